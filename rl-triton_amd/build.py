@@ -53,7 +53,8 @@ def sources() -> list[str]:
 
 def deps() -> list[str]:
     return sources() + sorted(glob.glob(os.path.join(CSRC, "*.hpp"))) + [
-        os.path.join(INCLUDE, "rl_triton_amd.h"), os.path.join(INCLUDE, "rlk_time_major.h"), os.path.abspath(__file__)]
+        os.path.join(INCLUDE, "rl_triton_amd.h"), os.path.join(INCLUDE, "rlk_time_major.h"),
+        os.path.join(INCLUDE, "rl_triton_policy.h"), os.path.abspath(__file__)]
 
 
 def up_to_date(target: str, inputs: list[str]) -> bool:

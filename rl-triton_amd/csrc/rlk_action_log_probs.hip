@@ -1,0 +1,109 @@
+// rlk_action_log_probs.hip -- log-probabilities and entropies of the taken actions
+// (include/rl_triton_policy.h; the mathematics is in rlk_action_rows.hpp).
+#include "rlk_action_rows.hpp"
+
+namespace rlk {
+namespace {
+
+template <class E, int LANES, int NV>
+__global__ __launch_bounds__(rows_threads<LANES>()) void log_probs_kernel(const ActionRows<E> a, float* __restrict__ log_probs,
+                                                                           float* __restrict__ entropies,
+                                                                           float* __restrict__ norms) {
+  constexpr int NT = rows_threads<LANES>(), PER = NT / LANES;
+  __shared__ float lds[LANES > 64 ? 3 * (LANES / 64) + 2 : 1];
+  const int lane = threadIdx.x % LANES;
+  for (int64_t row = (int64_t)blockIdx.x * PER + threadIdx.x / LANES; row < a.rows; row += (int64_t)gridDim.x * PER) {
+    const Frame<E> f(row_base(a, row), a.A);
+    RowStats r;
+    if constexpr (NV > 0) {
+      RowHolder<E, LANES, NV> h;
+      h.load(f, lane);
+      r = h.stats(f, lane, a.c, lds);
+    } else {
+      r = streamed_stats<E, LANES>(f, lane, a.c, lds);
+    }
+    if (lane == 0) {
+      const int64_t act = a.actions[row];
+      const float x = act >= 0 && act < a.A ? load_one(f.base + act) : NAN;
+      const float log2s = r.log2s();
+      const bool empty = r.s == 0.f;
+      log_probs[row] = empty && x == x ? -INFINITY : ((x - r.m) * a.c - log2s) * kLn2;
+      entropies[row] = empty ? 0.f : (log2s - r.u / r.s) * kLn2;
+      if (norms) norms[2 * row] = r.m, norms[2 * row + 1] = empty ? INFINITY : log2s;  // (inf: p = 0)
+    }
+    if constexpr (LANES > 64) __syncthreads();
+  }
+}
+
+template <class E, int LANES>
+__global__ __launch_bounds__(256) void backward_kernel(const ActionRows<E> a, const float* __restrict__ entropies,
+                                                       const float* __restrict__ norms, const float* __restrict__ gl,
+                                                       const float* __restrict__ ge, E* __restrict__ out) {
+  constexpr int PER = 256 / LANES;
+  const int lane = threadIdx.x % LANES;
+  for (int64_t row = (int64_t)blockIdx.x * PER + threadIdx.x / LANES; row < a.rows; row += (int64_t)gridDim.x * PER) {
+    const Frame<E> f(row_base(a, row), a.A);
+    const float log2s = norms[2 * row + 1];
+    const RowGrad g(gl ? gl[row] : 0.f, ge ? ge[row] : 0.f, entropies[row], norms[2 * row], log2s, a.inv_tau, a.actions[row],
+                    log2s == INFINITY);
+    write_grad<E, LANES, 0>(f, nullptr, out + row * a.A, g, a.c, lane);
+  }
+}
+
+template <class E>
+int forward(const rlk_action_rows* rows, float* lp, float* ent, float* norms, hipStream_t s) {
+  const ActionRows<E> a = action_rows<E>(rows);
+  constexpr int VEC = Frame<E>::VEC;
+  return dispatch_row((a.A + VEC - 1) / VEC, [&](auto lanes, auto nv) {
+    constexpr int L = decltype(lanes)::value, NV = decltype(nv)::value, NT = rows_threads<L>();
+    int64_t blocks = (a.rows + NT / L - 1) / (NT / L);
+    if (blocks > kMaxLossBlocks) blocks = kMaxLossBlocks;
+    log_probs_kernel<E, L, NV><<<dim3((unsigned)blocks), dim3(NT), 0, s>>>(a, lp, ent, norms);
+    return hipGetLastError() == hipSuccess ? RLK_OK : RLK_ERR_LAUNCH;
+  });
+}
+
+template <class E>
+int backward(const rlk_action_rows* rows, const float* ent, const float* norms, const float* gl, const float* ge, void* out,
+             hipStream_t s) {
+  const ActionRows<E> a = action_rows<E>(rows);
+  constexpr int VEC = Frame<E>::VEC;
+  const int64_t vecs = (a.A + VEC - 1) / VEC;
+  auto run = [&](auto lanes) {
+    constexpr int L = decltype(lanes)::value;
+    int64_t blocks = (a.rows + 256 / L - 1) / (256 / L);
+    if (blocks > 8192) blocks = 8192;
+    backward_kernel<E, L><<<dim3((unsigned)blocks), dim3(256), 0, s>>>(a, ent, norms, gl, ge, static_cast<E*>(out));
+    return hipGetLastError() == hipSuccess ? RLK_OK : RLK_ERR_LAUNCH;
+  };
+  if (vecs <= 8) return run(std::integral_constant<int, 4>{});
+  if (vecs <= 64) return run(std::integral_constant<int, 16>{});
+  return run(std::integral_constant<int, 256>{});
+}
+
+}  // namespace
+}  // namespace rlk
+
+using namespace rlk;
+
+extern "C" {
+
+int rlk_action_log_probs(const rlk_action_rows* rows, float* log_probs, float* entropies, float* norms, void* stream) {
+  if (!valid_rows(rows)) return RLK_ERR_INVALID_ARGUMENT;
+  if (rows->num_envs * rows->seq_len == 0) return RLK_OK;
+  if (!log_probs || !entropies) return RLK_ERR_INVALID_ARGUMENT;
+  const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  return rows->bf16 ? forward<bf16>(rows, log_probs, entropies, norms, s) : forward<float>(rows, log_probs, entropies, norms, s);
+}
+
+int rlk_action_log_probs_backward(const rlk_action_rows* rows, const float* entropies, const float* norms,
+                                  const float* grad_log_probs, const float* grad_entropies, void* grad_logits, void* stream) {
+  if (!valid_rows(rows)) return RLK_ERR_INVALID_ARGUMENT;
+  if (rows->num_envs * rows->seq_len == 0) return RLK_OK;
+  if (!entropies || !norms || !grad_logits) return RLK_ERR_INVALID_ARGUMENT;
+  const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  return rows->bf16 ? backward<bf16>(rows, entropies, norms, grad_log_probs, grad_entropies, grad_logits, s)
+                    : backward<float>(rows, entropies, norms, grad_log_probs, grad_entropies, grad_logits, s);
+}
+
+}  // extern "C"

@@ -1,0 +1,305 @@
+// rlk_action_rows.hpp -- rows of logits: softmax statistics in one read, and the gradient written from the
+// registers that still hold the row.
+//
+// For a row x and temperature tau, with c = log2(e) / tau, m = max x and y_j = (x_j - m) c:
+//   s = sum 2^y,  u = sum 2^y y,  log p_j = ln2 (y_j - log2 s),  H = ln2 (log2 s - u / s)
+// and for upstream gradients g of log p_a and h of H
+//   dx_j = (g ([j = a] - p_j) - h p_j (log p_j + H)) / tau.
+// x - m is formed before the product: a row whose logits are all the type's lowest value is then uniform
+// and not NaN.  Logits of -inf have no part (p = 0, nothing in u); a row of them alone has log p = -inf,
+// H = 0 and a zero gradient.  NaN and +inf make the row's outputs NaN through s.
+#pragma once
+#include "rlk_policy.hpp"
+
+namespace rlk {
+
+template <class E>
+struct ActionRows {
+  const E* logits;
+  const int64_t* actions;
+  int64_t rows, seq_len, env_stride, step_stride;
+  int A;
+  float c, inv_tau;
+};
+
+// The row as the lanes of a group hold it: `nfull` vectors of 16 bytes at 16-byte boundaries from element
+// `head` on, lane l holding vectors l, l + LANES, ...; the at most 2 (VEC - 1) elements before and after
+// them are held one by one.
+template <class E>
+struct Frame {
+  static constexpr int VEC = 16 / (int)sizeof(E);
+  const E* base;
+  int A, head, nfull;
+  __device__ Frame(const E* row, int A_) : base(row), A(A_) {
+    const int off = (int)((reinterpret_cast<uintptr_t>(row) / sizeof(E)) & (VEC - 1));
+    head = (VEC - off) & (VEC - 1);
+    if (head > A) head = A;
+    nfull = (A - head) / VEC;
+  }
+  // the element that edge slot `i` (0 .. 2 VEC - 1) stands for, or -1
+  __device__ int edge(int i) const {
+    if (i < VEC) return i < head ? i : -1;
+    const int j = head + nfull * VEC + (i - VEC);
+    return j < A ? j : -1;
+  }
+};
+
+__device__ __forceinline__ u32x4 load_words(const void* p) {
+  return __builtin_nontemporal_load(static_cast<const u32x4*>(p));
+}
+__device__ __forceinline__ void store_words(void* p, u32x4 w) {
+  __builtin_nontemporal_store(w, static_cast<u32x4*>(p));
+}
+
+template <class E>
+__device__ __forceinline__ void unpack(u32x4 w, float (&x)[16 / sizeof(E)]) {
+  constexpr int P = Words<E>::kPerWord;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int k = 0; k < P; ++k) x[i * P + k] = Words<E>::get(w[i], k);
+}
+template <class E>
+__device__ __forceinline__ u32x4 pack(const float (&x)[16 / sizeof(E)]) {
+  constexpr int P = Words<E>::kPerWord;
+  u32x4 w;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w[i] = Words<E>::put(x[i * P], x[i * P + P - 1]);
+  return w;
+}
+
+// Sums and maxima over the LANES lanes that hold a row: lanes of a wavefront, or the whole workgroup
+// (s: LANES / 64 floats, used alternately by two reductions).
+template <int LANES>
+__device__ __forceinline__ float group_max(float x, float* s) {
+#pragma unroll
+  for (int d = (LANES < 64 ? LANES : 64) / 2; d > 0; d >>= 1) x = fmaxf(x, __shfl_xor(x, d));
+  if constexpr (LANES > 64) {
+    if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = x;
+    __syncthreads();
+    x = s[0];
+#pragma unroll
+    for (int i = 1; i < LANES / 64; ++i) x = fmaxf(x, s[i]);
+  }
+  return x;
+}
+template <int LANES>
+__device__ __forceinline__ void group_sum2(float& a, float& b, float* s) {
+#pragma unroll
+  for (int d = (LANES < 64 ? LANES : 64) / 2; d > 0; d >>= 1) a += __shfl_xor(a, d), b += __shfl_xor(b, d);
+  if constexpr (LANES > 64) {
+    if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = a, s[LANES / 64 + (threadIdx.x >> 6)] = b;
+    __syncthreads();
+    a = s[0], b = s[LANES / 64];
+#pragma unroll
+    for (int i = 1; i < LANES / 64; ++i) a += s[i], b += s[LANES / 64 + i];
+  }
+}
+
+constexpr float kDeep = -1024.f;  // 2^kDeep is 0: below it y only has to be finite where it multiplies 2^y
+
+__device__ __forceinline__ void softmax_add(float x, float m, float c, float& s, float& u) {
+  const float y = (x - m) * c;
+  const float e = __builtin_amdgcn_exp2f(y);
+  s += e;
+  u = fmaf(e, fmaxf(y, kDeep), u);  // (y = -inf: e = 0 counts as 0)
+}
+
+struct RowStats {
+  float m, s, u;       // of a row without any finite logit: m = 0, s = u = 0
+  __device__ float log2s() const { return s == 0.f ? 0.f : __log2f(s); }
+};
+
+constexpr float kLn2 = 0.69314718055994531f;
+
+// What the writer of a gradient needs: p = 2^(y - log2 s), dx = p (a1 + b1 (y - log2 s)), plus g at the action.
+struct RowGrad {
+  float m, log2s, a1, b1, at;
+  int action;
+  bool zero;
+  __device__ RowGrad(float g, float h, float entropy, float m_, float log2s_, float inv_tau, int64_t a, bool empty)
+      : m(m_), log2s(log2s_), a1((-g - h * entropy) * inv_tau), b1(-h * kLn2 * inv_tau), at(g * inv_tau),
+        action(a >= 0 && a < (int64_t{1} << 30) ? (int)a : -1), zero(empty) {}
+  __device__ float operator()(float x, float c, int j) const {
+    const float y = fmaf(x - m, c, -log2s);
+    float d = __builtin_amdgcn_exp2f(y) * fmaf(b1, fmaxf(y, kDeep), a1);
+    return j == action ? d + at : d;
+  }
+};
+
+template <class E, int LANES, int NV>
+struct RowHolder {
+  static constexpr int VEC = Frame<E>::VEC;
+  static constexpr int EDGES = (2 * VEC + LANES - 1) / LANES;
+  u32x4 v[NV];
+  float edge[EDGES];
+
+  __device__ __forceinline__ void load(const Frame<E>& f, int lane) {
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const int i = lane + LANES * k;
+      if (i < f.nfull) v[k] = load_words(f.base + f.head + i * VEC);
+    }
+#pragma unroll
+    for (int k = 0; k < EDGES; ++k) {
+      const int j = lane + LANES * k < 2 * VEC ? f.edge(lane + LANES * k) : -1;
+      edge[k] = j >= 0 ? load_one(f.base + j) : -INFINITY;
+    }
+  }
+  __device__ __forceinline__ RowStats stats(const Frame<E>& f, int lane, float c, float* lds) const {
+    float m = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < EDGES; ++k) m = fmaxf(m, edge[k]);
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
+      if (lane + LANES * k < f.nfull) {
+        float x[VEC];
+        unpack<E>(v[k], x);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) m = fmaxf(m, x[i]);
+      }
+    RowStats r{group_max<LANES>(m, lds), 0.f, 0.f};
+    if (r.m == -INFINITY) r.m = 0.f;
+#pragma unroll
+    for (int k = 0; k < EDGES; ++k) softmax_add(edge[k], r.m, c, r.s, r.u);
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
+      if (lane + LANES * k < f.nfull) {
+        float x[VEC];
+        unpack<E>(v[k], x);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) softmax_add(x[i], r.m, c, r.s, r.u);
+      }
+    group_sum2<LANES>(r.s, r.u, lds + LANES / 64 + 1);
+    return r;
+  }
+};
+
+// Writes the gradient of a row, `held` (NV > 0) or read again.
+template <class E, int LANES, int NV>
+__device__ __forceinline__ void write_grad(const Frame<E>& f, const RowHolder<E, LANES, NV>* held, E* out, const RowGrad& g,
+                                           float c, int lane) {
+  constexpr int VEC = Frame<E>::VEC;
+  // the output has the input's place in its 16 bytes unless the logits' rows are strided
+  const bool same = ((reinterpret_cast<uintptr_t>(out) ^ reinterpret_cast<uintptr_t>(f.base)) & 15u) == 0;
+  auto vec = [&](u32x4 w, int i) {
+    const int j0 = f.head + i * VEC;
+    float x[VEC];
+    unpack<E>(w, x);
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) x[k] = g.zero ? 0.f : g(x[k], c, j0 + k);
+    if (same) {
+      store_words(out + j0, pack<E>(x));
+    } else {
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) out[j0 + k] = from_f32<E>(x[k]);
+    }
+  };
+  if constexpr (NV > 0) {
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
+      if (lane + LANES * k < f.nfull) vec(held->v[k], lane + LANES * k);
+  } else {
+#pragma unroll 4
+    for (int i = lane; i < f.nfull; i += LANES) vec(load_words(f.base + f.head + i * VEC), i);
+  }
+  for (int i = lane; i < 2 * VEC; i += LANES) {
+    const int j = f.edge(i);
+    if (j >= 0) out[j] = from_f32<E>(g.zero ? 0.f : g(load_one(f.base + j), c, j));
+  }
+}
+
+template <class E, int LANES>
+__device__ __forceinline__ void write_zeros(E* out, int A, int lane) {
+  const Frame<E> f(out, A);
+  for (int i = lane; i < f.nfull; i += LANES) store_words(out + f.head + i * Frame<E>::VEC, u32x4{0, 0, 0, 0});
+  for (int i = lane; i < 2 * Frame<E>::VEC; i += LANES) {
+    const int j = f.edge(i);
+    if (j >= 0) out[j] = from_f32<E>(0.f);
+  }
+}
+
+// Statistics of a row too long to hold: read once, with a running maximum per lane.
+template <class E, int LANES>
+__device__ __forceinline__ RowStats streamed_stats(const Frame<E>& f, int lane, float c, float* lds) {
+  constexpr int VEC = Frame<E>::VEC;
+  float m = -INFINITY, s = 0.f, u = 0.f;
+  auto rebase = [&](float to) {  // sums about `to` in place of m
+    if (m == to) return;
+    if (m != -INFINITY) {  // (else they are 0, or NaN from a NaN)
+      const float d = (m - to) * c, f2 = __builtin_amdgcn_exp2f(d);
+      u = f2 * fmaf(d, s, u);
+      s = f2 * s;
+    }
+    m = to;
+  };
+  for (int i = lane; i < 2 * VEC; i += LANES) {
+    const int j = f.edge(i);
+    const float x = j >= 0 ? load_one(f.base + j) : -INFINITY;
+    if (x != -INFINITY) {
+      rebase(fmaxf(m, x));
+      softmax_add(x, m, c, s, u);
+    }
+  }
+#pragma unroll 4
+  for (int i = lane; i < f.nfull; i += LANES) {
+    float x[VEC];
+    unpack<E>(load_words(f.base + f.head + i * VEC), x);
+    float t = x[0];
+    bool nan = x[0] != x[0];
+#pragma unroll
+    for (int k = 1; k < VEC; ++k) t = fmaxf(t, x[k]), nan |= x[k] != x[k];
+    if (nan) {
+      s = NAN;
+    } else if (t != -INFINITY) {
+      rebase(fmaxf(m, t));
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) softmax_add(x[k], m, c, s, u);
+    }
+  }
+  float top = group_max<LANES>(m, lds);
+  if (top != -INFINITY) rebase(top);
+  else top = 0.f;
+  group_sum2<LANES>(s, u, lds + LANES / 64 + 1);
+  return RowStats{top, s, u};
+}
+
+template <int LANES>
+constexpr int rows_threads() { return LANES > 256 ? LANES : 256; }
+
+// Calls f(integral constants LANES, NV) for rows of `vecs` 16-byte vectors: the fewest lanes that hold one
+// in at most 4 vectors each (8 and 16 for the longest rows, NV = 0 beyond: those are read twice).
+template <class F>
+int dispatch_row(int64_t vecs, F f) {
+  using std::integral_constant;
+  if (vecs <= 8) return f(integral_constant<int, 4>{}, integral_constant<int, 2>{});
+  if (vecs <= 64) return f(integral_constant<int, 16>{}, integral_constant<int, 4>{});
+  if (vecs <= 256) return f(integral_constant<int, 64>{}, integral_constant<int, 4>{});
+  if (vecs <= 1024) return f(integral_constant<int, 256>{}, integral_constant<int, 4>{});
+  if (vecs <= 2048) return f(integral_constant<int, 256>{}, integral_constant<int, 8>{});
+  if (vecs <= 8192) return f(integral_constant<int, 1024>{}, integral_constant<int, 8>{});
+  if (vecs <= 16384) return f(integral_constant<int, 1024>{}, integral_constant<int, 16>{});
+  return f(integral_constant<int, 1024>{}, integral_constant<int, 0>{});
+}
+
+inline bool valid_rows(const rlk_action_rows* r) {
+  if (!r || r->num_envs < 0 || r->seq_len < 0 || r->num_actions < 1 || r->num_actions > (int64_t{1} << 30)) return false;
+  if (!(r->temperature > 0.f) || !std::isfinite(r->temperature)) return false;
+  return r->num_envs * r->seq_len == 0 || (r->logits && r->actions && (reinterpret_cast<uintptr_t>(r->logits) & (r->bf16 ? 1u : 3u)) == 0);
+}
+
+template <class E>
+ActionRows<E> action_rows(const rlk_action_rows* r) {
+  const double inv = 1.0 / (double)r->temperature;
+  return {static_cast<const E*>(r->logits), r->actions, r->num_envs * r->seq_len, r->seq_len, r->env_stride, r->step_stride,
+          (int)r->num_actions, (float)(1.4426950408889634 * inv), (float)inv};
+}
+
+template <class E>
+__device__ __forceinline__ const E* row_base(const ActionRows<E>& a, int64_t row) {
+  if (a.env_stride == a.seq_len * a.step_stride) return a.logits + row * a.step_stride;
+  const int64_t e = row / a.seq_len;
+  return a.logits + e * a.env_stride + (row - e * a.seq_len) * a.step_stride;
+}
+
+}  // namespace rlk

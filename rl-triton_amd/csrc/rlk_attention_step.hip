@@ -1,0 +1,103 @@
+// rlk_attention_step.hip -- one step of linear attention for every environment (include/rl_triton_policy.h):
+//   S' = lambda (1 - done) S + k v^T,  out = scale S'^T q.
+// The state is read and written once and is nearly all there is to move: a workgroup per (environment, head),
+// each thread a quad of columns, the rows dealt out over the workgroup.
+#include "rlk_attention.hpp"
+
+namespace rlk {
+namespace {
+
+constexpr int kNT = 256;
+
+template <class E, int LANES, bool VEC>  // LANES lanes cover a row of the state in quads
+__global__ __launch_bounds__(kNT) void step_kernel(const Walk<E> w, int heads, const float* __restrict__ decay,
+                                                   const float* __restrict__ dones) {
+  constexpr int ROWS = kNT / LANES;
+  __shared__ float qs[128], ks[128];
+  __shared__ float4 part[ROWS][LANES];
+  const int head = blockIdx.x % heads, tid = threadIdx.x;
+  const int64_t env = blockIdx.x / heads, eh = blockIdx.x;
+  const int lane = tid % LANES, row0 = tid / LANES, j = lane * 4;
+  if (tid < w.da) {
+    qs[tid] = load_one(w.a.data + env * w.a.env_stride + head * w.a.head_stride + tid);
+    ks[tid] = load_one(w.b.data + env * w.b.env_stride + head * w.b.head_stride + tid);
+  }
+  const bool cut = dones != nullptr && dones[env] != 0.f;
+  const float lambda = decay[head];
+  const E* gv = w.c.data + env * w.c.env_stride + head * w.c.head_stride;
+  float v[4];
+#pragma unroll
+  for (int x = 0; x < 4; ++x) v[x] = j + x < w.dc ? load_one(gv + j + x) : 0.f;
+  __syncthreads();
+  const float* src = w.state + eh * (int64_t)(w.da * w.dc);
+  float* dst = w.state_out + eh * (int64_t)(w.da * w.dc);
+  float4 acc{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
+  for (int i = row0; i < w.da; i += ROWS) {
+    float4 x{0.f, 0.f, 0.f, 0.f};
+    if (j < w.dc) {
+      const int at = i * w.dc + j;
+      if (!cut) {  // (what a cut state held has no part, NaN included)
+        if constexpr (VEC) {
+          x = *reinterpret_cast<const float4*>(src + at);
+        } else {
+          x.x = src[at];
+          if (j + 1 < w.dc) x.y = src[at + 1];
+          if (j + 2 < w.dc) x.z = src[at + 2];
+          if (j + 3 < w.dc) x.w = src[at + 3];
+        }
+      }
+      const float k = ks[i], q = qs[i];
+      x.x = fmaf(lambda, x.x, k * v[0]), x.y = fmaf(lambda, x.y, k * v[1]);
+      x.z = fmaf(lambda, x.z, k * v[2]), x.w = fmaf(lambda, x.w, k * v[3]);
+      if constexpr (VEC) {
+        *reinterpret_cast<float4*>(dst + at) = x;
+      } else {
+        dst[at] = x.x;
+        if (j + 1 < w.dc) dst[at + 1] = x.y;
+        if (j + 2 < w.dc) dst[at + 2] = x.z;
+        if (j + 3 < w.dc) dst[at + 3] = x.w;
+      }
+      acc.x = fmaf(q, x.x, acc.x), acc.y = fmaf(q, x.y, acc.y), acc.z = fmaf(q, x.z, acc.z), acc.w = fmaf(q, x.w, acc.w);
+    }
+  }
+  part[row0][lane] = acc;
+  __syncthreads();
+  if (tid < w.dc) {
+    float y = 0.f;
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) y += reinterpret_cast<const float*>(&part[r][0])[tid];
+    w.y.data[env * w.y.env_stride + head * w.y.head_stride + tid] = from_f32<E>(y * w.scale);
+  }
+}
+
+template <class E>
+int step_impl(const rlk_attention& c, hipStream_t s) {
+  Walk<E> w = {};
+  w.a = sequence<const E>(c.q), w.b = sequence<const E>(c.k), w.c = sequence<const E>(c.v), w.y = sequence<E>(c.out);
+  w.da = (int)c.dim_k, w.dc = (int)c.dim_v, w.state = c.state, w.state_out = c.state_out, w.scale = c.scale;
+  const bool vec = c.dim_v % 4 == 0 && ((reinterpret_cast<uintptr_t>(c.state) | reinterpret_cast<uintptr_t>(c.state_out)) & 15u) == 0;
+  const dim3 grid((unsigned)(c.num_envs * c.heads)), block(kNT);
+  const int heads = (int)c.heads;
+  if (c.dim_v <= 64) {
+    if (vec) step_kernel<E, 16, true><<<grid, block, 0, s>>>(w, heads, c.decay, c.dones);
+    else step_kernel<E, 16, false><<<grid, block, 0, s>>>(w, heads, c.decay, c.dones);
+  } else {
+    if (vec) step_kernel<E, 32, true><<<grid, block, 0, s>>>(w, heads, c.decay, c.dones);
+    else step_kernel<E, 32, false><<<grid, block, 0, s>>>(w, heads, c.decay, c.dones);
+  }
+  return hipGetLastError() == hipSuccess ? RLK_OK : RLK_ERR_LAUNCH;
+}
+
+}  // namespace
+}  // namespace rlk
+
+using namespace rlk;
+
+extern "C" int rlk_linear_attention_step(const rlk_attention* call, void* stream) {
+  if (!call || !valid_attention(*call)) return RLK_ERR_INVALID_ARGUMENT;
+  if (call->num_envs == 0 || call->heads == 0) return RLK_OK;
+  if (!call->state || !call->state_out || call->num_envs * call->heads > kMaxGrid) return RLK_ERR_INVALID_ARGUMENT;
+  const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  return call->bf16 ? step_impl<bf16>(*call, s) : step_impl<float>(*call, s);
+}

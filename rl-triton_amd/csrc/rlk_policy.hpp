@@ -1,0 +1,164 @@
+// rlk_policy.hpp -- what the learner's operators share: 16-byte vectors of either storage type, group and
+// workgroup reductions, the policy loss's terms, and the weights of its mean.
+#pragma once
+#include <hip/hip_runtime.h>
+
+#include <cmath>
+#include <cstdint>
+
+#include "rl_triton_policy.h"
+#include "rlk_ops.hpp"
+
+namespace rlk {
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+
+// N consecutive elements of E as they are stored, in words.
+template <class E>
+struct Words;
+template <>
+struct Words<float> {
+  static constexpr int kPerWord = 1;
+  __device__ static float get(uint32_t w, int) { return __uint_as_float(w); }
+  __device__ static uint32_t put(float a, float) { return __float_as_uint(a); }
+};
+template <>
+struct Words<bf16> {
+  static constexpr int kPerWord = 2;
+  __device__ static float get(uint32_t w, int i) { return __uint_as_float(i == 0 ? w << 16 : w & 0xffff0000u); }
+  __device__ static uint32_t put(float a, float b) { return pack_bf16x2(a, b); }
+};
+
+__device__ __forceinline__ float load_one(const float* p) { return *p; }
+__device__ __forceinline__ float load_one(const bf16* p) { return to_f32(*p); }
+
+// The sum of `x` over a workgroup of NT threads, in a fixed order, in every thread.  `s`: NT / 64 elements.
+template <int NT, class T>
+__device__ __forceinline__ T block_sum(T x, T* s) {
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) x += __shfl_xor(x, d);
+  if constexpr (NT == 64) return x;
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = x;
+  __syncthreads();
+  T r = s[0];
+#pragma unroll
+  for (int i = 1; i < NT / 64; ++i) r += s[i];
+  return r;
+}
+
+// ---------------------------------------------------------------------------------------
+// The policy loss, step by step.
+//
+// With D = log pi - log pi_old, r = e^D and advantage A the loss of a step is max(-A r, -A clip(r)).  The
+// maximum takes the clipped side only where A > 0 and r is above, or A < 0 and r below; which side is told by
+// comparing D with the logarithms of the bounds, so no rounding of the exponential decides it.  On the
+// clipped side, and where the dual clip caps it, the gradient is zero, elsewhere d/d(log pi) = -A r.  The KL
+// term is e^d - 1 - d with d = log pi_ref - log pi, derivative 1 - e^d.
+// ---------------------------------------------------------------------------------------
+struct LossConsts {
+  float log_low, log_high, log_dual;  // thresholds of D; log_dual = inf: no cap
+  float low, high, dual;              // the values themselves
+  float kl_coef, entropy_coef;
+};
+
+constexpr int kTerms = 5;  // policy, KL, clipped share, KL to the old policy, entropy
+
+struct StepTerms {
+  float v[4];
+  float slope;
+};
+
+// e^x - 1 - x >= 0 without the cancellation near zero: its series up to 1/2 in size (the first dropped
+// term is below 2^-25 of the sum), the plain difference beyond, where it loses at most two bits.
+__device__ __forceinline__ float exp_minus_linear(float x, float ex) {
+  float p = 1.f / 362880.f;
+  p = fmaf(p, x, 1.f / 40320.f);
+  p = fmaf(p, x, 1.f / 5040.f);
+  p = fmaf(p, x, 1.f / 720.f);
+  p = fmaf(p, x, 1.f / 120.f);
+  p = fmaf(p, x, 1.f / 24.f);
+  p = fmaf(p, x, 1.f / 6.f);
+  p = fmaf(p, x, 0.5f);
+  return fabsf(x) < 0.5f ? p * x * x : (ex - 1.f) - x;
+}
+
+__device__ __forceinline__ StepTerms step_terms(float lp, float old, float adv, float ref, bool has_ref,
+                                                const LossConsts& c) {
+  StepTerms t;
+  const float d = lp - old;
+  const float r = expf(d);
+  const bool up = d > c.log_high && adv > 0.f, down = d < c.log_low && adv < 0.f;
+  const bool cap = d > c.log_dual && adv < 0.f;
+  const bool flat = up || down || cap;
+  const float held = cap ? c.dual : up ? c.high : down ? c.low : r;
+  t.v[0] = -adv * held;
+  t.slope = flat ? 0.f : -adv * r;
+  t.v[2] = flat ? 1.f : 0.f;
+  t.v[3] = exp_minus_linear(d, r);
+  t.v[1] = 0.f;
+  if (has_ref) {
+    const float e = ref - lp;
+    const float ee = expf(e);
+    t.v[1] = exp_minus_linear(e, ee);
+    t.slope -= c.kl_coef * (t.v[1] + e);  // e^e - 1
+  }
+  return t;
+}
+
+// ---------------------------------------------------------------------------------------
+// Weights of the mean.  `steps`: 1 / (number of steps that take part).  `rows`: 1 / (n_row * rows with any).
+// With a mask these numbers come from count_kernel: a number per row, and per workgroup the sums of what
+// the mean divides by, which every workgroup that needs them adds up in the same order (whole numbers: exact).
+// ---------------------------------------------------------------------------------------
+constexpr int kCountBlocks = 256;
+
+struct Weights {
+  const int64_t* parts;  // [kCountBlocks], or NULL: no mask
+  const int* row_counts;  // [num_envs] (per_row with a mask)
+  int num_parts;
+  int per_row;
+  float all;  // without a mask: every step's weight
+};
+
+// What all steps' weights have in common, in every thread of the workgroup.
+template <int NT>
+__device__ __forceinline__ float weight_scale(const Weights& w, int64_t* s) {
+  if (w.parts == nullptr) return w.all;
+  int64_t n = 0;
+  for (int i = threadIdx.x; i < w.num_parts; i += NT) n += w.parts[i];
+  n = block_sum<NT>(n, s);
+  return n > 0 ? (float)(1.0 / (double)n) : 0.f;
+}
+
+// Partial sums of the loss's terms, one set of kTerms doubles per workgroup, and the small kernel that adds
+// them up (rlk_policy_loss.hip).
+constexpr int kMaxLossBlocks = 4096;
+
+struct LossPlan {
+  LossConsts consts;
+  Weights weights;
+  double* partials;
+  int64_t* count_parts;
+  int* row_counts;
+};
+
+// Checks the terms and lays out the workspace; RLK_OK or an error.
+int plan_loss(const rlk_policy_terms* t, int64_t num_envs, int64_t seq_len, LossPlan* plan);
+// Counts the steps that take part (when there is a mask).
+int launch_count(const rlk_policy_terms* t, int64_t num_envs, int64_t seq_len, LossPlan* plan, hipStream_t s);
+// loss and means from `blocks` sets of partial sums.
+int launch_finish(const rlk_policy_terms* t, const LossPlan& plan, int blocks, int means, hipStream_t s);
+
+// Adds a thread's terms to its workgroup's and writes the workgroup's partial sums.
+template <int NT>
+__device__ __forceinline__ void write_partials(const float (&acc)[kTerms], double* partials, double* s) {
+#pragma unroll
+  for (int i = 0; i < kTerms; ++i) {
+    const double x = block_sum<NT>((double)acc[i], s);
+    if (threadIdx.x == 0) partials[(int64_t)blockIdx.x * kTerms + i] = x;
+  }
+}
+
+}  // namespace rlk

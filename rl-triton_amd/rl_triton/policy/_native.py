@@ -1,0 +1,188 @@
+"""ctypes binding of the learner's operators (include/rl_triton_policy.h) in librl_triton_amd.so.
+
+Tensors reaching this module are on one GPU, of the right type and shape; this turns them into
+the C ABI's structures, launches on torch's current stream of their device and owns the
+workspaces, one per (device, stream), as rl_triton._native does for the estimators.
+"""
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from rl_triton import _native
+
+_P, _I64, _F, _INT, _SZ = ctypes.c_void_p, ctypes.c_int64, ctypes.c_float, ctypes.c_int, ctypes.c_size_t
+
+
+class ActionRows(ctypes.Structure):
+    _fields_ = [("logits", _P), ("actions", _P), ("num_envs", _I64), ("seq_len", _I64), ("num_actions", _I64),
+                ("env_stride", _I64), ("step_stride", _I64), ("temperature", _F), ("bf16", _INT)]
+
+
+class PolicyTerms(ctypes.Structure):
+    _fields_ = [("old_log_probs", _P), ("advantages", _P), ("ref_log_probs", _P), ("mask", _P), ("clip_low", _F),
+                ("clip_high", _F), ("dual_clip", _F), ("kl_coef", _F), ("entropy_coef", _F), ("per_row", _INT),
+                ("bf16", _INT), ("loss", _P), ("means", _P), ("workspace", _P), ("workspace_bytes", _SZ)]
+
+
+class Sequence(ctypes.Structure):
+    _fields_ = [("data", _P), ("env_stride", _I64), ("step_stride", _I64), ("head_stride", _I64)]
+
+
+class Attention(ctypes.Structure):
+    _fields_ = [("q", Sequence), ("k", Sequence), ("v", Sequence), ("out", Sequence), ("num_envs", _I64),
+                ("seq_len", _I64), ("heads", _I64), ("dim_k", _I64), ("dim_v", _I64), ("decay", _P), ("dones", _P),
+                ("state", _P), ("state_transposed", _INT), ("state_out", _P), ("scale", _F), ("state_scale", _F),
+                ("state_out_scale", _F), ("reverse", _INT), ("bf16", _INT), ("workspace", _P),
+                ("workspace_bytes", _SZ)]
+
+
+# name -> argtypes (must match include/rl_triton_policy.h)
+SIGNATURES = {
+    "rlk_action_log_probs": [ctypes.POINTER(ActionRows), _P, _P, _P, _P],
+    "rlk_action_log_probs_backward": [ctypes.POINTER(ActionRows), _P, _P, _P, _P, _P, _P],
+    "rlk_policy_workspace_bytes": [_I64],
+    "rlk_policy_loss": [_P, _I64, _I64, ctypes.POINTER(PolicyTerms), _P, _P],
+    "rlk_policy_loss_from_logits": [ctypes.POINTER(ActionRows), ctypes.POINTER(PolicyTerms), _P, _P],
+    "rlk_attention_workspace_bytes": [_I64, _I64, _I64, _I64, _I64],
+    "rlk_linear_attention": [ctypes.POINTER(Attention), _INT, _P],
+    "rlk_linear_attention_step": [ctypes.POINTER(Attention), _P],
+}
+_RESTYPES = {"rlk_policy_workspace_bytes": _SZ, "rlk_attention_workspace_bytes": _SZ}
+
+_lib = None
+
+
+def load():
+    global _lib
+    if _lib is None:
+        lib = _native.load()
+        for name, argtypes in SIGNATURES.items():
+            fn = getattr(lib, name)
+            fn.argtypes = argtypes
+            fn.restype = _RESTYPES.get(name, _INT)
+        _lib = lib
+    return _lib
+
+
+_BF16 = torch.bfloat16
+_workspaces: dict = {}
+
+
+def _workspace(dev: int, stream: int, need: int):
+    """Scratch memory of the current call: kept per (device, stream) and grown by doubling; a call being
+    captured into a graph gets memory of its own, kept for the life of the process."""
+    if need == 0:
+        return None, 0
+    if _native._capturing():
+        ws = torch.empty(need, dtype=torch.uint8, device=torch.device("cuda", dev))
+        _native._captured.append(ws)
+        return ws.data_ptr(), need
+    ws = _workspaces.get((dev, stream))
+    if ws is None or ws.numel() < need:
+        ws = torch.empty(max(need, 2 * ws.numel() if ws is not None else 0), dtype=torch.uint8,
+                         device=torch.device("cuda", dev))
+        _workspaces[(dev, stream)] = ws
+    return ws.data_ptr(), ws.numel()
+
+
+def _on_device(fn):
+    """Runs `fn(dev, stream, ...)` with its first tensor's device current."""
+    def call(lead, *args):
+        dev = lead.get_device()
+        if dev != _native._cur_device():
+            with torch.cuda.device(dev):
+                return fn(dev, _native._raw_stream(dev), lead, *args)
+        return fn(dev, _native._raw_stream(dev), lead, *args)
+    return call
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _rows(logits, actions, temperature):
+    e, t, a = logits.shape
+    se, st, _ = logits.stride()
+    return ActionRows(logits.data_ptr(), actions.data_ptr(), e, t, a, se, st, temperature, logits.dtype is _BF16)
+
+
+@_on_device
+def action_log_probs(dev, stream, logits, actions, temperature, log_probs, entropies, norms):
+    _native._check((_lib or load()).rlk_action_log_probs(ctypes.byref(_rows(logits, actions, temperature)),
+                                                        log_probs.data_ptr(), entropies.data_ptr(), _ptr(norms), stream),
+                   "rlk_action_log_probs")
+
+
+@_on_device
+def action_log_probs_backward(dev, stream, logits, actions, temperature, entropies, norms, grad_log_probs,
+                              grad_entropies, grad_logits):
+    _native._check((_lib or load()).rlk_action_log_probs_backward(
+        ctypes.byref(_rows(logits, actions, temperature)), entropies.data_ptr(), norms.data_ptr(), _ptr(grad_log_probs),
+        _ptr(grad_entropies), grad_logits.data_ptr(), stream), "rlk_action_log_probs_backward")
+
+
+def _terms(dev, stream, num_envs, old, advantages, ref, mask, clip, kl_coef, entropy_coef, per_row, loss, means):
+    ws, wsb = _workspace(dev, stream, (_lib or load()).rlk_policy_workspace_bytes(num_envs))
+    low, high, dual = clip
+    return PolicyTerms(old.data_ptr(), advantages.data_ptr(), _ptr(ref), _ptr(mask), low, high, dual, kl_coef,
+                       entropy_coef, per_row, old.dtype is _BF16, loss.data_ptr(), means.data_ptr(), ws, wsb)
+
+
+@_on_device
+def policy_loss(dev, stream, log_probs, old, advantages, ref, mask, clip, kl_coef, per_row, loss, means, grad):
+    e, t = log_probs.shape
+    terms = _terms(dev, stream, e, old, advantages, ref, mask, clip, kl_coef, 0.0, per_row, loss, means)
+    _native._check(_lib.rlk_policy_loss(log_probs.data_ptr(), e, t, ctypes.byref(terms), grad.data_ptr(), stream),
+                   "rlk_policy_loss")
+
+
+@_on_device
+def policy_loss_from_logits(dev, stream, logits, actions, temperature, old, advantages, ref, mask, clip, kl_coef,
+                            entropy_coef, per_row, loss, means, grad):
+    terms = _terms(dev, stream, logits.shape[0], old, advantages, ref, mask, clip, kl_coef, entropy_coef, per_row, loss,
+                   means)
+    _native._check(_lib.rlk_policy_loss_from_logits(ctypes.byref(_rows(logits, actions, temperature)),
+                                                   ctypes.byref(terms), grad.data_ptr(), stream),
+                   "rlk_policy_loss_from_logits")
+
+
+def _sequence(t):
+    if t.dim() == 3:  # one step: [num_envs, heads, dim]
+        return Sequence(t.data_ptr(), t.stride(0), 0, t.stride(1))
+    return Sequence(t.data_ptr(), t.stride(0), t.stride(1), t.stride(2))
+
+
+class Pass:
+    """One recurrence of a linear attention call: arrays by role, states, scales and direction."""
+    __slots__ = ("a", "b", "c", "y", "state", "transposed", "state_out", "scale", "state_scale", "out_scale", "reverse")
+
+    def __init__(self, a, b, c, y, state, state_out, scale, transposed=False, reverse=False, state_scale=1.0, out_scale=1.0):
+        self.a, self.b, self.c, self.y = a, b, c, y
+        self.state, self.state_out, self.transposed = state, state_out, transposed
+        self.scale, self.state_scale, self.out_scale, self.reverse = scale, state_scale, out_scale, reverse
+
+    def struct(self, decay, dones, ws, wsb):
+        a, y = self.a, self.y
+        seq = a.shape[1] if a.dim() == 4 else 1
+        return Attention(_sequence(a), _sequence(self.b), _sequence(self.c), _sequence(y), a.shape[0], seq, a.shape[-2],
+                         a.shape[-1], y.shape[-1], decay.data_ptr(), _ptr(dones), _ptr(self.state), self.transposed,
+                         _ptr(self.state_out), self.scale, self.state_scale, self.out_scale, self.reverse,
+                         a.dtype is _BF16, ws, wsb)
+
+
+@_on_device
+def linear_attention(dev, stream, decay, dones, passes):
+    lib = _lib or load()
+    e, t, h = passes[0].a.shape[:3]
+    need = sum(lib.rlk_attention_workspace_bytes(e, t, h, p.a.shape[-1], p.y.shape[-1]) for p in passes)
+    ws, wsb = _workspace(dev, stream, need)
+    calls = (Attention * len(passes))(*(p.struct(decay, dones, ws, wsb) for p in passes))
+    _native._check(lib.rlk_linear_attention(calls, len(passes), stream), "rlk_linear_attention")
+
+
+@_on_device
+def linear_attention_step(dev, stream, decay, dones, step):
+    _native._check((_lib or load()).rlk_linear_attention_step(ctypes.byref(step.struct(decay, dones, None, 0)), stream),
+                   "rlk_linear_attention_step")
