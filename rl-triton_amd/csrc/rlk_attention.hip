@@ -13,8 +13,8 @@
 //   U'  = lambda^L [no cut in the chunk] U + sum_j lambda^{L-j} same(j, L-1) b_j c_j^T
 // Every factor is a power with an exponent >= 0 (no quotient of powers, which would leave float's range).
 //
-// A workgroup of 4 wavefronts walks the chunks of its (environment, head, segment); wavefront w owns a quarter of
-// the columns of c.  Its part of U stays in the accumulators of the matrix instructions for the whole walk: the
+// A workgroup walks the chunks of its (environment, head, segment) with a wavefront for every 16 columns of c (4
+// wavefronts for dims of up to 64, 8 for up to 128).  A wavefront's part of U stays in the accumulators of the matrix instructions for the whole walk: the
 // accumulator layout (4 consecutive rows of a column per lane) is also an operand layout once the inner index is
 // taken in that order, so U feeds U^T a without a trip through LDS.
 #include "rlk_attention.hpp"
@@ -23,10 +23,14 @@ namespace rlk {
 namespace {
 
 constexpr int C = 64;       // steps per chunk
-constexpr int kNT = 256;    // 4 wavefronts
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+
+// Two floats as bfloat16, rounded to nearest even as the instruction does it (a NaN keeps its own bits).
+__device__ __forceinline__ uint32_t bf16_pair(float lo, float hi) {
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2_t){lo, hi}, bf16x2_t));
+}
 
 // 8 consecutive (in the inner index) elements of an operand row: the unit of a matrix instruction's operands.
 template <class E>
@@ -42,8 +46,8 @@ struct Frag<bf16> {
   }
   __device__ static Frag from(f32x4 a, f32x4 b) {
     union { uint32_t w[4]; bf16x8 v; } u;
-    u.w[0] = pack_bf16x2(a[0], a[1]), u.w[1] = pack_bf16x2(a[2], a[3]);
-    u.w[2] = pack_bf16x2(b[0], b[1]), u.w[3] = pack_bf16x2(b[2], b[3]);
+    u.w[0] = bf16_pair(a[0], a[1]), u.w[1] = bf16_pair(a[2], a[3]);
+    u.w[2] = bf16_pair(b[0], b[1]), u.w[3] = bf16_pair(b[2], b[3]);
     return {u.v};
   }
 };
@@ -77,18 +81,32 @@ struct Quad;
 template <>
 struct Quad<bf16> {
   u32x2 w;
-  __device__ float get(int i) const { return Words<bf16>::get(w[i >> 1], i & 1); }
-  __device__ static Quad of(float a, float b, float c, float d) { return {{pack_bf16x2(a, b), pack_bf16x2(c, d)}}; }
+  __device__ static Quad of(f32x4 x) { return {{bf16_pair(x[0], x[1]), bf16_pair(x[2], x[3])}}; }
+  __device__ static Quad bits(bf16 a, bf16 b, bf16 c, bf16 d) {
+    return {{(uint32_t)a.bits | (uint32_t)b.bits << 16, (uint32_t)c.bits | (uint32_t)d.bits << 16}};
+  }
   __device__ static Quad load(const bf16* p) { return {*reinterpret_cast<const u32x2*>(p)}; }
   __device__ void store(bf16* p) const { *reinterpret_cast<u32x2*>(p) = w; }
+  __device__ void clear() { w = u32x2{0, 0}; }
+  // element x of four quads
+  template <int X>
+  __device__ static Quad across(const Quad& a, const Quad& b, const Quad& c, const Quad& d) {
+    constexpr uint32_t sel = X & 1 ? 0x07060302u : 0x05040100u;
+    return {{__builtin_amdgcn_perm(b.w[X >> 1], a.w[X >> 1], sel), __builtin_amdgcn_perm(d.w[X >> 1], c.w[X >> 1], sel)}};
+  }
 };
 template <>
 struct Quad<float> {
   f32x4 w;
-  __device__ float get(int i) const { return w[i]; }
-  __device__ static Quad of(float a, float b, float c, float d) { return {{a, b, c, d}}; }
+  __device__ static Quad of(f32x4 x) { return {x}; }
+  __device__ static Quad bits(float a, float b, float c, float d) { return {{a, b, c, d}}; }
   __device__ static Quad load(const float* p) { return {*reinterpret_cast<const f32x4*>(p)}; }
   __device__ void store(float* p) const { *reinterpret_cast<f32x4*>(p) = w; }
+  __device__ void clear() { w = f32x4{0.f, 0.f, 0.f, 0.f}; }
+  template <int X>
+  __device__ static Quad across(const Quad& a, const Quad& b, const Quad& c, const Quad& d) {
+    return {{a.w[X], b.w[X], c.w[X], d.w[X]}};
+  }
 };
 
 // x^n for n >= 0 from log2 x (x = 0: 1, 0, 0, ...).
@@ -97,53 +115,93 @@ __device__ __forceinline__ float power(float log2x, int n) { return n == 0 ? 1.f
 template <class E, int D>
 struct Tiles {
   static constexpr int PAD = 16 / (int)sizeof(E);
-  E a[C][D + PAD];    // rows of a chunk
+  E a[C][D + PAD];   // rows of a chunk
   E b[C][D + PAD];
-  E bt[D][C + PAD];   // b transposed
-  E ct[D][C + PAD];   // c transposed
-  E p[C][C + PAD];    // (a_i . b_j) lambda^{i-j} same(j, i)
+  E bt[D * C];       // b and c transposed, at transposed(d, j)
+  E ct[D * C];
+  E p[C][C + PAD];   // (a_i . b_j) lambda^{i-j} same(j, i)
 };
+
+// Where a transposed tile holds row d, column j.  The 16-byte units of a row are exchanged with d's low bits: a write has
+// lanes at every fourth row, a read at consecutive ones, and f takes all 8 values over either set, so both spread over
+// all banks (with padded rows the writes met in an eighth of them: 20 of 75 us of a [64,1024,8,64] call).
+template <class E>
+__device__ __forceinline__ int transposed(int d, int j) {
+  constexpr int UNIT = 16 / (int)sizeof(E);
+  const int f = (d & 7) ^ ((d >> 3) & 3);
+  return d * C + (((j / UNIT) ^ f) * UNIT) + j % UNIT;
+}
+template <class E>
+__device__ __forceinline__ Frag<E> load_transposed(const E* tile, int d, int j) {
+  if constexpr (sizeof(E) == 2) return Frag<E>::load(tile + transposed<E>(d, j));
+  else return Frag<E>::load2(tile + transposed<E>(d, j), tile + transposed<E>(d, j + 4));
+}
 
 // One array's part of a chunk, held by a thread: R rows of 4 columns.
 template <class E, int D>
 struct Part {
-  static constexpr int GROUPS = D / 4, R = C * GROUPS / kNT;
+  static constexpr int GROUPS = D / 4, R = C * GROUPS / (4 * D);
+  static_assert(R == 4, "a square of 4 x 4 elements per thread");
   Quad<E> x[R];
-};
+  const E* p;     // the first row's place
+  int64_t step;   // from a walk's step to the next, in elements
+  bool columns;   // this thread's columns exist
 
-template <class E, int D, bool VEC>
-__device__ __forceinline__ void fetch(Part<E, D>& part, const E* base, int64_t step_stride, int dim, int64_t first, int count,
-                                      int64_t T, bool reverse) {
-  constexpr int R = Part<E, D>::R;
-  const int col = (threadIdx.x % Part<E, D>::GROUPS) * 4, row0 = (threadIdx.x / Part<E, D>::GROUPS) * R;
+  __device__ __forceinline__ void start(const E* base, int64_t stride, int dim, int64_t first, int64_t T, bool reverse) {
+    const int col = (threadIdx.x % GROUPS) * 4, row0 = (threadIdx.x / GROUPS) * R;
+    columns = col < dim;
+    step = reverse ? -stride : stride;
+    p = base + (reverse ? T - 1 : 0) * stride + (first + row0) * step + (columns ? col : 0);
+  }
+  // Loads the next chunk's rows, of which `count` exist; rows beyond are loaded from the last one and cleared
+  // when the part is put down.  No branch on a lane's own position: the loads leave together.
+  template <bool VEC>
+  __device__ __forceinline__ Quad<E> quad(const E* q, int dim) const {
+    if constexpr (VEC) return Quad<E>::load(q);
+    const int left = dim - (threadIdx.x % GROUPS) * 4 - 1;  // the last column's offset, if these exist
+    return Quad<E>::bits(q[0], q[columns && left > 0 ? 1 : 0], q[columns && left > 1 ? 2 : 0], q[columns && left > 2 ? 3 : 0]);
+  }
+  template <bool VEC>
+  __device__ __forceinline__ void fetch(int dim) {
 #pragma unroll
-  for (int r = 0; r < R; ++r) {
-    const int i = row0 + r;
-    part.x[r] = Quad<E>::of(0.f, 0.f, 0.f, 0.f);
-    if (i < count && col < dim) {
-      const int64_t t = reverse ? T - 1 - (first + i) : first + i;
-      const E* p = base + t * step_stride + col;
-      if constexpr (VEC) {
-        part.x[r] = Quad<E>::load(p);
-      } else {
-        part.x[r] = Quad<E>::of(load_one(p), col + 1 < dim ? load_one(p + 1) : 0.f, col + 2 < dim ? load_one(p + 2) : 0.f,
-                                col + 3 < dim ? load_one(p + 3) : 0.f);
+    for (int r = 0; r < R; ++r) x[r] = quad<VEC>(p + r * step, dim);
+    p += C * step;
+  }
+  template <bool VEC>
+  __device__ __forceinline__ void fetch_some(int dim, int count) {
+    const int row0 = (threadIdx.x / GROUPS) * R;
+#pragma unroll
+    for (int r = 0; r < R; ++r) x[r] = quad<VEC>(p + ((row0 + r < count ? row0 + r : count - 1) - row0) * step, dim);
+  }
+  // Clears what lies beyond the chunk's rows or the array's columns.
+  template <bool VEC>
+  __device__ __forceinline__ void clip(int dim, int count) {
+    const int col = (threadIdx.x % GROUPS) * 4, row0 = (threadIdx.x / GROUPS) * R;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      if (!columns || row0 + r >= count) x[r].clear();
+      if constexpr (!VEC) {
+        const E zero = from_f32<E>(0.f);
+        const E* e = reinterpret_cast<const E*>(&x[r]);
+        x[r] = Quad<E>::bits(e[0], col + 1 < dim ? e[1] : zero, col + 2 < dim ? e[2] : zero, col + 3 < dim ? e[3] : zero);
       }
     }
   }
-}
-
-// Puts the R x 4 part down as 4 rows of R consecutive elements.
-template <class E, int D>
-__device__ __forceinline__ void put_transposed(const Part<E, D>& part, E (*dst)[C + Tiles<E, D>::PAD]) {
-  constexpr int R = Part<E, D>::R;
-  const int col = (threadIdx.x % Part<E, D>::GROUPS) * 4, row0 = (threadIdx.x / Part<E, D>::GROUPS) * R;
+  template <int STRIDE>
+  __device__ __forceinline__ void put(E (*dst)[STRIDE]) const {
+    const int col = (threadIdx.x % GROUPS) * 4, row0 = (threadIdx.x / GROUPS) * R;
 #pragma unroll
-  for (int x = 0; x < 4; ++x)
-#pragma unroll
-    for (int r = 0; r < R; r += 4)
-      Quad<E>::of(part.x[r].get(x), part.x[r + 1].get(x), part.x[r + 2].get(x), part.x[r + 3].get(x)).store(&dst[col + x][row0 + r]);
-}
+    for (int r = 0; r < R; ++r) x[r].store(&dst[row0 + r][col]);
+  }
+  // as 4 rows of 4 consecutive elements
+  __device__ __forceinline__ void put_transposed(E* tile) const {
+    const int col = (threadIdx.x % GROUPS) * 4, row0 = (threadIdx.x / GROUPS) * R;
+    Quad<E>::template across<0>(x[0], x[1], x[2], x[3]).store(tile + transposed<E>(col, row0));
+    Quad<E>::template across<1>(x[0], x[1], x[2], x[3]).store(tile + transposed<E>(col + 1, row0));
+    Quad<E>::template across<2>(x[0], x[1], x[2], x[3]).store(tile + transposed<E>(col + 2, row0));
+    Quad<E>::template across<3>(x[0], x[1], x[2], x[3]).store(tile + transposed<E>(col + 3, row0));
+  }
+};
 
 // acc += a (w * c) for an operand row c and weights w of its inner indices.  The weighted bfloat16 operand is
 // taken as the sum of two bfloat16 numbers (the product's upper 8 bits and the next 8): the state is a float32
@@ -167,8 +225,8 @@ struct Weighted<bf16> {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const float a = Words<bf16>::get(in.u[i], 0) * w[2 * i], b = Words<bf16>::get(in.u[i], 1) * w[2 * i + 1];
-      h.u[i] = pack_bf16x2(a, b);
-      l.u[i] = pack_bf16x2(a - Words<bf16>::get(h.u[i], 0), b - Words<bf16>::get(h.u[i], 1));
+      h.u[i] = bf16_pair(a, b);
+      l.u[i] = bf16_pair(a - Words<bf16>::get(h.u[i], 0), b - Words<bf16>::get(h.u[i], 1));
     }
     hi.x = h.v, lo.x = l.v;
   }
@@ -176,249 +234,277 @@ struct Weighted<bf16> {
 };
 
 // The walk over a segment.  STATE: only the state at its end, from zero, for the segments after it.
-template <class E, int D, bool VEC, bool STATE>
-__global__ __launch_bounds__(kNT) void walk_kernel(const Walks<E> walks) {
+//
+// Wavefront w owns the columns 16 w .. 16 w + 15 of c.  Everything a whole chunk without a cut needs of the
+// decay is in registers before the walk, and such chunks run through code without a question about them.
+// FORM 2: dims of exactly D; 1: dims are multiples of 4, tiles of the padded dims that hold nothing are skipped;
+// 0: any dims and alignment, element by element.
+template <class E, int D, int FORM, bool STATE>
+__global__ __launch_bounds__(4 * D, D == 64 && sizeof(E) == 4 ? 1 : 2) void walk_kernel(const Walks<E> walks) {
   __shared__ __align__(16) Tiles<E, D> tiles;
-  constexpr int MT = D / 16, NT = D / 64;  // tiles of 16: rows of the state; this wavefront's columns
+  constexpr int MT = D / 16, KK = D / 32;
+  constexpr int SHARE = D / 64, TILES = 4 / SHARE;  // wavefronts that share 16 rows of p; tiles of p a wavefront at most
   const Walk<E>& w = walks.w[blockIdx.z];
   const int head = blockIdx.x % walks.heads, seg = blockIdx.y;
   const int64_t env = blockIdx.x / walks.heads, T = walks.seq_len;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l16 = lane & 15, l4 = lane >> 4;
-  const int n0 = wave * (D / 4);  // this wavefront's columns
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l16 = lane & 15, l4 = lane >> 4;
+  constexpr bool VEC = FORM > 0, FULL = FORM == 2;
+  const int da = FULL ? D : w.da, dc = FULL ? D : w.dc;
   const int64_t first = (int64_t)seg * walks.seg_len, last = first + walks.seg_len < T ? first + walks.seg_len : T;
   const float lambda = walks.decay[head], lg = __log2f(lambda);
   const float* dones = walks.dones ? walks.dones + env * T : nullptr;
-  const E* ga = w.a.data + env * w.a.env_stride + head * w.a.head_stride;
-  const E* gb = w.b.data + env * w.b.env_stride + head * w.b.head_stride;
-  const E* gc = w.c.data + env * w.c.env_stride + head * w.c.head_stride;
   const bool reverse = w.reverse;
 
-  // U[da][dc]: lane holds column n0 + 16 n + l16, rows 16 m + 4 l4 + 0..3
-  f32x4 U[MT][NT];
-  const int64_t eh = env * walks.heads + head;
-  if (!STATE && seg > 0) {
-    const float* p = w.seg_states + (eh * walks.segs + seg) * (int64_t)(w.da * w.dc);
-#pragma unroll
-    for (int m = 0; m < MT; ++m)
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int i = 16 * m + 4 * l4 + r, j = n0 + 16 * n + l16;
-          U[m][n][r] = i < w.da && j < w.dc ? p[i * w.dc + j] : 0.f;
-        }
-  } else {
-    const float f = reverse ? w.state_scale : w.state_scale * lambda;
-    const float* p = STATE || w.state == nullptr ? nullptr : w.state + eh * (int64_t)(w.da * w.dc);
-#pragma unroll
-    for (int m = 0; m < MT; ++m)
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int i = 16 * m + 4 * l4 + r, j = n0 + 16 * n + l16;
-          U[m][n][r] = p != nullptr && i < w.da && j < w.dc ? p[w.transposed ? j * w.da + i : i * w.dc + j] * f : 0.f;
-        }
-  }
-
-  // lambda^{i-j}, j <= i, of this lane's elements of p (computed transposed: row j, column i): i = 16 wave + l16
-  f32x4 among[4];
-#pragma unroll
-  for (int jt = 0; jt < 4; ++jt)
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int d = 16 * wave + l16 - (16 * jt + 4 * l4 + r);
-      among[jt][r] = d < 0 ? 0.f : power(lg, d);
-    }
-  float back[4];  // lambda^i of the output rows i = 16 t + l16
-#pragma unroll
-  for (int t = 0; t < 4; ++t) back[t] = power(lg, 16 * t + l16);
-
   Part<E, D> pa, pb, pc;
-  uint64_t cuts, next_cuts = 0;
+  if constexpr (!STATE) pa.start(w.a.data + env * w.a.env_stride + head * w.a.head_stride, w.a.step_stride, da, first, T, reverse);
+  pb.start(w.b.data + env * w.b.env_stride + head * w.b.head_stride, w.b.step_stride, da, first, T, reverse);
+  pc.start(w.c.data + env * w.c.env_stride + head * w.c.head_stride, w.c.step_stride, dc, first, T, reverse);
+  float done = 0.f;  // of this lane's step of the next chunk: looked at when the chunk's other loads are (a ballot
+                     // when it is loaded would wait for all of them)
   auto fetch_all = [&](int64_t s0) {
-    const int count = (int)(last - s0 < C ? last - s0 : C);
-    if (!STATE) fetch<E, D, VEC>(pa, ga, w.a.step_stride, w.da, s0, count, T, reverse);
-    fetch<E, D, VEC>(pb, gb, w.b.step_stride, w.da, s0, count, T, reverse);
-    fetch<E, D, VEC>(pc, gc, w.c.step_stride, w.dc, s0, count, T, reverse);
-    bool cut = false;
-    if (dones != nullptr && lane < count) {
-      const int64_t s = s0 + lane;
-      if (reverse) cut = dones[T - 1 - s] != 0.f;
-      else cut = s > 0 && dones[s - 1] != 0.f;
+    if (last - s0 >= C) {
+      if constexpr (!STATE) pa.template fetch<VEC>(da);
+      pb.template fetch<VEC>(da);
+      pc.template fetch<VEC>(dc);
+    } else {
+      const int count = (int)(last - s0);
+      if constexpr (!STATE) pa.template fetch_some<VEC>(da, count);
+      pb.template fetch_some<VEC>(da, count);
+      pc.template fetch_some<VEC>(dc, count);
     }
-    next_cuts = __ballot(cut);
+    if (dones != nullptr) {
+      const int64_t s = s0 + lane < last ? s0 + lane : last - 1;
+      done = dones[reverse ? T - 1 - s : s > 0 ? s - 1 : 0];
+    }
   };
   fetch_all(first);
 
-  bool crossed = false;  // a cut anywhere in the segment
-  for (int64_t s0 = first; s0 < last; s0 += C) {
-    const int L = (int)(last - s0 < C ? last - s0 : C);
-    cuts = next_cuts;
-    crossed |= cuts != 0;
-    // the state that leaves the sequence forward is the one after the last step, not decayed by another
-    const bool end = !reverse && s0 + C >= T;
-    const int reach = end ? L - 1 : L;
-    __syncthreads();  // the chunk before has been read
-    {
-      constexpr int R = Part<E, D>::R;
-      const int col = (tid % Part<E, D>::GROUPS) * 4, row0 = (tid / Part<E, D>::GROUPS) * R;
-      if constexpr (!STATE) {
-#pragma unroll
-        for (int r = 0; r < R; ++r) pa.x[r].store(&tiles.a[row0 + r][col]), pb.x[r].store(&tiles.b[row0 + r][col]);
+  // U[da][dc]: lane holds column 16 wave + l16, rows 16 m + 4 l4 + 0..3
+  f32x4 U[MT];
+  const int64_t eh = env * walks.heads + head;
+  {
+    const float* p = nullptr;
+    float f = 1.f;
+    bool across = false;
+    if (!STATE) {
+      if (seg > 0) {
+        p = w.seg_states + (eh * walks.segs + seg) * (int64_t)(da * dc);
+      } else if (w.state != nullptr) {
+        p = w.state + eh * (int64_t)(da * dc);
+        f = reverse ? w.state_scale : w.state_scale * lambda;
+        across = w.transposed;
       }
-      put_transposed<E, D>(pc, tiles.ct);
-      put_transposed<E, D>(pb, tiles.bt);
     }
+    const int j = 16 * wave + l16, jc = j < dc ? j : 0;
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      U[m] = f32x4{0.f, 0.f, 0.f, 0.f};
+      if (p != nullptr && 16 * m < da)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int i = 16 * m + 4 * l4 + r, ic = i < da ? i : 0;
+          U[m][r] = p[across ? jc * da + ic : ic * dc + jc];
+        }
+    }
+    if (p != nullptr)
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) U[m][r] = 16 * m + 4 * l4 + r < da && j < dc ? U[m][r] * f : 0.f;
+  }
+
+  // This wavefront's part of p: rows i = 16 ti + l16, tiles of columns jt = wave % SHARE + SHARE u.  Computed
+  // transposed, so that a lane holds 4 consecutive j; scale lambda^{i-j} of its elements, 0 for j > i.
+  const int ti = wave / SHARE;
+  f32x4 among[STATE ? 1 : TILES];
+  float back[4];  // scale lambda^i of the output rows i = 16 t + l16
+  if constexpr (!STATE) {
+#pragma unroll
+    for (int u = 0; u < TILES; ++u)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int d = 16 * ti + l16 - (16 * (wave % SHARE + SHARE * u) + 4 * l4 + r);
+        among[u][r] = d < 0 ? 0.f : power(lg, d) * w.scale;
+      }
+#pragma unroll
+    for (int t = 0; t < 4; ++t) back[t] = power(lg, 16 * t + l16) * w.scale;
+    // the steps after a row's own tile, in the operand that ends with it: never written again
+    if ((ti & 1) == 0) Quad<E>::of(f32x4{0.f, 0.f, 0.f, 0.f}).store(&tiles.p[16 * ti + l16][16 * (ti + 1) + 4 * l4]);
+  }
+  float onward[2][8];  // lambda^{C-j} of the steps j = 32 kk + 8 l4 + x
+#pragma unroll
+  for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+    for (int x = 0; x < 8; ++x) onward[kk][x] = power(lg, C - (32 * kk + 8 * l4 + x));
+  const float whole = power(lg, C);
+
+  E* gy = nullptr;
+  int64_t ystep = 0;
+  if constexpr (!STATE) {
+    ystep = reverse ? -w.y.step_stride : w.y.step_stride;
+    gy = w.y.data + env * w.y.env_stride + head * w.y.head_stride + (reverse ? T - 1 : 0) * w.y.step_stride + (first + l16) * ystep +
+         16 * wave + 4 * l4;
+  }
+
+  bool crossed = false;  // a cut anywhere in the segment
+  // One chunk.  PLAIN: whole, without a cut, and not the one that a state leaves the sequence with.
+  auto chunk = [&](auto plain, int64_t s0, int L, uint64_t cuts, bool end) {
+    constexpr bool PLAIN = decltype(plain)::value;
+    // The lane's place again, for what only other chunks need: as a new value to the compiler, which would else compute
+    // all of it once before the walk and hold it in a hundred registers.
+    int v16 = l16, v4 = l4;
+    if constexpr (!PLAIN) asm volatile("" : "+v"(v16), "+v"(v4));
+    __syncthreads();  // the chunk before has been read
+    if (!PLAIN || !FULL) {
+      if constexpr (!STATE) pa.template clip<VEC>(da, L);
+      pb.template clip<VEC>(da, L);
+      pc.template clip<VEC>(dc, L);
+    }
+    if constexpr (!STATE) {
+      pa.put(tiles.a);
+      pb.put(tiles.b);
+    }
+    pb.put_transposed(tiles.bt);
+    pc.put_transposed(tiles.ct);
     __syncthreads();
     if (s0 + C < last) fetch_all(s0 + C);  // in flight while this chunk is worked on
 
     if constexpr (!STATE) {
-      // p^T: rows j, columns i = 16 wave + l16
-      f32x4 pt[4];
+      Frag<E> fa[KK];
 #pragma unroll
-      for (int jt = 0; jt < 4; ++jt) pt[jt] = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int kk = 0; kk < KK; ++kk)
+        if (FULL || 32 * kk < da) fa[kk] = Frag<E>::load(&tiles.a[16 * ti + l16][32 * kk + 8 * l4]);
 #pragma unroll
-      for (int kk = 0; kk < D / 32; ++kk) {
-        const Frag<E> fa = Frag<E>::load(&tiles.a[16 * wave + l16][32 * kk + 8 * l4]);
+      for (int u = 0; u < TILES; ++u) {
+        const int jt = wave % SHARE + SHARE * u;
+        if (jt > ti) continue;
+        f32x4 pt = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int jt = 0; jt < 4; ++jt)
-          if (jt <= wave) pt[jt] = mma(Frag<E>::load(&tiles.b[16 * jt + l16][32 * kk + 8 * l4]), fa, pt[jt]);
-      }
-      const int i = 16 * wave + l16;
-      // cuts before or at step i: two steps belong together when these numbers are the same
-      const int ep_i = __popcll(cuts & ((uint64_t)2 << i) - 1);
+        for (int kk = 0; kk < KK; ++kk)
+          if (FULL || 32 * kk < da) pt = mma(Frag<E>::load(&tiles.b[16 * jt + l16][32 * kk + 8 * l4]), fa[kk], pt);
+        pt *= among[u];
+        if (!PLAIN && cuts != 0) {
+          // two steps belong together when as many cuts lie before or at each of them
+          const int i = 16 * ti + v16, before = __popcll(cuts & (((uint64_t)2 << i) - 1));
 #pragma unroll
-      for (int jt = 0; jt < 4; ++jt) {
-        f32x4 x;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int j = 16 * jt + 4 * l4 + r;
-          const bool same = cuts == 0 || __popcll(cuts & ((uint64_t)2 << j) - 1) == ep_i;
-          x[r] = j <= i && same ? pt[jt][r] * among[jt][r] : 0.f;
+          for (int r = 0; r < 4; ++r)
+            if (__popcll(cuts & (((uint64_t)2 << (16 * jt + 4 * v4 + r)) - 1)) != before) pt[r] = 0.f;
         }
-        Quad<E>::of(x[0], x[1], x[2], x[3]).store(&tiles.p[i][16 * jt + 4 * l4]);
+        Quad<E>::of(pt).store(&tiles.p[16 * ti + l16][16 * jt + 4 * l4]);
       }
       __syncthreads();
+    }
 
+    Frag<E> fc[2];
+#pragma unroll
+    for (int kk = 0; kk < 2; ++kk) fc[kk] = load_transposed(tiles.ct, 16 * wave + l16, 32 * kk + 8 * l4);
+    const bool mine = FULL || 16 * wave < dc;  // else this wavefront only helps with p
+
+    if (!STATE && mine) {
       // y^T: rows = this wavefront's columns of c, columns i = 16 t + l16
-      f32x4 y[4][NT];
+      f32x4 y[4];
 #pragma unroll
-      for (int t = 0; t < 4; ++t)
+      for (int t = 0; t < 4; ++t) y[t] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int n = 0; n < NT; ++n) y[t][n] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int kk = 0; kk < D / 32; ++kk) {
-        Frag<E> fu[NT];
-#pragma unroll
-        for (int n = 0; n < NT; ++n) fu[n] = Frag<E>::from(U[2 * kk][n], U[2 * kk + 1][n]);
+      for (int kk = 0; kk < KK; ++kk) {
+        if (!FULL && 32 * kk >= da) continue;
+        const Frag<E> fu = Frag<E>::from(U[2 * kk], U[2 * kk + 1]);
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
           const E* row = &tiles.a[16 * t + l16][32 * kk + 4 * l4];
-          const Frag<E> fa = Frag<E>::load2(row, row + 16);
-#pragma unroll
-          for (int n = 0; n < NT; ++n) y[t][n] = mma(fu[n], fa, y[t][n]);
+          y[t] = mma(fu, Frag<E>::load2(row, row + 16), y[t]);
         }
       }
-      const int until = cuts == 0 ? C : __ffsll((long long)cuts) - 1;  // the first step that the state does not reach
+      // the first step that the state does not reach
+      const int until = PLAIN || cuts == 0 ? C : __ffsll((long long)cuts) - 1;
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
-        const float f = 16 * t + l16 < until ? back[t] : 0.f;
+        y[t] *= back[t];
+        if (!PLAIN && 16 * t + v16 >= until) y[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+      }
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+      for (int kk = 0; kk < 2; ++kk)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) y[t][n][r] = f == 0.f ? 0.f : y[t][n][r] * f;
+        for (int t = 2 * kk; t < 4; ++t)  // (rows before the steps 32 kk + 0..31 have none of them)
+          y[t] = mma(fc[kk], Frag<E>::load(&tiles.p[16 * t + l16][32 * kk + 8 * l4]), y[t]);
+      const int j = 16 * wave + 4 * l4;
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        E* p = gy + (16 * t) * ystep;
+        const Quad<E> v = Quad<E>::of(y[t]);
+        if (VEC) {
+          if ((PLAIN || 16 * t + v16 < L) && (FULL || j < dc)) v.store(p);
+        } else if (PLAIN || 16 * t + v16 < L) {
+          const E* e = reinterpret_cast<const E*>(&v);
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (j + r < dc) p[r] = e[r];
+        }
+      }
+      gy += C * ystep;
+    }
+
+    // U' = lambda^reach U + sum over steps from the last cut on of lambda^{reach-j} b_j c_j^T.  The state that
+    // leaves the sequence forward is the one after its last step, not decayed by another.
+    if (mine) {
+      const int reach = !PLAIN && end ? L - 1 : L, from = PLAIN || cuts == 0 ? 0 : 63 - __clzll((long long)cuts);
+      const float keep = PLAIN ? whole : power(lg, reach);
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+        U[m] *= keep;
+        if (!PLAIN && cuts != 0) U[m] = f32x4{0.f, 0.f, 0.f, 0.f};
       }
 #pragma unroll
       for (int kk = 0; kk < 2; ++kk) {
-        Frag<E> fc[NT];
+        float f[8];
 #pragma unroll
-        for (int n = 0; n < NT; ++n) fc[n] = Frag<E>::load(&tiles.ct[n0 + 16 * n + l16][32 * kk + 8 * l4]);
-#pragma unroll
-        for (int t = 2 * kk; t < 4; ++t) {  // (rows before the steps 32 kk + 0..31 have none of them)
-          const Frag<E> fp = Frag<E>::load(&tiles.p[16 * t + l16][32 * kk + 8 * l4]);
-#pragma unroll
-          for (int n = 0; n < NT; ++n) y[t][n] = mma(fc[n], fp, y[t][n]);
+        for (int x = 0; x < 8; ++x) {
+          const int j = 32 * kk + 8 * v4 + x;
+          f[x] = PLAIN ? onward[kk][x] : j >= from && j < L ? power(lg, reach - j) : 0.f;
         }
-      }
-      E* gy = w.y.data + env * w.y.env_stride + head * w.y.head_stride;
-#pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        const int row = 16 * t + l16;
-        if (row < L) {
-          const int64_t at = reverse ? T - 1 - (s0 + row) : s0 + row;
-#pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            const int j = n0 + 16 * n + 4 * l4;
-            E* p = gy + at * w.y.step_stride + j;
-            const f32x4 v = y[t][n] * w.scale;
-            if (VEC) {
-              if (j < w.dc) Quad<E>::of(v[0], v[1], v[2], v[3]).store(p);
-            } else {
-#pragma unroll
-              for (int r = 0; r < 4; ++r)
-                if (j + r < w.dc) p[r] = from_f32<E>(v[r]);
-            }
-          }
-        }
-      }
-    }
-
-    // U' = lambda^reach U + sum over steps from the last cut on of lambda^{reach-j} b_j c_j^T
-    const float keep = cuts == 0 ? power(lg, reach) : 0.f;
-    const int from = cuts == 0 ? 0 : 63 - __clzll((long long)cuts);
-#pragma unroll
-    for (int m = 0; m < MT; ++m)
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) U[m][n][r] = keep == 0.f ? 0.f : U[m][n][r] * keep;
-#pragma unroll
-    for (int kk = 0; kk < 2; ++kk) {
-      float f[8];
-#pragma unroll
-      for (int x = 0; x < 8; ++x) {
-        const int j = 32 * kk + 8 * l4 + x;
-        f[x] = j >= from && j < L ? power(lg, reach - j) : 0.f;
-      }
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        const Weighted<E> fc(Frag<E>::load(&tiles.ct[n0 + 16 * n + l16][32 * kk + 8 * l4]), f);
+        const Weighted<E> wc(fc[kk], f);
 #pragma unroll
         for (int m = 0; m < MT; ++m)
-          U[m][n] = fc.mma_with(Frag<E>::load(&tiles.bt[16 * m + l16][32 * kk + 8 * l4]), U[m][n]);
+          if (FULL || 16 * m < da) U[m] = wc.mma_with(load_transposed(tiles.bt, 16 * m + l16, 32 * kk + 8 * l4), U[m]);
       }
     }
+  };
+
+  for (int64_t s0 = first; s0 < last; s0 += C) {
+    const int L = (int)(last - s0 < C ? last - s0 : C);
+    const bool end = !reverse && s0 + C >= T;
+    const uint64_t cuts = __ballot(lane < L && done != 0.f && (reverse || s0 + lane > 0));
+    crossed |= cuts != 0;
+    if (L == C && cuts == 0 && !end) chunk(std::true_type{}, s0, L, cuts, end);
+    else chunk(std::false_type{}, s0, L, cuts, end);
   }
 
   float* out = nullptr;
   float f = 1.f;
   if (STATE) {
-    out = w.seg_states + (eh * walks.segs + seg + 1) * (int64_t)(w.da * w.dc);
-    if (tid == 0) w.seg_keep[eh * walks.segs + seg + 1] = crossed ? 0.f : power(lg, (int)(last - first));
+    out = w.seg_states + (eh * walks.segs + seg + 1) * (int64_t)(da * dc);
+    if (threadIdx.x == 0) w.seg_keep[eh * walks.segs + seg + 1] = crossed ? 0.f : power(lg, (int)(last - first));
   } else if (last == T && w.state_out != nullptr) {
-    out = w.state_out + eh * (int64_t)(w.da * w.dc);
+    out = w.state_out + eh * (int64_t)(da * dc);
     f = !reverse && dones != nullptr && dones[T - 1] != 0.f ? 0.f : w.state_out_scale;
   }
   if (out != nullptr)
 #pragma unroll
     for (int m = 0; m < MT; ++m)
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int i = 16 * m + 4 * l4 + r, j = n0 + 16 * n + l16;
-          if (i < w.da && j < w.dc) out[i * w.dc + j] = f == 0.f ? 0.f : U[m][n][r] * f;
-        }
+      for (int r = 0; r < 4; ++r) {
+        const int i = 16 * m + 4 * l4 + r, j = 16 * wave + l16;
+        if (i < da && j < dc) out[i * dc + j] = f == 0.f ? 0.f : U[m][r] * f;
+      }
 }
 
 // The states that enter the segments: in place, from what each segment added and how much of what enters it leaves.
 template <class E>
-__global__ __launch_bounds__(kNT) void join_kernel(const Walks<E> walks) {
+__global__ __launch_bounds__(256) void join_kernel(const Walks<E> walks) {
   const Walk<E>& w = walks.w[blockIdx.z];
   const int n = w.da * w.dc;
   const int64_t eh = blockIdx.x;
-  const int i = blockIdx.y * kNT + threadIdx.x;
+  const int i = blockIdx.y * 256 + threadIdx.x;
   if (i >= n) return;
   float u = 0.f;
   if (w.state != nullptr) {
@@ -433,20 +519,20 @@ __global__ __launch_bounds__(kNT) void join_kernel(const Walks<E> walks) {
   }
 }
 
-template <class E, int D, bool VEC>
+template <class E, int D, int FORM>
 int launch_walks(const Walks<E>& k, int count, hipStream_t s) {
   const dim3 grid((unsigned)(k.num_envs * k.heads), (unsigned)k.segs, (unsigned)count);
   if (k.segs > 1) {
     dim3 g = grid;
     g.y = (unsigned)k.segs - 1;
-    walk_kernel<E, D, VEC, true><<<g, dim3(kNT), 0, s>>>(k);
+    walk_kernel<E, D, FORM, true><<<g, dim3(4 * D), 0, s>>>(k);
     if (hipGetLastError() != hipSuccess) return RLK_ERR_LAUNCH;
     int most = 0;
     for (int i = 0; i < count; ++i) most = most < k.w[i].da * k.w[i].dc ? k.w[i].da * k.w[i].dc : most;
-    join_kernel<E><<<dim3(grid.x, (unsigned)(most + kNT - 1) / kNT, (unsigned)count), dim3(kNT), 0, s>>>(k);
+    join_kernel<E><<<dim3(grid.x, (unsigned)(most + 255) / 256, (unsigned)count), dim3(256), 0, s>>>(k);
     if (hipGetLastError() != hipSuccess) return RLK_ERR_LAUNCH;
   }
-  walk_kernel<E, D, VEC, false><<<grid, dim3(kNT), 0, s>>>(k);
+  walk_kernel<E, D, FORM, false><<<grid, dim3(4 * D), 0, s>>>(k);
   return hipGetLastError() == hipSuccess ? RLK_OK : RLK_ERR_LAUNCH;
 }
 
@@ -463,6 +549,7 @@ int walk_impl(const rlk_attention* c, int count, hipStream_t s) {
   const SegmentPlan plan = plan_segments(c->num_envs * c->heads, c->seq_len);
   k.segs = plan.segs, k.seg_len = plan.seg_len;
   bool vec = true, small = true;
+  int full = 0;  // the one size that all dims have, or -1
   char* ws = static_cast<char*>(c->workspace);
   size_t left = c->workspace_bytes;
   for (int i = 0; i < count; ++i) {
@@ -474,6 +561,7 @@ int walk_impl(const rlk_attention* c, int count, hipStream_t s) {
     w.scale = q.scale, w.state_scale = q.state_scale, w.state_out_scale = q.state_out_scale, w.reverse = q.reverse;
     vec = vec && quads(w.a, w.da) && quads(w.b, w.da) && quads(w.c, w.dc) && quads(w.y, w.dc);
     small = small && w.da <= 64 && w.dc <= 64;
+    full = w.da == w.dc && (full == 0 || full == w.da) ? w.da : -1;
     if (k.segs > 1) {
       const size_t states = (size_t)k.num_envs * k.heads * k.segs * w.da * w.dc, keeps = (size_t)k.num_envs * k.heads * k.segs;
       if ((states + keeps) * sizeof(float) > left || ws == nullptr || (reinterpret_cast<uintptr_t>(ws) & 3u) != 0)
@@ -482,8 +570,12 @@ int walk_impl(const rlk_attention* c, int count, hipStream_t s) {
       ws += (states + keeps) * sizeof(float), left -= (states + keeps) * sizeof(float);
     }
   }
-  if (small) return vec ? launch_walks<E, 64, true>(k, count, s) : launch_walks<E, 64, false>(k, count, s);
-  return vec ? launch_walks<E, 128, true>(k, count, s) : launch_walks<E, 128, false>(k, count, s);
+  if (small) {
+    if (vec && full == 64) return launch_walks<E, 64, 2>(k, count, s);
+    return vec ? launch_walks<E, 64, 1>(k, count, s) : launch_walks<E, 64, 0>(k, count, s);
+  }
+  if (vec && full == 128) return launch_walks<E, 128, 2>(k, count, s);
+  return vec ? launch_walks<E, 128, 1>(k, count, s) : launch_walks<E, 128, 0>(k, count, s);
 }
 
 }  // namespace
