@@ -53,7 +53,8 @@ typedef struct rlk_policy_terms {
   float *means; /* [4]: policy term, KL term (without its coefficient), share of steps whose gradient the
                    clipping removed, KL estimate to the old policy; from logits a fifth: the entropy */
   void *workspace;
-  size_t workspace_bytes; /* at least rlk_policy_workspace_bytes(num_envs), no initial contents needed */
+  size_t workspace_bytes; /* at least rlk_policy_workspace_bytes(num_envs); zero-filled before its first use
+                             and left ready for the next call on its stream */
 } rlk_policy_terms;
 
 size_t rlk_policy_workspace_bytes(int64_t num_envs);

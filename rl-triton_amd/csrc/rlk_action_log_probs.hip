@@ -12,7 +12,7 @@ __global__ __launch_bounds__(rows_threads<LANES>()) void log_probs_kernel(const 
   constexpr int NT = rows_threads<LANES>(), PER = NT / LANES;
   __shared__ float lds[LANES > 64 ? 3 * (LANES / 64) + 2 : 1];
   const int lane = threadIdx.x % LANES;
-  for (int64_t row = (int64_t)blockIdx.x * PER + threadIdx.x / LANES; row < a.rows; row += (int64_t)gridDim.x * PER) {
+  for (int64_t row = first_row<LANES>(); row < a.rows; row += (int64_t)gridDim.x * PER) {
     const Frame<E> f(row_base(a, row), a.A);
     RowStats r;
     if constexpr (NV > 0) {
@@ -35,29 +35,65 @@ __global__ __launch_bounds__(rows_threads<LANES>()) void log_probs_kernel(const 
   }
 }
 
+template <class E, int K>
+__global__ __launch_bounds__(kFewRows) void few_log_probs_kernel(const ActionRows<E> a, const FewRows f, float* __restrict__ log_probs,
+                                                                 float* __restrict__ entropies, float* __restrict__ norms) {
+  extern __shared__ float lds[];
+  for (int64_t row0 = (int64_t)blockIdx.x * kFewRows; row0 < a.rows; row0 += (int64_t)gridDim.x * kFewRows) {
+    const int rows = (int)(a.rows - row0 < kFewRows ? a.rows - row0 : kFewRows);
+    const int64_t row = row0 + threadIdx.x;
+    const int64_t act = (int)threadIdx.x < rows ? a.actions[row] : 0;
+    f.take(a.logits + row0 * a.A, rows * a.A, lds);
+    __syncthreads();
+    if ((int)threadIdx.x < rows) {
+      const float* mine = lds + threadIdx.x * f.pitch;
+      FewLogits<K> h;
+      h.load(mine, a.A);
+      const RowStats r = h.stats(a.c);
+      const float x = act >= 0 && act < a.A ? mine[act] : NAN;
+      const float log2s = r.log2s();
+      const bool empty = r.s == 0.f;
+      log_probs[row] = empty && x == x ? -INFINITY : ((x - r.m) * a.c - log2s) * kLn2;
+      entropies[row] = empty ? 0.f : (log2s - r.u / r.s) * kLn2;
+      if (norms) norms[2 * row] = r.m, norms[2 * row + 1] = empty ? INFINITY : log2s;
+    }
+    __syncthreads();
+  }
+}
+
 template <class E, int LANES>
 __global__ __launch_bounds__(256) void backward_kernel(const ActionRows<E> a, const float* __restrict__ entropies,
                                                        const float* __restrict__ norms, const float* __restrict__ gl,
                                                        const float* __restrict__ ge, E* __restrict__ out) {
   constexpr int PER = 256 / LANES;
   const int lane = threadIdx.x % LANES;
-  for (int64_t row = (int64_t)blockIdx.x * PER + threadIdx.x / LANES; row < a.rows; row += (int64_t)gridDim.x * PER) {
+  for (int64_t row = first_row<LANES>(); row < a.rows; row += (int64_t)gridDim.x * PER) {
     const Frame<E> f(row_base(a, row), a.A);
     const float log2s = norms[2 * row + 1];
-    const RowGrad g(gl ? gl[row] : 0.f, ge ? ge[row] : 0.f, entropies[row], norms[2 * row], log2s, a.inv_tau, a.actions[row],
+    const RowGrad g(gl ? gl[row] : 0.f, ge ? ge[row] : 0.f, entropies[row], norms[2 * row], a.c, log2s, a.inv_tau, a.actions[row],
                     log2s == INFINITY);
-    write_grad<E, LANES, 0>(f, nullptr, out + row * a.A, g, a.c, lane);
+    write_grad<E, LANES, 0>(f, nullptr, out + row * a.A, g, lane);
   }
 }
 
 template <class E>
 int forward(const rlk_action_rows* rows, float* lp, float* ent, float* norms, hipStream_t s) {
   const ActionRows<E> a = action_rows<E>(rows);
+  FewRows few;
+  if (few_rows(a, nullptr, &few)) {
+    int64_t blocks = (a.rows + kFewRows - 1) / kFewRows;
+    if (blocks > 2048) blocks = 2048;
+    return dispatch_few(a.A, [&](auto k) {
+      few_log_probs_kernel<E, decltype(k)::value><<<dim3((unsigned)blocks), dim3(kFewRows), few.pitch * kFewRows * sizeof(float), s>>>(
+          a, few, lp, ent, norms);
+      return hipGetLastError() == hipSuccess ? RLK_OK : RLK_ERR_LAUNCH;
+    });
+  }
   constexpr int VEC = Frame<E>::VEC;
-  return dispatch_row((a.A + VEC - 1) / VEC, [&](auto lanes, auto nv) {
+  return dispatch_read((a.A + VEC - 1) / VEC, a.rows, [&](auto lanes, auto nv, int64_t most) {
     constexpr int L = decltype(lanes)::value, NV = decltype(nv)::value, NT = rows_threads<L>();
     int64_t blocks = (a.rows + NT / L - 1) / (NT / L);
-    if (blocks > kMaxLossBlocks) blocks = kMaxLossBlocks;
+    if (blocks > most) blocks = most;
     log_probs_kernel<E, L, NV><<<dim3((unsigned)blocks), dim3(NT), 0, s>>>(a, lp, ent, norms);
     return hipGetLastError() == hipSuccess ? RLK_OK : RLK_ERR_LAUNCH;
   });

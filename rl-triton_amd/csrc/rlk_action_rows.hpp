@@ -5,8 +5,9 @@
 //   s = sum 2^y,  u = sum 2^y y,  log p_j = ln2 (y_j - log2 s),  H = ln2 (log2 s - u / s)
 // and for upstream gradients g of log p_a and h of H
 //   dx_j = (g ([j = a] - p_j) - h p_j (log p_j + H)) / tau.
-// x - m is formed before the product: a row whose logits are all the type's lowest value is then uniform
-// and not NaN.  Logits of -inf have no part (p = 0, nothing in u); a row of them alone has log p = -inf,
+// x - m is formed before the product: the largest logit's y is then 0 (one fma, x c - (m c rounded), leaves a residue
+// there, and log-probabilities above 0), and a row whose logits are all the type's lowest value is uniform and
+// not NaN.  Logits of -inf have no part (p = 0, nothing in u); a row of them alone has log p = -inf,
 // H = 0 and a zero gradient.  NaN and +inf make the row's outputs NaN through s.
 #pragma once
 #include "rlk_policy.hpp"
@@ -49,6 +50,23 @@ __device__ __forceinline__ u32x4 load_words(const void* p) {
 }
 __device__ __forceinline__ void store_words(void* p, u32x4 w) {
   __builtin_nontemporal_store(w, static_cast<u32x4*>(p));
+}
+
+// The k-th vector of a lane of LANES from `first`, a row's first whole vector: the same address for the wavefront plus a
+// 32-bit offset for the lane (as one offset, formed in 64 bits for every k, they filled 32 registers of a held row).
+template <int LANES, class T>
+__device__ __forceinline__ T* vector_at(T* first, int k, int lane) {
+  typedef std::conditional_t<std::is_const_v<T>, const char, char> Byte;
+  return reinterpret_cast<T*>(reinterpret_cast<Byte*>(first) + (int64_t)k * (LANES * 16) + (uint32_t)(lane * 16));
+}
+
+// The row that a group of LANES threads works on: one for a whole wavefront, and known to be.
+template <int LANES>
+__device__ __forceinline__ int64_t first_row() {
+  constexpr int PER = LANES > 256 ? 1 : 256 / LANES;
+  int group = threadIdx.x / LANES;
+  if constexpr (LANES >= 64) group = __builtin_amdgcn_readfirstlane(group);
+  return (int64_t)blockIdx.x * PER + group;
 }
 
 template <class E>
@@ -98,15 +116,14 @@ __device__ __forceinline__ void group_sum2(float& a, float& b, float* s) {
 
 constexpr float kDeep = -1024.f;  // 2^kDeep is 0: below it y only has to be finite where it multiplies 2^y
 
-__device__ __forceinline__ void softmax_add(float x, float m, float c, float& s, float& u) {
-  const float y = (x - m) * c;
+__device__ __forceinline__ void softmax_add(float y, float& s, float& u) {
   const float e = __builtin_amdgcn_exp2f(y);
   s += e;
   u = fmaf(e, fmaxf(y, kDeep), u);  // (y = -inf: e = 0 counts as 0)
 }
 
 struct RowStats {
-  float m, s, u;       // of a row without any finite logit: m = 0, s = u = 0
+  float m, s, u;  // of a row without any finite logit: m = 0, s = u = 0
   __device__ float log2s() const { return s == 0.f ? 0.f : __log2f(s); }
 };
 
@@ -114,18 +131,26 @@ constexpr float kLn2 = 0.69314718055994531f;
 
 // What the writer of a gradient needs: p = 2^(y - log2 s), dx = p (a1 + b1 (y - log2 s)), plus g at the action.
 struct RowGrad {
-  float m, log2s, a1, b1, at;
+  float m, c, log2s, a1, b1, at;
   int action;
   bool zero;
-  __device__ RowGrad(float g, float h, float entropy, float m_, float log2s_, float inv_tau, int64_t a, bool empty)
-      : m(m_), log2s(log2s_), a1((-g - h * entropy) * inv_tau), b1(-h * kLn2 * inv_tau), at(g * inv_tau),
+  __device__ RowGrad(float g, float h, float entropy, float m_, float c_, float log2s_, float inv_tau, int64_t a, bool empty)
+      : m(m_), c(c_), log2s(log2s_), a1((-g - h * entropy) * inv_tau), b1(-h * kLn2 * inv_tau), at(g * inv_tau),
         action(a >= 0 && a < (int64_t{1} << 30) ? (int)a : -1), zero(empty) {}
-  __device__ float operator()(float x, float c, int j) const {
+  // but for what the taken action adds, `at`
+  __device__ __forceinline__ float operator()(float x) const {
     const float y = fmaf(x - m, c, -log2s);
-    float d = __builtin_amdgcn_exp2f(y) * fmaf(b1, fmaxf(y, kDeep), a1);
-    return j == action ? d + at : d;
+    return __builtin_amdgcn_exp2f(y) * fmaf(b1, fmaxf(y, kDeep), a1);
   }
+  __device__ __forceinline__ float operator()(float x, int j) const { return (*this)(x) + (j == action ? at : 0.f); }
 };
+
+// Keeps the work on one held vector from being mixed with the next one's: where most registers hold the row the
+// mixture's do not fit any more.
+template <int NV>
+__device__ __forceinline__ void apart() {
+  if constexpr (NV >= 8) __builtin_amdgcn_sched_barrier(0);
+}
 
 template <class E, int LANES, int NV>
 struct RowHolder {
@@ -137,8 +162,7 @@ struct RowHolder {
   __device__ __forceinline__ void load(const Frame<E>& f, int lane) {
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-      const int i = lane + LANES * k;
-      if (i < f.nfull) v[k] = load_words(f.base + f.head + i * VEC);
+      if (lane + LANES * k < f.nfull) v[k] = load_words(vector_at<LANES>(f.base + f.head, k, lane));
     }
 #pragma unroll
     for (int k = 0; k < EDGES; ++k) {
@@ -161,14 +185,15 @@ struct RowHolder {
     RowStats r{group_max<LANES>(m, lds), 0.f, 0.f};
     if (r.m == -INFINITY) r.m = 0.f;
 #pragma unroll
-    for (int k = 0; k < EDGES; ++k) softmax_add(edge[k], r.m, c, r.s, r.u);
+    for (int k = 0; k < EDGES; ++k) softmax_add((edge[k] - r.m) * c, r.s, r.u);
 #pragma unroll
     for (int k = 0; k < NV; ++k)
       if (lane + LANES * k < f.nfull) {
         float x[VEC];
         unpack<E>(v[k], x);
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) softmax_add(x[i], r.m, c, r.s, r.u);
+        for (int i = 0; i < VEC; ++i) softmax_add((x[i] - r.m) * c, r.s, r.u);
+        apart<NV>();
       }
     group_sum2<LANES>(r.s, r.u, lds + LANES / 64 + 1);
     return r;
@@ -178,41 +203,49 @@ struct RowHolder {
 // Writes the gradient of a row, `held` (NV > 0) or read again.
 template <class E, int LANES, int NV>
 __device__ __forceinline__ void write_grad(const Frame<E>& f, const RowHolder<E, LANES, NV>* held, E* out, const RowGrad& g,
-                                           float c, int lane) {
+                                           int lane) {
   constexpr int VEC = Frame<E>::VEC;
   // the output has the input's place in its 16 bytes unless the logits' rows are strided
   const bool same = ((reinterpret_cast<uintptr_t>(out) ^ reinterpret_cast<uintptr_t>(f.base)) & 15u) == 0;
-  auto vec = [&](u32x4 w, int i) {
-    const int j0 = f.head + i * VEC;
+  auto vec = [&](u32x4 w, int r) {
+    E* to = vector_at<LANES>(out + f.head, r, lane);
+    const int j0 = f.head + (lane + LANES * r) * VEC;
     float x[VEC];
     unpack<E>(w, x);
 #pragma unroll
-    for (int k = 0; k < VEC; ++k) x[k] = g.zero ? 0.f : g(x[k], c, j0 + k);
+    for (int k = 0; k < VEC; ++k) x[k] = g.zero ? 0.f : g(x[k]);
+    if ((uint32_t)(g.action - j0) < (uint32_t)VEC && !g.zero) {
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) x[k] += j0 + k == g.action ? g.at : 0.f;
+    }
     if (same) {
-      store_words(out + j0, pack<E>(x));
+      store_words(to, pack<E>(x));
     } else {
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) out[j0 + k] = from_f32<E>(x[k]);
+      for (int k = 0; k < VEC; ++k) to[k] = from_f32<E>(x[k]);
     }
   };
   if constexpr (NV > 0) {
 #pragma unroll
     for (int k = 0; k < NV; ++k)
-      if (lane + LANES * k < f.nfull) vec(held->v[k], lane + LANES * k);
+      if (lane + LANES * k < f.nfull) {
+        vec(held->v[k], k);
+        apart<NV>();
+      }
   } else {
 #pragma unroll 4
-    for (int i = lane; i < f.nfull; i += LANES) vec(load_words(f.base + f.head + i * VEC), i);
+    for (int k = 0; lane + LANES * k < f.nfull; ++k) vec(load_words(vector_at<LANES>(f.base + f.head, k, lane)), k);
   }
   for (int i = lane; i < 2 * VEC; i += LANES) {
     const int j = f.edge(i);
-    if (j >= 0) out[j] = from_f32<E>(g.zero ? 0.f : g(load_one(f.base + j), c, j));
+    if (j >= 0) out[j] = from_f32<E>(g.zero ? 0.f : g(load_one(f.base + j), j));
   }
 }
 
 template <class E, int LANES>
 __device__ __forceinline__ void write_zeros(E* out, int A, int lane) {
   const Frame<E> f(out, A);
-  for (int i = lane; i < f.nfull; i += LANES) store_words(out + f.head + i * Frame<E>::VEC, u32x4{0, 0, 0, 0});
+  for (int k = 0; lane + LANES * k < f.nfull; ++k) store_words(vector_at<LANES>(out + f.head, k, lane), u32x4{0, 0, 0, 0});
   for (int i = lane; i < 2 * Frame<E>::VEC; i += LANES) {
     const int j = f.edge(i);
     if (j >= 0) out[j] = from_f32<E>(0.f);
@@ -238,13 +271,13 @@ __device__ __forceinline__ RowStats streamed_stats(const Frame<E>& f, int lane, 
     const float x = j >= 0 ? load_one(f.base + j) : -INFINITY;
     if (x != -INFINITY) {
       rebase(fmaxf(m, x));
-      softmax_add(x, m, c, s, u);
+      softmax_add((x - m) * c, s, u);
     }
   }
 #pragma unroll 4
-  for (int i = lane; i < f.nfull; i += LANES) {
+  for (int r = 0; lane + LANES * r < f.nfull; ++r) {
     float x[VEC];
-    unpack<E>(load_words(f.base + f.head + i * VEC), x);
+    unpack<E>(load_words(vector_at<LANES>(f.base + f.head, r, lane)), x);
     float t = x[0];
     bool nan = x[0] != x[0];
 #pragma unroll
@@ -254,7 +287,7 @@ __device__ __forceinline__ RowStats streamed_stats(const Frame<E>& f, int lane, 
     } else if (t != -INFINITY) {
       rebase(fmaxf(m, t));
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) softmax_add(x[k], m, c, s, u);
+      for (int k = 0; k < VEC; ++k) softmax_add((x[k] - m) * c, s, u);
     }
   }
   float top = group_max<LANES>(m, lds);
@@ -264,22 +297,146 @@ __device__ __forceinline__ RowStats streamed_stats(const Frame<E>& f, int lane, 
   return RowStats{top, s, u};
 }
 
+// ---------------------------------------------------------------------------------------
+// Few actions, rows one after the other in memory: a thread per row.  A workgroup takes 256 rows in 16-byte
+// accesses through LDS, where a row starts at an odd word (A | 1 apart), so that lanes that read the same column
+// of their rows meet in different banks.  No lane is idle past the row's end, nothing is reduced over lanes, and what a
+// step computes beside its logits it computes once.
+// ---------------------------------------------------------------------------------------
+constexpr int kFewActions = 32, kFewRows = 256;
+
+struct FewRows {
+  int A, pitch;
+  uint32_t magic;  // ceil(2^32 / A): i / A = umulhi(i, magic) for i < 2^13 (A > 1)
+  bool quads;      // the arrays are aligned to 4 elements
+  __device__ int row(int i) const { return A == 1 ? i : (int)__umulhi((uint32_t)i, magic); }
+
+  // LDS <- `count` elements at `src`
+  template <class E>
+  __device__ void take(const E* src, int count, float* lds) const {
+    const int whole = quads ? count / 4 : 0;
+    for (int q = threadIdx.x; q < whole; q += kFewRows) {
+      const float4 v = load_quad<true>(src + 4 * q);
+      const float* x = &v.x;
+      int r = row(4 * q), j = 4 * q - r * A;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        lds[r * pitch + j] = x[k];
+        if (++j == A) j = 0, ++r;
+      }
+    }
+    for (int i = 4 * whole + threadIdx.x; i < count; i += kFewRows) {
+      const int r = row(i);
+      lds[r * pitch + i - r * A] = load_one(src + i);
+    }
+  }
+  template <class E>
+  __device__ void put(E* dst, int count, const float* lds) const {
+    const int whole = quads ? count / 4 : 0;
+    for (int q = threadIdx.x; q < whole; q += kFewRows) {
+      float4 v;
+      float* x = &v.x;
+      int r = row(4 * q), j = 4 * q - r * A;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        x[k] = lds[r * pitch + j];
+        if (++j == A) j = 0, ++r;
+      }
+      store_quad<true>(dst + 4 * q, v);
+    }
+    for (int i = 4 * whole + threadIdx.x; i < count; i += kFewRows) {
+      const int r = row(i);
+      dst[i] = from_f32<E>(lds[r * pitch + i - r * A]);
+    }
+  }
+};
+
+// A thread's row: K >= A logits, -inf beyond A.
+template <int K>
+struct FewLogits {
+  float x[K];
+  __device__ __forceinline__ void load(const float* row, int A) {
+#pragma unroll
+    for (int j = 0; j < K; ++j) x[j] = j < K - 3 || j < A ? row[j] : -INFINITY;
+  }
+  __device__ __forceinline__ RowStats stats(float c) const {
+    float m = x[0];
+#pragma unroll
+    for (int j = 1; j < K; ++j) m = fmaxf(m, x[j]);
+    RowStats r{m == -INFINITY ? 0.f : m, 0.f, 0.f};
+#pragma unroll
+    for (int j = 0; j < K; ++j) softmax_add((x[j] - r.m) * c, r.s, r.u);
+    return r;
+  }
+};
+
+// Calls f(integral constant K) with the multiple of 4 that holds A.
+template <class F>
+int dispatch_few(int A, F f) {
+  switch ((A + 3) / 4) {
+    case 1: return f(std::integral_constant<int, 4>{});
+    case 2: return f(std::integral_constant<int, 8>{});
+    case 3: return f(std::integral_constant<int, 12>{});
+    case 4: return f(std::integral_constant<int, 16>{});
+    case 5: return f(std::integral_constant<int, 20>{});
+    case 6: return f(std::integral_constant<int, 24>{});
+    case 7: return f(std::integral_constant<int, 28>{});
+    default: return f(std::integral_constant<int, 32>{});
+  }
+}
+
+template <class E>
+bool few_rows(const ActionRows<E>& a, const void* out, FewRows* f) {
+  if (a.A > kFewActions || a.step_stride != a.A || a.env_stride != a.seq_len * a.step_stride) return false;
+  const uintptr_t low = (reinterpret_cast<uintptr_t>(a.logits) | reinterpret_cast<uintptr_t>(out)) & (4 * sizeof(E) - 1);
+  *f = {a.A, a.A | 1, (uint32_t)(((uint64_t{1} << 32) + (uint32_t)a.A - 1) / (uint32_t)a.A), low == 0};
+  return true;
+}
+
 template <int LANES>
 constexpr int rows_threads() { return LANES > 256 ? LANES : 256; }
 
-// Calls f(integral constants LANES, NV) for rows of `vecs` 16-byte vectors: the fewest lanes that hold one
-// in at most 4 vectors each (8 and 16 for the longest rows, NV = 0 beyond: those are read twice).
+// Calls f(integral constants LANES, NV, most workgroups) for `rows` rows of `vecs` 16-byte vectors.
+//
+// Rows of up to 256 vectors are held by as few lanes as hold them in four vectors each (two in the shortest): whole
+// wavefronts' lanes are busy and what is computed once a row is repeated in few lanes (float32, 84 MB read: 40 actions 25.7 us with 8 lanes,
+// 37.6 with 16; 128: 13.8 with 8, 17.2 with 16; 511: 14.3 with 32, 17.8 with 64).  Longer ones:
+//  - only read (log-probabilities): streamed (NV = 0), a workgroup per row, many small workgroups so that one loads while
+//    another reduces; wider ones where there are too few rows for that.  16384 rows of 32768 bfloat16: 256 lanes 183 us,
+//    512 199, 1024 233, held by 1024 lanes 284; a round of 256 rows of 65536: 9.3 us with 1024 lanes, 13 with 512, 22 with 256.
+//  - read and written (losses): held, in the fewest lanes whose registers leave room for a second workgroup per CU
+//    (4096 vectors: 512 lanes 313 us, 256 lanes 351, 1024 lanes 380; 1000 vectors: 256 lanes 355, 512 420, 1024 727); rows of
+//    more than 256 KB are read twice.
 template <class F>
-int dispatch_row(int64_t vecs, F f) {
+int dispatch_short(int64_t vecs, F f) {
   using std::integral_constant;
-  if (vecs <= 8) return f(integral_constant<int, 4>{}, integral_constant<int, 2>{});
-  if (vecs <= 64) return f(integral_constant<int, 16>{}, integral_constant<int, 4>{});
-  if (vecs <= 256) return f(integral_constant<int, 64>{}, integral_constant<int, 4>{});
-  if (vecs <= 1024) return f(integral_constant<int, 256>{}, integral_constant<int, 4>{});
-  if (vecs <= 2048) return f(integral_constant<int, 256>{}, integral_constant<int, 8>{});
-  if (vecs <= 8192) return f(integral_constant<int, 1024>{}, integral_constant<int, 8>{});
-  if (vecs <= 16384) return f(integral_constant<int, 1024>{}, integral_constant<int, 16>{});
-  return f(integral_constant<int, 1024>{}, integral_constant<int, 0>{});
+  if (vecs <= 8) return f(integral_constant<int, 4>{}, integral_constant<int, 2>{}, 2048);
+  if (vecs <= 16) return f(integral_constant<int, 8>{}, integral_constant<int, 2>{}, 2048);
+  if (vecs <= 32) return f(integral_constant<int, 8>{}, integral_constant<int, 4>{}, 2048);
+  if (vecs <= 64) return f(integral_constant<int, 16>{}, integral_constant<int, 4>{}, 2048);
+  if (vecs <= 128) return f(integral_constant<int, 32>{}, integral_constant<int, 4>{}, 2048);
+  if (vecs <= 256) return f(integral_constant<int, 64>{}, integral_constant<int, 4>{}, 2048);
+  return f(integral_constant<int, 256>{}, integral_constant<int, 2>{}, 2048);
+}
+template <class F>
+int dispatch_read(int64_t vecs, int64_t rows, F f) {
+  using std::integral_constant;
+  if (vecs <= 512) return dispatch_short(vecs, f);
+  const int64_t many = int64_t{1} << 22;
+  if (rows < 512) return f(integral_constant<int, 1024>{}, integral_constant<int, 0>{}, many);
+  if (rows < 1024) return f(integral_constant<int, 512>{}, integral_constant<int, 0>{}, many);
+  return f(integral_constant<int, 256>{}, integral_constant<int, 0>{}, many);
+}
+template <class F>
+int dispatch_update(int64_t vecs, F f) {
+  using std::integral_constant;
+  if (vecs <= 512) return dispatch_short(vecs, f);
+  if (vecs <= 1024) return f(integral_constant<int, 256>{}, integral_constant<int, 4>{}, 2048);
+  if (vecs <= 2048) return f(integral_constant<int, 256>{}, integral_constant<int, 8>{}, 2048);
+  if (vecs <= 4096) return f(integral_constant<int, 512>{}, integral_constant<int, 8>{}, 2048);
+  if (vecs <= 8192) return f(integral_constant<int, 1024>{}, integral_constant<int, 8>{}, 1024);
+  if (vecs <= 16384) return f(integral_constant<int, 1024>{}, integral_constant<int, 16>{}, 1024);
+  return f(integral_constant<int, 512>{}, integral_constant<int, 0>{}, 2048);
 }
 
 inline bool valid_rows(const rlk_action_rows* r) {

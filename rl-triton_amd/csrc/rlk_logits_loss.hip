@@ -12,15 +12,14 @@ struct StepArrays {
 template <class E, int LANES, int NV>
 __global__ __launch_bounds__(rows_threads<LANES>()) void logits_loss_kernel(const ActionRows<E> a, const StepArrays t,
                                                                              const LossConsts c, const Weights w,
-                                                                             double* __restrict__ partials, E* __restrict__ grad) {
+                                                                             const LossOut sums, E* __restrict__ grad) {
   constexpr int NT = rows_threads<LANES>(), PER = NT / LANES;
   __shared__ float lds[LANES > 64 ? 3 * (LANES / 64) + 2 : 1];
   __shared__ int64_t sc[NT / 64];
-  __shared__ double sd[NT / 64];
   const float scale = weight_scale<NT>(w, sc);
   const int lane = threadIdx.x % LANES;
   float acc[kTerms] = {};
-  for (int64_t row = (int64_t)blockIdx.x * PER + threadIdx.x / LANES; row < a.rows; row += (int64_t)gridDim.x * PER) {
+  for (int64_t row = first_row<LANES>(); row < a.rows; row += (int64_t)gridDim.x * PER) {
     E* out = grad + row * a.A;
     if (t.mask != nullptr && t.mask[row] == 0.f) {  // (the same for the whole group)
       write_zeros<E, LANES>(out, a.A, lane);
@@ -43,11 +42,11 @@ __global__ __launch_bounds__(rows_threads<LANES>()) void logits_loss_kernel(cons
     const float lp = empty && x == x ? -INFINITY : ((x - r.m) * a.c - log2s) * kLn2;
     const float entropy = empty ? 0.f : (log2s - r.u / r.s) * kLn2;
     const StepTerms st = step_terms(lp, t.old[row], t.adv[row], t.ref ? t.ref[row] : 0.f, t.ref != nullptr, c);
-    const RowGrad g(wt * st.slope, -c.entropy_coef * wt, entropy, r.m, log2s, a.inv_tau, act, empty);
+    const RowGrad g(wt * st.slope, -c.entropy_coef * wt, entropy, r.m, a.c, log2s, a.inv_tau, act, empty);
     if constexpr (NV > 0)
-      write_grad<E, LANES, NV>(f, &h, out, g, a.c, lane);
+      write_grad<E, LANES, NV>(f, &h, out, g, lane);
     else
-      write_grad<E, LANES, 0>(f, nullptr, out, g, a.c, lane);
+      write_grad<E, LANES, 0>(f, nullptr, out, g, lane);
     if (lane == 0) {
 #pragma unroll
       for (int k = 0; k < 4; ++k) acc[k] += wt * st.v[k];
@@ -55,31 +54,95 @@ __global__ __launch_bounds__(rows_threads<LANES>()) void logits_loss_kernel(cons
     }
     if constexpr (LANES > 64) __syncthreads();
   }
-  write_partials<NT>(acc, partials, sd);
+  finish_loss<NT>(acc, c, sums);
+}
+
+template <class E, int K>
+__global__ __launch_bounds__(kFewRows) void few_loss_kernel(const ActionRows<E> a, const FewRows f, const StepArrays t,
+                                                            const LossConsts c, const Weights w, const LossOut sums,
+                                                            E* __restrict__ grad) {
+  extern __shared__ float lds[];
+  __shared__ int64_t sc[kFewRows / 64];
+  const float scale = weight_scale<kFewRows>(w, sc);
+  float acc[kTerms] = {};
+  for (int64_t row0 = (int64_t)blockIdx.x * kFewRows; row0 < a.rows; row0 += (int64_t)gridDim.x * kFewRows) {
+    const int rows = (int)(a.rows - row0 < kFewRows ? a.rows - row0 : kFewRows);
+    const int64_t row = row0 + threadIdx.x;
+    const bool mine = (int)threadIdx.x < rows, kept = mine && (t.mask == nullptr || t.mask[row] != 0.f);
+    int64_t act = 0;
+    float old = 0.f, adv = 0.f, ref = 0.f, wt = scale;
+    if (kept) {
+      act = a.actions[row], old = t.old[row], adv = t.adv[row];
+      if (t.ref) ref = t.ref[row];
+      if (w.row_counts != nullptr) wt = scale / (float)w.row_counts[row / a.seq_len];
+    }
+    f.take(a.logits + row0 * a.A, rows * a.A, lds);
+    __syncthreads();
+    float* x = lds + threadIdx.x * f.pitch;
+    if (kept) {
+      FewLogits<K> h;
+      h.load(x, a.A);
+      const RowStats r = h.stats(a.c);
+      const float xa = act >= 0 && act < a.A ? x[act] : NAN;
+      const bool empty = r.s == 0.f;
+      const float log2s = r.log2s();
+        const float lp = empty && xa == xa ? -INFINITY : ((xa - r.m) * a.c - log2s) * kLn2;
+      const float entropy = empty ? 0.f : (log2s - r.u / r.s) * kLn2;
+      const StepTerms st = step_terms(lp, old, adv, ref, t.ref != nullptr, c);
+      const RowGrad g(wt * st.slope, -c.entropy_coef * wt, entropy, r.m, a.c, log2s, a.inv_tau, act, empty);
+      if (__any(empty)) {
+#pragma unroll
+        for (int j = 0; j < K; ++j)
+          if (j < K - 3 || j < a.A) x[j] = empty ? 0.f : g(h.x[j], j);
+      } else {
+#pragma unroll
+        for (int j = 0; j < K; ++j)
+          if (j < K - 3 || j < a.A) x[j] = g(h.x[j]);
+        if (g.action >= 0 && g.action < a.A) x[g.action] += g.at;
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) acc[k] += wt * st.v[k];
+      acc[4] += wt * entropy;
+    } else if (mine) {
+      for (int j = 0; j < a.A; ++j) x[j] = 0.f;
+    }
+    __syncthreads();
+    f.put(grad + row0 * a.A, rows * a.A, lds);
+    __syncthreads();
+  }
+  finish_loss<kFewRows>(acc, c, sums);
 }
 
 template <class E>
 int impl(const rlk_action_rows* rows, const rlk_policy_terms* t, void* grad, hipStream_t s) {
   LossPlan plan;
-  int st = plan_loss(t, rows->num_envs, rows->seq_len, &plan);
+  int st = plan_loss(t, rows->num_envs, rows->seq_len, kTerms, &plan);
   if (st != RLK_OK) return st;
   const ActionRows<E> a = action_rows<E>(rows);
-  if (a.rows == 0) return launch_finish(t, plan, 0, kTerms, s);
+  if (a.rows == 0) return launch_no_steps(plan, s);
   if (!grad) return RLK_ERR_INVALID_ARGUMENT;
   if ((st = launch_count(t, rows->num_envs, rows->seq_len, &plan, s)) != RLK_OK) return st;
   const StepArrays arrays{static_cast<const float*>(t->old_log_probs), static_cast<const float*>(t->advantages),
                           static_cast<const float*>(t->ref_log_probs), static_cast<const float*>(t->mask)};
-  constexpr int VEC = Frame<E>::VEC;
-  int64_t blocks = 0;
-  st = dispatch_row((a.A + VEC - 1) / VEC, [&](auto lanes, auto nv) {
-    constexpr int L = decltype(lanes)::value, NV = decltype(nv)::value, NT = rows_threads<L>();
-    blocks = (a.rows + NT / L - 1) / (NT / L);
+  FewRows few;
+  if (few_rows(a, grad, &few)) {
+    int64_t blocks = (a.rows + kFewRows - 1) / kFewRows;
     if (blocks > kMaxLossBlocks) blocks = kMaxLossBlocks;
-    logits_loss_kernel<E, L, NV><<<dim3((unsigned)blocks), dim3(NT), 0, s>>>(a, arrays, plan.consts, plan.weights, plan.partials,
+    return dispatch_few(a.A, [&](auto k) {
+      few_loss_kernel<E, decltype(k)::value><<<dim3((unsigned)blocks), dim3(kFewRows), few.pitch * kFewRows * sizeof(float), s>>>(
+          a, few, arrays, plan.consts, plan.weights, plan.out, static_cast<E*>(grad));
+      return hipGetLastError() == hipSuccess ? RLK_OK : RLK_ERR_LAUNCH;
+    });
+  }
+  constexpr int VEC = Frame<E>::VEC;
+  return dispatch_update((a.A + VEC - 1) / VEC, [&](auto lanes, auto nv, int64_t most) {
+    constexpr int L = decltype(lanes)::value, NV = decltype(nv)::value, NT = rows_threads<L>();
+    int64_t blocks = (a.rows + NT / L - 1) / (NT / L);
+    if (blocks > most) blocks = most;
+    logits_loss_kernel<E, L, NV><<<dim3((unsigned)blocks), dim3(NT), 0, s>>>(a, arrays, plan.consts, plan.weights, plan.out,
                                                                            static_cast<E*>(grad));
     return hipGetLastError() == hipSuccess ? RLK_OK : RLK_ERR_LAUNCH;
   });
-  return st != RLK_OK ? st : launch_finish(t, plan, (int)blocks, kTerms, s);
 }
 
 }  // namespace

@@ -132,33 +132,93 @@ __device__ __forceinline__ float weight_scale(const Weights& w, int64_t* s) {
   return n > 0 ? (float)(1.0 / (double)n) : 0.f;
 }
 
-// Partial sums of the loss's terms, one set of kTerms doubles per workgroup, and the small kernel that adds
-// them up (rlk_policy_loss.hip).
-constexpr int kMaxLossBlocks = 4096;
+// Partial sums of the loss's terms: one set of kTerms doubles per workgroup, at most this many.
+constexpr int kMaxLossBlocks = 2048, kPartials = 8;  // (64 bytes each)
+
+// The workgroups draw tickets in this many groups, and the last of each group draws one of the groups: 1024 draws
+// from one word took 10 us more than the kernel around them.
+constexpr int kTicketGroups = 32, kTicketStride = 16;
+constexpr size_t kTicketBytes = (kTicketGroups + 1) * kTicketStride * sizeof(uint32_t);
+
+// Where a call's sums meet and what they become.
+struct LossOut {
+  double* partials;  // [workgroups, kPartials]
+  uint32_t* tickets;  // [kTicketGroups + 1], kTicketStride apart, 0 between calls
+  float *loss, *means;
+  int num_means;
+};
 
 struct LossPlan {
   LossConsts consts;
   Weights weights;
-  double* partials;
+  LossOut out;
   int64_t* count_parts;
   int* row_counts;
 };
 
 // Checks the terms and lays out the workspace; RLK_OK or an error.
-int plan_loss(const rlk_policy_terms* t, int64_t num_envs, int64_t seq_len, LossPlan* plan);
+int plan_loss(const rlk_policy_terms* t, int64_t num_envs, int64_t seq_len, int means, LossPlan* plan);
 // Counts the steps that take part (when there is a mask).
 int launch_count(const rlk_policy_terms* t, int64_t num_envs, int64_t seq_len, LossPlan* plan, hipStream_t s);
-// loss and means from `blocks` sets of partial sums.
-int launch_finish(const rlk_policy_terms* t, const LossPlan& plan, int blocks, int means, hipStream_t s);
+// Writes the loss and means of no steps: zeros.
+int launch_no_steps(const LossPlan& plan, hipStream_t s);
 
-// Adds a thread's terms to its workgroup's and writes the workgroup's partial sums.
+// The sums of kTerms doubles over a workgroup of NT threads: term k in thread k.  `s`: NT / 64 * kTerms.
 template <int NT>
-__device__ __forceinline__ void write_partials(const float (&acc)[kTerms], double* partials, double* s) {
+__device__ __forceinline__ double sum_terms(double (&v)[kTerms], double* s) {
 #pragma unroll
-  for (int i = 0; i < kTerms; ++i) {
-    const double x = block_sum<NT>((double)acc[i], s);
-    if (threadIdx.x == 0) partials[(int64_t)blockIdx.x * kTerms + i] = x;
+  for (int k = 0; k < kTerms; ++k)
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) v[k] += __shfl_xor(v[k], d);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0)
+#pragma unroll
+    for (int k = 0; k < kTerms; ++k) s[(threadIdx.x >> 6) * kTerms + k] = v[k];
+  __syncthreads();
+  double x = 0.0;
+  if (threadIdx.x < kTerms)
+    for (int i = 0; i < NT / 64; ++i) x += s[i * kTerms + threadIdx.x];
+  return x;
+}
+
+// The end of a loss kernel: the workgroups' sums, and from the last one to arrive the loss and the means, added up in the
+// workgroups' order whichever that is.  (A launch of its own for that took 2.7 us and a gap.)  The sums go through stores
+// and loads at agent scope, which every XCD sees, and are complete before the ticket is drawn: the wait is all the order
+// that takes.  A release at the ticket would also write back the L2's gradients, once per workgroup ([512,6000] 47 us of a
+// kernel that takes 11).
+template <int NT>
+__device__ __forceinline__ void finish_loss(const float (&acc)[kTerms], const LossConsts& c, const LossOut& o) {
+  __shared__ double s[NT / 64 * kTerms];
+  __shared__ bool last;
+  double v[kTerms];
+#pragma unroll
+  for (int k = 0; k < kTerms; ++k) v[k] = (double)acc[k];
+  double x = sum_terms<NT>(v, s);
+  if (gridDim.x > 1) {
+    if (threadIdx.x < kTerms)
+      __hip_atomic_store(o.partials + (int64_t)blockIdx.x * kPartials + threadIdx.x, x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (threadIdx.x == 0) {
+      const uint32_t group = blockIdx.x % kTicketGroups, members = (gridDim.x - group + kTicketGroups - 1) / kTicketGroups;
+      const uint32_t groups = gridDim.x < kTicketGroups ? gridDim.x : kTicketGroups;
+      uint32_t *mine = o.tickets + group * kTicketStride, *all = o.tickets + kTicketGroups * kTicketStride;
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (the wavefront's stores: the sums' among them)
+      last = __hip_atomic_fetch_add(mine, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == members - 1 &&
+             __hip_atomic_fetch_add(all, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == groups - 1;
+    }
+    __syncthreads();
+    if (!last) return;
+#pragma unroll
+    for (int k = 0; k < kTerms; ++k) v[k] = 0.0;
+    for (int b = threadIdx.x; b < (int)gridDim.x; b += NT)
+#pragma unroll
+      for (int k = 0; k < kTerms; ++k)
+        v[k] += __hip_atomic_load(o.partials + (int64_t)b * kPartials + k, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    x = sum_terms<NT>(v, s);
+    if (threadIdx.x <= kTicketGroups) o.tickets[threadIdx.x * kTicketStride] = 0;
   }
+  if ((int)threadIdx.x < o.num_means) o.means[threadIdx.x] = (float)x;
+  const double kl = __shfl(x, 1), entropy = __shfl(x, 4);
+  if (threadIdx.x == 0) *o.loss = (float)(x + (double)c.kl_coef * kl - (double)c.entropy_coef * entropy);
 }
 
 }  // namespace rlk

@@ -1,5 +1,6 @@
 // rlk_policy_loss.hip -- the clipped policy loss from log-probabilities, and the counting and summing that
 // the loss from logits shares (include/rl_triton_policy.h).
+#include "rlk_launch.hpp"
 #include "rlk_policy.hpp"
 
 namespace rlk {
@@ -7,23 +8,48 @@ namespace {
 
 constexpr int kNT = 256;
 
-// What the mean divides by: the steps with mask != 0 or, per_row, the rows that have any (and each row's
-// number).  A wavefront per row, or the whole workgroup where there are few.
+// Four consecutive elements as floats; `whole`: one aligned access, else the `left` (1..4) that exist.
 template <class E>
-__global__ __launch_bounds__(kNT) void count_kernel(const E* __restrict__ mask, int64_t num_envs, int64_t seq_len,
-                                                    int per_row, int64_t* __restrict__ parts, int* __restrict__ row_counts) {
+__device__ __forceinline__ float4 load4(const E* p, bool whole, int left) {
+  if (whole) return load_quad<false>(p);
+  return {load_one(p), left > 1 ? load_one(p + 1) : 0.f, left > 2 ? load_one(p + 2) : 0.f, left > 3 ? load_one(p + 3) : 0.f};
+}
+
+// What the mean divides by: the steps with mask != 0 or, per_row, the rows that have any (and each row's number: a
+// wavefront per row for short rows, the workgroup for others).
+template <class E, int ROW_LANES>  // 0: steps
+__global__ __launch_bounds__(kNT) void count_kernel(const E* __restrict__ mask, int64_t num_envs, int64_t seq_len, bool whole,
+                                                    int64_t* __restrict__ parts, int* __restrict__ row_counts) {
   __shared__ int64_t s[kNT / 64];
+  __shared__ int part[2][kNT / 64];
   int64_t total = 0;
-  if (!per_row) {
-    const int64_t n = num_envs * seq_len, step = (int64_t)gridDim.x * kNT;
-    for (int64_t i = (int64_t)blockIdx.x * kNT + threadIdx.x; i < n; i += step) total += load_one(mask + i) != 0.f;
+  auto kept = [](float4 m) { return (m.x != 0.f) + (m.y != 0.f) + (m.z != 0.f) + (m.w != 0.f); };
+  if constexpr (ROW_LANES == 0) {
+    const int64_t n = num_envs * seq_len, step = (int64_t)gridDim.x * kNT * 4;
+    for (int64_t i = ((int64_t)blockIdx.x * kNT + threadIdx.x) * 4; i < n; i += step) {
+      const int left = (int)(n - i < 4 ? n - i : 4);
+      total += kept(load4(mask + i, whole && left == 4, left));
+    }
   } else {
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    for (int64_t e = (int64_t)blockIdx.x * (kNT / 64) + wave; e < num_envs; e += (int64_t)gridDim.x * (kNT / 64)) {
+    constexpr int PER = kNT / ROW_LANES;
+    const int lane = threadIdx.x % ROW_LANES;
+    int turn = 0;
+    for (int64_t e = (int64_t)blockIdx.x * PER + threadIdx.x / ROW_LANES; e < num_envs; e += (int64_t)gridDim.x * PER) {
+      const E* row = mask + e * seq_len;
       int n = 0;
-      for (int64_t t = lane; t < seq_len; t += 64) n += load_one(mask + e * seq_len + t) != 0.f;
+      for (int64_t t = lane * 4; t < seq_len; t += ROW_LANES * 4) {
+        const int left = (int)(seq_len - t < 4 ? seq_len - t : 4);
+        n += kept(load4(row + t, whole && left == 4, left));
+      }
 #pragma unroll
       for (int d = 32; d > 0; d >>= 1) n += __shfl_xor(n, d);
+      if constexpr (ROW_LANES > 64) {
+        if ((threadIdx.x & 63) == 0) part[turn][threadIdx.x >> 6] = n;
+        __syncthreads();
+        n = 0;
+        for (int i = 0; i < kNT / 64; ++i) n += part[turn][i];
+        turn ^= 1;
+      }
       if (lane == 0) {
         row_counts[e] = n;
         total += n > 0;
@@ -39,71 +65,169 @@ struct LossArgs {
   const E *lp, *old, *adv, *ref, *mask;
   E* grad;
   int64_t n, seq_len;
+  bool whole;  // arrays aligned to 4 elements
   LossConsts c;
   Weights w;
-  double* partials;
+  LossOut out;
 };
+
+// Steps i .. i + 3 (`left` of them exist): their gradients, their terms added to `acc`.  row_weight(step): what a
+// row's steps count for.
+template <class E, class F>
+__device__ __forceinline__ void four_steps(const LossArgs<E>& a, int64_t i, int left, float4 m, float (&acc)[kTerms], F weight) {
+  const bool whole = a.whole && left == 4;
+  const float4 lp = load4(a.lp + i, whole, left), old = load4(a.old + i, whole, left), adv = load4(a.adv + i, whole, left);
+  const float4 ref = a.ref ? load4(a.ref + i, whole, left) : float4{0.f, 0.f, 0.f, 0.f};
+  float g[4];
+  const float *pl = &lp.x, *po = &old.x, *pa = &adv.x, *pr = &ref.x, *pm = &m.x;
+#pragma unroll
+  for (int x = 0; x < 4; ++x) {
+    g[x] = 0.f;
+    if (pm[x] != 0.f && x < left) {
+      const float w = weight(i, x);
+      const StepTerms t = step_terms(pl[x], po[x], pa[x], pr[x], a.ref != nullptr, a.c);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) acc[k] += w * t.v[k];
+      g[x] = w * t.slope;
+    }
+  }
+  if (whole) {
+    store_quad(a.grad + i, float4{g[0], g[1], g[2], g[3]});
+  } else {
+#pragma unroll
+    for (int x = 0; x < 4; ++x)
+      if (x < left) a.grad[i + x] = from_f32<E>(g[x]);
+  }
+}
+
+constexpr float4 kAll{1.f, 1.f, 1.f, 1.f};
 
 template <class E>
 __global__ __launch_bounds__(kNT) void loss_kernel(const LossArgs<E> a) {
   __shared__ int64_t sc[kNT / 64];
-  __shared__ double sd[kNT / 64];
   const float scale = weight_scale<kNT>(a.w, sc);
   float acc[kTerms] = {};
-  const int64_t step = (int64_t)gridDim.x * kNT;
-  for (int64_t i = (int64_t)blockIdx.x * kNT + threadIdx.x; i < a.n; i += step) {
-    float g = 0.f;
-    if (a.mask == nullptr || load_one(a.mask + i) != 0.f) {
-      float w = scale;
-      if (a.w.row_counts != nullptr) w /= (float)a.w.row_counts[i / a.seq_len];
-      const StepTerms t = step_terms(load_one(a.lp + i), load_one(a.old + i), load_one(a.adv + i),
-                                     a.ref ? load_one(a.ref + i) : 0.f, a.ref != nullptr, a.c);
-#pragma unroll
-      for (int k = 0; k < 4; ++k) acc[k] += w * t.v[k];
-      g = w * t.slope;
+  const int64_t step = (int64_t)gridDim.x * kNT * 4;
+  for (int64_t i = ((int64_t)blockIdx.x * kNT + threadIdx.x) * 4; i < a.n; i += step) {
+    const int left = (int)(a.n - i < 4 ? a.n - i : 4);
+    const float4 m = a.mask ? load4(a.mask + i, a.whole && left == 4, left) : kAll;
+    if (a.w.row_counts == nullptr) {
+      four_steps(a, i, left, m, acc, [&](int64_t, int) { return scale; });
+    } else {
+      int64_t row = a.n <= 0x7fffffff ? (int64_t)((uint32_t)i / (uint32_t)a.seq_len) : i / a.seq_len;
+      int64_t ends = (row + 1) * a.seq_len;
+      float w = scale / (float)a.w.row_counts[row];  // (a row of none is asked for nothing)
+      four_steps(a, i, left, m, acc, [&](int64_t at, int x) {
+        while (at + x >= ends) w = scale / (float)a.w.row_counts[++row], ends += a.seq_len;
+        return w;
+      });
     }
-    a.grad[i] = from_f32<E>(g);
   }
-  write_partials<kNT>(acc, a.partials, sd);
+  finish_loss<kNT>(acc, a.c, a.out);
 }
 
-__global__ __launch_bounds__(kNT) void finish_kernel(const double* __restrict__ partials, int blocks, int means,
-                                                     float kl_coef, float entropy_coef, float* __restrict__ loss,
-                                                     float* __restrict__ out) {
-  __shared__ double s[kNT / 64];
-  double v[kTerms] = {};
-  for (int b = threadIdx.x; b < blocks; b += kNT)
+// Small calls: one workgroup counts, computes and sums, and there is one launch to wait for.
+constexpr int kSmallNT = 1024, kSmallSteps = 8192;
+
+template <class E>
+__global__ __launch_bounds__(kSmallNT) void small_loss_kernel(const LossArgs<E> a) {
+  __shared__ int counts[kSmallSteps];
+  __shared__ int sums[kSmallNT / 64];
+  constexpr int Q = kSmallSteps / (4 * kSmallNT);
+  const int n = (int)a.n, T = (int)a.seq_len;
+  float4 m[Q];
+  float scale = a.w.all;
+  const bool rows = a.mask != nullptr && a.w.per_row;
 #pragma unroll
-    for (int k = 0; k < kTerms; ++k) v[k] += partials[(int64_t)b * kTerms + k];
-#pragma unroll
-  for (int k = 0; k < kTerms; ++k) v[k] = block_sum<kNT>(v[k], s);
-  if (threadIdx.x == 0) {
-    *loss = (float)(v[0] + (double)kl_coef * v[1] - (double)entropy_coef * v[4]);
-    for (int k = 0; k < means; ++k) out[k] = (float)v[k];
+  for (int q = 0; q < Q; ++q) {
+    const int i = (q * kSmallNT + threadIdx.x) * 4, left = n - i < 4 ? n - i : 4;
+    m[q] = i >= n ? float4{0.f, 0.f, 0.f, 0.f} : a.mask ? load4(a.mask + i, a.whole && left == 4, left) : kAll;
   }
+  if (a.mask != nullptr) {
+    int count = 0;
+    if (rows) {
+      for (int e = threadIdx.x; e * T < n; e += kSmallNT) counts[e] = 0;
+      __syncthreads();
+    }
+#pragma unroll
+    for (int q = 0; q < Q; ++q) {
+      const float* pm = &m[q].x;
+#pragma unroll
+      for (int x = 0; x < 4; ++x)
+        if (pm[x] != 0.f) {
+          if (rows) atomicAdd(&counts[((q * kSmallNT + threadIdx.x) * 4 + x) / T], 1);
+          else ++count;
+        }
+    }
+    if (rows) {
+      __syncthreads();
+      for (int e = threadIdx.x; e * T < n; e += kSmallNT) count += counts[e] > 0;
+    }
+    count = block_sum<kSmallNT>(count, sums);
+    scale = count > 0 ? 1.f / (float)count : 0.f;
+  }
+  float acc[kTerms] = {};
+#pragma unroll
+  for (int q = 0; q < Q; ++q) {
+    const int i = (q * kSmallNT + threadIdx.x) * 4;
+    if (i < n)
+      four_steps(a, i, n - i < 4 ? n - i : 4, m[q], acc,
+                 [&](int64_t at, int x) { return rows ? scale / (float)counts[((int)at + x) / T] : scale; });
+  }
+  finish_loss<kSmallNT>(acc, a.c, a.out);
+}
+
+__global__ void no_steps_kernel(LossOut o) {
+  if (threadIdx.x == 0) *o.loss = 0.f;
+  if ((int)threadIdx.x < o.num_means) o.means[threadIdx.x] = 0.f;
 }
 
 template <class E>
 int loss_impl(const void* lp, int64_t E_, int64_t T, const rlk_policy_terms* t, void* grad, hipStream_t s) {
   LossPlan plan;
-  int st = plan_loss(t, E_, T, &plan);
+  int st = plan_loss(t, E_, T, 4, &plan);
   if (st != RLK_OK) return st;
   const int64_t n = E_ * T;
-  if (n > 0 && (!lp || !grad)) return RLK_ERR_INVALID_ARGUMENT;
-  if ((st = launch_count(t, E_, T, &plan, s)) != RLK_OK) return st;
-  int64_t blocks = (n + kNT * 4 - 1) / (kNT * 4);
-  blocks = blocks < 1 ? 1 : blocks > 2048 ? 2048 : blocks;
+  if (n == 0) return launch_no_steps(plan, s);
+  if (!lp || !grad) return RLK_ERR_INVALID_ARGUMENT;
   LossArgs<E> a{static_cast<const E*>(lp), static_cast<const E*>(t->old_log_probs), static_cast<const E*>(t->advantages),
                 static_cast<const E*>(t->ref_log_probs), static_cast<const E*>(t->mask), static_cast<E*>(grad),
-                n, T, plan.consts, plan.weights, plan.partials};
-  loss_kernel<E><<<dim3((unsigned)blocks), dim3(kNT), 0, s>>>(a);
-  if (hipGetLastError() != hipSuccess) return RLK_ERR_LAUNCH;
-  return launch_finish(t, plan, (int)blocks, 4, s);
+                n, T, false, plan.consts, plan.weights, plan.out};
+  a.whole = quad_aligned(a.lp, a.old, a.adv, a.ref, a.mask, a.grad);
+  a.c.entropy_coef = 0.f;  // (there are no entropies here)
+  if (n <= kSmallSteps) {
+    small_loss_kernel<E><<<dim3(1), dim3(kSmallNT), 0, s>>>(a);
+  } else {
+    if ((st = launch_count(t, E_, T, &plan, s)) != RLK_OK) return st;
+    a.w = plan.weights;
+    // as many rounds as the most workgroups need, and as many workgroups as fill them
+    const int64_t units = (n + kNT * 4 - 1) / (kNT * 4), rounds = (units + kMaxLossBlocks - 1) / kMaxLossBlocks;
+    loss_kernel<E><<<dim3((unsigned)((units + rounds - 1) / rounds)), dim3(kNT), 0, s>>>(a);
+  }
+  return hipGetLastError() == hipSuccess ? RLK_OK : RLK_ERR_LAUNCH;
+}
+
+template <class E>
+int count_impl(const rlk_policy_terms* t, int64_t E_, int64_t T, LossPlan* p, hipStream_t s) {
+  const E* mask = static_cast<const E*>(t->mask);
+  Weights& w = p->weights;
+  const bool whole = quad_aligned(mask) && (!w.per_row || T % 4 == 0);
+  // a workgroup per row from rows that give each of its threads a quad
+  const bool wide = T >= kNT * 4;
+  const int64_t units = !w.per_row ? (E_ * T + kNT * 4 - 1) / (kNT * 4) : wide ? E_ : (E_ + kNT / 64 - 1) / (kNT / 64);
+  const int blocks = (int)(units < kCountBlocks ? units : kCountBlocks);
+  w.parts = p->count_parts, w.num_parts = blocks;
+  if (w.per_row) w.row_counts = p->row_counts;
+  const dim3 grid(blocks), block(kNT);
+  if (!w.per_row) count_kernel<E, 0><<<grid, block, 0, s>>>(mask, E_, T, whole, p->count_parts, p->row_counts);
+  else if (wide) count_kernel<E, kNT><<<grid, block, 0, s>>>(mask, E_, T, whole, p->count_parts, p->row_counts);
+  else count_kernel<E, 64><<<grid, block, 0, s>>>(mask, E_, T, whole, p->count_parts, p->row_counts);
+  return hipGetLastError() == hipSuccess ? RLK_OK : RLK_ERR_LAUNCH;
 }
 
 }  // namespace
 
-int plan_loss(const rlk_policy_terms* t, int64_t num_envs, int64_t seq_len, LossPlan* p) {
+int plan_loss(const rlk_policy_terms* t, int64_t num_envs, int64_t seq_len, int means, LossPlan* p) {
   if (!t || num_envs < 0 || seq_len < 0 || !t->loss || !t->means) return RLK_ERR_INVALID_ARGUMENT;
   if (num_envs * seq_len > 0 && (!t->old_log_probs || !t->advantages)) return RLK_ERR_INVALID_ARGUMENT;
   if (!(t->clip_low >= 0.f) || !(t->clip_high >= 0.f) || !(t->dual_clip == 0.f || t->dual_clip > 1.f))
@@ -118,8 +242,9 @@ int plan_loss(const rlk_policy_terms* t, int64_t num_envs, int64_t seq_len, Loss
   c.log_high = (float)std::log1p((double)t->clip_high);
   c.dual = t->dual_clip, c.log_dual = t->dual_clip > 0.f ? (float)std::log((double)t->dual_clip) : INFINITY;
   c.kl_coef = t->kl_coef, c.entropy_coef = t->entropy_coef;
-  p->partials = static_cast<double*>(t->workspace);
-  p->count_parts = reinterpret_cast<int64_t*>(p->partials + (int64_t)kMaxLossBlocks * kTerms);
+  char* ws = static_cast<char*>(t->workspace);
+  p->out = {reinterpret_cast<double*>(ws + kTicketBytes), reinterpret_cast<uint32_t*>(ws), t->loss, t->means, means};
+  p->count_parts = reinterpret_cast<int64_t*>(p->out.partials + (int64_t)kMaxLossBlocks * kPartials);
   p->row_counts = reinterpret_cast<int*>(p->count_parts + kCountBlocks);
   Weights& w = p->weights;
   w.parts = nullptr, w.row_counts = nullptr, w.num_parts = 0, w.per_row = t->per_row != 0;
@@ -130,23 +255,11 @@ int plan_loss(const rlk_policy_terms* t, int64_t num_envs, int64_t seq_len, Loss
 
 int launch_count(const rlk_policy_terms* t, int64_t num_envs, int64_t seq_len, LossPlan* p, hipStream_t s) {
   if (t->mask == nullptr || num_envs * seq_len == 0) return RLK_OK;
-  Weights& w = p->weights;
-  const int64_t units = w.per_row ? (num_envs + kNT / 64 - 1) / (kNT / 64) : (num_envs * seq_len + kNT - 1) / kNT;
-  const int blocks = (int)(units < kCountBlocks ? units : kCountBlocks);
-  w.parts = p->count_parts, w.num_parts = blocks;
-  if (w.per_row) w.row_counts = p->row_counts;
-  if (t->bf16)
-    count_kernel<bf16><<<dim3(blocks), dim3(kNT), 0, s>>>(static_cast<const bf16*>(t->mask), num_envs, seq_len, w.per_row,
-                                                         p->count_parts, p->row_counts);
-  else
-    count_kernel<float><<<dim3(blocks), dim3(kNT), 0, s>>>(static_cast<const float*>(t->mask), num_envs, seq_len, w.per_row,
-                                                          p->count_parts, p->row_counts);
-  return hipGetLastError() == hipSuccess ? RLK_OK : RLK_ERR_LAUNCH;
+  return t->bf16 ? count_impl<bf16>(t, num_envs, seq_len, p, s) : count_impl<float>(t, num_envs, seq_len, p, s);
 }
 
-int launch_finish(const rlk_policy_terms* t, const LossPlan& p, int blocks, int means, hipStream_t s) {
-  finish_kernel<<<dim3(1), dim3(kNT), 0, s>>>(p.partials, blocks, means, t->kl_coef, means > 4 ? t->entropy_coef : 0.f,
-                                              t->loss, t->means);
+int launch_no_steps(const LossPlan& p, hipStream_t s) {
+  no_steps_kernel<<<dim3(1), dim3(64), 0, s>>>(p.out);
   return hipGetLastError() == hipSuccess ? RLK_OK : RLK_ERR_LAUNCH;
 }
 
@@ -158,7 +271,7 @@ extern "C" {
 
 size_t rlk_policy_workspace_bytes(int64_t num_envs) {
   const size_t rows = num_envs > 0 ? (size_t)num_envs : 0;
-  return sizeof(double) * kMaxLossBlocks * kTerms + sizeof(int64_t) * kCountBlocks + (sizeof(int) * rows + 7) / 8 * 8;
+  return kTicketBytes + sizeof(double) * kMaxLossBlocks * kPartials + sizeof(int64_t) * kCountBlocks + (sizeof(int) * rows + 7) / 8 * 8;
 }
 
 int rlk_policy_loss(const void* log_probs, int64_t num_envs, int64_t seq_len, const rlk_policy_terms* terms,

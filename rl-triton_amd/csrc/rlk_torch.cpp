@@ -19,12 +19,14 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <ATen/core/grad_mode.h>
 #include <ATen/hip/EmptyTensor.h>
 #include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <algorithm>
+#include <cmath>
 #include <cstddef>
 #include <cstdint>
 #include <cstdlib>
@@ -34,6 +36,7 @@
 #include <utility>
 
 #include "rl_triton_amd.h"
+#include "rl_triton_policy.h"
 #include "rlk_time_major.h"
 
 namespace {
@@ -700,6 +703,8 @@ PyObject* op_affine_scan(PyObject* const* a, Py_ssize_t n) {
   return finish(st, "rlk_affine_scan", THPVariable_Wrap(std::move(out)));
 }
 
+#include "rlk_torch_policy.hpp"
+
 // C++ exceptions (an allocation that fails, say) must not cross into the interpreter: such
 // a call is declined, and the Python path raises torch's own exception for it.
 template <PyObject* (*F)(PyObject* const*, Py_ssize_t)>
@@ -824,6 +829,11 @@ const OpName kOps[] = {
     {"discounted_returns", guarded<op_discounted_returns<true>>},
     {"eligibility_traces", guarded<op_eligibility_traces<true>>},
     {"prefix_sum", guarded<op_prefix_sum_api>},
+    {"action_log_probs", guarded<op_action_log_probs>},
+    {"policy_loss", guarded<op_policy_loss>},
+    {"policy_loss_from_logits", guarded<op_policy_loss_from_logits>},
+    {"linear_attention", guarded<op_linear_attention>},
+    {"linear_attention_step", guarded<op_linear_attention_step>},
 };
 
 // entry(op, names, npos, defaults, required, fallback): a public function over fast op `op`

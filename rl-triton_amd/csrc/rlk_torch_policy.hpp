@@ -1,0 +1,244 @@
+// rlk_torch_policy.hpp -- the fast path of rl_triton.policy's functions, included by rlk_torch.cpp.
+//
+// As for the estimators: a call is taken when it can go to the C ABI (include/rl_triton_policy.h) as it stands and needs
+// no graph of gradients; any other is declined and the Python implementation checks it, copies what it has to
+// and raises.
+#pragma once
+
+// Checks of one call, on the device of its first tensor.
+struct PolicyCall {
+  c10::DeviceIndex dev = -1;
+  bool ok = true;
+
+  const at::Tensor* fail() {
+    ok = false;
+    return nullptr;
+  }
+  // A tensor on the current GPU that is an ordinary one and, where `graph` says that the function is differentiable
+  // in it, needs no gradient now.
+  const at::Tensor* tensor(PyObject* o, bool graph) {
+    if (!ok || !THPVariable_Check(o)) return fail();
+    const at::Tensor& t = THPVariable_Unpack(o);
+    if (!t.is_cuda() || t.is_neg() || (graph && t.requires_grad() && at::GradMode::is_enabled())) return fail();
+    if (dev < 0) {
+      dev = t.get_device();
+      if (dev != c10::hip::current_device()) return fail();
+    } else if (t.get_device() != dev) {
+      return fail();
+    }
+    return &t;
+  }
+  const at::Tensor* array(PyObject* o, at::ScalarType st, at::IntArrayRef sizes, bool graph = false) {
+    const at::Tensor* t = tensor(o, graph);
+    if (!t || t->scalar_type() != st || !t->is_contiguous() || t->sizes() != sizes) return fail();
+    return t;
+  }
+  const at::Tensor* opt(PyObject* o, at::ScalarType st, at::IntArrayRef sizes, bool graph = false) {
+    return o == Py_None ? nullptr : array(o, st, sizes, graph);
+  }
+  double number(PyObject* o, double low) {
+    double d = NAN;
+    if (PyFloat_CheckExact(o)) d = PyFloat_AS_DOUBLE(o);
+    else if (PyLong_CheckExact(o)) d = PyLong_AsDouble(o);
+    if (PyErr_Occurred()) PyErr_Clear(), d = NAN;
+    if (!std::isfinite(d) || d < low) fail();
+    return d;
+  }
+  void* stream() const { return c10::hip::getCurrentHIPStream(dev).stream(); }
+};
+
+at::Tensor policy_output(at::IntArrayRef sizes, at::ScalarType st, const at::Tensor& like) {
+  return at::Tensor(at::detail::empty_cuda(sizes, st, like.device(), std::nullopt));
+}
+
+const void* data_or_null(const at::Tensor* t) { return t ? t->data_ptr() : nullptr; }
+
+// Scratch memory, one of each kind per (device, stream), as rl_triton.policy._native keeps it; none (declined) while
+// the stream is capturing a graph.
+struct PolicyScratch {
+  at::Tensor sums, states;
+};
+bool policy_scratch(const PolicyCall& c, at::Tensor PolicyScratch::* kind, size_t need, const at::Tensor& like, void** ptr,
+                    size_t* bytes) {
+  *ptr = nullptr, *bytes = 0;
+  if (need == 0) return true;
+  static auto* all = new std::map<std::pair<int, uintptr_t>, PolicyScratch>();
+  hipStream_t s = static_cast<hipStream_t>(c.stream());
+  hipStreamCaptureStatus cs = hipStreamCaptureStatusNone;
+  if (hipStreamIsCapturing(s, &cs) != hipSuccess || cs != hipStreamCaptureStatusNone) return false;
+  at::Tensor& buf = (*all)[{(int)c.dev, reinterpret_cast<uintptr_t>(s)}].*kind;
+  if (!buf.defined() || (size_t)buf.numel() < need)
+    buf = zeroed((int64_t)(buf.defined() ? std::max(need, 2 * (size_t)buf.numel()) : need), like);
+  *ptr = buf.data_ptr(), *bytes = (size_t)buf.numel();
+  return true;
+}
+
+bool float_type(at::ScalarType st) { return st == at::kFloat || st == at::kBFloat16; }
+
+// logits [envs, steps, actions] with contiguous actions, or contiguous ones of any other rank.
+bool logit_rows(PolicyCall& c, PyObject* logits, PyObject* actions, PyObject* temperature, bool graph, rlk_action_rows* r,
+                const at::Tensor** x, const at::Tensor** a) {
+  const at::Tensor* t = *x = c.tensor(logits, graph);
+  if (!t || !float_type(t->scalar_type()) || t->dim() < 1 || t->numel() == 0) return false;
+  const int64_t n = t->size(-1);
+  r->num_actions = n;
+  if (t->dim() == 3 && (t->stride(2) == 1 || n == 1)) {
+    r->num_envs = t->size(0), r->seq_len = t->size(1), r->env_stride = t->stride(0), r->step_stride = t->stride(1);
+  } else if (t->is_contiguous()) {
+    r->num_envs = 1, r->seq_len = t->numel() / n, r->env_stride = t->numel(), r->step_stride = n;
+  } else {
+    return false;
+  }
+  *a = c.array(actions, at::kLong, t->sizes().slice(0, t->dim() - 1));
+  const double tau = c.number(temperature, 0.0);
+  if (!c.ok || !(tau > 0.0)) return false;
+  r->logits = t->data_ptr(), r->actions = static_cast<const int64_t*>((*a)->data_ptr());
+  r->temperature = (float)tau, r->bf16 = t->scalar_type() == at::kBFloat16;
+  return true;
+}
+
+// action_log_probs(logits, actions, temperature)
+PyObject* op_action_log_probs(PyObject* const* a, Py_ssize_t n) {
+  if (n != 3 || correctness_warnings()) return decline();
+  PolicyCall c;
+  rlk_action_rows r = {};
+  const at::Tensor *x, *act;
+  if (!logit_rows(c, a[0], a[1], a[2], true, &r, &x, &act)) return decline();
+  at::Tensor lp = policy_output(act->sizes(), at::kFloat, *x), ent = policy_output(act->sizes(), at::kFloat, *x);
+  const int st = rlk_action_log_probs(&r, static_cast<float*>(lp.data_ptr()), static_cast<float*>(ent.data_ptr()), nullptr, c.stream());
+  return finish(st, "rlk_action_log_probs", pair(lp, ent));
+}
+
+// What both losses read: (old, advantages, ref, clip_low, clip_high, kl_coef, dual_clip, mask, reduction).
+bool loss_terms(PolicyCall& c, PyObject* old, PyObject* adv, PyObject* ref, PyObject* low, PyObject* high, PyObject* kl, PyObject* dual,
+                PyObject* mask, PyObject* reduction, at::ScalarType st, at::IntArrayRef sizes, const at::Tensor& like,
+                rlk_policy_terms* t) {
+  const at::Tensor *o = c.array(old, st, sizes), *ad = c.array(adv, st, sizes), *r = c.opt(ref, st, sizes), *m = c.opt(mask, st, sizes);
+  t->clip_low = (float)c.number(low, 0.0), t->clip_high = (float)c.number(high, 0.0);
+  t->kl_coef = (float)c.number(kl, -HUGE_VAL);
+  if (dual != Py_None) {
+    const double d = c.number(dual, 1.0);
+    if (!((float)d > 1.f)) return false;
+    t->dual_clip = (float)d;
+  }
+  if (!c.ok || !PyUnicode_Check(reduction)) return false;
+  if (PyUnicode_CompareWithASCIIString(reduction, "rows") == 0) t->per_row = 1;
+  else if (PyUnicode_CompareWithASCIIString(reduction, "steps") != 0) return false;
+  t->old_log_probs = o->data_ptr(), t->advantages = ad->data_ptr(), t->ref_log_probs = data_or_null(r), t->mask = data_or_null(m);
+  t->bf16 = st == at::kBFloat16;
+  return policy_scratch(c, &PolicyScratch::sums, rlk_policy_workspace_bytes(sizes[0]), like, &t->workspace, &t->workspace_bytes);
+}
+
+PyObject* loss_result(int st, const char* what, at::Tensor& loss, at::Tensor& grad, at::Tensor& means) {
+  PyObject* r = PyTuple_New(3);
+  if (!r) return nullptr;
+  PyTuple_SET_ITEM(r, 0, THPVariable_Wrap(std::move(loss)));
+  PyTuple_SET_ITEM(r, 1, THPVariable_Wrap(std::move(grad)));
+  PyTuple_SET_ITEM(r, 2, THPVariable_Wrap(std::move(means)));
+  return finish(st, what, r);
+}
+
+// policy_loss(log_probs, old_log_probs, advantages, ref_log_probs, clip_low, clip_high, kl_coef, dual_clip, mask, reduction)
+PyObject* op_policy_loss(PyObject* const* a, Py_ssize_t n) {
+  if (n != 10 || correctness_warnings()) return decline();
+  PolicyCall c;
+  const at::Tensor* lp = c.tensor(a[0], false);
+  if (!lp || lp->dim() != 2 || !lp->is_contiguous() || !float_type(lp->scalar_type())) return decline();
+  rlk_policy_terms t = {};
+  if (!loss_terms(c, a[1], a[2], a[3], a[4], a[5], a[6], a[7], a[8], a[9], lp->scalar_type(), lp->sizes(), *lp, &t)) return decline();
+  at::Tensor loss = policy_output({}, at::kFloat, *lp), grad = policy_output(lp->sizes(), lp->scalar_type(), *lp),
+             means = policy_output({4}, at::kFloat, *lp);
+  t.loss = static_cast<float*>(loss.data_ptr()), t.means = static_cast<float*>(means.data_ptr());
+  const int st = rlk_policy_loss(lp->data_ptr(), lp->size(0), lp->size(1), &t, grad.data_ptr(), c.stream());
+  return loss_result(st, "rlk_policy_loss", loss, grad, means);
+}
+
+// policy_loss_from_logits(logits, actions, old_log_probs, advantages, ref_log_probs, clip_low, clip_high, kl_coef, entropy_coef,
+//                         temperature, dual_clip, mask, reduction)
+PyObject* op_policy_loss_from_logits(PyObject* const* a, Py_ssize_t n) {
+  if (n != 13 || correctness_warnings()) return decline();
+  PolicyCall c;
+  rlk_action_rows r = {};
+  const at::Tensor *x, *act;
+  if (!logit_rows(c, a[0], a[1], a[9], false, &r, &x, &act) || x->dim() != 3) return decline();
+  rlk_policy_terms t = {};
+  t.entropy_coef = (float)c.number(a[8], -HUGE_VAL);
+  if (!loss_terms(c, a[2], a[3], a[4], a[5], a[6], a[7], a[10], a[11], a[12], at::kFloat, act->sizes(), *x, &t)) return decline();
+  at::Tensor loss = policy_output({}, at::kFloat, *x), grad = policy_output(x->sizes(), x->scalar_type(), *x),
+             means = policy_output({5}, at::kFloat, *x);
+  t.loss = static_cast<float*>(loss.data_ptr()), t.means = static_cast<float*>(means.data_ptr());
+  const int st = rlk_policy_loss_from_logits(&r, &t, grad.data_ptr(), c.stream());
+  return loss_result(st, "rlk_policy_loss_from_logits", loss, grad, means);
+}
+
+// q, k, v of a sequence ([envs, steps, heads, dim]) or of a step ([envs, heads, dim]) and what goes with them.
+bool attention_args(PolicyCall& c, PyObject* q_, PyObject* k_, PyObject* v_, PyObject* decay_, PyObject* dones_, PyObject* state_,
+                    PyObject* scale_, bool steps, rlk_attention* t, const at::Tensor** v, at::Tensor* flags) {
+  const at::Tensor *q = c.tensor(q_, steps), *k = c.tensor(k_, steps);
+  *v = c.tensor(v_, steps);
+  if (!c.ok || !float_type(q->scalar_type()) || k->scalar_type() != q->scalar_type() || (*v)->scalar_type() != q->scalar_type()) return false;
+  const int64_t rank = steps ? 4 : 3;
+  if (q->dim() != rank || (*v)->dim() != rank || k->sizes() != q->sizes() ||
+      (*v)->sizes().slice(0, rank - 1) != q->sizes().slice(0, rank - 1) || q->numel() == 0 || (*v)->numel() == 0)
+    return false;
+  t->num_envs = q->size(0), t->seq_len = steps ? q->size(1) : 1, t->heads = q->size(rank - 2);
+  t->dim_k = q->size(rank - 1), t->dim_v = (*v)->size(rank - 1);
+  if (t->dim_k > 128 || t->dim_v > 128) return false;
+  auto seq = [&](const at::Tensor& x) {
+    return rlk_sequence{x.data_ptr(), x.stride(0), steps ? x.stride(1) : 0, x.stride(rank - 2)};
+  };
+  for (const at::Tensor* x : {q, k, *v})
+    if (x->size(rank - 1) > 1 && x->stride(rank - 1) != 1) return false;
+  t->q = seq(*q), t->k = seq(*k), t->v = seq(**v);
+  const at::Tensor* decay = c.array(decay_, at::kFloat, {t->heads});
+  const at::Tensor* dones = dones_ == Py_None ? nullptr : c.tensor(dones_, false);
+  if (!c.ok || (dones && (dones->scalar_type() != at::kFloat || dones->sizes() != q->sizes().slice(0, steps ? 2 : 1)))) return false;
+  if (dones && !dones->is_contiguous()) {  // (a step's column of a rollout buffer)
+    *flags = dones->contiguous();
+    dones = flags;
+  }
+  const at::Tensor* state = c.opt(state_, at::kFloat, {t->num_envs, t->heads, t->dim_k, t->dim_v}, steps);
+  if (!c.ok || decay->requires_grad()) return false;  // (refused by the Python path)
+  const double scale = scale_ == Py_None ? 1.0 / std::sqrt((double)t->dim_k) : c.number(scale_, -HUGE_VAL);
+  if (!c.ok || (float)scale == 0.f || !std::isfinite((float)scale)) return false;
+  t->decay = static_cast<const float*>(decay->data_ptr()), t->dones = static_cast<const float*>(data_or_null(dones));
+  t->state = static_cast<const float*>(data_or_null(state));
+  t->scale = (float)scale, t->state_scale = t->state_out_scale = 1.f, t->bf16 = q->scalar_type() == at::kBFloat16;
+  return true;
+}
+
+// The outputs: contiguous like v, and a state.
+at::Tensor attention_out(const at::Tensor& v, rlk_attention* t) {
+  at::Tensor out = policy_output(v.sizes(), v.scalar_type(), v);
+  const bool steps = v.dim() == 4;
+  t->out = {out.data_ptr(), out.stride(0), steps ? out.stride(1) : 0, out.stride(v.dim() - 2)};
+  return out;
+}
+
+// linear_attention(q, k, v, decay, dones, state, scale)
+PyObject* op_linear_attention(PyObject* const* a, Py_ssize_t n) {
+  if (n != 7 || correctness_warnings()) return decline();
+  PolicyCall c;
+  rlk_attention t = {};
+  const at::Tensor* v;
+  at::Tensor flags;
+  if (!attention_args(c, a[0], a[1], a[2], a[3], a[4], a[5], a[6], true, &t, &v, &flags)) return decline();
+  const size_t need = rlk_attention_workspace_bytes(t.num_envs, t.seq_len, t.heads, t.dim_k, t.dim_v);
+  if (!policy_scratch(c, &PolicyScratch::states, need, *v, &t.workspace, &t.workspace_bytes)) return decline();
+  at::Tensor out = attention_out(*v, &t), last = policy_output({t.num_envs, t.heads, t.dim_k, t.dim_v}, at::kFloat, *v);
+  t.state_out = static_cast<float*>(last.data_ptr());
+  return finish(rlk_linear_attention(&t, 1, c.stream()), "rlk_linear_attention", pair(out, last));
+}
+
+// linear_attention_step(q, k, v, decay, state, dones, scale, out_state)
+PyObject* op_linear_attention_step(PyObject* const* a, Py_ssize_t n) {
+  if (n != 8 || a[7] != Py_None || correctness_warnings()) return decline();
+  PolicyCall c;
+  rlk_attention t = {};
+  const at::Tensor* v;
+  at::Tensor flags;
+  if (!attention_args(c, a[0], a[1], a[2], a[3], a[5], a[4], a[6], false, &t, &v, &flags) || !t.state) return decline();
+  at::Tensor out = attention_out(*v, &t), next = policy_output({t.num_envs, t.heads, t.dim_k, t.dim_v}, at::kFloat, *v);
+  t.state_out = static_cast<float*>(next.data_ptr());
+  return finish(rlk_linear_attention_step(&t, c.stream()), "rlk_linear_attention_step", pair(out, next));
+}

@@ -67,23 +67,26 @@ def load():
 
 
 _BF16 = torch.bfloat16
+# Scratch memory, one of each kind per (device, stream): "sums" of the losses, whose head is zero between calls, and
+# "states" of sequences cut into segments.
 _workspaces: dict = {}
 
 
-def _workspace(dev: int, stream: int, need: int):
-    """Scratch memory of the current call: kept per (device, stream) and grown by doubling; a call being
-    captured into a graph gets memory of its own, kept for the life of the process."""
+def _workspace(kind: str, dev: int, stream: int, need: int):
+    """Scratch memory of the current call: kept per (device, stream), grown by doubling, zero-filled when made; a
+    call being captured into a graph gets memory of its own (zero-filled by a kernel the graph records), kept for
+    the life of the process."""
     if need == 0:
         return None, 0
+    device = torch.device("cuda", dev)
     if _native._capturing():
-        ws = torch.empty(need, dtype=torch.uint8, device=torch.device("cuda", dev))
+        ws = torch.zeros(need, dtype=torch.uint8, device=device)
         _native._captured.append(ws)
         return ws.data_ptr(), need
-    ws = _workspaces.get((dev, stream))
+    ws = _workspaces.get((kind, dev, stream))
     if ws is None or ws.numel() < need:
-        ws = torch.empty(max(need, 2 * ws.numel() if ws is not None else 0), dtype=torch.uint8,
-                         device=torch.device("cuda", dev))
-        _workspaces[(dev, stream)] = ws
+        ws = torch.zeros(max(need, 2 * ws.numel() if ws is not None else 0), dtype=torch.uint8, device=device)
+        _workspaces[(kind, dev, stream)] = ws
     return ws.data_ptr(), ws.numel()
 
 
@@ -124,7 +127,7 @@ def action_log_probs_backward(dev, stream, logits, actions, temperature, entropi
 
 
 def _terms(dev, stream, num_envs, old, advantages, ref, mask, clip, kl_coef, entropy_coef, per_row, loss, means):
-    ws, wsb = _workspace(dev, stream, (_lib or load()).rlk_policy_workspace_bytes(num_envs))
+    ws, wsb = _workspace("sums", dev, stream, (_lib or load()).rlk_policy_workspace_bytes(num_envs))
     low, high, dual = clip
     return PolicyTerms(old.data_ptr(), advantages.data_ptr(), _ptr(ref), _ptr(mask), low, high, dual, kl_coef,
                        entropy_coef, per_row, old.dtype is _BF16, loss.data_ptr(), means.data_ptr(), ws, wsb)
@@ -177,7 +180,7 @@ def linear_attention(dev, stream, decay, dones, passes):
     lib = _lib or load()
     e, t, h = passes[0].a.shape[:3]
     need = sum(lib.rlk_attention_workspace_bytes(e, t, h, p.a.shape[-1], p.y.shape[-1]) for p in passes)
-    ws, wsb = _workspace(dev, stream, need)
+    ws, wsb = _workspace("states", dev, stream, need)
     calls = (Attention * len(passes))(*(p.struct(decay, dones, ws, wsb) for p in passes))
     _native._check(lib.rlk_linear_attention(calls, len(passes), stream), "rlk_linear_attention")
 

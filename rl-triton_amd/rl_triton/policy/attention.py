@@ -185,6 +185,8 @@ def compute_linear_attention_step(
     else:
         assert out_state.get_device() == state.get_device() and out_state.dtype == torch.float32 and \
             out_state.shape == state.shape and out_state.is_contiguous(), "out_state must be a contiguous float32 tensor like state"
+        apart = abs(out_state.data_ptr() - state.data_ptr())
+        assert apart == 0 or apart >= 4 * state.numel(), "out_state overlaps state without being it"
     out = torch.empty(v.shape, dtype=v.dtype, device=v.device)
     if q.shape[0] and q.shape[1]:
         _native.linear_attention_step(decay.contiguous(), _dones(dones),
