@@ -112,7 +112,7 @@ __device__ __forceinline__ StepTerms step_terms(float lp, float old, float adv, 
 // With a mask these numbers come from count_kernel: a number per row, and per workgroup the sums of what
 // the mean divides by, which every workgroup that needs them adds up in the same order (whole numbers: exact).
 // ---------------------------------------------------------------------------------------
-constexpr int kCountBlocks = 256;
+constexpr int kCountBlocks = 512;
 
 struct Weights {
   const int64_t* parts;  // [kCountBlocks], or NULL: no mask
