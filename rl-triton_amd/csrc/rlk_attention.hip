@@ -38,8 +38,8 @@ struct Frag;
 template <>
 struct Frag<bf16> {
   bf16x8 x;
-  __device__ static Frag load(const bf16* p) { return {*reinterpret_cast<const bf16x8*>(p)}; }
-  __device__ static Frag load2(const bf16* p, const bf16* q) {
+  __device__ static Frag load(const char* p) { return {*reinterpret_cast<const bf16x8*>(p)}; }
+  __device__ static Frag load2(const char* p, const char* q) {
     union { u32x2 h[2]; bf16x8 v; } u;
     u.h[0] = *reinterpret_cast<const u32x2*>(p), u.h[1] = *reinterpret_cast<const u32x2*>(q);
     return {u.v};
@@ -54,8 +54,8 @@ struct Frag<bf16> {
 template <>
 struct Frag<float> {
   f32x4 lo, hi;
-  __device__ static Frag load(const float* p) { return load2(p, p + 4); }
-  __device__ static Frag load2(const float* p, const float* q) {
+  __device__ static Frag load(const char* p) { return load2(p, p + 16); }
+  __device__ static Frag load2(const char* p, const char* q) {
     return {*reinterpret_cast<const f32x4*>(p), *reinterpret_cast<const f32x4*>(q)};
   }
   __device__ static Frag from(f32x4 a, f32x4 b) { return {a, b}; }
@@ -112,29 +112,28 @@ struct Quad<float> {
 // x^n for n >= 0 from log2 x (x = 0: 1, 0, 0, ...).
 __device__ __forceinline__ float power(float log2x, int n) { return n == 0 ? 1.f : __builtin_amdgcn_exp2f(log2x * (float)n); }
 
+// A chunk in LDS, in bytes.  Accesses are a lane's offset, formed once, plus a constant: the offsets are made opaque, or the
+// compiler would fold the tiles' places (past the 64 KB that an instruction's own offset reaches) into an address of its own
+// for every access and hold them all.
 template <class E, int D>
-struct Tiles {
-  static constexpr int PAD = 16 / (int)sizeof(E);
-  E a[C][D + PAD];   // rows of a chunk
-  E b[C][D + PAD];
-  E bt[D * C];       // b and c transposed, at transposed(d, j)
-  E ct[D * C];
-  E p[C][C + PAD];   // (a_i . b_j) lambda^{i-j} same(j, i)
+struct Lds {
+  static constexpr int S = (int)sizeof(E), PAD = 16;
+  static constexpr int ROW = D * S + PAD, PROW = C * S + PAD, TROW = C * S;
+  static constexpr int BT = 0, CT = D * TROW;                // b and c transposed, at transposed(d, j)
+  static constexpr int A = 2 * D * TROW, B = A + C * ROW;    // rows of a and b
+  static constexpr int P = B + C * ROW;                      // (a_i . b_j) lambda^{i-j} same(j, i)
+  static constexpr int BYTES = P + C * PROW;
+  // Where a transposed tile holds row d, column j.  The 16-byte units of a row are exchanged with d's low bits: a write has
+  // lanes at every fourth row, a read at consecutive ones, and f takes all 8 values over either set, so both spread over
+  // all banks (with padded rows the writes met in an eighth of them: 20 of 75 us of a [64,1024,8,64] call).
+  __device__ static int transposed(int d, int j) {
+    const int f = (d & 7) ^ ((d >> 3) & 3);
+    return d * TROW + (((j * S / 16) ^ f) * 16) + j * S % 16;
+  }
 };
-
-// Where a transposed tile holds row d, column j.  The 16-byte units of a row are exchanged with d's low bits: a write has
-// lanes at every fourth row, a read at consecutive ones, and f takes all 8 values over either set, so both spread over
-// all banks (with padded rows the writes met in an eighth of them: 20 of 75 us of a [64,1024,8,64] call).
-template <class E>
-__device__ __forceinline__ int transposed(int d, int j) {
-  constexpr int UNIT = 16 / (int)sizeof(E);
-  const int f = (d & 7) ^ ((d >> 3) & 3);
-  return d * C + (((j / UNIT) ^ f) * UNIT) + j % UNIT;
-}
-template <class E>
-__device__ __forceinline__ Frag<E> load_transposed(const E* tile, int d, int j) {
-  if constexpr (sizeof(E) == 2) return Frag<E>::load(tile + transposed<E>(d, j));
-  else return Frag<E>::load2(tile + transposed<E>(d, j), tile + transposed<E>(d, j + 4));
+__device__ __forceinline__ int opaque(int x) {
+  asm("" : "+v"(x));
+  return x;
 }
 
 // One array's part of a chunk, held by a thread: R rows of 4 columns.
@@ -187,19 +186,17 @@ struct Part {
       }
     }
   }
-  template <int STRIDE>
-  __device__ __forceinline__ void put(E (*dst)[STRIDE]) const {
-    const int col = (threadIdx.x % GROUPS) * 4, row0 = (threadIdx.x / GROUPS) * R;
+  // to `at` and three rows on
+  __device__ __forceinline__ void put(char* at) const {
 #pragma unroll
-    for (int r = 0; r < R; ++r) x[r].store(&dst[row0 + r][col]);
+    for (int r = 0; r < R; ++r) x[r].store(reinterpret_cast<E*>(at + r * Lds<E, D>::ROW));
   }
   // as 4 rows of 4 consecutive elements
-  __device__ __forceinline__ void put_transposed(E* tile) const {
-    const int col = (threadIdx.x % GROUPS) * 4, row0 = (threadIdx.x / GROUPS) * R;
-    Quad<E>::template across<0>(x[0], x[1], x[2], x[3]).store(tile + transposed<E>(col, row0));
-    Quad<E>::template across<1>(x[0], x[1], x[2], x[3]).store(tile + transposed<E>(col + 1, row0));
-    Quad<E>::template across<2>(x[0], x[1], x[2], x[3]).store(tile + transposed<E>(col + 2, row0));
-    Quad<E>::template across<3>(x[0], x[1], x[2], x[3]).store(tile + transposed<E>(col + 3, row0));
+  __device__ __forceinline__ void put_transposed(char* tile, const int (&at)[4]) const {
+    Quad<E>::template across<0>(x[0], x[1], x[2], x[3]).store(reinterpret_cast<E*>(tile + at[0]));
+    Quad<E>::template across<1>(x[0], x[1], x[2], x[3]).store(reinterpret_cast<E*>(tile + at[1]));
+    Quad<E>::template across<2>(x[0], x[1], x[2], x[3]).store(reinterpret_cast<E*>(tile + at[2]));
+    Quad<E>::template across<3>(x[0], x[1], x[2], x[3]).store(reinterpret_cast<E*>(tile + at[3]));
   }
 };
 
@@ -241,7 +238,8 @@ struct Weighted<bf16> {
 // 0: any dims and alignment, element by element.
 template <class E, int D, int FORM, bool STATE>
 __global__ __launch_bounds__(4 * D, D == 64 && sizeof(E) == 4 ? 1 : 2) void walk_kernel(const Walks<E> walks) {
-  __shared__ __align__(16) Tiles<E, D> tiles;
+  typedef Lds<E, D> M;
+  __shared__ __align__(16) char lds[M::BYTES];
   constexpr int MT = D / 16, KK = D / 32;
   constexpr int SHARE = D / 64, TILES = 4 / SHARE;  // wavefronts that share 16 rows of p; tiles of p a wavefront at most
   const Walk<E>& w = walks.w[blockIdx.z];
@@ -329,13 +327,13 @@ __global__ __launch_bounds__(4 * D, D == 64 && sizeof(E) == 4 ? 1 : 2) void walk
 #pragma unroll
     for (int t = 0; t < 4; ++t) back[t] = power(lg, 16 * t + l16) * w.scale;
     // the steps after a row's own tile, in the operand that ends with it: never written again
-    if ((ti & 1) == 0) Quad<E>::of(f32x4{0.f, 0.f, 0.f, 0.f}).store(&tiles.p[16 * ti + l16][16 * (ti + 1) + 4 * l4]);
+    if ((ti & 1) == 0)
+      Quad<E>::of(f32x4{0.f, 0.f, 0.f, 0.f})
+          .store(reinterpret_cast<E*>(lds + M::P + (16 * ti + l16) * M::PROW + (16 * (ti + 1) + 4 * l4) * M::S));
   }
-  float onward[2][8];  // lambda^{C-j} of the steps j = 32 kk + 8 l4 + x
+  float onward[2];  // lambda^{C-j} of the steps j = 32 kk + 8 l4 + 7; the 7 before are lambda times the next
 #pragma unroll
-  for (int kk = 0; kk < 2; ++kk)
-#pragma unroll
-    for (int x = 0; x < 8; ++x) onward[kk][x] = power(lg, C - (32 * kk + 8 * l4 + x));
+  for (int kk = 0; kk < 2; ++kk) onward[kk] = power(lg, C - (32 * kk + 8 * l4 + 7));
   const float whole = power(lg, C);
 
   E* gy = nullptr;
@@ -346,10 +344,35 @@ __global__ __launch_bounds__(4 * D, D == 64 && sizeof(E) == 4 ? 1 : 2) void walk
          16 * wave + 4 * l4;
   }
 
+  // this lane's places in LDS
+  constexpr bool HALVES = sizeof(E) == 4;  // an operand of 8 elements is two 16-byte units; else the two chunk halves differ
+  const int col = (threadIdx.x % Part<E, D>::GROUPS) * 4, row0 = (threadIdx.x / Part<E, D>::GROUPS) * 4;
+  const int at_row = opaque(M::A + row0 * M::ROW + col * M::S);
+  const int at_col[4] = {opaque(M::transposed(col, row0)), opaque(M::transposed(col + 1, row0)), opaque(M::transposed(col + 2, row0)),
+                         opaque(M::transposed(col + 3, row0))};
+  const int at_a = opaque(M::A + (16 * ti + l16) * M::ROW + 8 * l4 * M::S);
+  const int at_b = opaque(M::B + (16 * (wave % SHARE) + l16) * M::ROW + 8 * l4 * M::S);
+  const int at_a2 = opaque(M::A + l16 * M::ROW + 4 * l4 * M::S);
+  const int at_p_put = opaque(M::P + (16 * ti + l16) * M::PROW + (16 * (wave % SHARE) + 4 * l4) * M::S);
+  const int at_p = opaque(M::P + l16 * M::PROW + 8 * l4 * M::S);
+  const int step2 = HALVES ? 4 : 32;
+  const int at_bt[2][2] = {{opaque(M::transposed(l16, 8 * l4)), opaque(M::transposed(l16, 8 * l4 + step2))},
+                           {opaque(M::transposed(16 + l16, 8 * l4)), opaque(M::transposed(16 + l16, 8 * l4 + step2))}};
+  const int at_ct[2] = {opaque(M::CT + M::transposed(16 * wave + l16, 8 * l4)), opaque(M::CT + M::transposed(16 * wave + l16, 8 * l4 + step2))};
+  // 8 elements of a transposed tile from column 32 kk on, `more` bytes further
+  auto load_t = [&](const int (&at)[2], int kk, int more) {
+    if constexpr (HALVES) return Frag<E>::load2(lds + at[0] + 32 * kk * M::S + more, lds + at[1] + 32 * kk * M::S + more);
+    else return Frag<E>::load(lds + at[kk] + more);
+  };
+
   bool crossed = false;  // a cut anywhere in the segment
   // One chunk.  PLAIN: whole, without a cut, and not the one that a state leaves the sequence with.
   auto chunk = [&](auto plain, int64_t s0, int L, uint64_t cuts, bool end) {
     constexpr bool PLAIN = decltype(plain)::value;
+    // float32 operands are twice the registers: loads of more than the next two are kept from moving up
+    auto apart = [] {
+      if constexpr (sizeof(E) == 4 || D == 128) __builtin_amdgcn_sched_barrier(0);
+    };
     // The lane's place again, for what only other chunks need: as a new value to the compiler, which would else compute
     // all of it once before the walk and hold it in a hundred registers.
     int v16 = l16, v4 = l4;
@@ -361,27 +384,33 @@ __global__ __launch_bounds__(4 * D, D == 64 && sizeof(E) == 4 ? 1 : 2) void walk
       pc.template clip<VEC>(dc, L);
     }
     if constexpr (!STATE) {
-      pa.put(tiles.a);
-      pb.put(tiles.b);
+      pa.put(lds + at_row);
+      pb.put(lds + at_row + (M::B - M::A));
     }
-    pb.put_transposed(tiles.bt);
-    pc.put_transposed(tiles.ct);
+    pb.put_transposed(lds, at_col);
+    pc.put_transposed(lds + M::CT, at_col);
     __syncthreads();
     if (s0 + C < last) fetch_all(s0 + C);  // in flight while this chunk is worked on
 
     if constexpr (!STATE) {
-      Frag<E> fa[KK];
+      f32x4 pts[TILES];
 #pragma unroll
-      for (int kk = 0; kk < KK; ++kk)
-        if (FULL || 32 * kk < da) fa[kk] = Frag<E>::load(&tiles.a[16 * ti + l16][32 * kk + 8 * l4]);
+      for (int u = 0; u < TILES; ++u) pts[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk) {
+        if (!FULL && 32 * kk >= da) continue;
+        const Frag<E> fa = Frag<E>::load(lds + at_a + 32 * kk * M::S);
+#pragma unroll
+        for (int u = 0; u < TILES; ++u) {
+          const int jt = wave % SHARE + SHARE * u;
+          if (jt <= ti) pts[u] = mma(Frag<E>::load(lds + at_b + 16 * SHARE * u * M::ROW + 32 * kk * M::S), fa, pts[u]);
+        }
+      }
 #pragma unroll
       for (int u = 0; u < TILES; ++u) {
         const int jt = wave % SHARE + SHARE * u;
         if (jt > ti) continue;
-        f32x4 pt = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int kk = 0; kk < KK; ++kk)
-          if (FULL || 32 * kk < da) pt = mma(Frag<E>::load(&tiles.b[16 * jt + l16][32 * kk + 8 * l4]), fa[kk], pt);
+        f32x4 pt = pts[u];
         pt *= among[u];
         if (!PLAIN && cuts != 0) {
           // two steps belong together when as many cuts lie before or at each of them
@@ -390,14 +419,14 @@ __global__ __launch_bounds__(4 * D, D == 64 && sizeof(E) == 4 ? 1 : 2) void walk
           for (int r = 0; r < 4; ++r)
             if (__popcll(cuts & (((uint64_t)2 << (16 * jt + 4 * v4 + r)) - 1)) != before) pt[r] = 0.f;
         }
-        Quad<E>::of(pt).store(&tiles.p[16 * ti + l16][16 * jt + 4 * l4]);
+        Quad<E>::of(pt).store(reinterpret_cast<E*>(lds + at_p_put + 16 * SHARE * u * M::S));
       }
       __syncthreads();
     }
 
     Frag<E> fc[2];
 #pragma unroll
-    for (int kk = 0; kk < 2; ++kk) fc[kk] = load_transposed(tiles.ct, 16 * wave + l16, 32 * kk + 8 * l4);
+    for (int kk = 0; kk < 2; ++kk) fc[kk] = load_t(at_ct, kk, 0);
     const bool mine = FULL || 16 * wave < dc;  // else this wavefront only helps with p
 
     if (!STATE && mine) {
@@ -411,8 +440,9 @@ __global__ __launch_bounds__(4 * D, D == 64 && sizeof(E) == 4 ? 1 : 2) void walk
         const Frag<E> fu = Frag<E>::from(U[2 * kk], U[2 * kk + 1]);
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
-          const E* row = &tiles.a[16 * t + l16][32 * kk + 4 * l4];
-          y[t] = mma(fu, Frag<E>::load2(row, row + 16), y[t]);
+          const char* row = lds + at_a2 + 16 * t * M::ROW + 32 * kk * M::S;
+          y[t] = mma(fu, Frag<E>::load2(row, row + 16 * M::S), y[t]);
+          if (t & 1) apart();
         }
       }
       // the first step that the state does not reach
@@ -426,7 +456,10 @@ __global__ __launch_bounds__(4 * D, D == 64 && sizeof(E) == 4 ? 1 : 2) void walk
       for (int kk = 0; kk < 2; ++kk)
 #pragma unroll
         for (int t = 2 * kk; t < 4; ++t)  // (rows before the steps 32 kk + 0..31 have none of them)
-          y[t] = mma(fc[kk], Frag<E>::load(&tiles.p[16 * t + l16][32 * kk + 8 * l4]), y[t]);
+        {
+          y[t] = mma(fc[kk], Frag<E>::load(lds + at_p + 16 * t * M::PROW + 32 * kk * M::S), y[t]);
+          if (t & 1) apart();
+        }
       const int j = 16 * wave + 4 * l4;
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
@@ -457,15 +490,23 @@ __global__ __launch_bounds__(4 * D, D == 64 && sizeof(E) == 4 ? 1 : 2) void walk
 #pragma unroll
       for (int kk = 0; kk < 2; ++kk) {
         float f[8];
+        f[7] = onward[kk];
 #pragma unroll
-        for (int x = 0; x < 8; ++x) {
-          const int j = 32 * kk + 8 * v4 + x;
-          f[x] = PLAIN ? onward[kk][x] : j >= from && j < L ? power(lg, reach - j) : 0.f;
+        for (int x = 6; x >= 0; --x) f[x] = f[x + 1] * lambda;
+        if constexpr (!PLAIN) {
+#pragma unroll
+          for (int x = 0; x < 8; ++x) {
+            const int j = 32 * kk + 8 * v4 + x;
+            f[x] = j >= from && j < L ? power(lg, reach - j) : 0.f;
+          }
         }
         const Weighted<E> wc(fc[kk], f);
 #pragma unroll
         for (int m = 0; m < MT; ++m)
-          if (FULL || 16 * m < da) U[m] = wc.mma_with(load_transposed(tiles.bt, 16 * m + l16, 32 * kk + 8 * l4), U[m]);
+        {
+          if (FULL || 16 * m < da) U[m] = wc.mma_with(load_t(at_bt[m & 1], kk, 16 * (m & ~1) * M::TROW), U[m]);
+          if (m & 1) apart();
+        }
       }
     }
   };
