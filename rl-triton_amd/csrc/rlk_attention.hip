@@ -587,7 +587,7 @@ template <class E>
 int walk_impl(const rlk_attention* c, int count, hipStream_t s) {
   Walks<E> k = {};
   k.num_envs = c->num_envs, k.seq_len = c->seq_len, k.heads = (int)c->heads, k.decay = c->decay, k.dones = c->dones;
-  const SegmentPlan plan = plan_segments(c->num_envs * c->heads, c->seq_len);
+  const SegmentPlan plan = plan_segments(c->num_envs * c->heads, c->seq_len, c->dim_k <= 64 && c->dim_v <= 64);
   k.segs = plan.segs, k.seg_len = plan.seg_len;
   bool vec = true, small = true;
   int full = 0;  // the one size that all dims have, or -1
@@ -628,7 +628,7 @@ extern "C" {
 
 size_t rlk_attention_workspace_bytes(int64_t num_envs, int64_t seq_len, int64_t heads, int64_t dim_k, int64_t dim_v) {
   if (num_envs <= 0 || seq_len <= 0 || heads <= 0 || dim_k <= 0 || dim_v <= 0) return 0;
-  const SegmentPlan plan = plan_segments(num_envs * heads, seq_len);
+  const SegmentPlan plan = plan_segments(num_envs * heads, seq_len, dim_k <= 64 && dim_v <= 64);
   return plan.segs <= 1 ? 0 : (size_t)num_envs * heads * plan.segs * (dim_k * dim_v + 1) * sizeof(float);
 }
 

@@ -56,12 +56,12 @@ struct SegmentPlan {
   int64_t seg_len;  // a multiple of 64
 };
 
-// Segments: none where the (environment, head) pairs fill the GPU by themselves; else as many as make two
-// workgroups per CU, of at least 4 chunks (a segment's k and v are read twice, and its state is written and
-// read once per segment).
-inline SegmentPlan plan_segments(int64_t rows, int64_t T) {
+// Segments: none where the (environment, head) pairs fill the GPU by themselves; else as many as make one round of
+// the workgroups that it holds (two per CU for dims of up to 64, one beyond), of at least 4 chunks (a segment's k and v are read
+// twice, and its state is written and read once per segment).
+inline SegmentPlan plan_segments(int64_t rows, int64_t T, bool small) {
   const int64_t cus = device_cus(), chunks = (T + 63) / 64;
-  int64_t segs = rows >= cus ? 1 : 2 * cus / rows;
+  int64_t segs = rows >= cus ? 1 : (small ? 2 : 1) * cus / rows;
   if (segs > chunks / 4) segs = chunks / 4;
   if (segs < 1) segs = 1;
   const int64_t per = (chunks + segs - 1) / segs;
