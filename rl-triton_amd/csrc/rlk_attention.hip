@@ -121,8 +121,13 @@ struct Lds {
   static constexpr int ROW = D * S + PAD, PROW = C * S + PAD, TROW = C * S;
   static constexpr int BT = 0, CT = D * TROW;                // b and c transposed, at transposed(d, j)
   static constexpr int A = 2 * D * TROW, B = A + C * ROW;    // rows of a and b
-  static constexpr int P = B + C * ROW;                      // (a_i . b_j) lambda^{i-j} same(j, i)
-  static constexpr int BYTES = P + C * PROW;
+  static constexpr int CHUNK = B + C * ROW;
+  // Two chunks where they fit (160 KB a CU; two workgroups of it for bfloat16 dims of up to 64): the next one is put down
+  // while this one is worked on.
+  static constexpr int P_BYTES = C * PROW;                   // (a_i . b_j) lambda^{i-j} same(j, i)
+  static constexpr int CHUNKS = 2 * CHUNK + P_BYTES <= 160 * 1024 ? 2 : 1;
+  static constexpr int P = CHUNKS * CHUNK;
+  static constexpr int BYTES = P + P_BYTES;
   // Where a transposed tile holds row d, column j.  The 16-byte units of a row are exchanged with d's low bits: a write has
   // lanes at every fourth row, a read at consecutive ones, and f takes all 8 values over either set, so both spread over
   // all banks (with padded rows the writes met in an eighth of them: 20 of 75 us of a [64,1024,8,64] call).
@@ -360,16 +365,36 @@ __global__ __launch_bounds__(4 * D, D == 64 && sizeof(E) == 4 ? 1 : 2) void walk
                            {opaque(M::transposed(16 + l16, 8 * l4)), opaque(M::transposed(16 + l16, 8 * l4 + step2))}};
   const int at_ct[2] = {opaque(M::CT + M::transposed(16 * wave + l16, 8 * l4)), opaque(M::CT + M::transposed(16 * wave + l16, 8 * l4 + step2))};
   // 8 elements of a transposed tile from column 32 kk on, `more` bytes further
-  auto load_t = [&](const int (&at)[2], int kk, int more) {
-    if constexpr (HALVES) return Frag<E>::load2(lds + at[0] + 32 * kk * M::S + more, lds + at[1] + 32 * kk * M::S + more);
-    else return Frag<E>::load(lds + at[kk] + more);
+  auto load_t = [&](const char* tile, const int (&at)[2], int kk, int more) {
+    if constexpr (HALVES) return Frag<E>::load2(tile + at[0] + 32 * kk * M::S + more, tile + at[1] + 32 * kk * M::S + more);
+    else return Frag<E>::load(tile + at[kk] + more);
   };
 
   bool crossed = false;  // a cut anywhere in the segment
+  // Puts the fetched chunk of the steps from s0 on down and has the one after it fetched; its cuts come back.
+  auto put_down = [&](int64_t s0, int buffer) {
+    const int L = (int)(last - s0 < C ? last - s0 : C);
+    const uint64_t found = __ballot(lane < L && done != 0.f && (reverse || s0 + lane > 0));
+    if (!FULL || L < C) {
+      if constexpr (!STATE) pa.template clip<VEC>(da, L);
+      pb.template clip<VEC>(da, L);
+      pc.template clip<VEC>(dc, L);
+    }
+    char* to = lds + buffer;
+    if constexpr (!STATE) {
+      pa.put(to + at_row);
+      pb.put(to + at_row + (M::B - M::A));
+    }
+    pb.put_transposed(to, at_col);
+    pc.put_transposed(to + M::CT, at_col);
+    if (s0 + C < last) fetch_all(s0 + C);
+    return found;
+  };
+
   // One chunk.  PLAIN: whole, without a cut, and not the one that a state leaves the sequence with.
-  auto chunk = [&](auto plain, int64_t s0, int L, uint64_t cuts, bool end) {
+  auto chunk = [&](auto plain, int64_t s0, int L, uint64_t cuts, bool end, const char* tile) {
     constexpr bool PLAIN = decltype(plain)::value;
-    // float32 operands are twice the registers: loads of more than the next two are kept from moving up
+    // operands that take more registers: loads of more than the next two are kept from moving up
     auto apart = [] {
       if constexpr (sizeof(E) == 4 || D == 128) __builtin_amdgcn_sched_barrier(0);
     };
@@ -377,21 +402,6 @@ __global__ __launch_bounds__(4 * D, D == 64 && sizeof(E) == 4 ? 1 : 2) void walk
     // all of it once before the walk and hold it in a hundred registers.
     int v16 = l16, v4 = l4;
     if constexpr (!PLAIN) asm volatile("" : "+v"(v16), "+v"(v4));
-    __syncthreads();  // the chunk before has been read
-    if (!PLAIN || !FULL) {
-      if constexpr (!STATE) pa.template clip<VEC>(da, L);
-      pb.template clip<VEC>(da, L);
-      pc.template clip<VEC>(dc, L);
-    }
-    if constexpr (!STATE) {
-      pa.put(lds + at_row);
-      pb.put(lds + at_row + (M::B - M::A));
-    }
-    pb.put_transposed(lds, at_col);
-    pc.put_transposed(lds + M::CT, at_col);
-    __syncthreads();
-    if (s0 + C < last) fetch_all(s0 + C);  // in flight while this chunk is worked on
-
     if constexpr (!STATE) {
       f32x4 pts[TILES];
 #pragma unroll
@@ -399,11 +409,11 @@ __global__ __launch_bounds__(4 * D, D == 64 && sizeof(E) == 4 ? 1 : 2) void walk
 #pragma unroll
       for (int kk = 0; kk < KK; ++kk) {
         if (!FULL && 32 * kk >= da) continue;
-        const Frag<E> fa = Frag<E>::load(lds + at_a + 32 * kk * M::S);
+        const Frag<E> fa = Frag<E>::load(tile + at_a + 32 * kk * M::S);
 #pragma unroll
         for (int u = 0; u < TILES; ++u) {
           const int jt = wave % SHARE + SHARE * u;
-          if (jt <= ti) pts[u] = mma(Frag<E>::load(lds + at_b + 16 * SHARE * u * M::ROW + 32 * kk * M::S), fa, pts[u]);
+          if (jt <= ti) pts[u] = mma(Frag<E>::load(tile + at_b + 16 * SHARE * u * M::ROW + 32 * kk * M::S), fa, pts[u]);
         }
       }
 #pragma unroll
@@ -426,7 +436,7 @@ __global__ __launch_bounds__(4 * D, D == 64 && sizeof(E) == 4 ? 1 : 2) void walk
 
     Frag<E> fc[2];
 #pragma unroll
-    for (int kk = 0; kk < 2; ++kk) fc[kk] = load_t(at_ct, kk, 0);
+    for (int kk = 0; kk < 2; ++kk) fc[kk] = load_t(tile, at_ct, kk, 0);
     const bool mine = FULL || 16 * wave < dc;  // else this wavefront only helps with p
 
     if (!STATE && mine) {
@@ -440,7 +450,7 @@ __global__ __launch_bounds__(4 * D, D == 64 && sizeof(E) == 4 ? 1 : 2) void walk
         const Frag<E> fu = Frag<E>::from(U[2 * kk], U[2 * kk + 1]);
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
-          const char* row = lds + at_a2 + 16 * t * M::ROW + 32 * kk * M::S;
+          const char* row = tile + at_a2 + 16 * t * M::ROW + 32 * kk * M::S;
           y[t] = mma(fu, Frag<E>::load2(row, row + 16 * M::S), y[t]);
           if (t & 1) apart();
         }
@@ -504,20 +514,27 @@ __global__ __launch_bounds__(4 * D, D == 64 && sizeof(E) == 4 ? 1 : 2) void walk
 #pragma unroll
         for (int m = 0; m < MT; ++m)
         {
-          if (FULL || 16 * m < da) U[m] = wc.mma_with(load_t(at_bt[m & 1], kk, 16 * (m & ~1) * M::TROW), U[m]);
+          if (FULL || 16 * m < da) U[m] = wc.mma_with(load_t(tile, at_bt[m & 1], kk, 16 * (m & ~1) * M::TROW), U[m]);
           if (m & 1) apart();
         }
       }
     }
   };
 
+  int buffer = 0;
+  uint64_t cuts = put_down(first, 0);
+  __syncthreads();
   for (int64_t s0 = first; s0 < last; s0 += C) {
     const int L = (int)(last - s0 < C ? last - s0 : C);
     const bool end = !reverse && s0 + C >= T;
-    const uint64_t cuts = __ballot(lane < L && done != 0.f && (reverse || s0 + lane > 0));
     crossed |= cuts != 0;
-    if (L == C && cuts == 0 && !end) chunk(std::true_type{}, s0, L, cuts, end);
-    else chunk(std::false_type{}, s0, L, cuts, end);
+    if (L == C && cuts == 0 && !end) chunk(std::true_type{}, s0, L, cuts, end, lds + buffer);
+    else chunk(std::false_type{}, s0, L, cuts, end, lds + buffer);
+    if (s0 + C >= last) break;
+    if constexpr (M::CHUNKS == 2) buffer ^= M::CHUNK;
+    else __syncthreads();  // the chunk has been read
+    cuts = put_down(s0 + C, buffer);
+    __syncthreads();
   }
 
   float* out = nullptr;
