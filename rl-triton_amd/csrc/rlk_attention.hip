@@ -235,6 +235,24 @@ struct Weighted<bf16> {
   __device__ f32x4 mma_with(const Frag<bf16>& a, f32x4 acc) const { return mma(a, hi, mma(a, lo, acc)); }
 };
 
+// Which walk of which environment and head a workgroup takes.  Workgroups go round the 8 XCDs, so the walks over the same
+// arrays (a backward pass's three) are 8 apart: on one XCD, one after the other, where they find what the others
+// have read in its L2.
+struct Place {
+  int walk, head;
+  int64_t env;
+  bool there;
+  template <class W>
+  __device__ explicit Place(const W& walks) {
+    const uint32_t x = blockIdx.x, count = (uint32_t)walks.count;
+    const uint32_t eh = x / (8 * count) * 8 + x % 8;
+    walk = (int)(x / 8 % count);
+    head = (int)(eh % (uint32_t)walks.heads);
+    env = eh / (uint32_t)walks.heads;
+    there = env < walks.num_envs;
+  }
+};
+
 // The walk over a segment.  STATE: only the state at its end, from zero, for the segments after it.
 //
 // Wavefront w owns the columns 16 w .. 16 w + 15 of c.  Everything a whole chunk without a cut needs of the
@@ -247,9 +265,11 @@ __global__ __launch_bounds__(4 * D, D == 64 && sizeof(E) == 4 ? 1 : 2) void walk
   __shared__ __align__(16) char lds[M::BYTES];
   constexpr int MT = D / 16, KK = D / 32;
   constexpr int SHARE = D / 64, TILES = 4 / SHARE;  // wavefronts that share 16 rows of p; tiles of p a wavefront at most
-  const Walk<E>& w = walks.w[blockIdx.z];
-  const int head = blockIdx.x % walks.heads, seg = blockIdx.y;
-  const int64_t env = blockIdx.x / walks.heads, T = walks.seq_len;
+  const Place place(walks);
+  if (!place.there) return;
+  const Walk<E>& w = walks.w[place.walk];
+  const int head = place.head, seg = blockIdx.y;
+  const int64_t env = place.env, T = walks.seq_len;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l16 = lane & 15, l4 = lane >> 4;
   constexpr bool VEC = FORM > 0, FULL = FORM == 2;
   const int da = FULL ? D : w.da, dc = FULL ? D : w.dc;
@@ -579,7 +599,8 @@ __global__ __launch_bounds__(256) void join_kernel(const Walks<E> walks) {
 
 template <class E, int D, int FORM>
 int launch_walks(const Walks<E>& k, int count, hipStream_t s) {
-  const dim3 grid((unsigned)(k.num_envs * k.heads), (unsigned)k.segs, (unsigned)count);
+  const unsigned rows = (unsigned)(k.num_envs * k.heads);
+  const dim3 grid((rows + 7) / 8 * 8 * (unsigned)count, (unsigned)k.segs);
   if (k.segs > 1) {
     dim3 g = grid;
     g.y = (unsigned)k.segs - 1;
@@ -587,7 +608,7 @@ int launch_walks(const Walks<E>& k, int count, hipStream_t s) {
     if (hipGetLastError() != hipSuccess) return RLK_ERR_LAUNCH;
     int most = 0;
     for (int i = 0; i < count; ++i) most = most < k.w[i].da * k.w[i].dc ? k.w[i].da * k.w[i].dc : most;
-    join_kernel<E><<<dim3(grid.x, (unsigned)(most + 255) / 256, (unsigned)count), dim3(256), 0, s>>>(k);
+    join_kernel<E><<<dim3(rows, (unsigned)(most + 255) / 256, (unsigned)count), dim3(256), 0, s>>>(k);
     if (hipGetLastError() != hipSuccess) return RLK_ERR_LAUNCH;
   }
   walk_kernel<E, D, FORM, false><<<grid, dim3(4 * D), 0, s>>>(k);
@@ -603,7 +624,7 @@ bool quads(const Sequence<E>& x, int dim) {
 template <class E>
 int walk_impl(const rlk_attention* c, int count, hipStream_t s) {
   Walks<E> k = {};
-  k.num_envs = c->num_envs, k.seq_len = c->seq_len, k.heads = (int)c->heads, k.decay = c->decay, k.dones = c->dones;
+  k.count = count, k.num_envs = c->num_envs, k.seq_len = c->seq_len, k.heads = (int)c->heads, k.decay = c->decay, k.dones = c->dones;
   const SegmentPlan plan = plan_segments(c->num_envs * c->heads, c->seq_len, c->dim_k <= 64 && c->dim_v <= 64);
   k.segs = plan.segs, k.seg_len = plan.seg_len;
   bool vec = true, small = true;

@@ -6,8 +6,8 @@
 
 namespace rlk {
 
-// One workgroup of 256 per (environment, head): as many as a launch's 2^32 - 1 work-items allow.
-constexpr int64_t kMaxGrid = (int64_t{1} << 24) - 1;
+// (environment, head) pairs a launch takes: three workgroups of 512 each stay below its 2^32 - 1 work-items.
+constexpr int64_t kMaxGrid = (int64_t{1} << 21) - 8;
 
 template <class E>
 struct Sequence {
@@ -32,7 +32,7 @@ template <class E>
 struct Walks {
   Walk<E> w[3];
   int64_t num_envs, seq_len, seg_len;
-  int heads, segs;
+  int count, heads, segs;
   const float *decay, *dones;
 };
 
