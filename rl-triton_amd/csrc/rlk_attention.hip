@@ -250,6 +250,7 @@ struct Place {
     head = (int)(eh % (uint32_t)walks.heads);
     env = eh / (uint32_t)walks.heads;
     there = env < walks.num_envs;
+    env += walks.first_env;
   }
 };
 
@@ -485,8 +486,7 @@ __global__ __launch_bounds__(4 * D, D == 64 && sizeof(E) == 4 ? 1 : 2) void walk
 #pragma unroll
       for (int kk = 0; kk < 2; ++kk)
 #pragma unroll
-        for (int t = 2 * kk; t < 4; ++t)  // (rows before the steps 32 kk + 0..31 have none of them)
-        {
+        for (int t = 2 * kk; t < 4; ++t) {  // (rows before the steps 32 kk + 0..31 have none of them)
           y[t] = mma(fc[kk], Frag<E>::load(lds + at_p + 16 * t * M::PROW + 32 * kk * M::S), y[t]);
           if (t & 1) apart();
         }
@@ -532,8 +532,7 @@ __global__ __launch_bounds__(4 * D, D == 64 && sizeof(E) == 4 ? 1 : 2) void walk
         }
         const Weighted<E> wc(fc[kk], f);
 #pragma unroll
-        for (int m = 0; m < MT; ++m)
-        {
+        for (int m = 0; m < MT; ++m) {
           if (FULL || 16 * m < da) U[m] = wc.mma_with(load_t(tile, at_bt[m & 1], kk, 16 * (m & ~1) * M::TROW), U[m]);
           if (m & 1) apart();
         }
@@ -581,7 +580,7 @@ template <class E>
 __global__ __launch_bounds__(256) void join_kernel(const Walks<E> walks) {
   const Walk<E>& w = walks.w[blockIdx.z];
   const int n = w.da * w.dc;
-  const int64_t eh = blockIdx.x;
+  const int64_t eh = walks.first_env * walks.heads + blockIdx.x;
   const int i = blockIdx.y * 256 + threadIdx.x;
   if (i >= n) return;
   float u = 0.f;
@@ -598,21 +597,22 @@ __global__ __launch_bounds__(256) void join_kernel(const Walks<E> walks) {
 }
 
 template <class E, int D, int FORM>
-int launch_walks(const Walks<E>& k, int count, hipStream_t s) {
-  const unsigned rows = (unsigned)(k.num_envs * k.heads);
-  const dim3 grid((rows + 7) / 8 * 8 * (unsigned)count, (unsigned)k.segs);
-  if (k.segs > 1) {
-    dim3 g = grid;
-    g.y = (unsigned)k.segs - 1;
-    walk_kernel<E, D, FORM, true><<<g, dim3(4 * D), 0, s>>>(k);
-    if (hipGetLastError() != hipSuccess) return RLK_ERR_LAUNCH;
-    int most = 0;
-    for (int i = 0; i < count; ++i) most = most < k.w[i].da * k.w[i].dc ? k.w[i].da * k.w[i].dc : most;
-    join_kernel<E><<<dim3(rows, (unsigned)(most + 255) / 256, (unsigned)count), dim3(256), 0, s>>>(k);
+int launch_walks(Walks<E> k, int count, hipStream_t s) {
+  const int64_t envs = k.num_envs, most = kMaxPairs / k.heads;
+  for (k.first_env = 0; k.first_env < envs; k.first_env += most) {
+    k.num_envs = envs - k.first_env < most ? envs - k.first_env : most;
+    const unsigned rows = (unsigned)(k.num_envs * k.heads);
+    const dim3 grid((rows + 7) / 8 * 8 * (unsigned)count, (unsigned)k.segs);
+    if (k.segs > 1) {
+      walk_kernel<E, D, FORM, true><<<dim3(grid.x, grid.y - 1), dim3(4 * D), 0, s>>>(k);
+      int most_state = 0;
+      for (int i = 0; i < count; ++i) most_state = most_state < k.w[i].da * k.w[i].dc ? k.w[i].da * k.w[i].dc : most_state;
+      join_kernel<E><<<dim3(rows, (unsigned)(most_state + 255) / 256, (unsigned)count), dim3(256), 0, s>>>(k);
+    }
+    walk_kernel<E, D, FORM, false><<<grid, dim3(4 * D), 0, s>>>(k);
     if (hipGetLastError() != hipSuccess) return RLK_ERR_LAUNCH;
   }
-  walk_kernel<E, D, FORM, false><<<grid, dim3(4 * D), 0, s>>>(k);
-  return hipGetLastError() == hipSuccess ? RLK_OK : RLK_ERR_LAUNCH;
+  return RLK_OK;
 }
 
 template <class E>
@@ -679,7 +679,7 @@ int rlk_linear_attention(const rlk_attention* calls, int count, void* stream) {
       return RLK_ERR_INVALID_ARGUMENT;
   }
   if (calls->num_envs == 0 || calls->heads == 0 || calls->seq_len == 0) return RLK_OK;
-  if (calls->num_envs * calls->heads > kMaxGrid || calls->seq_len > (int64_t{1} << 30)) return RLK_ERR_INVALID_ARGUMENT;
+  if (calls->heads > kMaxPairs || calls->seq_len > (int64_t{1} << 30)) return RLK_ERR_INVALID_ARGUMENT;
   const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   return calls->bf16 ? walk_impl<bf16>(calls, count, s) : walk_impl<float>(calls, count, s);
 }

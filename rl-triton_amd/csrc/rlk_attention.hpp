@@ -6,8 +6,9 @@
 
 namespace rlk {
 
-// (environment, head) pairs a launch takes: three workgroups of 512 each stay below its 2^32 - 1 work-items.
-constexpr int64_t kMaxGrid = (int64_t{1} << 21) - 8;
+// (environment, head) pairs of one launch, whose work-items are at most 2^32 - 1 (three workgroups of 512 a pair); more
+// environments go in further launches.
+constexpr int64_t kMaxPairs = (int64_t{1} << 21) - 8;
 
 template <class E>
 struct Sequence {
@@ -32,6 +33,7 @@ template <class E>
 struct Walks {
   Walk<E> w[3];
   int64_t num_envs, seq_len, seg_len;
+  int64_t first_env;  // of this launch, which has num_envs of them
   int count, heads, segs;
   const float *decay, *dones;
 };

@@ -10,13 +10,13 @@ namespace {
 constexpr int kNT = 256;
 
 template <class E, int LANES, bool VEC>  // LANES lanes cover a row of the state in quads
-__global__ __launch_bounds__(kNT) void step_kernel(const Walk<E> w, int heads, const float* __restrict__ decay,
+__global__ __launch_bounds__(kNT) void step_kernel(const Walk<E> w, int heads, int64_t first, const float* __restrict__ decay,
                                                    const float* __restrict__ dones) {
   constexpr int ROWS = kNT / LANES;
   __shared__ float qs[128], ks[128];
   __shared__ float4 part[ROWS][LANES];
-  const int head = blockIdx.x % heads, tid = threadIdx.x;
-  const int64_t env = blockIdx.x / heads, eh = blockIdx.x;
+  const int64_t eh = first + blockIdx.x, env = eh / heads;
+  const int head = (int)(eh - env * heads), tid = threadIdx.x;
   const int lane = tid % LANES, row0 = tid / LANES, j = lane * 4;
   if (tid < w.da) {
     qs[tid] = load_one(w.a.data + env * w.a.env_stride + head * w.a.head_stride + tid);
@@ -77,16 +77,20 @@ int step_impl(const rlk_attention& c, hipStream_t s) {
   w.a = sequence<const E>(c.q), w.b = sequence<const E>(c.k), w.c = sequence<const E>(c.v), w.y = sequence<E>(c.out);
   w.da = (int)c.dim_k, w.dc = (int)c.dim_v, w.state = c.state, w.state_out = c.state_out, w.scale = c.scale;
   const bool vec = c.dim_v % 4 == 0 && ((reinterpret_cast<uintptr_t>(c.state) | reinterpret_cast<uintptr_t>(c.state_out)) & 15u) == 0;
-  const dim3 grid((unsigned)(c.num_envs * c.heads)), block(kNT);
   const int heads = (int)c.heads;
-  if (c.dim_v <= 64) {
-    if (vec) step_kernel<E, 16, true><<<grid, block, 0, s>>>(w, heads, c.decay, c.dones);
-    else step_kernel<E, 16, false><<<grid, block, 0, s>>>(w, heads, c.decay, c.dones);
-  } else {
-    if (vec) step_kernel<E, 32, true><<<grid, block, 0, s>>>(w, heads, c.decay, c.dones);
-    else step_kernel<E, 32, false><<<grid, block, 0, s>>>(w, heads, c.decay, c.dones);
+  const int64_t pairs = c.num_envs * c.heads, most = int64_t{1} << 23;  // (of one launch: 2^31 work-items)
+  for (int64_t first = 0; first < pairs; first += most) {
+    const dim3 grid((unsigned)(pairs - first < most ? pairs - first : most)), block(kNT);
+    if (c.dim_v <= 64) {
+      if (vec) step_kernel<E, 16, true><<<grid, block, 0, s>>>(w, heads, first, c.decay, c.dones);
+      else step_kernel<E, 16, false><<<grid, block, 0, s>>>(w, heads, first, c.decay, c.dones);
+    } else {
+      if (vec) step_kernel<E, 32, true><<<grid, block, 0, s>>>(w, heads, first, c.decay, c.dones);
+      else step_kernel<E, 32, false><<<grid, block, 0, s>>>(w, heads, first, c.decay, c.dones);
+    }
+    if (hipGetLastError() != hipSuccess) return RLK_ERR_LAUNCH;
   }
-  return hipGetLastError() == hipSuccess ? RLK_OK : RLK_ERR_LAUNCH;
+  return RLK_OK;
 }
 
 }  // namespace
@@ -97,7 +101,7 @@ using namespace rlk;
 extern "C" int rlk_linear_attention_step(const rlk_attention* call, void* stream) {
   if (!call || !valid_attention(*call)) return RLK_ERR_INVALID_ARGUMENT;
   if (call->num_envs == 0 || call->heads == 0) return RLK_OK;
-  if (!call->state || !call->state_out || call->num_envs * call->heads > kMaxGrid) return RLK_ERR_INVALID_ARGUMENT;
+  if (!call->state || !call->state_out || call->heads > 0x7fffffff) return RLK_ERR_INVALID_ARGUMENT;
   const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   return call->bf16 ? step_impl<bf16>(*call, s) : step_impl<float>(*call, s);
 }

@@ -206,6 +206,26 @@ def test_a_cut_state_has_no_part():
     assert bool(o.isfinite().all()) and bool(new.isfinite().all())
 
 
+def test_more_pairs_than_a_launch_takes():
+    """Two million sequences of two steps, nine million single steps: several launches over ranges of environments.  Two
+    products and a sum a result: 8 u of the sizes."""
+    E, g = (1 << 21) + 77, torch.Generator(device="cuda").manual_seed(1)
+    n = lambda *s: torch.randn(s, generator=g, device="cuda")  # noqa: E731
+    q, k, v, s = n(E, 2, 1, 1), n(E, 2, 1, 1), n(E, 2, 1, 1), n(E, 1, 1, 1)
+    decay = torch.tensor([0.5], device="cuda")
+    out, last = policy.compute_linear_attention(q, k, v, decay, None, s, 1.0)
+    s1 = 0.5 * s[:, 0].double() + (k * v)[:, 0].double()
+    s2 = 0.5 * s1 + (k * v)[:, 1].double()
+    for got, want in ((out[:, 0], q[:, 0] * s1), (out[:, 1], q[:, 1] * s2), (last[:, 0], s2)):
+        assert bool(((got.double() - want).abs() <= 8 * U32 * 8 * (1 + want.abs())).all())
+    E = (1 << 23) + 77
+    q, k, v, s = n(E, 1, 1), n(E, 1, 1), n(E, 1, 1), n(E, 1, 1, 1)
+    out, new = policy.compute_linear_attention_step(q, k, v, decay, s, None, 1.0)
+    s1 = 0.5 * s[:, 0].double() + (k * v).double()
+    assert bool(((new[:, 0].double() - s1).abs() <= 64 * U32 * (1 + s1.abs())).all())
+    assert bool(((out.double() - q * s1).abs() <= 64 * U32 * (1 + (q * s1).abs())).all())
+
+
 def test_nothing_to_do():
     z = torch.zeros(2, 0, 3, 8, device="cuda", requires_grad=True)
     s = torch.randn(2, 3, 8, 8, device="cuda")

@@ -66,7 +66,7 @@ def test_entry_points_refuse_without_launching():
                                                    decay=p, state=p, scale=1.0, state_scale=1.0, state_out_scale=1.0), **kw})
     none = _native.Sequence(None, 0, 0, 0)
     for bad in (dict(q=none), dict(out=none), dict(decay=None), dict(dim_k=0), dict(dim_v=129), dict(scale=float("inf")),
-                dict(seq_len=-1), dict(num_envs=-2), dict(num_envs=1 << 24)):
+                dict(seq_len=-1), dict(num_envs=-2), dict(heads=1 << 21)):
         assert lib.rlk_linear_attention(ctypes.byref(att(**bad)), 1, None) == -1, bad
     assert lib.rlk_linear_attention(ctypes.byref(att()), 4, None) == -1
     two = (_native.Attention * 2)(att(), att(heads=2))
