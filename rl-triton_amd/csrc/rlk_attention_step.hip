@@ -9,7 +9,8 @@ namespace {
 
 constexpr int kNT = 256;
 
-template <class E, int LANES, bool VEC>  // LANES lanes cover a row of the state in quads
+// LANES lanes cover a row of the state in quads.  NT: non-temporal accesses to it.
+template <class E, int LANES, bool VEC, bool NT>
 __global__ __launch_bounds__(kNT) void step_kernel(const Walk<E> w, int heads, int64_t first, const float* __restrict__ decay,
                                                    const float* __restrict__ dones) {
   constexpr int ROWS = kNT / LANES;
@@ -39,7 +40,7 @@ __global__ __launch_bounds__(kNT) void step_kernel(const Walk<E> w, int heads, i
       const int at = i * w.dc + j;
       if (!cut) {  // (what a cut state held has no part, NaN included)
         if constexpr (VEC) {
-          x = *reinterpret_cast<const float4*>(src + at);
+          x = load_quad<NT>(src + at);
         } else {
           x.x = src[at];
           if (j + 1 < w.dc) x.y = src[at + 1];
@@ -51,7 +52,7 @@ __global__ __launch_bounds__(kNT) void step_kernel(const Walk<E> w, int heads, i
       x.x = fmaf(lambda, x.x, k * v[0]), x.y = fmaf(lambda, x.y, k * v[1]);
       x.z = fmaf(lambda, x.z, k * v[2]), x.w = fmaf(lambda, x.w, k * v[3]);
       if constexpr (VEC) {
-        *reinterpret_cast<float4*>(dst + at) = x;
+        store_quad<NT>(dst + at, x);
       } else {
         dst[at] = x.x;
         if (j + 1 < w.dc) dst[at + 1] = x.y;
@@ -78,16 +79,22 @@ int step_impl(const rlk_attention& c, hipStream_t s) {
   w.da = (int)c.dim_k, w.dc = (int)c.dim_v, w.state = c.state, w.state_out = c.state_out, w.scale = c.scale;
   const bool vec = c.dim_v % 4 == 0 && ((reinterpret_cast<uintptr_t>(c.state) | reinterpret_cast<uintptr_t>(c.state_out)) & 15u) == 0;
   const int heads = (int)c.heads;
+  // A state that the 256 MB of last-level cache cannot keep for the next step goes past the caches (512 MB: 192 us, 206 through
+  // them; 256 MB: 99 and 99 to 107); a smaller one is found there again (64 MB: 23.5 us, 26 past them).
+  const bool large = c.num_envs * c.heads * c.dim_k * c.dim_v * (int64_t)sizeof(float) >= int64_t{1} << 28;
   const int64_t pairs = c.num_envs * c.heads, most = int64_t{1} << 23;  // (of one launch: 2^31 work-items)
   for (int64_t first = 0; first < pairs; first += most) {
     const dim3 grid((unsigned)(pairs - first < most ? pairs - first : most)), block(kNT);
-    if (c.dim_v <= 64) {
-      if (vec) step_kernel<E, 16, true><<<grid, block, 0, s>>>(w, heads, first, c.decay, c.dones);
-      else step_kernel<E, 16, false><<<grid, block, 0, s>>>(w, heads, first, c.decay, c.dones);
-    } else {
-      if (vec) step_kernel<E, 32, true><<<grid, block, 0, s>>>(w, heads, first, c.decay, c.dones);
-      else step_kernel<E, 32, false><<<grid, block, 0, s>>>(w, heads, first, c.decay, c.dones);
-    }
+    auto launch = [&](auto lanes, auto v, auto nt) {
+      step_kernel<E, decltype(lanes)::value, decltype(v)::value, decltype(nt)::value><<<grid, block, 0, s>>>(w, heads, first, c.decay, c.dones);
+    };
+    auto by_size = [&](auto v, auto nt) {
+      if (c.dim_v <= 64) launch(std::integral_constant<int, 16>{}, v, nt);
+      else launch(std::integral_constant<int, 32>{}, v, nt);
+    };
+    if (!vec) by_size(std::false_type{}, std::false_type{});
+    else if (large) by_size(std::true_type{}, std::true_type{});
+    else by_size(std::true_type{}, std::false_type{});
     if (hipGetLastError() != hipSuccess) return RLK_ERR_LAUNCH;
   }
   return RLK_OK;
