@@ -260,7 +260,7 @@ __device__ __forceinline__ RowStats streamed_stats(const Frame<E>& f, int lane, 
   auto rebase = [&](float to) {  // sums about `to` in place of m
     if (m == to) return;
     if (m != -INFINITY) {  // (else they are 0, or NaN from a NaN)
-      const float d = (m - to) * c, f2 = __builtin_amdgcn_exp2f(d);
+      const float d = fmaxf((m - to) * c, kDeep), f2 = __builtin_amdgcn_exp2f(d);  // (finite: d s where f2 is 0)
       u = f2 * fmaf(d, s, u);
       s = f2 * s;
     }

@@ -90,6 +90,38 @@ def test_values_that_masks_leave(A, dtype):
     assert lp[5].isnan() and lp[6].isnan() and ent[5].isfinite() and ent[6].isfinite()
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("A", [5, 18, 60, 300, 3000, 9000, 50001, 140001])
+@pytest.mark.parametrize("rows", [(1, 3), (2, 700)])
+def test_masks_of_the_lowest_value(A, rows, dtype):
+    """Logits of the type's lowest value count as nothing beside others, wherever they lie: first, last, most of the row."""
+    if rows[1] > 3 and A > 9000:
+        rows = (2, 300)
+    x, a = _make(rows, A, A + 1, dtype)
+    g = torch.Generator().manual_seed(A)
+    low = torch.rand(x.shape, generator=g) < torch.tensor([0.1, 0.9, 0.99])[torch.randint(0, 3, rows, generator=g)][..., None]
+    low[..., :A // 3] = True
+    low.scatter_(-1, a[..., None], False)
+    _check(torch.where(low, torch.finfo(dtype).min, x.float()).to(dtype), a, 0.6)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows", [1, 2, 7, 33, 130, 256, 257])
+def test_few_long_rows(rows, dtype):
+    """Rows shared by several workgroups, of every alignment, with parts that hold nothing but -inf."""
+    for A in (8192, 20011, 33333):
+        x, a = _make((1, rows), A, A + rows, dtype, "invalid")
+        x[0, 0, A // 4:3 * A // 4] = -math.inf
+        a[0, 0] = A - 1
+        x[0, 0, A - 1] = 1.0
+        if rows > 2:
+            x[0, 1] = -math.inf
+            x[0, 2, A // 2] = math.nan
+        if A % 2 and dtype == torch.bfloat16 and rows > 100:
+            continue
+        _check(x, a, 0.9)
+
+
 def _grad_check(x, a, tau, xd, seed=3):
     g = torch.Generator().manual_seed(seed)
     gl, ge = torch.randn(a.shape, generator=g), torch.randn(a.shape, generator=g)
