@@ -26,7 +26,13 @@ typedef struct rlk_action_rows {
   int64_t env_stride, step_stride;
   float temperature; /* logits are divided by it: > 0 */
   int bf16;          /* logits (and their gradient) */
+  /* NULL, or RLK_ROWS_WORKSPACE_BYTES (no initial contents needed) with which log-probabilities of few long rows are
+   * shared by several workgroups a row.  The losses use their own. */
+  void *workspace;
+  size_t workspace_bytes;
 } rlk_action_rows;
+
+#define RLK_ROWS_WORKSPACE_BYTES 12288
 
 /* log_probs[e,t] = x_a - log sum_j exp x_j with x = logits / temperature, and the entropy of every row.
  * norms: NULL, or [num_envs, seq_len, 2] for the backward call: the row's largest logit and the binary

@@ -5,6 +5,19 @@
 namespace rlk {
 namespace {
 
+// What a row's statistics come to.
+template <class E>
+__device__ __forceinline__ void write_row(const ActionRows<E>& a, const E* base, int64_t row, const RowStats& r, float* log_probs,
+                                          float* entropies, float* norms) {
+  const int64_t act = a.actions[row];
+  const float x = act >= 0 && act < a.A ? load_one(base + act) : NAN;
+  const float log2s = r.log2s();
+  const bool empty = r.s == 0.f;
+  log_probs[row] = empty && x == x ? -INFINITY : ((x - r.m) * a.c - log2s) * kLn2;
+  entropies[row] = empty ? 0.f : (log2s - r.u / r.s) * kLn2;
+  if (norms) norms[2 * row] = r.m, norms[2 * row + 1] = empty ? INFINITY : log2s;  // (inf: p = 0)
+}
+
 template <class E, int LANES, int NV>
 __global__ __launch_bounds__(rows_threads<LANES>()) void log_probs_kernel(const ActionRows<E> a, float* __restrict__ log_probs,
                                                                            float* __restrict__ entropies,
@@ -20,19 +33,20 @@ __global__ __launch_bounds__(rows_threads<LANES>()) void log_probs_kernel(const 
       h.load(f, lane);
       r = h.stats(f, lane, a.c, lds);
     } else {
-      r = streamed_stats<E, LANES>(f, lane, a.c, lds);
+      r = streamed_stats<E, LANES>(f, lane, a.c, lds, Part{0, f.nfull, true});
     }
-    if (lane == 0) {
-      const int64_t act = a.actions[row];
-      const float x = act >= 0 && act < a.A ? load_one(f.base + act) : NAN;
-      const float log2s = r.log2s();
-      const bool empty = r.s == 0.f;
-      log_probs[row] = empty && x == x ? -INFINITY : ((x - r.m) * a.c - log2s) * kLn2;
-      entropies[row] = empty ? 0.f : (log2s - r.u / r.s) * kLn2;
-      if (norms) norms[2 * row] = r.m, norms[2 * row + 1] = empty ? INFINITY : log2s;  // (inf: p = 0)
-    }
+    if (lane == 0) write_row(a, f.base, row, r, log_probs, entropies, norms);
     if constexpr (LANES > 64) __syncthreads();
   }
+}
+
+template <class E>
+__global__ __launch_bounds__(256) void join_log_probs_kernel(const ActionRows<E> a, const RowParts p, float* __restrict__ log_probs,
+                                                             float* __restrict__ entropies, float* __restrict__ norms) {
+  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (row >= a.rows) return;
+  const RowStats r = join_parts(p, row, a.c);
+  if ((threadIdx.x & 63) == 0) write_row(a, row_base(a, row), row, r, log_probs, entropies, norms);
 }
 
 template <class E, int K>
@@ -72,7 +86,7 @@ __global__ __launch_bounds__(256) void backward_kernel(const ActionRows<E> a, co
     const float log2s = norms[2 * row + 1];
     const RowGrad g(gl ? gl[row] : 0.f, ge ? ge[row] : 0.f, entropies[row], norms[2 * row], a.c, log2s, a.inv_tau, a.actions[row],
                     log2s == INFINITY);
-    write_grad<E, LANES, 0>(f, nullptr, out + row * a.A, g, lane);
+    write_grad<E, LANES, 0>(f, nullptr, out + row * a.A, g, lane, Part{0, f.nfull, true});
   }
 }
 
@@ -90,6 +104,12 @@ int forward(const rlk_action_rows* rows, float* lp, float* ent, float* norms, hi
     });
   }
   constexpr int VEC = Frame<E>::VEC;
+  const RowParts parts = plan_parts(a.rows, (a.A + VEC - 1) / VEC, false, rows->workspace, rows->workspace_bytes);
+  if (parts.parts > 0) {
+    part_stats_kernel<E><<<dim3((unsigned)(a.rows * parts.parts)), dim3(256), 0, s>>>(a, parts, nullptr);
+    join_log_probs_kernel<E><<<dim3((unsigned)((a.rows + 3) / 4)), dim3(256), 0, s>>>(a, parts, lp, ent, norms);
+    return hipGetLastError() == hipSuccess ? RLK_OK : RLK_ERR_LAUNCH;
+  }
   return dispatch_read((a.A + VEC - 1) / VEC, a.rows, [&](auto lanes, auto nv, int64_t most) {
     constexpr int L = decltype(lanes)::value, NV = decltype(nv)::value, NT = rows_threads<L>();
     int64_t blocks = (a.rows + NT / L - 1) / (NT / L);

@@ -23,6 +23,13 @@ struct ActionRows {
   float c, inv_tau;
 };
 
+template <class E>
+__device__ __forceinline__ const E* row_base(const ActionRows<E>& a, int64_t row) {
+  if (a.env_stride == a.seq_len * a.step_stride) return a.logits + row * a.step_stride;
+  const int64_t e = row / a.seq_len;
+  return a.logits + e * a.env_stride + (row - e * a.seq_len) * a.step_stride;
+}
+
 // The row as the lanes of a group hold it: `nfull` vectors of 16 bytes at 16-byte boundaries from element
 // `head` on, lane l holding vectors l, l + LANES, ...; the at most 2 (VEC - 1) elements before and after
 // them are held one by one.
@@ -200,16 +207,22 @@ struct RowHolder {
   }
 };
 
-// Writes the gradient of a row, `held` (NV > 0) or read again.
+// A part of a row: its whole vectors v0 .. v1 - 1 and, `edges`, the elements around all of them.
+struct Part {
+  int v0, v1;
+  bool edges;
+};
+
+// Writes the gradient of a row, `held` (NV > 0), or of a part of it that is read again.
 template <class E, int LANES, int NV>
 __device__ __forceinline__ void write_grad(const Frame<E>& f, const RowHolder<E, LANES, NV>* held, E* out, const RowGrad& g,
-                                           int lane) {
+                                           int lane, const Part& part) {
   constexpr int VEC = Frame<E>::VEC;
   // the output has the input's place in its 16 bytes unless the logits' rows are strided
   const bool same = ((reinterpret_cast<uintptr_t>(out) ^ reinterpret_cast<uintptr_t>(f.base)) & 15u) == 0;
   auto vec = [&](u32x4 w, int r) {
-    E* to = vector_at<LANES>(out + f.head, r, lane);
-    const int j0 = f.head + (lane + LANES * r) * VEC;
+    E* to = vector_at<LANES>(out + f.head + part.v0 * VEC, r, lane);
+    const int j0 = f.head + (part.v0 + lane + LANES * r) * VEC;
     float x[VEC];
     unpack<E>(w, x);
 #pragma unroll
@@ -234,8 +247,10 @@ __device__ __forceinline__ void write_grad(const Frame<E>& f, const RowHolder<E,
       }
   } else {
 #pragma unroll 4
-    for (int k = 0; lane + LANES * k < f.nfull; ++k) vec(load_words(vector_at<LANES>(f.base + f.head, k, lane)), k);
+    for (int k = 0; part.v0 + lane + LANES * k < part.v1; ++k)
+      vec(load_words(vector_at<LANES>(f.base + f.head + part.v0 * VEC, k, lane)), k);
   }
+  if (!part.edges) return;
   for (int i = lane; i < 2 * VEC; i += LANES) {
     const int j = f.edge(i);
     if (j >= 0) out[j] = from_f32<E>(g.zero ? 0.f : g(load_one(f.base + j), j));
@@ -243,18 +258,19 @@ __device__ __forceinline__ void write_grad(const Frame<E>& f, const RowHolder<E,
 }
 
 template <class E, int LANES>
-__device__ __forceinline__ void write_zeros(E* out, int A, int lane) {
+__device__ __forceinline__ void write_zeros(E* out, int A, int lane, int part = 0, int parts = 1) {
   const Frame<E> f(out, A);
-  for (int k = 0; lane + LANES * k < f.nfull; ++k) store_words(vector_at<LANES>(out + f.head, k, lane), u32x4{0, 0, 0, 0});
+  for (int i = lane + LANES * part; i < f.nfull; i += LANES * parts) store_words(out + f.head + (int64_t)i * Frame<E>::VEC, u32x4{0, 0, 0, 0});
+  if (part > 0) return;
   for (int i = lane; i < 2 * Frame<E>::VEC; i += LANES) {
     const int j = f.edge(i);
     if (j >= 0) out[j] = from_f32<E>(0.f);
   }
 }
 
-// Statistics of a row too long to hold: read once, with a running maximum per lane.
+// Statistics of a row too long to hold, or of a part of it: read once, with a running maximum per lane.
 template <class E, int LANES>
-__device__ __forceinline__ RowStats streamed_stats(const Frame<E>& f, int lane, float c, float* lds) {
+__device__ __forceinline__ RowStats streamed_stats(const Frame<E>& f, int lane, float c, float* lds, const Part& part) {
   constexpr int VEC = Frame<E>::VEC;
   float m = -INFINITY, s = 0.f, u = 0.f;
   auto rebase = [&](float to) {  // sums about `to` in place of m
@@ -266,7 +282,7 @@ __device__ __forceinline__ RowStats streamed_stats(const Frame<E>& f, int lane, 
     }
     m = to;
   };
-  for (int i = lane; i < 2 * VEC; i += LANES) {
+  for (int i = lane; part.edges && i < 2 * VEC; i += LANES) {
     const int j = f.edge(i);
     const float x = j >= 0 ? load_one(f.base + j) : -INFINITY;
     if (x != -INFINITY) {
@@ -275,9 +291,9 @@ __device__ __forceinline__ RowStats streamed_stats(const Frame<E>& f, int lane, 
     }
   }
 #pragma unroll 4
-  for (int r = 0; lane + LANES * r < f.nfull; ++r) {
+  for (int r = 0; part.v0 + lane + LANES * r < part.v1; ++r) {
     float x[VEC];
-    unpack<E>(load_words(vector_at<LANES>(f.base + f.head, r, lane)), x);
+    unpack<E>(load_words(vector_at<LANES>(f.base + f.head + part.v0 * VEC, r, lane)), x);
     float t = x[0];
     bool nan = x[0] != x[0];
 #pragma unroll
@@ -294,6 +310,68 @@ __device__ __forceinline__ RowStats streamed_stats(const Frame<E>& f, int lane, 
   if (top != -INFINITY) rebase(top);
   else top = 0.f;
   group_sum2<LANES>(s, u, lds + LANES / 64 + 1);
+  return RowStats{top, s, u};
+}
+
+// ---------------------------------------------------------------------------------------
+// Few rows, and long: each is shared by `parts` workgroups.  A first launch writes the parts' statistics, the second joins
+// a row's (a wavefront, in the parts' order) and goes on from there.
+// ---------------------------------------------------------------------------------------
+struct RowParts {
+  int parts;     // 0: rows are not shared
+  int per;       // vectors of a part
+  float* stats;  // [row, part, 3]: largest logit (-inf: none), s, u
+  __device__ Part part(int i, int nfull) const {
+    const int v0 = i * per < nfull ? i * per : nfull;
+    return {v0, v0 + per < nfull ? v0 + per : nfull, i == 0};
+  }
+};
+constexpr int kMaxShares = 1024, kMaxParts = 64;
+static_assert(RLK_ROWS_WORKSPACE_BYTES == sizeof(float) * 3 * kMaxShares, "the workspace of shared rows");
+
+// Shared where a workgroup each would leave most of the GPU idle for longer than a second launch takes (us, alone -> shared).
+// Only read: from 12288 vectors (float32: 16 rows of 131072 25.5 -> 11.8, 160 28.2 -> 23.4, 64 of 50001 12.3 -> 11.9; but 10 of 33776
+// 8.0 -> 11.4).  Read and written: up to 64 rows from 4096 vectors (bfloat16: 10 of 33776 17.1 -> 13.4, 64 of 50001 19.9 -> 16.8, 16 of
+// 131072 32.7 -> 14.7; but 200 of 32768 16.2 -> 24.3, 32 of 8192 9.4 -> 13.9), and up to 256 that are too long to be held (float32: 160 of
+// 131072 103 -> 60).
+inline RowParts plan_parts(int64_t rows, int64_t vecs, bool written, void* workspace, size_t bytes) {
+  RowParts p{0, 0, static_cast<float*>(workspace)};
+  if (workspace == nullptr || bytes < sizeof(float) * 3 * kMaxShares || rows < 1 || rows > 256) return p;
+  if (written ? vecs < 4096 || (rows > 64 && vecs <= 16384) : vecs < 12288) return p;
+  int64_t n = kMaxShares / rows;
+  if (n > kMaxParts) n = kMaxParts;
+  if (n > vecs / 512) n = vecs / 512;
+  p.parts = (int)n, p.per = (int)((vecs + n - 1) / n);
+  return p;
+}
+
+template <class E>
+__global__ __launch_bounds__(256) void part_stats_kernel(const ActionRows<E> a, const RowParts p, const float* __restrict__ mask) {
+  __shared__ float lds[3 * 4 + 2];
+  const int part = blockIdx.x % p.parts;
+  const int64_t row = blockIdx.x / p.parts;
+  if (mask != nullptr && mask[row] == 0.f) return;
+  const Frame<E> f(row_base(a, row), a.A);
+  const RowStats r = streamed_stats<E, 256>(f, threadIdx.x, a.c, lds, p.part(part, f.nfull));
+  if (threadIdx.x == 0) {
+    float* to = p.stats + 3 * (int64_t)blockIdx.x;
+    to[0] = r.s == 0.f ? -INFINITY : r.m, to[1] = r.s, to[2] = r.u;
+  }
+}
+
+// The row's statistics, in every lane of a wavefront.
+__device__ __forceinline__ RowStats join_parts(const RowParts& p, int64_t row, float c) {
+  const int lane = threadIdx.x & 63;
+  float m = -INFINITY, s = 0.f, u = 0.f;
+  if (lane < p.parts) {
+    const float* from = p.stats + 3 * (row * p.parts + lane);
+    m = from[0], s = from[1], u = from[2];
+  }
+  float top = group_max<64>(m, nullptr);
+  if (top == -INFINITY) top = 0.f;
+  const float d = fmaxf((m - top) * c, kDeep), f = __builtin_amdgcn_exp2f(d);
+  u = f * fmaf(d, s, u), s = f * s;
+  group_sum2<64>(s, u, nullptr);
   return RowStats{top, s, u};
 }
 
@@ -450,13 +528,6 @@ ActionRows<E> action_rows(const rlk_action_rows* r) {
   const double inv = 1.0 / (double)r->temperature;
   return {static_cast<const E*>(r->logits), r->actions, r->num_envs * r->seq_len, r->seq_len, r->env_stride, r->step_stride,
           (int)r->num_actions, (float)(1.4426950408889634 * inv), (float)inv};
-}
-
-template <class E>
-__device__ __forceinline__ const E* row_base(const ActionRows<E>& a, int64_t row) {
-  if (a.env_stride == a.seq_len * a.step_stride) return a.logits + row * a.step_stride;
-  const int64_t e = row / a.seq_len;
-  return a.logits + e * a.env_stride + (row - e * a.seq_len) * a.step_stride;
 }
 
 }  // namespace rlk

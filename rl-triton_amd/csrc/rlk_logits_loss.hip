@@ -35,7 +35,7 @@ __global__ __launch_bounds__(rows_threads<LANES>()) void logits_loss_kernel(cons
       h.load(f, lane);
       r = h.stats(f, lane, a.c, lds);
     } else {
-      r = streamed_stats<E, LANES>(f, lane, a.c, lds);
+      r = streamed_stats<E, LANES>(f, lane, a.c, lds, Part{0, f.nfull, true});
     }
     const bool empty = r.s == 0.f;
     const float log2s = r.log2s();
@@ -44,9 +44,9 @@ __global__ __launch_bounds__(rows_threads<LANES>()) void logits_loss_kernel(cons
     const StepTerms st = step_terms(lp, t.old[row], t.adv[row], t.ref ? t.ref[row] : 0.f, t.ref != nullptr, c);
     const RowGrad g(wt * st.slope, -c.entropy_coef * wt, entropy, r.m, a.c, log2s, a.inv_tau, act, empty);
     if constexpr (NV > 0)
-      write_grad<E, LANES, NV>(f, &h, out, g, lane);
+      write_grad<E, LANES, NV>(f, &h, out, g, lane, Part{0, f.nfull, true});
     else
-      write_grad<E, LANES, 0>(f, nullptr, out, g, lane);
+      write_grad<E, LANES, 0>(f, nullptr, out, g, lane, Part{0, f.nfull, true});
     if (lane == 0) {
 #pragma unroll
       for (int k = 0; k < 4; ++k) acc[k] += wt * st.v[k];
@@ -55,6 +55,40 @@ __global__ __launch_bounds__(rows_threads<LANES>()) void logits_loss_kernel(cons
     if constexpr (LANES > 64) __syncthreads();
   }
   finish_loss<NT>(acc, c, sums);
+}
+
+// The second launch for rows that several workgroups share: the loss by the first part's, the gradient by each for its own.
+template <class E>
+__global__ __launch_bounds__(256) void join_loss_kernel(const ActionRows<E> a, const RowParts p, const StepArrays t, const LossConsts c,
+                                                        const Weights w, const LossOut sums, E* __restrict__ grad) {
+  __shared__ int64_t sc[4];
+  const float scale = weight_scale<256>(w, sc);
+  float acc[kTerms] = {};
+  const int part = blockIdx.x % p.parts;
+  const int64_t row = blockIdx.x / p.parts;
+  E* out = grad + row * a.A;
+  if (t.mask != nullptr && t.mask[row] == 0.f) {
+    write_zeros<E, 256>(out, a.A, threadIdx.x, part, p.parts);
+  } else {
+    const float wt = w.row_counts != nullptr ? scale / (float)w.row_counts[row / a.seq_len] : scale;
+    const Frame<E> f(row_base(a, row), a.A);
+    const int64_t act = a.actions[row];
+    const float x = act >= 0 && act < a.A ? load_one(f.base + act) : NAN;
+    const RowStats r = join_parts(p, row, a.c);
+    const bool empty = r.s == 0.f;
+    const float log2s = r.log2s();
+    const float lp = empty && x == x ? -INFINITY : ((x - r.m) * a.c - log2s) * kLn2;
+    const float entropy = empty ? 0.f : (log2s - r.u / r.s) * kLn2;
+    const StepTerms st = step_terms(lp, t.old[row], t.adv[row], t.ref ? t.ref[row] : 0.f, t.ref != nullptr, c);
+    const RowGrad g(wt * st.slope, -c.entropy_coef * wt, entropy, r.m, a.c, log2s, a.inv_tau, act, empty);
+    write_grad<E, 256, 0>(f, nullptr, out, g, threadIdx.x, p.part(part, f.nfull));
+    if (threadIdx.x == 0 && part == 0) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) acc[k] = wt * st.v[k];
+      acc[4] = wt * entropy;
+    }
+  }
+  finish_loss<256>(acc, c, sums);
 }
 
 template <class E, int K>
@@ -135,6 +169,13 @@ int impl(const rlk_action_rows* rows, const rlk_policy_terms* t, void* grad, hip
     });
   }
   constexpr int VEC = Frame<E>::VEC;
+  const RowParts parts = plan_parts(a.rows, (a.A + VEC - 1) / VEC, true, plan.shares, kShareBytes);
+  if (parts.parts > 0) {
+    const dim3 grid((unsigned)(a.rows * parts.parts));
+    part_stats_kernel<E><<<grid, dim3(256), 0, s>>>(a, parts, arrays.mask);
+    join_loss_kernel<E><<<grid, dim3(256), 0, s>>>(a, parts, arrays, plan.consts, plan.weights, plan.out, static_cast<E*>(grad));
+    return hipGetLastError() == hipSuccess ? RLK_OK : RLK_ERR_LAUNCH;
+  }
   return dispatch_update((a.A + VEC - 1) / VEC, [&](auto lanes, auto nv, int64_t most) {
     constexpr int L = decltype(lanes)::value, NV = decltype(nv)::value, NT = rows_threads<L>();
     int64_t blocks = (a.rows + NT / L - 1) / (NT / L);

@@ -154,7 +154,9 @@ struct LossPlan {
   LossOut out;
   int64_t* count_parts;
   int* row_counts;
+  void* shares;  // kShareBytes for rows of logits that several workgroups share
 };
+constexpr size_t kShareBytes = RLK_ROWS_WORKSPACE_BYTES;
 
 // Checks the terms and lays out the workspace; RLK_OK or an error.
 int plan_loss(const rlk_policy_terms* t, int64_t num_envs, int64_t seq_len, int means, LossPlan* plan);

@@ -245,7 +245,8 @@ int plan_loss(const rlk_policy_terms* t, int64_t num_envs, int64_t seq_len, int 
   char* ws = static_cast<char*>(t->workspace);
   p->out = {reinterpret_cast<double*>(ws + kTicketBytes), reinterpret_cast<uint32_t*>(ws), t->loss, t->means, means};
   p->count_parts = reinterpret_cast<int64_t*>(p->out.partials + (int64_t)kMaxLossBlocks * kPartials);
-  p->row_counts = reinterpret_cast<int*>(p->count_parts + kCountBlocks);
+  p->shares = p->count_parts + kCountBlocks;
+  p->row_counts = reinterpret_cast<int*>(static_cast<char*>(p->shares) + kShareBytes);
   Weights& w = p->weights;
   w.parts = nullptr, w.row_counts = nullptr, w.num_parts = 0, w.per_row = t->per_row != 0;
   const int64_t n = num_envs * seq_len;
@@ -271,7 +272,8 @@ extern "C" {
 
 size_t rlk_policy_workspace_bytes(int64_t num_envs) {
   const size_t rows = num_envs > 0 ? (size_t)num_envs : 0;
-  return kTicketBytes + sizeof(double) * kMaxLossBlocks * kPartials + sizeof(int64_t) * kCountBlocks + (sizeof(int) * rows + 7) / 8 * 8;
+  return kTicketBytes + sizeof(double) * kMaxLossBlocks * kPartials + sizeof(int64_t) * kCountBlocks + kShareBytes +
+         (sizeof(int) * rows + 7) / 8 * 8;
 }
 
 int rlk_policy_loss(const void* log_probs, int64_t num_envs, int64_t seq_len, const rlk_policy_terms* terms,

@@ -56,7 +56,7 @@ const void* data_or_null(const at::Tensor* t) { return t ? t->data_ptr() : nullp
 // Scratch memory, one of each kind per (device, stream), as rl_triton.policy._native keeps it; none (declined) while
 // the stream is capturing a graph.
 struct PolicyScratch {
-  at::Tensor sums, states;
+  at::Tensor sums, rows, states;
 };
 bool policy_scratch(const PolicyCall& c, at::Tensor PolicyScratch::* kind, size_t need, const at::Tensor& like, void** ptr,
                     size_t* bytes) {
@@ -104,6 +104,9 @@ PyObject* op_action_log_probs(PyObject* const* a, Py_ssize_t n) {
   rlk_action_rows r = {};
   const at::Tensor *x, *act;
   if (!logit_rows(c, a[0], a[1], a[2], true, &r, &x, &act)) return decline();
+  if (act->numel() <= 256 && r.num_actions >= 32768 &&
+      !policy_scratch(c, &PolicyScratch::rows, RLK_ROWS_WORKSPACE_BYTES, *x, &r.workspace, &r.workspace_bytes))
+    return decline();
   at::Tensor lp = policy_output(act->sizes(), at::kFloat, *x), ent = policy_output(act->sizes(), at::kFloat, *x);
   const int st = rlk_action_log_probs(&r, static_cast<float*>(lp.data_ptr()), static_cast<float*>(ent.data_ptr()), nullptr, c.stream());
   return finish(st, "rlk_action_log_probs", pair(lp, ent));

@@ -17,7 +17,11 @@ _P, _I64, _F, _INT, _SZ = ctypes.c_void_p, ctypes.c_int64, ctypes.c_float, ctype
 
 class ActionRows(ctypes.Structure):
     _fields_ = [("logits", _P), ("actions", _P), ("num_envs", _I64), ("seq_len", _I64), ("num_actions", _I64),
-                ("env_stride", _I64), ("step_stride", _I64), ("temperature", _F), ("bf16", _INT)]
+                ("env_stride", _I64), ("step_stride", _I64), ("temperature", _F), ("bf16", _INT),
+                ("workspace", _P), ("workspace_bytes", _SZ)]
+
+
+ROWS_WORKSPACE_BYTES = 12288
 
 
 class PolicyTerms(ctypes.Structure):
@@ -67,8 +71,8 @@ def load():
 
 
 _BF16 = torch.bfloat16
-# Scratch memory, one of each kind per (device, stream): "sums" of the losses, whose head is zero between calls, and
-# "states" of sequences cut into segments.
+# Scratch memory, one of each kind per (device, stream): "sums" of the losses, whose head is zero between calls,
+# "rows" of statistics of shared rows, and "states" of sequences cut into segments.
 _workspaces: dict = {}
 
 
@@ -113,7 +117,10 @@ def _rows(logits, actions, temperature):
 
 @_on_device
 def action_log_probs(dev, stream, logits, actions, temperature, log_probs, entropies, norms):
-    _native._check((_lib or load()).rlk_action_log_probs(ctypes.byref(_rows(logits, actions, temperature)),
+    rows = _rows(logits, actions, temperature)
+    if actions.numel() <= 256:
+        rows.workspace, rows.workspace_bytes = _workspace("rows", dev, stream, ROWS_WORKSPACE_BYTES)
+    _native._check((_lib or load()).rlk_action_log_probs(ctypes.byref(rows),
                                                         log_probs.data_ptr(), entropies.data_ptr(), _ptr(norms), stream),
                    "rlk_action_log_probs")
 

@@ -180,6 +180,17 @@ def test_from_logits(A, dtype):
     _logits_check(x, a, terms, x.cuda().transpose(0, 1).contiguous().transpose(0, 1), "rows")
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,A", [(1, 131072), (1, 16389), (3, 32771), (64, 33000), (65, 33000), (70, 140001), (13, 70003)])
+def test_from_logits_few_long_rows(rows, A, dtype):
+    """Rows shared by several workgroups, masked ones among them."""
+    if rows > 20 and A > 100000 and dtype == torch.float32:
+        rows = 5
+    for mask in (None, "random"):
+        x, a, terms = _make_logits(1, rows, A, A + rows, dtype, mask=mask, ref=True)
+        _logits_check(x, a, terms, x.cuda(), "rows")
+
+
 def test_from_logits_many_rows():
     """More rows than workgroups: every group of lanes takes several."""
     x, a, terms = _make_logits(600, 500, 6, 2, torch.float32, mask="random", ref=True)
