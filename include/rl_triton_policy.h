@@ -24,7 +24,7 @@ typedef struct rlk_action_rows {
   const int64_t *actions; /* [num_envs, seq_len], contiguous */
   int64_t num_envs, seq_len, num_actions;
   int64_t env_stride, step_stride;
-  float temperature; /* logits are divided by it: > 0 */
+  double temperature; /* logits are divided by it: > 0 */
   int bf16;          /* logits (and their gradient) */
   /* NULL, or RLK_ROWS_WORKSPACE_BYTES (no initial contents needed) with which log-probabilities of few long rows are
    * shared by several workgroups a row.  The losses use their own. */
@@ -50,9 +50,9 @@ typedef struct rlk_policy_terms {
   const void *old_log_probs, *advantages;
   const void *ref_log_probs; /* NULL: no KL term */
   const void *mask;          /* NULL: every step takes part; else those with mask != 0 */
-  float clip_low, clip_high; /* ratios are held to [1 - clip_low, 1 + clip_high] */
-  float dual_clip;           /* > 1: the least that negative advantages count with, -A * dual_clip; 0: none */
-  float kl_coef, entropy_coef;
+  double clip_low, clip_high; /* ratios are held to [1 - clip_low, 1 + clip_high] */
+  double dual_clip;           /* > 1: the least that negative advantages count with, -A * dual_clip; 0: none */
+  double kl_coef, entropy_coef;
   int per_row; /* 0: mean over the steps that take part; 1: mean over rows of their means */
   int bf16;    /* the arrays above (rlk_policy_loss: log_probs and the gradient too) */
   float *loss;  /* [1] */

@@ -519,13 +519,13 @@ int dispatch_update(int64_t vecs, F f) {
 
 inline bool valid_rows(const rlk_action_rows* r) {
   if (!r || r->num_envs < 0 || r->seq_len < 0 || r->num_actions < 1 || r->num_actions > (int64_t{1} << 30)) return false;
-  if (!(r->temperature > 0.f) || !std::isfinite(r->temperature)) return false;
+  if (!(r->temperature > 0.0) || !std::isfinite(r->temperature)) return false;
   return r->num_envs * r->seq_len == 0 || (r->logits && r->actions && (reinterpret_cast<uintptr_t>(r->logits) & (r->bf16 ? 1u : 3u)) == 0);
 }
 
 template <class E>
 ActionRows<E> action_rows(const rlk_action_rows* r) {
-  const double inv = 1.0 / (double)r->temperature;
+  const double inv = 1.0 / r->temperature;
   return {static_cast<const E*>(r->logits), r->actions, r->num_envs * r->seq_len, r->seq_len, r->env_stride, r->step_stride,
           (int)r->num_actions, (float)(1.4426950408889634 * inv), (float)inv};
 }

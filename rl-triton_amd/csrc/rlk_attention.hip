@@ -205,9 +205,10 @@ struct Part {
   }
 };
 
-// acc += a (w * c) for an operand row c and weights w of its inner indices.  The weighted bfloat16 operand is
-// taken as the sum of two bfloat16 numbers (the product's upper 8 bits and the next 8): the state is a float32
-// result and sums over all steps, and one rounding of every term to 8 bits would be 2^-9 of it.
+// acc += a (w * c) for an operand row c and weights w of its inner indices.  The weighted bfloat16 operand is taken as the sum
+// of three bfloat16 numbers, the product's upper, middle and lower 8 bits: the state is a float32 result and sums over
+// all steps (with one rounding of a term to 8 bits it would be off by 2^-9 of itself, with two numbers by 2.5e-6; three are
+// the float32 product).
 template <class E>
 struct Weighted;
 template <>
@@ -221,18 +222,23 @@ struct Weighted<float> {
 };
 template <>
 struct Weighted<bf16> {
-  Frag<bf16> hi, lo;
+  Frag<bf16> hi, mid, lo;
   __device__ Weighted(const Frag<bf16>& c, const float (&w)[8]) {
-    union { bf16x8 v; uint32_t u[4]; } in{c.x}, h, l;
+    union { bf16x8 v; uint32_t u[4]; } in{c.x}, h, m, l;
+    auto upper = [](float x) { return __uint_as_float(__float_as_uint(x) & 0xffff0000u); };
+    auto uppers = [](float x, float y) { return __builtin_amdgcn_perm(__float_as_uint(y), __float_as_uint(x), 0x07060302u); };
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const float a = Words<bf16>::get(in.u[i], 0) * w[2 * i], b = Words<bf16>::get(in.u[i], 1) * w[2 * i + 1];
-      h.u[i] = bf16_pair(a, b);
-      l.u[i] = bf16_pair(a - Words<bf16>::get(h.u[i], 0), b - Words<bf16>::get(h.u[i], 1));
+      float a = Words<bf16>::get(in.u[i], 0) * w[2 * i], b = Words<bf16>::get(in.u[i], 1) * w[2 * i + 1];
+      h.u[i] = uppers(a, b);
+      a -= upper(a), b -= upper(b);
+      m.u[i] = uppers(a, b);
+      a -= upper(a), b -= upper(b);
+      l.u[i] = uppers(a, b);
     }
-    hi.x = h.v, lo.x = l.v;
+    hi.x = h.v, mid.x = m.v, lo.x = l.v;
   }
-  __device__ f32x4 mma_with(const Frag<bf16>& a, f32x4 acc) const { return mma(a, hi, mma(a, lo, acc)); }
+  __device__ f32x4 mma_with(const Frag<bf16>& a, f32x4 acc) const { return mma(a, hi, mma(a, mid, mma(a, lo, acc))); }
 };
 
 // Which walk of which environment and head a workgroup takes.  Workgroups go round the 8 XCDs, so the walks over the same

@@ -18,7 +18,11 @@ __global__ __launch_bounds__(rows_threads<LANES>()) void logits_loss_kernel(cons
   __shared__ int64_t sc[NT / 64];
   const float scale = weight_scale<NT>(w, sc);
   const int lane = threadIdx.x % LANES;
-  float acc[kTerms] = {};
+  // (a workgroup's rows: one thread adds, and in LDS, since the held row needs the registers)
+  __shared__ double total[kTerms];
+  double acc[kTerms] = {};
+  if (LANES > 64 && threadIdx.x < kTerms) total[threadIdx.x] = 0.0;
+  __syncthreads();
   for (int64_t row = first_row<LANES>(); row < a.rows; row += (int64_t)gridDim.x * PER) {
     E* out = grad + row * a.A;
     if (t.mask != nullptr && t.mask[row] == 0.f) {  // (the same for the whole group)
@@ -42,17 +46,26 @@ __global__ __launch_bounds__(rows_threads<LANES>()) void logits_loss_kernel(cons
     const float lp = empty && x == x ? -INFINITY : ((x - r.m) * a.c - log2s) * kLn2;
     const float entropy = empty ? 0.f : (log2s - r.u / r.s) * kLn2;
     const StepTerms st = step_terms(lp, t.old[row], t.adv[row], t.ref ? t.ref[row] : 0.f, t.ref != nullptr, c);
-    const RowGrad g(wt * st.slope, -c.entropy_coef * wt, entropy, r.m, a.c, log2s, a.inv_tau, act, empty);
+    const RowGrad g(wt * st.slope, -(float)c.entropy_coef * wt, entropy, r.m, a.c, log2s, a.inv_tau, act, empty);
     if constexpr (NV > 0)
       write_grad<E, LANES, NV>(f, &h, out, g, lane, Part{0, f.nfull, true});
     else
       write_grad<E, LANES, 0>(f, nullptr, out, g, lane, Part{0, f.nfull, true});
     if (lane == 0) {
-#pragma unroll
-      for (int k = 0; k < 4; ++k) acc[k] += wt * st.v[k];
-      acc[4] += wt * entropy;
+      if constexpr (LANES > 64) {
+        add_terms(total, st, wt);
+        total[4] += (double)(wt * entropy);
+      } else {
+        add_terms(acc, st, wt);
+        acc[4] += (double)(wt * entropy);
+      }
     }
     if constexpr (LANES > 64) __syncthreads();
+  }
+  if constexpr (LANES > 64) {
+    if (threadIdx.x == 0)
+#pragma unroll
+      for (int k = 0; k < kTerms; ++k) acc[k] = total[k];
   }
   finish_loss<NT>(acc, c, sums);
 }
@@ -63,7 +76,7 @@ __global__ __launch_bounds__(256) void join_loss_kernel(const ActionRows<E> a, c
                                                         const Weights w, const LossOut sums, E* __restrict__ grad) {
   __shared__ int64_t sc[4];
   const float scale = weight_scale<256>(w, sc);
-  float acc[kTerms] = {};
+  double acc[kTerms] = {};
   const int part = blockIdx.x % p.parts;
   const int64_t row = blockIdx.x / p.parts;
   E* out = grad + row * a.A;
@@ -80,12 +93,11 @@ __global__ __launch_bounds__(256) void join_loss_kernel(const ActionRows<E> a, c
     const float lp = empty && x == x ? -INFINITY : ((x - r.m) * a.c - log2s) * kLn2;
     const float entropy = empty ? 0.f : (log2s - r.u / r.s) * kLn2;
     const StepTerms st = step_terms(lp, t.old[row], t.adv[row], t.ref ? t.ref[row] : 0.f, t.ref != nullptr, c);
-    const RowGrad g(wt * st.slope, -c.entropy_coef * wt, entropy, r.m, a.c, log2s, a.inv_tau, act, empty);
+    const RowGrad g(wt * st.slope, -(float)c.entropy_coef * wt, entropy, r.m, a.c, log2s, a.inv_tau, act, empty);
     write_grad<E, 256, 0>(f, nullptr, out, g, threadIdx.x, p.part(part, f.nfull));
     if (threadIdx.x == 0 && part == 0) {
-#pragma unroll
-      for (int k = 0; k < 4; ++k) acc[k] = wt * st.v[k];
-      acc[4] = wt * entropy;
+      add_terms(acc, st, wt);
+      acc[4] = (double)(wt * entropy);
     }
   }
   finish_loss<256>(acc, c, sums);
@@ -98,7 +110,7 @@ __global__ __launch_bounds__(kFewRows) void few_loss_kernel(const ActionRows<E> 
   extern __shared__ float lds[];
   __shared__ int64_t sc[kFewRows / 64];
   const float scale = weight_scale<kFewRows>(w, sc);
-  float acc[kTerms] = {};
+  double acc[kTerms] = {};
   for (int64_t row0 = (int64_t)blockIdx.x * kFewRows; row0 < a.rows; row0 += (int64_t)gridDim.x * kFewRows) {
     const int rows = (int)(a.rows - row0 < kFewRows ? a.rows - row0 : kFewRows);
     const int64_t row = row0 + threadIdx.x;
@@ -123,7 +135,7 @@ __global__ __launch_bounds__(kFewRows) void few_loss_kernel(const ActionRows<E> 
         const float lp = empty && xa == xa ? -INFINITY : ((xa - r.m) * a.c - log2s) * kLn2;
       const float entropy = empty ? 0.f : (log2s - r.u / r.s) * kLn2;
       const StepTerms st = step_terms(lp, old, adv, ref, t.ref != nullptr, c);
-      const RowGrad g(wt * st.slope, -c.entropy_coef * wt, entropy, r.m, a.c, log2s, a.inv_tau, act, empty);
+      const RowGrad g(wt * st.slope, -(float)c.entropy_coef * wt, entropy, r.m, a.c, log2s, a.inv_tau, act, empty);
       if (__any(empty)) {
 #pragma unroll
         for (int j = 0; j < K; ++j)
@@ -134,9 +146,8 @@ __global__ __launch_bounds__(kFewRows) void few_loss_kernel(const ActionRows<E> 
           if (j < K - 3 || j < a.A) x[j] = g(h.x[j]);
         if (g.action >= 0 && g.action < a.A) x[g.action] += g.at;
       }
-#pragma unroll
-      for (int k = 0; k < 4; ++k) acc[k] += wt * st.v[k];
-      acc[4] += wt * entropy;
+      add_terms(acc, st, wt);
+      acc[4] += (double)(wt * entropy);
     } else if (mine) {
       for (int j = 0; j < a.A; ++j) x[j] = 0.f;
     }

@@ -59,16 +59,25 @@ __device__ __forceinline__ T block_sum(T x, T* s) {
 // ---------------------------------------------------------------------------------------
 struct LossConsts {
   float log_low, log_high, log_dual;  // thresholds of D; log_dual = inf: no cap
-  float low, high, dual;              // the values themselves
-  float kl_coef, entropy_coef;
+  float low, high, dual;              // the values themselves, and what float32 leaves out of them
+  float low_rest, high_rest, dual_rest;
+  double kl_coef, entropy_coef;
 };
 
 constexpr int kTerms = 5;  // policy, KL, clipped share, KL to the old policy, entropy
 
+// The bounds come as two floats each: terms of both signs leave a loss that is far smaller than they are, and a bound rounded
+// to one float is off alike in every step that it holds.
 struct StepTerms {
-  float v[4];
+  float policy, kl, clipped, old_kl;
   float slope;
 };
+
+// Adds a step's terms with weight w.
+__device__ __forceinline__ void add_terms(double (&acc)[5], const StepTerms& t, float w) {
+  acc[0] += (double)w * (double)t.policy;
+  acc[1] += (double)(w * t.kl), acc[2] += (double)(w * t.clipped), acc[3] += (double)(w * t.old_kl);
+}
 
 // e^x - 1 - x >= 0 without the cancellation near zero: its series up to 1/2 in size (the first dropped
 // term is below 2^-25 of the sum), the plain difference beyond, where it loses at most two bits.
@@ -93,16 +102,17 @@ __device__ __forceinline__ StepTerms step_terms(float lp, float old, float adv, 
   const bool cap = d > c.log_dual && adv < 0.f;
   const bool flat = up || down || cap;
   const float held = cap ? c.dual : up ? c.high : down ? c.low : r;
-  t.v[0] = -adv * held;
+  const float rest = cap ? c.dual_rest : up ? c.high_rest : down ? c.low_rest : 0.f;
+  t.policy = -fmaf(adv, held, adv * rest);
   t.slope = flat ? 0.f : -adv * r;
-  t.v[2] = flat ? 1.f : 0.f;
-  t.v[3] = exp_minus_linear(d, r);
-  t.v[1] = 0.f;
+  t.clipped = flat ? 1.f : 0.f;
+  t.old_kl = exp_minus_linear(d, r);
+  t.kl = 0.f;
   if (has_ref) {
     const float e = ref - lp;
     const float ee = expf(e);
-    t.v[1] = exp_minus_linear(e, ee);
-    t.slope -= c.kl_coef * (t.v[1] + e);  // e^e - 1
+    t.kl = exp_minus_linear(e, ee);
+    t.slope -= (float)c.kl_coef * (t.kl + e);  // e^e - 1
   }
   return t;
 }
@@ -189,12 +199,12 @@ __device__ __forceinline__ double sum_terms(double (&v)[kTerms], double* s) {
 // that takes.  A release at the ticket would also write back the L2's gradients, once per workgroup ([512,6000] 47 us of a
 // kernel that takes 11).
 template <int NT>
-__device__ __forceinline__ void finish_loss(const float (&acc)[kTerms], const LossConsts& c, const LossOut& o) {
+__device__ __forceinline__ void finish_loss(const double (&acc)[kTerms], const LossConsts& c, const LossOut& o) {
   __shared__ double s[NT / 64 * kTerms];
   __shared__ bool last;
   double v[kTerms];
 #pragma unroll
-  for (int k = 0; k < kTerms; ++k) v[k] = (double)acc[k];
+  for (int k = 0; k < kTerms; ++k) v[k] = acc[k];
   double x = sum_terms<NT>(v, s);
   if (gridDim.x > 1) {
     if (threadIdx.x < kTerms)
@@ -220,7 +230,7 @@ __device__ __forceinline__ void finish_loss(const float (&acc)[kTerms], const Lo
   }
   if ((int)threadIdx.x < o.num_means) o.means[threadIdx.x] = (float)x;
   const double kl = __shfl(x, 1), entropy = __shfl(x, 4);
-  if (threadIdx.x == 0) *o.loss = (float)(x + (double)c.kl_coef * kl - (double)c.entropy_coef * entropy);
+  if (threadIdx.x == 0) *o.loss = (float)(x + c.kl_coef * kl - c.entropy_coef * entropy);
 }
 
 }  // namespace rlk

@@ -74,11 +74,11 @@ struct LossArgs {
 // Steps i .. i + 3 (`left` of them exist): their gradients, their terms added to `acc`.  row_weight(step): what a
 // row's steps count for.
 template <class E, class F>
-__device__ __forceinline__ void four_steps(const LossArgs<E>& a, int64_t i, int left, float4 m, float (&acc)[kTerms], F weight) {
+__device__ __forceinline__ void four_steps(const LossArgs<E>& a, int64_t i, int left, float4 m, double (&acc)[kTerms], F weight) {
   const bool whole = a.whole && left == 4;
   const float4 lp = load4(a.lp + i, whole, left), old = load4(a.old + i, whole, left), adv = load4(a.adv + i, whole, left);
   const float4 ref = a.ref ? load4(a.ref + i, whole, left) : float4{0.f, 0.f, 0.f, 0.f};
-  float g[4];
+  float g[4], policy = 0.f, kl = 0.f, clipped = 0.f, old_kl = 0.f;
   const float *pl = &lp.x, *po = &old.x, *pa = &adv.x, *pr = &ref.x, *pm = &m.x;
 #pragma unroll
   for (int x = 0; x < 4; ++x) {
@@ -86,11 +86,12 @@ __device__ __forceinline__ void four_steps(const LossArgs<E>& a, int64_t i, int 
     if (pm[x] != 0.f && x < left) {
       const float w = weight(i, x);
       const StepTerms t = step_terms(pl[x], po[x], pa[x], pr[x], a.ref != nullptr, a.c);
-#pragma unroll
-      for (int k = 0; k < 4; ++k) acc[k] += w * t.v[k];
+      policy = fmaf(w, t.policy, policy);
+      kl = fmaf(w, t.kl, kl), clipped = fmaf(w, t.clipped, clipped), old_kl = fmaf(w, t.old_kl, old_kl);
       g[x] = w * t.slope;
     }
   }
+  acc[0] += policy, acc[1] += kl, acc[2] += clipped, acc[3] += old_kl;
   if (whole) {
     store_quad(a.grad + i, float4{g[0], g[1], g[2], g[3]});
   } else {
@@ -106,7 +107,7 @@ template <class E>
 __global__ __launch_bounds__(kNT) void loss_kernel(const LossArgs<E> a) {
   __shared__ int64_t sc[kNT / 64];
   const float scale = weight_scale<kNT>(a.w, sc);
-  float acc[kTerms] = {};
+  double acc[kTerms] = {};
   const int64_t step = (int64_t)gridDim.x * kNT * 4;
   for (int64_t i = ((int64_t)blockIdx.x * kNT + threadIdx.x) * 4; i < a.n; i += step) {
     const int left = (int)(a.n - i < 4 ? a.n - i : 4);
@@ -166,7 +167,7 @@ __global__ __launch_bounds__(kSmallNT) void small_loss_kernel(const LossArgs<E> 
     count = block_sum<kSmallNT>(count, sums);
     scale = count > 0 ? 1.f / (float)count : 0.f;
   }
-  float acc[kTerms] = {};
+  double acc[kTerms] = {};
 #pragma unroll
   for (int q = 0; q < Q; ++q) {
     const int i = (q * kSmallNT + threadIdx.x) * 4;
@@ -194,7 +195,7 @@ int loss_impl(const void* lp, int64_t E_, int64_t T, const rlk_policy_terms* t, 
                 static_cast<const E*>(t->ref_log_probs), static_cast<const E*>(t->mask), static_cast<E*>(grad),
                 n, T, false, plan.consts, plan.weights, plan.out};
   a.whole = quad_aligned(a.lp, a.old, a.adv, a.ref, a.mask, a.grad);
-  a.c.entropy_coef = 0.f;  // (there are no entropies here)
+  a.c.entropy_coef = 0.0;  // (there are no entropies here)
   if (n <= kSmallSteps) {
     small_loss_kernel<E><<<dim3(1), dim3(kSmallNT), 0, s>>>(a);
   } else {
@@ -230,17 +231,19 @@ int count_impl(const rlk_policy_terms* t, int64_t E_, int64_t T, LossPlan* p, hi
 int plan_loss(const rlk_policy_terms* t, int64_t num_envs, int64_t seq_len, int means, LossPlan* p) {
   if (!t || num_envs < 0 || seq_len < 0 || !t->loss || !t->means) return RLK_ERR_INVALID_ARGUMENT;
   if (num_envs * seq_len > 0 && (!t->old_log_probs || !t->advantages)) return RLK_ERR_INVALID_ARGUMENT;
-  if (!(t->clip_low >= 0.f) || !(t->clip_high >= 0.f) || !(t->dual_clip == 0.f || t->dual_clip > 1.f))
+  if (!(t->clip_low >= 0.0) || !(t->clip_high >= 0.0) || !(t->dual_clip == 0.0 || t->dual_clip > 1.0))
     return RLK_ERR_INVALID_ARGUMENT;
   if (seq_len > (int64_t{1} << 30)) return RLK_ERR_INVALID_ARGUMENT;  // (a row's count is an int)
   if (!t->workspace || t->workspace_bytes < rlk_policy_workspace_bytes(num_envs) ||
       (reinterpret_cast<uintptr_t>(t->workspace) & 7u) != 0)
     return RLK_ERR_WORKSPACE;
   LossConsts& c = p->consts;
-  c.low = 1.f - t->clip_low, c.high = 1.f + t->clip_high;
-  c.log_low = t->clip_low < 1.f ? (float)std::log1p(-(double)t->clip_low) : -INFINITY;
-  c.log_high = (float)std::log1p((double)t->clip_high);
-  c.dual = t->dual_clip, c.log_dual = t->dual_clip > 0.f ? (float)std::log((double)t->dual_clip) : INFINITY;
+  const double low = 1.0 - t->clip_low, high = 1.0 + t->clip_high, dual = t->dual_clip;
+  c.low = (float)low, c.high = (float)high, c.dual = (float)dual;
+  c.low_rest = (float)(low - (double)c.low), c.high_rest = (float)(high - (double)c.high), c.dual_rest = (float)(dual - (double)c.dual);
+  c.log_low = t->clip_low < 1.0 ? (float)std::log1p(-t->clip_low) : -INFINITY;
+  c.log_high = (float)std::log1p(t->clip_high);
+  c.log_dual = t->dual_clip > 0.0 ? (float)std::log(t->dual_clip) : INFINITY;
   c.kl_coef = t->kl_coef, c.entropy_coef = t->entropy_coef;
   char* ws = static_cast<char*>(t->workspace);
   p->out = {reinterpret_cast<double*>(ws + kTicketBytes), reinterpret_cast<uint32_t*>(ws), t->loss, t->means, means};

@@ -93,7 +93,7 @@ bool logit_rows(PolicyCall& c, PyObject* logits, PyObject* actions, PyObject* te
   const double tau = c.number(temperature, 0.0);
   if (!c.ok || !(tau > 0.0)) return false;
   r->logits = t->data_ptr(), r->actions = static_cast<const int64_t*>((*a)->data_ptr());
-  r->temperature = (float)tau, r->bf16 = t->scalar_type() == at::kBFloat16;
+  r->temperature = tau, r->bf16 = t->scalar_type() == at::kBFloat16;
   return true;
 }
 
@@ -117,12 +117,12 @@ bool loss_terms(PolicyCall& c, PyObject* old, PyObject* adv, PyObject* ref, PyOb
                 PyObject* mask, PyObject* reduction, at::ScalarType st, at::IntArrayRef sizes, const at::Tensor& like,
                 rlk_policy_terms* t) {
   const at::Tensor *o = c.array(old, st, sizes), *ad = c.array(adv, st, sizes), *r = c.opt(ref, st, sizes), *m = c.opt(mask, st, sizes);
-  t->clip_low = (float)c.number(low, 0.0), t->clip_high = (float)c.number(high, 0.0);
-  t->kl_coef = (float)c.number(kl, -HUGE_VAL);
+  t->clip_low = c.number(low, 0.0), t->clip_high = c.number(high, 0.0);
+  t->kl_coef = c.number(kl, -HUGE_VAL);
   if (dual != Py_None) {
     const double d = c.number(dual, 1.0);
-    if (!((float)d > 1.f)) return false;
-    t->dual_clip = (float)d;
+    if (!(d > 1.0)) return false;
+    t->dual_clip = d;
   }
   if (!c.ok || !PyUnicode_Check(reduction)) return false;
   if (PyUnicode_CompareWithASCIIString(reduction, "rows") == 0) t->per_row = 1;
@@ -165,7 +165,7 @@ PyObject* op_policy_loss_from_logits(PyObject* const* a, Py_ssize_t n) {
   const at::Tensor *x, *act;
   if (!logit_rows(c, a[0], a[1], a[9], false, &r, &x, &act) || x->dim() != 3) return decline();
   rlk_policy_terms t = {};
-  t.entropy_coef = (float)c.number(a[8], -HUGE_VAL);
+  t.entropy_coef = c.number(a[8], -HUGE_VAL);
   if (!loss_terms(c, a[2], a[3], a[4], a[5], a[6], a[7], a[10], a[11], a[12], at::kFloat, act->sizes(), *x, &t)) return decline();
   at::Tensor loss = policy_output({}, at::kFloat, *x), grad = policy_output(x->sizes(), x->scalar_type(), *x),
              means = policy_output({5}, at::kFloat, *x);

@@ -12,12 +12,13 @@ import torch
 
 from rl_triton import _native
 
-_P, _I64, _F, _INT, _SZ = ctypes.c_void_p, ctypes.c_int64, ctypes.c_float, ctypes.c_int, ctypes.c_size_t
+_P, _I64, _F, _D, _INT, _SZ = (ctypes.c_void_p, ctypes.c_int64, ctypes.c_float, ctypes.c_double, ctypes.c_int,
+                               ctypes.c_size_t)
 
 
 class ActionRows(ctypes.Structure):
     _fields_ = [("logits", _P), ("actions", _P), ("num_envs", _I64), ("seq_len", _I64), ("num_actions", _I64),
-                ("env_stride", _I64), ("step_stride", _I64), ("temperature", _F), ("bf16", _INT),
+                ("env_stride", _I64), ("step_stride", _I64), ("temperature", _D), ("bf16", _INT),
                 ("workspace", _P), ("workspace_bytes", _SZ)]
 
 
@@ -25,8 +26,8 @@ ROWS_WORKSPACE_BYTES = 12288
 
 
 class PolicyTerms(ctypes.Structure):
-    _fields_ = [("old_log_probs", _P), ("advantages", _P), ("ref_log_probs", _P), ("mask", _P), ("clip_low", _F),
-                ("clip_high", _F), ("dual_clip", _F), ("kl_coef", _F), ("entropy_coef", _F), ("per_row", _INT),
+    _fields_ = [("old_log_probs", _P), ("advantages", _P), ("ref_log_probs", _P), ("mask", _P), ("clip_low", _D),
+                ("clip_high", _D), ("dual_clip", _D), ("kl_coef", _D), ("entropy_coef", _D), ("per_row", _INT),
                 ("bf16", _INT), ("loss", _P), ("means", _P), ("workspace", _P), ("workspace_bytes", _SZ)]
 
 
