@@ -211,10 +211,11 @@ __device__ __forceinline__ void finish_loss(const double (&acc)[kTerms], const L
       __hip_atomic_store(o.partials + (int64_t)blockIdx.x * kPartials + threadIdx.x, x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     if (threadIdx.x == 0) {
       const uint32_t group = blockIdx.x % kTicketGroups, members = (gridDim.x - group + kTicketGroups - 1) / kTicketGroups;
-      const uint32_t groups = gridDim.x < kTicketGroups ? gridDim.x : kTicketGroups;
+      const bool grouped = gridDim.x > kTicketGroups;
+      const uint32_t groups = grouped ? kTicketGroups : gridDim.x;
       uint32_t *mine = o.tickets + group * kTicketStride, *all = o.tickets + kTicketGroups * kTicketStride;
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (the wavefront's stores: the sums' among them)
-      last = __hip_atomic_fetch_add(mine, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == members - 1 &&
+      last = (!grouped || __hip_atomic_fetch_add(mine, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == members - 1) &&
              __hip_atomic_fetch_add(all, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == groups - 1;
     }
     __syncthreads();

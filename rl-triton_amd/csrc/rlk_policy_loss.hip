@@ -127,54 +127,39 @@ __global__ __launch_bounds__(kNT) void loss_kernel(const LossArgs<E> a) {
   finish_loss<kNT>(acc, a.c, a.out);
 }
 
-// Small calls: one workgroup counts, computes and sums, and there is one launch to wait for.
-constexpr int kSmallNT = 1024, kSmallSteps = 8192;
+// Small masked calls: one workgroup counts, computes and sums, in one launch ([16,128] 8.8 us in a graph, 10.7 in two; at
+// [32,128] 10.3 and 10.7, at [64,128] 13.1 and 10.9).  Without a mask there is nothing to count, and loss_kernel is one launch.
+constexpr int kSmallNT = 512, kSmallSteps = 4 * kSmallNT;
 
 template <class E>
 __global__ __launch_bounds__(kSmallNT) void small_loss_kernel(const LossArgs<E> a) {
   __shared__ int counts[kSmallSteps];
   __shared__ int sums[kSmallNT / 64];
-  constexpr int Q = kSmallSteps / (4 * kSmallNT);
-  const int n = (int)a.n, T = (int)a.seq_len;
-  float4 m[Q];
-  float scale = a.w.all;
-  const bool rows = a.mask != nullptr && a.w.per_row;
-#pragma unroll
-  for (int q = 0; q < Q; ++q) {
-    const int i = (q * kSmallNT + threadIdx.x) * 4, left = n - i < 4 ? n - i : 4;
-    m[q] = i >= n ? float4{0.f, 0.f, 0.f, 0.f} : a.mask ? load4(a.mask + i, a.whole && left == 4, left) : kAll;
+  const int n = (int)a.n, T = (int)a.seq_len, i = 4 * threadIdx.x, left = n - i < 4 ? n - i : 4;
+  const bool rows = a.w.per_row;
+  float4 m{0.f, 0.f, 0.f, 0.f};
+  if (i < n) m = load4(a.mask + i, a.whole && left == 4, left);
+  int count = 0;
+  if (rows) {
+    for (int e = threadIdx.x; e * T < n; e += kSmallNT) counts[e] = 0;
+    __syncthreads();
   }
-  if (a.mask != nullptr) {
-    int count = 0;
-    if (rows) {
-      for (int e = threadIdx.x; e * T < n; e += kSmallNT) counts[e] = 0;
-      __syncthreads();
-    }
+  const float* pm = &m.x;
 #pragma unroll
-    for (int q = 0; q < Q; ++q) {
-      const float* pm = &m[q].x;
-#pragma unroll
-      for (int x = 0; x < 4; ++x)
-        if (pm[x] != 0.f) {
-          if (rows) atomicAdd(&counts[((q * kSmallNT + threadIdx.x) * 4 + x) / T], 1);
-          else ++count;
-        }
+  for (int x = 0; x < 4; ++x)
+    if (pm[x] != 0.f) {
+      if (rows) atomicAdd(&counts[(i + x) / T], 1);
+      else ++count;
     }
-    if (rows) {
-      __syncthreads();
-      for (int e = threadIdx.x; e * T < n; e += kSmallNT) count += counts[e] > 0;
-    }
-    count = block_sum<kSmallNT>(count, sums);
-    scale = count > 0 ? 1.f / (float)count : 0.f;
+  if (rows) {
+    __syncthreads();
+    for (int e = threadIdx.x; e * T < n; e += kSmallNT) count += counts[e] > 0;
   }
+  count = block_sum<kSmallNT>(count, sums);
+  const float scale = count > 0 ? 1.f / (float)count : 0.f;
   double acc[kTerms] = {};
-#pragma unroll
-  for (int q = 0; q < Q; ++q) {
-    const int i = (q * kSmallNT + threadIdx.x) * 4;
-    if (i < n)
-      four_steps(a, i, n - i < 4 ? n - i : 4, m[q], acc,
-                 [&](int64_t at, int x) { return rows ? scale / (float)counts[((int)at + x) / T] : scale; });
-  }
+  if (i < n)
+    four_steps(a, i, left, m, acc, [&](int64_t at, int x) { return rows ? scale / (float)counts[((int)at + x) / T] : scale; });
   finish_loss<kSmallNT>(acc, a.c, a.out);
 }
 
@@ -196,7 +181,7 @@ int loss_impl(const void* lp, int64_t E_, int64_t T, const rlk_policy_terms* t, 
                 n, T, false, plan.consts, plan.weights, plan.out};
   a.whole = quad_aligned(a.lp, a.old, a.adv, a.ref, a.mask, a.grad);
   a.c.entropy_coef = 0.0;  // (there are no entropies here)
-  if (n <= kSmallSteps) {
+  if (t->mask && n <= kSmallSteps) {
     small_loss_kernel<E><<<dim3(1), dim3(kSmallNT), 0, s>>>(a);
   } else {
     if ((st = launch_count(t, E_, T, &plan, s)) != RLK_OK) return st;
