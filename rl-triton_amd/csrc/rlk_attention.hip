@@ -88,6 +88,12 @@ struct Quad<bf16> {
   __device__ static Quad load(const bf16* p) { return {*reinterpret_cast<const u32x2*>(p)}; }
   __device__ void store(bf16* p) const { *reinterpret_cast<u32x2*>(p) = w; }
   __device__ void clear() { w = u32x2{0, 0}; }
+  // sum + each element's square
+  __device__ float squares(float sum) const {
+    typedef __bf16 pair __attribute__((ext_vector_type(2)));
+    const pair x = __builtin_bit_cast(pair, (uint32_t)w[0]), y = __builtin_bit_cast(pair, (uint32_t)w[1]);
+    return __builtin_amdgcn_fdot2_f32_bf16(y, y, __builtin_amdgcn_fdot2_f32_bf16(x, x, sum, false), false);
+  }
   // element x of four quads
   template <int X>
   __device__ static Quad across(const Quad& a, const Quad& b, const Quad& c, const Quad& d) {
@@ -103,6 +109,7 @@ struct Quad<float> {
   __device__ static Quad load(const float* p) { return {*reinterpret_cast<const f32x4*>(p)}; }
   __device__ void store(float* p) const { *reinterpret_cast<f32x4*>(p) = w; }
   __device__ void clear() { w = f32x4{0.f, 0.f, 0.f, 0.f}; }
+  __device__ float squares(float sum) const { return fmaf(w[3], w[3], fmaf(w[2], w[2], fmaf(w[1], w[1], fmaf(w[0], w[0], sum)))); }
   template <int X>
   __device__ static Quad across(const Quad& a, const Quad& b, const Quad& c, const Quad& d) {
     return {{a.w[X], b.w[X], c.w[X], d.w[X]}};
@@ -125,9 +132,10 @@ struct Lds {
   // Two chunks where they fit (160 KB a CU; two workgroups of it for bfloat16 dims of up to 64): the next one is put down
   // while this one is worked on.
   static constexpr int P_BYTES = C * PROW;                   // (a_i . b_j) lambda^{i-j} same(j, i)
-  static constexpr int CHUNKS = 2 * CHUNK + P_BYTES <= 160 * 1024 ? 2 : 1;
+  static constexpr int CHUNKS = 2 * (CHUNK + 32) + P_BYTES <= 160 * 1024 ? 2 : 1;
   static constexpr int P = CHUNKS * CHUNK;
-  static constexpr int BYTES = P + P_BYTES;
+  static constexpr int TAINT = P + P_BYTES;  // [CHUNKS][8]: whether a wavefront has put down an inf, a NaN or a value near the type's largest
+  static constexpr int BYTES = TAINT + CHUNKS * 32;
   // Where a transposed tile holds row d, column j.  The 16-byte units of a row are exchanged with d's low bits: a write has
   // lanes at every fourth row, a read at consecutive ones, and f takes all 8 values over either set, so both spread over
   // all banks (with padded rows the writes met in an eighth of them: 20 of 75 us of a [64,1024,8,64] call).
@@ -190,6 +198,11 @@ struct Part {
         x[r] = Quad<E>::bits(e[0], col + 1 < dim ? e[1] : zero, col + 2 < dim ? e[2] : zero, col + 3 < dim ? e[3] : zero);
       }
     }
+  }
+  __device__ __forceinline__ float squares(float sum) const {
+#pragma unroll
+    for (int r = 0; r < R; ++r) sum = x[r].squares(sum);
+    return sum;
   }
   // to `at` and three rows on
   __device__ __forceinline__ void put(char* at) const {
@@ -408,6 +421,10 @@ __global__ __launch_bounds__(4 * D, D == 64 && sizeof(E) == 4 ? 1 : 2) void walk
       pc.template clip<VEC>(dc, L);
     }
     char* to = lds + buffer;
+    float sum = pc.squares(pb.squares(0.f));
+    if constexpr (!STATE) sum = pa.squares(sum);
+    const bool tainted = __any(!(sum < 0x1p120f));  // (else each is below 2^60, and no product of two rows overflows)
+    if (lane == 0) *reinterpret_cast<int*>(lds + M::TAINT + (buffer != 0 ? 32 : 0) + 4 * wave) = tainted;
     if constexpr (!STATE) {
       pa.put(to + at_row);
       pb.put(to + at_row + (M::B - M::A));
@@ -418,9 +435,12 @@ __global__ __launch_bounds__(4 * D, D == 64 && sizeof(E) == 4 ? 1 : 2) void walk
     return found;
   };
 
-  // One chunk.  PLAIN: whole, without a cut, and not the one that a state leaves the sequence with.
+  // One chunk, unless it is tainted.  PLAIN: whole, without a cut, and not the one that a state leaves the sequence with.
   auto chunk = [&](auto plain, int64_t s0, int L, uint64_t cuts, bool end, const char* tile) {
     constexpr bool PLAIN = decltype(plain)::value;
+    const int4* marks = reinterpret_cast<const int4*>(lds + M::TAINT + (tile != lds ? 32 : 0));
+    int4 mark = marks[0];
+    if constexpr (D == 128) mark.x |= marks[1].x | marks[1].y | marks[1].z | marks[1].w;
     // operands that take more registers: loads of more than the next two are kept from moving up
     auto apart = [] {
       if constexpr (sizeof(E) == 4 || D == 128) __builtin_amdgcn_sched_barrier(0);
@@ -460,6 +480,7 @@ __global__ __launch_bounds__(4 * D, D == 64 && sizeof(E) == 4 ? 1 : 2) void walk
       }
       __syncthreads();
     }
+    if (__builtin_amdgcn_readfirstlane(mark.x | mark.y | mark.z | mark.w) != 0) return false;
 
     Frag<E> fc[2];
 #pragma unroll
@@ -544,6 +565,44 @@ __global__ __launch_bounds__(4 * D, D == 64 && sizeof(E) == 4 ? 1 : 2) void walk
         }
       }
     }
+    return true;
+  };
+
+  // A chunk that holds an inf, a NaN or values whose products overflow, step by step: as products of matrices it would put
+  // them (0 inf = NaN) where the recurrence does not, in steps before them and past an episode's end.  bfloat16 [1,16384,16,128]: 122 us
+  // without such a chunk, 2539 with one in every chunk; looking for them costs 3% ([64,1024,8,64] training 264 -> 269).
+  auto careful = [&](int64_t s0, int L, uint64_t cuts, bool end, const char* tile) {
+    int v16 = l16, v4 = l4;
+    for (int i = 0; i < L; ++i) {
+      asm volatile("" : "+v"(v16), "+v"(v4));  // (as in `chunk`)
+      const int j = 16 * wave + v16;
+      const float c = load_one(reinterpret_cast<const E*>(tile + M::CT + M::transposed(j, i)));
+      const float keep = i == 0 ? 1.f : lambda;
+      const bool cut = (cuts >> i) & 1;
+      float sum = 0.f;
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int d = 16 * m + 4 * v4 + r;
+          const float b = load_one(reinterpret_cast<const E*>(tile + M::BT + M::transposed(d, i)));
+          U[m][r] = fmaf(b, c, cut || keep == 0.f ? 0.f : U[m][r] * keep);
+          if constexpr (!STATE) sum = fmaf(load_one(reinterpret_cast<const E*>(tile + M::A + i * M::ROW + d * M::S)), U[m][r], sum);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      if constexpr (!STATE) {
+        sum += __shfl_xor(sum, 16);
+        sum += __shfl_xor(sum, 32);
+        if (v4 == 0 && j < dc) gy[(i - v16) * ystep + v16] = from_f32<E>(sum * w.scale);
+      }
+    }
+    if constexpr (!STATE) gy += C * ystep;
+    if (!end)
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) U[m][r] = lambda == 0.f ? 0.f : U[m][r] * lambda;
   };
 
   int buffer = 0;
@@ -553,8 +612,9 @@ __global__ __launch_bounds__(4 * D, D == 64 && sizeof(E) == 4 ? 1 : 2) void walk
     const int L = (int)(last - s0 < C ? last - s0 : C);
     const bool end = !reverse && s0 + C >= T;
     crossed |= cuts != 0;
-    if (L == C && cuts == 0 && !end) chunk(std::true_type{}, s0, L, cuts, end, lds + buffer);
-    else chunk(std::false_type{}, s0, L, cuts, end, lds + buffer);
+    const bool whole_chunk = L == C && cuts == 0 && !end;
+    if (!(whole_chunk ? chunk(std::true_type{}, s0, L, cuts, end, lds + buffer) : chunk(std::false_type{}, s0, L, cuts, end, lds + buffer)))
+      careful(s0, L, cuts, end, lds + buffer);
     if (s0 + C >= last) break;
     if constexpr (M::CHUNKS == 2) buffer ^= M::CHUNK;
     else __syncthreads();  // the chunk has been read

@@ -119,8 +119,8 @@ def compute_linear_attention(
     calls round the products of queries and keys, and the state where outputs are read from it, to bfloat16.
     Differentiable in q, k, v and state.
 
-    A chunk is multiplied as a whole: an inf or NaN in q, k or v makes outputs of its environment and head NaN from up to
-    63 steps before it, across an episode's end too.
+    What is not finite, in padded steps for one, reaches no step before it and none past its episode's end; a chunk that
+    holds such values is computed step by step, in some twenty times the time.
 
     Args:
         q, k:  [num_envs, seq_len, heads, dim_k], float32 or bfloat16, GPU; any strides with a contiguous last axis

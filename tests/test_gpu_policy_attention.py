@@ -206,6 +206,70 @@ def test_a_cut_state_has_no_part():
     assert bool(o.isfinite().all()) and bool(new.isfinite().all())
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("d", [24, 64, 100, 128])
+def test_values_that_are_not_finite_stay_where_they_belong(d, dtype):
+    """An inf, a NaN or a value whose products overflow, in q, k, v or an upstream gradient (garbage in padded steps is such a
+    value), reaches what it reaches in the recurrence: nothing before it, nothing past its episode's end."""
+    E, T, H = 2, 200, 2
+    q, k, v, decay, _, s = _make(E, T, H, d, d, 7, dtype)
+    dones = torch.zeros(E, T)
+    dones[:, [59, 70, 71, 150]] = 1
+    gen = torch.Generator().manual_seed(1)
+    go, gs = torch.randn(E, T, H, d, generator=gen).to(dtype), torch.randn(E, H, d, d, generator=gen)
+    # head 0 of environment 0, the episode of the steps 60..70: what is not finite
+    q[0, 65, 0, 3], k[0, 66, 0, 1], v[0, 67, 0, 2], v[0, 68, 0, 5], go[0, 66, 0, 0] = math.nan, math.inf, -math.inf, math.nan, math.inf
+    k[0, 70, 0] = math.nan
+    # head 1 of environment 1: the type's lowest and largest values
+    low = torch.finfo(dtype).min
+    q[1, 65:68, 1], k[1, 65:68, 1], v[1, 65:68, 1], go[1, 65:68, 1] = low, low, -low, -low
+    huge = torch.zeros(E, T, H, dtype=torch.bool)
+    huge[1, 60:71, 1] = True
+
+    leaves = [t.requires_grad_() for t in _cuda(q, k, v, s)]
+    out, last = policy.compute_linear_attention(leaves[0], leaves[1], leaves[2], *_cuda(decay, dones), leaves[3], 0.3)
+    got = (out, last, *torch.autograd.grad((out, last), leaves, _cuda(go, gs)))
+    q, k, v, s = (t.detach() for t in (q, k, v, s))
+    args = (q, k, v, decay, dones, s, 0.3)
+    want = (*attention(*args), *attention_grads(*args, go, gs))
+    by, bs = _bounds(args, dtype, T)
+    sizes = attention_grads(q.abs(), k.abs(), v.abs(), decay, dones, s.abs(), 0.3, go.abs(), gs.abs())
+    wide = dtype == torch.bfloat16
+    bounds = (by, bs, *[x * ((T + 128) * U32 + ((U16 * U16 if i == 3 else U16) if wide else 0)) for i, x in enumerate(sizes)])
+    for i, (x, w, bound) in enumerate(zip(got, want, bounds)):
+        unit = (U16 if wide and i not in (1, 5) else 0) + U32
+        x = x.detach().cpu().double()
+        if i not in (1, 5):  # (a state belongs to no step)
+            before = huge.clone()
+            before[:, 65:] = False  # outputs and their queries' gradients from before them
+            seen = ~huge | before if i == 0 else ~huge
+            x, w, bound = x[seen], w[seen], bound[seen]
+        kept = w.isfinite()
+        assert bool((x.isfinite() == kept).all()), i
+        _within(x[kept], w[kept], bound[kept], unit)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_step_of_large_states(dtype):
+    """States of 256 MB and more, which take another path through the caches; bounds as above."""
+    E, H, d = 4096 + 3, 1, 128
+    g = torch.Generator(device="cuda").manual_seed(3)
+    q, k, v = (torch.randn(E, H, d, generator=g, device="cuda").to(dtype) for _ in range(3))
+    s, decay = torch.randn(E, H, d, d, generator=g, device="cuda"), torch.tensor([0.75], device="cuda")
+    done = (torch.rand(E, generator=g, device="cuda") < 0.25).float()
+    out, new = policy.compute_linear_attention_step(q, k, v, decay, s, done, 0.5)
+    lam = torch.where(done != 0, 0.0, 0.75)[:, None, None, None]
+    for part in (slice(0, 300), slice(E - 300, E)):
+        S = s[part].double() * lam[part] + k[part].double()[..., :, None] * v[part].double()[..., None, :]
+        size = s[part].double().abs() * lam[part] + k[part].double().abs()[..., :, None] * v[part].double().abs()[..., None, :]
+        assert bool(((new[part].double() - S).abs() <= 4 * U32 * size).all())
+        y = (q[part].double()[..., :, None] * S).sum(-2) * 0.5
+        bound = (d + 8) * U32 * (q[part].double().abs()[..., :, None] * size).sum(-2) * 0.5
+        assert bool(((out[part].double() - y).abs() <= bound + (U16 if dtype == torch.bfloat16 else 0) * y.abs()).all())
+    again, same = policy.compute_linear_attention_step(q, k, v, decay, s, done, 0.5, out_state=s)
+    assert same is s and torch.equal(again, out) and torch.equal(s, new)
+
+
 def test_more_pairs_than_a_launch_takes():
     """Two million sequences of two steps, nine million single steps: several launches over ranges of environments.  Two
     products and a sum a result: 8 u of the sizes."""
