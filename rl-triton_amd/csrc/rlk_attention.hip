@@ -116,6 +116,15 @@ struct Quad<float> {
   }
 };
 
+// After matrix products that branches lead around: a copy of a result, which such a way reaches within a few instructions, was
+// emitted without the wait that it needs, and read the sums of before (states wrong in two rows of four).  So the wait
+// stands here, in the way of everything.
+__device__ __forceinline__ void settle() {
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("s_nop 9");
+  __builtin_amdgcn_sched_barrier(0);
+}
+
 // x^n for n >= 0 from log2 x (x = 0: 1, 0, 0, ...).
 __device__ __forceinline__ float power(float log2x, int n) { return n == 0 ? 1.f : __builtin_amdgcn_exp2f(log2x * (float)n); }
 
@@ -371,10 +380,6 @@ __global__ __launch_bounds__(4 * D, D == 64 && sizeof(E) == 4 ? 1 : 2) void walk
       }
 #pragma unroll
     for (int t = 0; t < 4; ++t) back[t] = power(lg, 16 * t + l16) * w.scale;
-    // the steps after a row's own tile, in the operand that ends with it: never written again
-    if ((ti & 1) == 0)
-      Quad<E>::of(f32x4{0.f, 0.f, 0.f, 0.f})
-          .store(reinterpret_cast<E*>(lds + M::P + (16 * ti + l16) * M::PROW + (16 * (ti + 1) + 4 * l4) * M::S));
   }
   float onward[2];  // lambda^{C-j} of the steps j = 32 kk + 8 l4 + 7; the 7 before are lambda times the next
 #pragma unroll
@@ -450,6 +455,11 @@ __global__ __launch_bounds__(4 * D, D == 64 && sizeof(E) == 4 ? 1 : 2) void walk
     int v16 = l16, v4 = l4;
     if constexpr (!PLAIN) asm volatile("" : "+v"(v16), "+v"(v4));
     if constexpr (!STATE) {
+      int begin = 0;  // of row i's episode: the last cut at or before it
+      if (!PLAIN && cuts != 0) {
+        const uint64_t before = cuts & (((uint64_t)2 << (16 * ti + v16)) - 1);
+        begin = before != 0 ? 63 - __clzll((long long)before) : 0;
+      }
       f32x4 pts[TILES];
 #pragma unroll
       for (int u = 0; u < TILES; ++u) pts[u] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -459,22 +469,20 @@ __global__ __launch_bounds__(4 * D, D == 64 && sizeof(E) == 4 ? 1 : 2) void walk
         const Frag<E> fa = Frag<E>::load(tile + at_a + 32 * kk * M::S);
 #pragma unroll
         for (int u = 0; u < TILES; ++u) {
-          const int jt = wave % SHARE + SHARE * u;
-          if (jt <= ti) pts[u] = mma(Frag<E>::load(tile + at_b + 16 * SHARE * u * M::ROW + 32 * kk * M::S), fa, pts[u]);
+          // (tiles past the diagonal too, whose `among` is 0: the wavefront with the last rows has none, the others would wait for it)
+          pts[u] = mma(Frag<E>::load(tile + at_b + 16 * SHARE * u * M::ROW + 32 * kk * M::S), fa, pts[u]);
         }
       }
+      if constexpr (!FULL) settle();
 #pragma unroll
       for (int u = 0; u < TILES; ++u) {
         const int jt = wave % SHARE + SHARE * u;
-        if (jt > ti) continue;
         f32x4 pt = pts[u];
         pt *= among[u];
         if (!PLAIN && cuts != 0) {
-          // two steps belong together when as many cuts lie before or at each of them
-          const int i = 16 * ti + v16, before = __popcll(cuts & (((uint64_t)2 << i) - 1));
 #pragma unroll
           for (int r = 0; r < 4; ++r)
-            if (__popcll(cuts & (((uint64_t)2 << (16 * jt + 4 * v4 + r)) - 1)) != before) pt[r] = 0.f;
+            if (16 * jt + 4 * v4 + r < begin) pt[r] = 0.f;
         }
         Quad<E>::of(pt).store(reinterpret_cast<E*>(lds + at_p_put + 16 * SHARE * u * M::S));
       }
@@ -503,6 +511,7 @@ __global__ __launch_bounds__(4 * D, D == 64 && sizeof(E) == 4 ? 1 : 2) void walk
           if (t & 1) apart();
         }
       }
+      if constexpr (!FULL) settle();
       // the first step that the state does not reach
       const int until = PLAIN || cuts == 0 ? C : __ffsll((long long)cuts) - 1;
 #pragma unroll
@@ -551,11 +560,13 @@ __global__ __launch_bounds__(4 * D, D == 64 && sizeof(E) == 4 ? 1 : 2) void walk
 #pragma unroll
         for (int x = 6; x >= 0; --x) f[x] = f[x + 1] * lambda;
         if constexpr (!PLAIN) {
+          const int j = 32 * kk + 8 * v4;
+          if (reach != C) {
 #pragma unroll
-          for (int x = 0; x < 8; ++x) {
-            const int j = 32 * kk + 8 * v4 + x;
-            f[x] = j >= from && j < L ? power(lg, reach - j) : 0.f;
+            for (int x = 0; x < 8; ++x) f[x] = j + x < L ? power(lg, reach - j - x) : 0.f;
           }
+#pragma unroll
+          for (int x = 0; x < 8; ++x) f[x] = j + x >= from ? f[x] : 0.f;
         }
         const Weighted<E> wc(fc[kk], f);
 #pragma unroll
@@ -564,6 +575,7 @@ __global__ __launch_bounds__(4 * D, D == 64 && sizeof(E) == 4 ? 1 : 2) void walk
           if (m & 1) apart();
         }
       }
+      settle();
     }
     return true;
   };
