@@ -141,9 +141,10 @@ struct Lds {
   // Two chunks where they fit (160 KB a CU; two workgroups of it for bfloat16 dims of up to 64): the next one is put down
   // while this one is worked on.
   static constexpr int P_BYTES = C * PROW;                   // (a_i . b_j) lambda^{i-j} same(j, i)
-  static constexpr int CHUNKS = 2 * (CHUNK + 32) + P_BYTES <= 160 * 1024 ? 2 : 1;
-  static constexpr int P = CHUNKS * CHUNK;
-  static constexpr int TAINT = P + P_BYTES;  // [CHUNKS][8]: whether a wavefront has put down an inf, a NaN or a value near the type's largest
+  static constexpr bool OVER = S == 4 && D == 64;            // p in the place of b's rows, which are read for nothing else
+  static constexpr int CHUNKS = !OVER && 2 * (CHUNK + 32) + P_BYTES <= 160 * 1024 ? 2 : 1;
+  static constexpr int P = OVER ? B : CHUNKS * CHUNK;
+  static constexpr int TAINT = CHUNKS * CHUNK + (OVER ? 0 : P_BYTES);  // [CHUNKS][8]: whether a wavefront has put down an inf, a NaN or a value near the type's largest
   static constexpr int BYTES = TAINT + CHUNKS * 32;
   // Where a transposed tile holds row d, column j.  The 16-byte units of a row are exchanged with d's low bits: a write has
   // lanes at every fourth row, a read at consecutive ones, and f takes all 8 values over either set, so both spread over
@@ -289,7 +290,7 @@ struct Place {
 // FORM 2: dims of exactly D; 1: dims are multiples of 4, tiles of the padded dims that hold nothing are skipped;
 // 0: any dims and alignment, element by element.
 template <class E, int D, int FORM, bool STATE>
-__global__ __launch_bounds__(4 * D, D == 64 && sizeof(E) == 4 ? 1 : 2) void walk_kernel(const Walks<E> walks) {
+__global__ __launch_bounds__(4 * D, 2) void walk_kernel(const Walks<E> walks) {
   typedef Lds<E, D> M;
   __shared__ __align__(16) char lds[M::BYTES];
   constexpr int MT = D / 16, KK = D / 32;
@@ -474,6 +475,7 @@ __global__ __launch_bounds__(4 * D, D == 64 && sizeof(E) == 4 ? 1 : 2) void walk
         }
       }
       if constexpr (!FULL) settle();
+      if constexpr (M::OVER) __syncthreads();
 #pragma unroll
       for (int u = 0; u < TILES; ++u) {
         const int jt = wave % SHARE + SHARE * u;
