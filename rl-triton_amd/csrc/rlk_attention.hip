@@ -75,6 +75,14 @@ __device__ __forceinline__ f32x4 mma(const Frag<float>& a, const Frag<float>& b,
   return acc;
 }
 
+// The first 16 of the inner indices only, where the operands' `lo` hold those.
+__device__ __forceinline__ f32x4 mma_half(const Frag<float>& a, const Frag<float>& b, f32x4 acc) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a.lo[i], b.lo[i], acc, 0, 0, 0);
+  return acc;
+}
+__device__ __forceinline__ f32x4 mma_half(const Frag<bf16>& a, const Frag<bf16>& b, f32x4 acc) { return mma(a, b, acc); }
+
 // 4 consecutive elements.
 template <class E>
 struct Quad;
@@ -401,8 +409,9 @@ __global__ __launch_bounds__(4 * D, 2) void walk_kernel(const Walks<E> walks) {
   const int at_row = opaque(M::A + row0 * M::ROW + col * M::S);
   const int at_col[4] = {opaque(M::transposed(col, row0)), opaque(M::transposed(col + 1, row0)), opaque(M::transposed(col + 2, row0)),
                          opaque(M::transposed(col + 3, row0))};
-  const int at_a = opaque(M::A + (16 * ti + l16) * M::ROW + 8 * l4 * M::S);
-  const int at_b = opaque(M::B + (16 * (wave % SHARE) + l16) * M::ROW + 8 * l4 * M::S);
+  constexpr int PER = HALVES ? 4 : 8;  // consecutive inner indices of a lane, of rows
+  const int at_a = opaque(M::A + (16 * ti + l16) * M::ROW + PER * l4 * M::S);
+  const int at_b = opaque(M::B + (16 * (wave % SHARE) + l16) * M::ROW + PER * l4 * M::S);
   const int at_a2 = opaque(M::A + l16 * M::ROW + 4 * l4 * M::S);
   const int at_p_put = opaque(M::P + (16 * ti + l16) * M::PROW + (16 * (wave % SHARE) + 4 * l4) * M::S);
   const int at_p = opaque(M::P + l16 * M::PROW + 8 * l4 * M::S);
@@ -414,6 +423,11 @@ __global__ __launch_bounds__(4 * D, 2) void walk_kernel(const Walks<E> walks) {
   auto load_t = [&](const char* tile, const int (&at)[2], int kk, int more) {
     if constexpr (HALVES) return Frag<E>::load2(tile + at[0] + 32 * kk * M::S + more, tile + at[1] + 32 * kk * M::S + more);
     else return Frag<E>::load(tile + at[kk] + more);
+  };
+
+  auto load_row = [](const char* p) {
+    if constexpr (HALVES) return Frag<E>::load2(p, p + 16 * M::S);
+    else return Frag<E>::load(p);
   };
 
   bool crossed = false;  // a cut anywhere in the segment
@@ -467,11 +481,13 @@ __global__ __launch_bounds__(4 * D, 2) void walk_kernel(const Walks<E> walks) {
 #pragma unroll
       for (int kk = 0; kk < KK; ++kk) {
         if (!FULL && 32 * kk >= da) continue;
-        const Frag<E> fa = Frag<E>::load(tile + at_a + 32 * kk * M::S);
+        const bool half = !FULL && da - 32 * kk <= 16;
+        const Frag<E> fa = load_row(tile + at_a + 32 * kk * M::S);
 #pragma unroll
         for (int u = 0; u < TILES; ++u) {
           // (tiles past the diagonal too, whose `among` is 0: the wavefront with the last rows has none, the others would wait for it)
-          pts[u] = mma(Frag<E>::load(tile + at_b + 16 * SHARE * u * M::ROW + 32 * kk * M::S), fa, pts[u]);
+          const Frag<E> fb = load_row(tile + at_b + 16 * SHARE * u * M::ROW + 32 * kk * M::S);
+          pts[u] = half ? mma_half(fb, fa, pts[u]) : mma(fb, fa, pts[u]);
         }
       }
       if constexpr (!FULL) settle();
@@ -505,11 +521,13 @@ __global__ __launch_bounds__(4 * D, 2) void walk_kernel(const Walks<E> walks) {
 #pragma unroll
       for (int kk = 0; kk < KK; ++kk) {
         if (!FULL && 32 * kk >= da) continue;
+        const bool half = !FULL && da - 32 * kk <= 16;
         const Frag<E> fu = Frag<E>::from(U[2 * kk], U[2 * kk + 1]);
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
           const char* row = tile + at_a2 + 16 * t * M::ROW + 32 * kk * M::S;
-          y[t] = mma(fu, Frag<E>::load2(row, row + 16 * M::S), y[t]);
+          const Frag<E> fr = Frag<E>::load2(row, row + 16 * M::S);
+          y[t] = half ? mma_half(fu, fr, y[t]) : mma(fu, fr, y[t]);
           if (t & 1) apart();
         }
       }
