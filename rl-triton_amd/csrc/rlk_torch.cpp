@@ -23,6 +23,8 @@
 #include <ATen/hip/EmptyTensor.h>
 #include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <algorithm>
@@ -32,8 +34,10 @@
 #include <cstdlib>
 #include <cstring>
 #include <map>
+#include <mutex>
 #include <type_traits>
 #include <utility>
+#include <vector>
 
 #include "rl_triton_amd.h"
 #include "rl_triton_policy.h"
@@ -706,13 +710,17 @@ PyObject* op_affine_scan(PyObject* const* a, Py_ssize_t n) {
 #include "rlk_torch_policy.hpp"
 
 // C++ exceptions (an allocation that fails, say) must not cross into the interpreter: such
-// a call is declined, and the Python path raises torch's own exception for it.
+// a call is declined, and the Python path raises torch's own exception for it.  Python's own (a saved tensor's hook that
+// raises) goes on as it is.
 template <PyObject* (*F)(PyObject* const*, Py_ssize_t)>
 PyObject* guarded(PyObject*, PyObject* const* a, Py_ssize_t n) {
   try {
     return F(a, n);
+  } catch (python_error& e) {
+    e.restore();
+    return nullptr;
   } catch (...) {
-    return decline();
+    return PyErr_Occurred() ? nullptr : decline();
   }
 }
 

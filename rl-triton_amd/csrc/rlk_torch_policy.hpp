@@ -1,25 +1,30 @@
 // rlk_torch_policy.hpp -- the fast path of rl_triton.policy's functions, included by rlk_torch.cpp.
 //
-// As for the estimators: a call is taken when it can go to the C ABI (include/rl_triton_policy.h) as it stands and needs
-// no graph of gradients; any other is declined and the Python implementation checks it, copies what it has to
-// and raises.
+// As for the estimators: a call is taken when it can go to the C ABI (include/rl_triton_policy.h) as it stands; any other is
+// declined and the Python implementation checks it, copies what it has to and raises.  Calls that need gradients
+// are nodes of torch's graph from here too: a forward and backward pass took 93 us of host time through Python's
+// functions, more than the GPU's for a minibatch of small sequences.
 #pragma once
 
 // Checks of one call, on the device of its first tensor.
 struct PolicyCall {
   c10::DeviceIndex dev = -1;
   bool ok = true;
+  bool wants_grad = false;  // by a tensor that the function is differentiable in
 
   const at::Tensor* fail() {
     ok = false;
     return nullptr;
   }
-  // A tensor on the current GPU that is an ordinary one and, where `graph` says that the function is differentiable
-  // in it, needs no gradient now.
+  // A tensor on the current GPU that is an ordinary one; `graph`: the function is differentiable in it.
   const at::Tensor* tensor(PyObject* o, bool graph) {
     if (!ok || !THPVariable_Check(o)) return fail();
     const at::Tensor& t = THPVariable_Unpack(o);
-    if (!t.is_cuda() || t.is_neg() || (graph && t.requires_grad() && at::GradMode::is_enabled())) return fail();
+    if (!t.is_cuda() || t.is_neg()) return fail();
+    if (graph && t.requires_grad() && at::GradMode::is_enabled()) {
+      if (t._fw_grad(0).defined()) return fail();  // (forward derivatives are refused by the Python path)
+      wants_grad = true;
+    }
     if (dev < 0) {
       dev = t.get_device();
       if (dev != c10::hip::current_device()) return fail();
@@ -73,29 +78,121 @@ bool policy_scratch(const PolicyCall& c, at::Tensor PolicyScratch::* kind, size_
   return true;
 }
 
+// Scratch memory of sequences cut into segments, held from its choice to the launch: a backward pass runs on torch's own
+// thread.  `keep`: a call that is being captured has memory of its own, for the graph's replays; else there is none.
+class StatesScratch {
+ public:
+  void* ptr = nullptr;
+  size_t bytes = 0;
+  bool ok = true;
+  StatesScratch(const PolicyCall& c, size_t need, const at::Tensor& like, bool keep) {
+    if (!lock().try_lock()) {  // (whoever holds it may need the interpreter before they let go)
+      PyThreadState* state = PyGILState_Check() ? PyEval_SaveThread() : nullptr;
+      lock().lock();
+      if (state) PyEval_RestoreThread(state);
+    }
+    try {
+      ok = policy_scratch(c, &PolicyScratch::states, need, like, &ptr, &bytes);
+      if (!ok && keep) {
+        static auto* kept = new std::vector<at::Tensor>();
+        kept->push_back(zeroed((int64_t)need, like));
+        ptr = kept->back().data_ptr(), bytes = need, ok = true;
+      }
+    } catch (...) {
+      lock().unlock();
+      throw;
+    }
+  }
+  ~StatesScratch() { lock().unlock(); }
+  StatesScratch(const StatesScratch&) = delete;
+
+ private:
+  static std::mutex& lock() {
+    static auto* m = new std::mutex;
+    return *m;
+  }
+};
+
+// A node's results cannot be differentiated once more: they say so when that is tried, as Python's functions do.
+struct DifferentiableOnce : torch::autograd::Function<DifferentiableOnce> {
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext*, const at::Tensor& x, const at::Tensor&) { return {x.detach()}; }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext*, torch::autograd::variable_list) {
+    TORCH_CHECK(false, "trying to differentiate twice a function of rl_triton.policy, whose gradients are not differentiable");
+  }
+};
+void once(torch::autograd::variable_list& grads, const torch::autograd::variable_list& from) {
+  if (!at::GradMode::is_enabled()) return;
+  for (const at::Tensor& f : from)
+    if (f.defined() && f.requires_grad()) {
+      for (at::Tensor& g : grads)
+        if (g.defined()) g = DifferentiableOnce::apply(g, f)[0];
+      return;
+    }
+}
+
 bool float_type(at::ScalarType st) { return st == at::kFloat || st == at::kBFloat16; }
 
 // logits [envs, steps, actions] with contiguous actions, or contiguous ones of any other rank.
-bool logit_rows(PolicyCall& c, PyObject* logits, PyObject* actions, PyObject* temperature, bool graph, rlk_action_rows* r,
-                const at::Tensor** x, const at::Tensor** a) {
-  const at::Tensor* t = *x = c.tensor(logits, graph);
-  if (!t || !float_type(t->scalar_type()) || t->dim() < 1 || t->numel() == 0) return false;
-  const int64_t n = t->size(-1);
+bool logit_layout(const at::Tensor& t, rlk_action_rows* r) {
+  const int64_t n = t.size(-1);
   r->num_actions = n;
-  if (t->dim() == 3 && (t->stride(2) == 1 || n == 1)) {
-    r->num_envs = t->size(0), r->seq_len = t->size(1), r->env_stride = t->stride(0), r->step_stride = t->stride(1);
-  } else if (t->is_contiguous()) {
-    r->num_envs = 1, r->seq_len = t->numel() / n, r->env_stride = t->numel(), r->step_stride = n;
+  r->logits = t.data_ptr(), r->bf16 = t.scalar_type() == at::kBFloat16;
+  if (t.dim() == 3 && (t.stride(2) == 1 || n == 1)) {
+    r->num_envs = t.size(0), r->seq_len = t.size(1), r->env_stride = t.stride(0), r->step_stride = t.stride(1);
+  } else if (t.is_contiguous()) {
+    r->num_envs = 1, r->seq_len = t.numel() / n, r->env_stride = t.numel(), r->step_stride = n;
   } else {
     return false;
   }
+  return true;
+}
+bool logit_rows(PolicyCall& c, PyObject* logits, PyObject* actions, PyObject* temperature, bool graph, rlk_action_rows* r,
+                const at::Tensor** x, const at::Tensor** a) {
+  const at::Tensor* t = *x = c.tensor(logits, graph);
+  if (!t || !float_type(t->scalar_type()) || t->dim() < 1 || t->numel() == 0 || !logit_layout(*t, r)) return false;
   *a = c.array(actions, at::kLong, t->sizes().slice(0, t->dim() - 1));
   const double tau = c.number(temperature, 0.0);
   if (!c.ok || !(tau > 0.0)) return false;
-  r->logits = t->data_ptr(), r->actions = static_cast<const int64_t*>((*a)->data_ptr());
-  r->temperature = tau, r->bf16 = t->scalar_type() == at::kBFloat16;
+  r->actions = static_cast<const int64_t*>((*a)->data_ptr());
+  r->temperature = tau;
   return true;
 }
+
+struct ActionLogProbs : torch::autograd::Function<ActionLogProbs> {
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const at::Tensor& logits, const at::Tensor& actions,
+                                                const rlk_action_rows* r, void* stream) {
+    std::vector<int64_t> two = actions.sizes().vec();
+    at::Tensor lp = policy_output(two, at::kFloat, logits), ent = policy_output(two, at::kFloat, logits);
+    two.push_back(2);
+    at::Tensor norms = policy_output(two, at::kFloat, logits);
+    const int st = rlk_action_log_probs(r, static_cast<float*>(lp.data_ptr()), static_cast<float*>(ent.data_ptr()),
+                                        static_cast<float*>(norms.data_ptr()), stream);
+    TORCH_CHECK(st == RLK_OK, "rlk_action_log_probs failed: ", rlk_status_string(st));
+    ctx->save_for_backward({logits, actions, ent, norms});
+    ctx->saved_data["temperature"] = r->temperature;
+    ctx->set_materialize_grads(false);
+    return {lp, ent};
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const at::Tensor &logits = saved[0], &actions = saved[1];
+    torch::autograd::variable_list out(4);
+    if (!grads[0].defined() && !grads[1].defined()) return out;
+    rlk_action_rows r = {};
+    logit_layout(logits, &r);
+    r.actions = static_cast<const int64_t*>(actions.data_ptr()), r.temperature = ctx->saved_data["temperature"].toDouble();
+    at::Tensor up[2];
+    const float* p[2] = {};
+    for (int i = 0; i < 2; ++i)
+      if (grads[i].defined()) up[i] = grads[i].contiguous(), p[i] = static_cast<const float*>(up[i].data_ptr());
+    out[0] = policy_output(logits.sizes(), logits.scalar_type(), logits);
+    const int st = rlk_action_log_probs_backward(&r, static_cast<const float*>(saved[2].data_ptr()), static_cast<const float*>(saved[3].data_ptr()),
+                                                 p[0], p[1], out[0].data_ptr(), c10::hip::getCurrentHIPStream(logits.get_device()).stream());
+    TORCH_CHECK(st == RLK_OK, "rlk_action_log_probs_backward failed: ", rlk_status_string(st));
+    once(out, {logits, grads[0], grads[1]});
+    return out;
+  }
+};
 
 // action_log_probs(logits, actions, temperature)
 PyObject* op_action_log_probs(PyObject* const* a, Py_ssize_t n) {
@@ -107,6 +204,10 @@ PyObject* op_action_log_probs(PyObject* const* a, Py_ssize_t n) {
   if (act->numel() <= 256 && r.num_actions >= 32768 &&
       !policy_scratch(c, &PolicyScratch::rows, RLK_ROWS_WORKSPACE_BYTES, *x, &r.workspace, &r.workspace_bytes))
     return decline();
+  if (c.wants_grad) {
+    torch::autograd::variable_list o = ActionLogProbs::apply(*x, *act, &r, c.stream());
+    return pair(o[0], o[1]);
+  }
   at::Tensor lp = policy_output(act->sizes(), at::kFloat, *x), ent = policy_output(act->sizes(), at::kFloat, *x);
   const int st = rlk_action_log_probs(&r, static_cast<float*>(lp.data_ptr()), static_cast<float*>(ent.data_ptr()), nullptr, c.stream());
   return finish(st, "rlk_action_log_probs", pair(lp, ent));
@@ -218,6 +319,83 @@ at::Tensor attention_out(const at::Tensor& v, rlk_attention* t) {
   return out;
 }
 
+rlk_sequence steps_of(const at::Tensor& x) { return {x.data_ptr(), x.stride(0), x.stride(1), x.stride(2)}; }
+
+// What a call has beside its tensors of every call (a node's arguments are defined tensors: `state` is any where there is none).
+struct AttentionCall {
+  rlk_attention* t;
+  at::Tensor dones;
+  bool state;
+  double scale;  // unrounded
+  size_t need;   // of scratch memory
+};
+
+struct LinearAttention : torch::autograd::Function<LinearAttention> {
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const at::Tensor& q, const at::Tensor& k,
+                                                const at::Tensor& v, const at::Tensor& state, const at::Tensor& decay,
+                                                const AttentionCall* call) {
+    rlk_attention* t = call->t;
+    at::Tensor out = attention_out(v, t), last = policy_output({t->num_envs, t->heads, t->dim_k, t->dim_v}, at::kFloat, v);
+    t->state_out = static_cast<float*>(last.data_ptr());
+    PolicyCall c;
+    c.dev = q.get_device();
+    const int st = [&] {
+      const StatesScratch scratch(c, call->need, q, true);
+      t->workspace = scratch.ptr, t->workspace_bytes = scratch.bytes;
+      return rlk_linear_attention(t, 1, c.stream());
+    }();
+    TORCH_CHECK(st == RLK_OK, "rlk_linear_attention failed: ", rlk_status_string(st));
+    ctx->save_for_backward({q, k, v, call->state ? state : at::Tensor(), decay, call->dones});
+    ctx->saved_data["scale"] = call->scale;
+    ctx->saved_data["state"] = call->state && state.requires_grad();
+    ctx->set_materialize_grads(false);
+    return {out, last};
+  }
+  // The gradients are the same recurrence over other arrays (rlk_attention.hip): dq = (g, v, k) forward, and in
+  // reverse dk = (v, g, q) and dv = (k, q, g), whose state at the first step is the state's gradient.
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const at::Tensor &q = saved[0], &k = saved[1], &v = saved[2], &state = saved[3], &decay = saved[4], &dones = saved[5];
+    torch::autograd::variable_list out(6);
+    if (!grads[0].defined() && !grads[1].defined()) return out;
+    const at::Tensor g = !grads[0].defined() ? at::zeros(v.sizes(), v.options())
+                         : grads[0].stride(3) == 1 || v.size(3) == 1 ? grads[0] : grads[0].contiguous();
+    const at::Tensor last = grads[1].defined() ? grads[1].contiguous() : grads[1];
+    const double scale = ctx->saved_data["scale"].toDouble();
+    rlk_attention t[3] = {};
+    const at::Tensor* roles[3][3] = {{&g, &v, &k}, {&v, &g, &q}, {&k, &q, &g}};
+    const at::Tensor* like[3] = {&q, &k, &v};
+    for (int i = 0; i < 3; ++i) {
+      rlk_attention& w = t[i];
+      out[i] = policy_output(like[i]->sizes(), like[i]->scalar_type(), *like[i]);
+      w.q = steps_of(*roles[i][0]), w.k = steps_of(*roles[i][1]), w.v = steps_of(*roles[i][2]), w.out = steps_of(out[i]);
+      w.num_envs = q.size(0), w.seq_len = q.size(1), w.heads = q.size(2);
+      w.dim_k = roles[i][0]->size(3), w.dim_v = out[i].size(3);
+      w.decay = static_cast<const float*>(decay.data_ptr()), w.dones = dones.defined() ? static_cast<const float*>(dones.data_ptr()) : nullptr;
+      const at::Tensor& enters = i == 0 ? state : last;
+      w.state = enters.defined() ? static_cast<const float*>(enters.data_ptr()) : nullptr;
+      w.state_transposed = i < 2, w.reverse = i > 0, w.bf16 = q.scalar_type() == at::kBFloat16;
+      w.scale = (float)scale, w.state_scale = i > 0 ? (float)(1.0 / scale) : 1.f, w.state_out_scale = i > 0 ? (float)scale : 1.f;
+    }
+    if (ctx->saved_data["state"].toBool()) {
+      out[3] = policy_output({q.size(0), q.size(2), q.size(3), v.size(3)}, at::kFloat, q);
+      t[2].state_out = static_cast<float*>(out[3].data_ptr());
+    }
+    PolicyCall c;
+    c.dev = q.get_device();
+    size_t need = 0;
+    for (const rlk_attention& w : t) need += rlk_attention_workspace_bytes(w.num_envs, w.seq_len, w.heads, w.dim_k, w.dim_v);
+    const int st = [&] {
+      const StatesScratch scratch(c, need, q, true);
+      for (rlk_attention& w : t) w.workspace = scratch.ptr, w.workspace_bytes = scratch.bytes;
+      return rlk_linear_attention(t, 3, c.stream());
+    }();
+    TORCH_CHECK(st == RLK_OK, "rlk_linear_attention failed: ", rlk_status_string(st));
+    once(out, {q, k, v, state, grads[0], grads[1]});
+    return out;
+  }
+};
+
 // linear_attention(q, k, v, decay, dones, state, scale)
 PyObject* op_linear_attention(PyObject* const* a, Py_ssize_t n) {
   if (n != 7 || correctness_warnings()) return decline();
@@ -227,7 +405,18 @@ PyObject* op_linear_attention(PyObject* const* a, Py_ssize_t n) {
   at::Tensor flags;
   if (!attention_args(c, a[0], a[1], a[2], a[3], a[4], a[5], a[6], true, &t, &v, &flags)) return decline();
   const size_t need = rlk_attention_workspace_bytes(t.num_envs, t.seq_len, t.heads, t.dim_k, t.dim_v);
-  if (!policy_scratch(c, &PolicyScratch::states, need, *v, &t.workspace, &t.workspace_bytes)) return decline();
+  if (c.wants_grad) {
+    const bool state = a[5] != Py_None;
+    const AttentionCall call{&t, flags.defined() ? flags : a[4] == Py_None ? at::Tensor() : THPVariable_Unpack(a[4]), state,
+                             a[6] == Py_None ? 1.0 / std::sqrt((double)t.dim_k) : c.number(a[6], -HUGE_VAL), need};
+    const at::Tensor& decay = THPVariable_Unpack(a[3]);
+    torch::autograd::variable_list o = LinearAttention::apply(THPVariable_Unpack(a[0]), THPVariable_Unpack(a[1]), *v,
+                                                              state ? THPVariable_Unpack(a[5]) : decay, decay, &call);
+    return pair(o[0], o[1]);
+  }
+  const StatesScratch scratch(c, need, *v, false);
+  if (!scratch.ok) return decline();
+  t.workspace = scratch.ptr, t.workspace_bytes = scratch.bytes;
   at::Tensor out = attention_out(*v, &t), last = policy_output({t.num_envs, t.heads, t.dim_k, t.dim_v}, at::kFloat, *v);
   t.state_out = static_cast<float*>(last.data_ptr());
   return finish(rlk_linear_attention(&t, 1, c.stream()), "rlk_linear_attention", pair(out, last));

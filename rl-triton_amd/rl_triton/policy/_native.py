@@ -7,6 +7,7 @@ workspaces, one per (device, stream), as rl_triton._native does for the estimato
 from __future__ import annotations
 
 import ctypes
+import threading
 
 import torch
 
@@ -75,6 +76,7 @@ _BF16 = torch.bfloat16
 # Scratch memory, one of each kind per (device, stream): "sums" of the losses, whose head is zero between calls,
 # "rows" of statistics of shared rows, and "states" of sequences cut into segments.
 _workspaces: dict = {}
+_launching = threading.Lock()  # from a workspace's choice to the launch: a backward pass runs on torch's own thread
 
 
 def _workspace(kind: str, dev: int, stream: int, need: int):
@@ -99,10 +101,11 @@ def _on_device(fn):
     """Runs `fn(dev, stream, ...)` with its first tensor's device current."""
     def call(lead, *args):
         dev = lead.get_device()
-        if dev != _native._cur_device():
-            with torch.cuda.device(dev):
-                return fn(dev, _native._raw_stream(dev), lead, *args)
-        return fn(dev, _native._raw_stream(dev), lead, *args)
+        with _launching:
+            if dev != _native._cur_device():
+                with torch.cuda.device(dev):
+                    return fn(dev, _native._raw_stream(dev), lead, *args)
+            return fn(dev, _native._raw_stream(dev), lead, *args)
     return call
 
 
