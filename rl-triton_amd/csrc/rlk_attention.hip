@@ -17,6 +17,15 @@
 // wavefronts for dims of up to 64, 8 for up to 128).  A wavefront's part of U stays in the accumulators of the matrix instructions for the whole walk: the
 // accumulator layout (4 consecutive rows of a column per lane) is also an operand layout once the inner index is
 // taken in that order, so U feeds U^T a without a trip through LDS.
+//
+// Measured (us; floors are bytes at the 5.2 TB/s of a large copy): bfloat16 [64,1024,8,64] 75 forward (floor 52) and 185 for
+// the three walks back (90 with each array read once); float32 185 and 460 (103, 181).  [1,16384,16,128], a row of
+// segments: states 43, join 8.5, walks 84 (52 for all).  [37,333,4,40 and 72] float32: 60 and 113 (18 for both; the
+// useful products alone 13), on 148 of 256 CUs forward, each with the wavefronts' fifth tile of columns on one SIMD.
+// Neither HBM nor the matrix units are the bound in bfloat16: the vector units are busy for 43% of the time (a chunk costs a
+// wavefront some 450 instructions, a quarter of them the weights' split into three), matrix products for 15%, and
+// the rest is waits for LDS and the two barriers of a chunk, with two wavefronts a SIMD to cover them.  In
+// float32 matrix products (16x16x4, a sixteenth of bfloat16's rate) take 34% of [37,333,4,40 and 72], over the SIMDs.
 #include "rlk_attention.hpp"
 
 namespace rlk {
@@ -147,7 +156,8 @@ struct Lds {
   static constexpr int A = 2 * D * TROW, B = A + C * ROW;    // rows of a and b
   static constexpr int CHUNK = B + C * ROW;
   // Two chunks where they fit (160 KB a CU; two workgroups of it for bfloat16 dims of up to 64): the next one is put down
-  // while this one is worked on.
+  // while this one is worked on.  float32 dims of up to 64 have one, and two workgroups a CU (training [64,1024,8,64] 645 us;
+  // two chunks and one workgroup 818).
   static constexpr int P_BYTES = C * PROW;                   // (a_i . b_j) lambda^{i-j} same(j, i)
   static constexpr bool OVER = S == 4 && D == 64;            // p in the place of b's rows, which are read for nothing else
   static constexpr int CHUNKS = !OVER && 2 * (CHUNK + 32) + P_BYTES <= 160 * 1024 ? 2 : 1;

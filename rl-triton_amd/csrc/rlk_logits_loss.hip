@@ -1,5 +1,8 @@
 // rlk_logits_loss.hip -- the clipped policy loss from logits and the logits' gradient in one pass over them
 // (include/rl_triton_policy.h; the mathematics is in rlk_action_rows.hpp and rlk_policy.hpp).
+// Bound by HBM where rows are long: [16,512] of 65536 bfloat16 378 us a call, 5.7 TB/s of reads and writes, [7,285] of 50001
+// float32 139, 5.7 TB/s (a large copy 5.2).  [4096,128] of 18 float32: 30 us, 2.8 TB/s (floor 16): rows of 72 bytes go through
+// LDS, and computing on them takes as long as moving them.
 #include "rlk_action_rows.hpp"
 
 namespace rlk {

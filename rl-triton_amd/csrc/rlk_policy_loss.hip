@@ -1,5 +1,9 @@
 // rlk_policy_loss.hip -- the clipped policy loss from log-probabilities, and the counting and summing that
 // the loss from logits shares (include/rl_triton_policy.h).
+//
+// [512,6000] with mask, reference and row means: counts 4.7 us, loss 21 (floor 14 for both): reads that end in a reduction, then
+// one exchange between workgroups through two levels of tickets.  [64,128]: 7 us, two loads' latencies, the reduction and the
+// exchange.
 #include "rlk_launch.hpp"
 #include "rlk_policy.hpp"
 

@@ -2,8 +2,8 @@
 //
 // As for the estimators: a call is taken when it can go to the C ABI (include/rl_triton_policy.h) as it stands; any other is
 // declined and the Python implementation checks it, copies what it has to and raises.  Calls that need gradients
-// are nodes of torch's graph from here too: a forward and backward pass took 93 us of host time through Python's
-// functions, more than the GPU's for a minibatch of small sequences.
+// are nodes of torch's graph from here too: a forward and backward pass of attention takes 68 us of host time and 158 through
+// Python's functions (torch's own q * k takes 55 in the same loop).
 #pragma once
 
 // Checks of one call, on the device of its first tensor.
