@@ -668,7 +668,7 @@ __global__ __launch_bounds__(4 * D, 2) void walk_kernel(const Walks<E> walks) {
   float f = 1.f;
   if (STATE) {
     out = w.seg_states + (eh * walks.segs + seg + 1) * (int64_t)(da * dc);
-    if (threadIdx.x == 0) w.seg_keep[eh * walks.segs + seg + 1] = crossed ? 0.f : power(lg, (int)(last - first));
+    if (threadIdx.x == 0) w.seg_keep[eh * walks.segs + seg + 1] = crossed || lambda == 0.f ? -1.f : power(lg, (int)(last - first));
   } else if (last == T && w.state_out != nullptr) {
     out = w.state_out + eh * (int64_t)(da * dc);
     f = !reverse && dones != nullptr && dones[T - 1] != 0.f ? 0.f : w.state_out_scale;
@@ -699,7 +699,7 @@ __global__ __launch_bounds__(256) void join_kernel(const Walks<E> walks) {
   for (int s = 1; s < walks.segs; ++s) {
     float* p = w.seg_states + (eh * walks.segs + s) * (int64_t)n + i;
     const float keep = w.seg_keep[eh * walks.segs + s];
-    u = keep == 0.f ? *p : fmaf(u, keep, *p);
+    u = keep < 0.f ? *p : fmaf(u, keep, *p);  // (no part of u, NaN included, passes an episode's end; one too small to see leaves a NaN)
     *p = u;
   }
 }

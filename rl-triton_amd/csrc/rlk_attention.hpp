@@ -24,7 +24,7 @@ struct Walk {
   const float* state;
   float* state_out;
   float* seg_states;  // [env, head, segment, da, dc]: what enters the segment (0 unused)
-  float* seg_keep;    // [env, head, segment]: how much of what enters the segment before leaves it
+  float* seg_keep;    // [env, head, segment]: how much of what enters the segment before leaves it; below 0: nothing, an episode ends in it
   float scale, state_scale, state_out_scale;
   int transposed, reverse;
 };

@@ -250,6 +250,36 @@ def test_values_that_are_not_finite_stay_where_they_belong(d, dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("d", [40, 128])
+def test_values_that_are_not_finite_in_sequences_cut_into_segments(d, dtype):
+    """The same over 20 chunks of one environment and head, whose segments' states are found first.  A NaN without an episode's
+    end after it reaches every later step, past the point where its decay is too small for float32."""
+    E, T, H = 1, 1280, 2
+    q, k, v, _, _, s = _make(E, T, H, d, d, 8, dtype)
+    decay = torch.tensor([0.99, 0.5])
+    dones = torch.zeros(E, T)
+    dones[0, [300, 420]] = 1
+    gen = torch.Generator().manual_seed(2)
+    go, gs = torch.randn(E, T, H, d, generator=gen).to(dtype), torch.randn(E, H, d, d, generator=gen)
+    k[0, 330, 0, 3], v[0, 350, 0, 2], k[0, 500, 1, 5], go[0, 310, 1, 1] = math.nan, math.inf, math.nan, -math.inf
+    leaves = [t.requires_grad_() for t in _cuda(q, k, v, s)]
+    out, last = policy.compute_linear_attention(leaves[0], leaves[1], leaves[2], *_cuda(decay, dones), leaves[3], 0.3)
+    got = (out, last, *torch.autograd.grad((out, last), leaves, _cuda(go, gs)))
+    q, k, v, s = (t.detach() for t in (q, k, v, s))
+    args = (q, k, v, decay, dones, s, 0.3)
+    want = (*attention(*args), *attention_grads(*args, go, gs))
+    assert bool(want[0][0, -1, 1].isnan().any()) and not bool(want[0][0, 421:, 0].isnan().any())
+    by, bs = _bounds(args, dtype, T)
+    sizes = attention_grads(q.abs(), k.abs(), v.abs(), decay, dones, s.abs(), 0.3, go.abs(), gs.abs())
+    wide = dtype == torch.bfloat16
+    bounds = (by, bs, *[x * ((T + 128) * U32 + ((U16 * U16 if i == 3 else U16) if wide else 0)) for i, x in enumerate(sizes)])
+    for i, (x, w, bound) in enumerate(zip(got, want, bounds)):
+        x, kept = x.detach().cpu().double(), w.isfinite()
+        assert bool((x.isfinite() == kept).all()), i
+        _within(x[kept], w[kept], bound[kept], (U16 if wide and i not in (1, 5) else 0) + U32)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_step_of_large_states(dtype):
     """States of 256 MB and more, which take another path through the caches; bounds as above."""
     E, H, d = 4096 + 3, 1, 128
