@@ -54,7 +54,7 @@ __global__ __launch_bounds__(256) void join_log_probs_kernel(const ActionRows<E>
 template <class E, int K>
 __global__ __launch_bounds__(kFewRows) void few_log_probs_kernel(const ActionRows<E> a, const FewRows f, float* __restrict__ log_probs,
                                                                  float* __restrict__ entropies, float* __restrict__ norms) {
-  extern __shared__ float lds[];
+  extern __shared__ __align__(16) float lds[];
   for (int64_t row0 = (int64_t)blockIdx.x * kFewRows; row0 < a.rows; row0 += (int64_t)gridDim.x * kFewRows) {
     const int rows = (int)(a.rows - row0 < kFewRows ? a.rows - row0 : kFewRows);
     const int64_t row = row0 + threadIdx.x;
@@ -100,7 +100,7 @@ int forward(const rlk_action_rows* rows, float* lp, float* ent, float* norms, hi
     int64_t blocks = (a.rows + kFewRows - 1) / kFewRows;
     if (blocks > 2048) blocks = 2048;
     return dispatch_few(a.A, [&](auto k) {
-      few_log_probs_kernel<E, decltype(k)::value><<<dim3((unsigned)blocks), dim3(kFewRows), few.pitch * kFewRows * sizeof(float), s>>>(
+      few_log_probs_kernel<E, decltype(k)::value><<<dim3((unsigned)blocks), dim3(kFewRows), FewRows::bytes(few.pitch), s>>>(
           a, few, lp, ent, norms);
       return hipGetLastError() == hipSuccess ? RLK_OK : RLK_ERR_LAUNCH;
     });

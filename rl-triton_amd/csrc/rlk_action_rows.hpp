@@ -377,55 +377,33 @@ __device__ __forceinline__ RowStats join_parts(const RowParts& p, int64_t row, f
 
 // ---------------------------------------------------------------------------------------
 // Few actions, rows one after the other in memory: a thread per row.  A workgroup takes 256 rows in 16-byte
-// accesses through LDS, where a row starts at an odd word (A | 1 apart), so that lanes that read the same column
-// of their rows meet in different banks.  No lane is idle past the row's end, nothing is reduced over lanes, and what a
+// accesses through LDS, which holds them as they are in memory: a lane reads its row in the widest words that divide it (4,
+// 8 or 16 bytes), whose places in a wavefront's rows lie in different banks; for rows of a multiple of 32 bytes 16
+// more keep them apart.  No lane is idle past the row's end, nothing is reduced over lanes, and what a
 // step computes beside its logits it computes once.
 // ---------------------------------------------------------------------------------------
 constexpr int kFewActions = 32, kFewRows = 256;
 
 struct FewRows {
-  int A, pitch;
+  int A, pitch;    // pitch: A, or A + 4 for a multiple of 8
   uint32_t magic;  // ceil(2^32 / A): i / A = umulhi(i, magic) for i < 2^13 (A > 1)
   bool quads;      // the arrays are aligned to 4 elements
-  __device__ int row(int i) const { return A == 1 ? i : (int)__umulhi((uint32_t)i, magic); }
+  static constexpr size_t bytes(int pitch) { return (size_t)pitch * kFewRows * sizeof(float); }
+  // where element i of the rows lies
+  __device__ int place(int i) const { return pitch == A ? i : i + 4 * (int)__umulhi((uint32_t)i, magic); }
 
   // LDS <- `count` elements at `src`
   template <class E>
   __device__ void take(const E* src, int count, float* lds) const {
     const int whole = quads ? count / 4 : 0;
-    for (int q = threadIdx.x; q < whole; q += kFewRows) {
-      const float4 v = load_quad<true>(src + 4 * q);
-      const float* x = &v.x;
-      int r = row(4 * q), j = 4 * q - r * A;
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        lds[r * pitch + j] = x[k];
-        if (++j == A) j = 0, ++r;
-      }
-    }
-    for (int i = 4 * whole + threadIdx.x; i < count; i += kFewRows) {
-      const int r = row(i);
-      lds[r * pitch + i - r * A] = load_one(src + i);
-    }
+    for (int q = threadIdx.x; q < whole; q += kFewRows) *reinterpret_cast<float4*>(lds + place(4 * q)) = load_quad<true>(src + 4 * q);
+    for (int i = 4 * whole + threadIdx.x; i < count; i += kFewRows) lds[place(i)] = load_one(src + i);
   }
   template <class E>
   __device__ void put(E* dst, int count, const float* lds) const {
     const int whole = quads ? count / 4 : 0;
-    for (int q = threadIdx.x; q < whole; q += kFewRows) {
-      float4 v;
-      float* x = &v.x;
-      int r = row(4 * q), j = 4 * q - r * A;
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        x[k] = lds[r * pitch + j];
-        if (++j == A) j = 0, ++r;
-      }
-      store_quad<true>(dst + 4 * q, v);
-    }
-    for (int i = 4 * whole + threadIdx.x; i < count; i += kFewRows) {
-      const int r = row(i);
-      dst[i] = from_f32<E>(lds[r * pitch + i - r * A]);
-    }
+    for (int q = threadIdx.x; q < whole; q += kFewRows) store_quad<true>(dst + 4 * q, *reinterpret_cast<const float4*>(lds + place(4 * q)));
+    for (int i = 4 * whole + threadIdx.x; i < count; i += kFewRows) dst[i] = from_f32<E>(lds[place(i)]);
   }
 };
 
@@ -433,9 +411,39 @@ struct FewRows {
 template <int K>
 struct FewLogits {
   float x[K];
+  // f(first element, vector type) for each of the widest words that divide the row, K of 4 at the most
+  template <class F>
+  __device__ __forceinline__ static void words(int A, F f) {
+    if ((A & 3) == 0) {
+#pragma unroll
+      for (int j = 0; j < K; j += 4) f(j, float4{});
+    } else if ((A & 1) == 0) {
+#pragma unroll
+      for (int j = 0; j < K; j += 2)
+        if (j < K - 2) f(j, float2{});
+    } else {
+#pragma unroll
+      for (int j = 0; j < K; ++j)
+        if (j < K - 3 || j < A) f(j, 0.f);
+    }
+  }
   __device__ __forceinline__ void load(const float* row, int A) {
 #pragma unroll
-    for (int j = 0; j < K; ++j) x[j] = j < K - 3 || j < A ? row[j] : -INFINITY;
+    for (int j = K - 3; j < K; ++j) x[j] = -INFINITY;
+    words(A, [&](int j, auto word) {
+      word = *reinterpret_cast<const decltype(word)*>(row + j);
+      const float* e = reinterpret_cast<const float*>(&word);
+#pragma unroll
+      for (int i = 0; i < (int)(sizeof(word) / 4); ++i) x[j + i] = e[i];
+    });
+  }
+  __device__ __forceinline__ void store(float* row, int A) const {
+    words(A, [&](int j, auto word) {
+      float* e = reinterpret_cast<float*>(&word);
+#pragma unroll
+      for (int i = 0; i < (int)(sizeof(word) / 4); ++i) e[i] = x[j + i];
+      *reinterpret_cast<decltype(word)*>(row + j) = word;
+    });
   }
   __device__ __forceinline__ RowStats stats(float c) const {
     float m = x[0];
@@ -467,7 +475,7 @@ template <class E>
 bool few_rows(const ActionRows<E>& a, const void* out, FewRows* f) {
   if (a.A > kFewActions || a.step_stride != a.A || a.env_stride != a.seq_len * a.step_stride) return false;
   const uintptr_t low = (reinterpret_cast<uintptr_t>(a.logits) | reinterpret_cast<uintptr_t>(out)) & (4 * sizeof(E) - 1);
-  *f = {a.A, a.A | 1, (uint32_t)(((uint64_t{1} << 32) + (uint32_t)a.A - 1) / (uint32_t)a.A), low == 0};
+  *f = {a.A, a.A % 8 == 0 ? a.A + 4 : a.A, (uint32_t)(((uint64_t{1} << 32) + (uint32_t)a.A - 1) / (uint32_t)a.A), low == 0};
   return true;
 }
 

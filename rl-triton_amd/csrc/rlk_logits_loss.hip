@@ -110,7 +110,7 @@ template <class E, int K>
 __global__ __launch_bounds__(kFewRows) void few_loss_kernel(const ActionRows<E> a, const FewRows f, const StepArrays t,
                                                             const LossConsts c, const Weights w, const LossOut sums,
                                                             E* __restrict__ grad) {
-  extern __shared__ float lds[];
+  extern __shared__ __align__(16) float lds[];
   __shared__ int64_t sc[kFewRows / 64];
   const float scale = weight_scale<kFewRows>(w, sc);
   double acc[kTerms] = {};
@@ -141,12 +141,13 @@ __global__ __launch_bounds__(kFewRows) void few_loss_kernel(const ActionRows<E> 
       const RowGrad g(wt * st.slope, -(float)c.entropy_coef * wt, entropy, r.m, a.c, log2s, a.inv_tau, act, empty);
       if (__any(empty)) {
 #pragma unroll
-        for (int j = 0; j < K; ++j)
-          if (j < K - 3 || j < a.A) x[j] = empty ? 0.f : g(h.x[j], j);
+        for (int j = 0; j < K; ++j) h.x[j] = empty ? 0.f : g(h.x[j], j);
+        h.store(x, a.A);
       } else {
 #pragma unroll
-        for (int j = 0; j < K; ++j)
-          if (j < K - 3 || j < a.A) x[j] = g(h.x[j]);
+        for (int j = 0; j < K; ++j) h.x[j] = g(h.x[j]);
+        h.store(x, a.A);
+        asm volatile("" ::: "memory");  // (the stores are of another type: the compiler might exchange them)
         if (g.action >= 0 && g.action < a.A) x[g.action] += g.at;
       }
       add_terms(acc, st, wt);
@@ -177,7 +178,7 @@ int impl(const rlk_action_rows* rows, const rlk_policy_terms* t, void* grad, hip
     int64_t blocks = (a.rows + kFewRows - 1) / kFewRows;
     if (blocks > kMaxLossBlocks) blocks = kMaxLossBlocks;
     return dispatch_few(a.A, [&](auto k) {
-      few_loss_kernel<E, decltype(k)::value><<<dim3((unsigned)blocks), dim3(kFewRows), few.pitch * kFewRows * sizeof(float), s>>>(
+      few_loss_kernel<E, decltype(k)::value><<<dim3((unsigned)blocks), dim3(kFewRows), FewRows::bytes(few.pitch), s>>>(
           a, few, arrays, plan.consts, plan.weights, plan.out, static_cast<E*>(grad));
       return hipGetLastError() == hipSuccess ? RLK_OK : RLK_ERR_LAUNCH;
     });

@@ -75,13 +75,23 @@ struct LossArgs {
   LossOut out;
 };
 
-// Steps i .. i + 3 (`left` of them exist): their gradients, their terms added to `acc`.  row_weight(step): what a
-// row's steps count for.
+// Steps i .. i + 3 (`left` of them exist).
+struct FourSteps {
+  float4 lp, old, adv, ref;
+  template <class E>
+  __device__ __forceinline__ void load(const LossArgs<E>& a, int64_t i, int left) {
+    const bool whole = a.whole && left == 4;
+    lp = load4(a.lp + i, whole, left), old = load4(a.old + i, whole, left), adv = load4(a.adv + i, whole, left);
+    ref = a.ref ? load4(a.ref + i, whole, left) : float4{0.f, 0.f, 0.f, 0.f};
+  }
+};
+
+// Their gradients, their terms added to `acc`.  weight(step, which of the four): what it counts for.
 template <class E, class F>
-__device__ __forceinline__ void four_steps(const LossArgs<E>& a, int64_t i, int left, float4 m, double (&acc)[kTerms], F weight) {
+__device__ __forceinline__ void four_steps(const LossArgs<E>& a, const FourSteps& x4, int64_t i, int left, float4 m, double (&acc)[kTerms],
+                                           F weight) {
   const bool whole = a.whole && left == 4;
-  const float4 lp = load4(a.lp + i, whole, left), old = load4(a.old + i, whole, left), adv = load4(a.adv + i, whole, left);
-  const float4 ref = a.ref ? load4(a.ref + i, whole, left) : float4{0.f, 0.f, 0.f, 0.f};
+  const float4 &lp = x4.lp, &old = x4.old, &adv = x4.adv, &ref = x4.ref;
   float g[4], policy = 0.f, kl = 0.f, clipped = 0.f, old_kl = 0.f;
   const float *pl = &lp.x, *po = &old.x, *pa = &adv.x, *pr = &ref.x, *pm = &m.x;
 #pragma unroll
@@ -110,23 +120,32 @@ constexpr float4 kAll{1.f, 1.f, 1.f, 1.f};
 template <class E>
 __global__ __launch_bounds__(kNT) void loss_kernel(const LossArgs<E> a) {
   __shared__ int64_t sc[kNT / 64];
+  const int64_t step = (int64_t)gridDim.x * kNT * 4;
+  int64_t i = ((int64_t)blockIdx.x * kNT + threadIdx.x) * 4;
+  float4 m = kAll;
+  FourSteps x;
+  auto load = [&](int64_t at) {
+    const int left = (int)(a.n - at < 4 ? a.n - at : 4);
+    if (a.mask) m = load4(a.mask + at, a.whole && left == 4, left);
+    x.load(a, at, left);
+  };
+  if (i < a.n) load(i);  // (on their way while the counts are added up)
   const float scale = weight_scale<kNT>(a.w, sc);
   double acc[kTerms] = {};
-  const int64_t step = (int64_t)gridDim.x * kNT * 4;
-  for (int64_t i = ((int64_t)blockIdx.x * kNT + threadIdx.x) * 4; i < a.n; i += step) {
+  for (; i < a.n; i += step) {
     const int left = (int)(a.n - i < 4 ? a.n - i : 4);
-    const float4 m = a.mask ? load4(a.mask + i, a.whole && left == 4, left) : kAll;
     if (a.w.row_counts == nullptr) {
-      four_steps(a, i, left, m, acc, [&](int64_t, int) { return scale; });
+      four_steps(a, x, i, left, m, acc, [&](int64_t, int) { return scale; });
     } else {
       int64_t row = a.n <= 0x7fffffff ? (int64_t)((uint32_t)i / (uint32_t)a.seq_len) : i / a.seq_len;
       int64_t ends = (row + 1) * a.seq_len;
       float w = scale / (float)a.w.row_counts[row];  // (a row of none is asked for nothing)
-      four_steps(a, i, left, m, acc, [&](int64_t at, int x) {
-        while (at + x >= ends) w = scale / (float)a.w.row_counts[++row], ends += a.seq_len;
+      four_steps(a, x, i, left, m, acc, [&](int64_t at, int which) {
+        while (at + which >= ends) w = scale / (float)a.w.row_counts[++row], ends += a.seq_len;
         return w;
       });
     }
+    if (i + step < a.n) load(i + step);
   }
   finish_loss<kNT>(acc, a.c, a.out);
 }
@@ -162,8 +181,11 @@ __global__ __launch_bounds__(kSmallNT) void small_loss_kernel(const LossArgs<E> 
   count = block_sum<kSmallNT>(count, sums);
   const float scale = count > 0 ? 1.f / (float)count : 0.f;
   double acc[kTerms] = {};
-  if (i < n)
-    four_steps(a, i, left, m, acc, [&](int64_t at, int x) { return rows ? scale / (float)counts[((int)at + x) / T] : scale; });
+  if (i < n) {
+    FourSteps x;
+    x.load(a, i, left);
+    four_steps(a, x, i, left, m, acc, [&](int64_t at, int which) { return rows ? scale / (float)counts[((int)at + which) / T] : scale; });
+  }
   finish_loss<kSmallNT>(acc, a.c, a.out);
 }
 
