@@ -1,7 +1,7 @@
 // rlk_logits_loss.hip -- the clipped policy loss from logits and the logits' gradient in one pass over them
 // (include/rl_triton_policy.h; the mathematics is in rlk_action_rows.hpp and rlk_policy.hpp).
 // Bound by HBM where rows are long: [16,512] of 65536 bfloat16 378 us a call, 5.7 TB/s of reads and writes, [7,285] of 50001
-// float32 139, 5.7 TB/s (a large copy 5.2).  [4096,128] of 18 float32: 30 us, 2.8 TB/s (floor 16): rows of 72 bytes go through
+// float32 139, 5.7 TB/s (a large copy 5.2).  [4096,128] of 18 float32: 23 to 25 us, 3.5 TB/s (floor 16): rows of 72 bytes go through
 // LDS, and computing on them takes as long as moving them.
 #include "rlk_action_rows.hpp"
 
@@ -176,7 +176,10 @@ int impl(const rlk_action_rows* rows, const rlk_policy_terms* t, void* grad, hip
   FewRows few;
   if (few_rows(a, grad, &few)) {
     int64_t blocks = (a.rows + kFewRows - 1) / kFewRows;
-    if (blocks > kMaxLossBlocks) blocks = kMaxLossBlocks;
+    // Two tiles a workgroup and more where LDS would hold a workgroup for every tile: one's loads go on beside another's
+    // sums ([4096,128], in a graph: 2 actions 17.2 -> 13.7 us, 18 28.7 -> 24.7; 28, of which fewer fit, 37.7 and 38.3).
+    const int64_t most = a.A <= 24 ? 1024 : kMaxLossBlocks;
+    if (blocks > most) blocks = most;
     return dispatch_few(a.A, [&](auto k) {
       few_loss_kernel<E, decltype(k)::value><<<dim3((unsigned)blocks), dim3(kFewRows), FewRows::bytes(few.pitch), s>>>(
           a, few, arrays, plan.consts, plan.weights, plan.out, static_cast<E*>(grad));
