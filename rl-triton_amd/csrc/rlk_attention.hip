@@ -20,7 +20,7 @@
 //
 // Measured (us; floors are bytes at the 5.2 TB/s of a large copy): bfloat16 [64,1024,8,64] 75 forward (floor 52) and 185 for
 // the three walks back (90 with each array read once); float32 185 and 460 (103, 181).  [1,16384,16,128], a row of
-// segments: states 43, join 8.5, walks 84 (52 for all).  [37,333,4,40 and 72] float32: 60 and 113 (18 for both; the
+// segments: states 43, join 7.8, walks 83 (52 for all).  [37,333,4,40 and 72] float32: 60 and 113 (18 for both; the
 // useful products alone 13), on 148 of 256 CUs forward, each with the wavefronts' fifth tile of columns on one SIMD.
 // Neither HBM nor the matrix units are the bound in bfloat16: the vector units are busy for 43% of the time (a chunk costs a
 // wavefront some 450 instructions, a quarter of them the weights' split into three), matrix products for 15%, and
@@ -683,7 +683,8 @@ __global__ __launch_bounds__(4 * D, 2) void walk_kernel(const Walks<E> walks) {
       }
 }
 
-// The states that enter the segments: in place, from what each segment added and how much of what enters it leaves.
+// The states that enter the segments: in place, from what each segment added and how much of what enters it leaves.  The chain is
+// one multiply-add a segment: what it waits for are the loads, so 16 are on their way at once.
 template <class E>
 __global__ __launch_bounds__(256) void join_kernel(const Walks<E> walks) {
   const Walk<E>& w = walks.w[blockIdx.z];
@@ -696,11 +697,22 @@ __global__ __launch_bounds__(256) void join_kernel(const Walks<E> walks) {
     const int64_t at = w.transposed ? (int64_t)(i % w.dc) * w.da + i / w.dc : i;
     u = w.state[eh * n + at] * (w.reverse ? w.state_scale : w.state_scale * walks.decay[eh % walks.heads]);
   }
-  for (int s = 1; s < walks.segs; ++s) {
-    float* p = w.seg_states + (eh * walks.segs + s) * (int64_t)n + i;
-    const float keep = w.seg_keep[eh * walks.segs + s];
-    u = keep < 0.f ? *p : fmaf(u, keep, *p);  // (no part of u, NaN included, passes an episode's end; one too small to see leaves a NaN)
-    *p = u;
+  constexpr int AHEAD = 16;
+  float* p = w.seg_states + eh * walks.segs * (int64_t)n + i;
+  const float* keeps = w.seg_keep + eh * walks.segs;
+  for (int s0 = 1; s0 < walks.segs; s0 += AHEAD) {
+    float x[AHEAD], keep[AHEAD];
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) {
+      const int s = s0 + k < walks.segs ? s0 + k : s0;  // (one that is there, for those past the last)
+      x[k] = p[(int64_t)s * n], keep[k] = keeps[s];
+    }
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) {
+      if (s0 + k >= walks.segs) break;
+      u = keep[k] < 0.f ? x[k] : fmaf(u, keep[k], x[k]);  // (no part of u, NaN included, passes an episode's end; one too small to see leaves a NaN)
+      p[(int64_t)(s0 + k) * n] = u;
+    }
   }
 }
 
