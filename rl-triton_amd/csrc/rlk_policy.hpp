@@ -61,6 +61,7 @@ struct LossConsts {
   float log_low, log_high, log_dual;  // thresholds of D; log_dual = inf: no cap
   float low, high, dual;              // the values themselves, and what float32 leaves out of them
   float low_rest, high_rest, dual_rest;
+  float kl;  // kl_coef
   double kl_coef, entropy_coef;
 };
 
@@ -80,7 +81,8 @@ __device__ __forceinline__ void add_terms(double (&acc)[5], const StepTerms& t, 
 }
 
 // e^x - 1 - x >= 0 without the cancellation near zero: its series up to 1/2 in size (the first dropped
-// term is below 2^-25 of the sum), the plain difference beyond, where it loses at most two bits.
+// term is below 2^-25 of the sum), the plain difference beyond, where it loses at most two bits.  From 64 on e^x is all that
+// float32 holds of it (and infinity is, where the difference would be NaN).
 __device__ __forceinline__ float exp_minus_linear(float x, float ex) {
   float p = 1.f / 362880.f;
   p = fmaf(p, x, 1.f / 40320.f);
@@ -90,7 +92,7 @@ __device__ __forceinline__ float exp_minus_linear(float x, float ex) {
   p = fmaf(p, x, 1.f / 24.f);
   p = fmaf(p, x, 1.f / 6.f);
   p = fmaf(p, x, 0.5f);
-  return fabsf(x) < 0.5f ? p * x * x : (ex - 1.f) - x;
+  return fabsf(x) < 0.5f ? p * x * x : x > 64.f ? ex : (ex - 1.f) - x;
 }
 
 __device__ __forceinline__ StepTerms step_terms(float lp, float old, float adv, float ref, bool has_ref,
@@ -112,7 +114,9 @@ __device__ __forceinline__ StepTerms step_terms(float lp, float old, float adv, 
     const float e = ref - lp;
     const float ee = expf(e);
     t.kl = exp_minus_linear(e, ee);
-    t.slope -= (float)c.kl_coef * (t.kl + e);  // e^e - 1
+    // e^e - 1: from the series near zero, else as it stands.  A reference far below (-inf: an action that it forbids) has a KL term
+    // that holds nothing but -e, from which it could not be had again.  Without a coefficient there is none to follow.
+    if (c.kl != 0.f) t.slope -= c.kl * (fabsf(e) < 0.5f ? t.kl + e : ee - 1.f);
   }
   return t;
 }
@@ -237,7 +241,8 @@ __device__ __forceinline__ void finish_loss(const double (&acc)[kTerms], const L
   }
   if ((int)threadIdx.x < o.num_means) o.means[threadIdx.x] = (float)x;
   const double kl = __shfl(x, 1), entropy = __shfl(x, 4);
-  if (threadIdx.x == 0) *o.loss = (float)(x + c.kl_coef * kl - c.entropy_coef * entropy);
+  // (a term without a coefficient has no part, infinite or not)
+  if (threadIdx.x == 0) *o.loss = (float)(x + (c.kl_coef != 0.0 ? c.kl_coef * kl : 0.0) - (c.entropy_coef != 0.0 ? c.entropy_coef * entropy : 0.0));
 }
 
 }  // namespace rlk

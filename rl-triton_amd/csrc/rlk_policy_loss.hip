@@ -256,7 +256,7 @@ int plan_loss(const rlk_policy_terms* t, int64_t num_envs, int64_t seq_len, int 
   c.log_low = t->clip_low < 1.0 ? (float)std::log1p(-t->clip_low) : -INFINITY;
   c.log_high = (float)std::log1p(t->clip_high);
   c.log_dual = t->dual_clip > 0.0 ? (float)std::log(t->dual_clip) : INFINITY;
-  c.kl_coef = t->kl_coef, c.entropy_coef = t->entropy_coef;
+  c.kl = (float)t->kl_coef, c.kl_coef = t->kl_coef, c.entropy_coef = t->entropy_coef;
   char* ws = static_cast<char*>(t->workspace);
   p->out = {reinterpret_cast<double*>(ws + kTicketBytes), reinterpret_cast<uint32_t*>(ws), t->loss, t->means, means};
   p->count_parts = reinterpret_cast<int64_t*>(p->out.partials + (int64_t)kMaxLossBlocks * kPartials);

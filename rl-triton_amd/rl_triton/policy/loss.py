@@ -64,7 +64,7 @@ def compute_policy_loss(
         advantages:    [num_envs, seq_len] (compute_gae, compute_gae_normalized, compute_vtrace).
         ref_log_probs: the same under a reference policy, or None.
         clip_low, clip_high: how far the ratio may leave 1 (default 0.2 each).
-        kl_coef:       what the KL term counts for.
+        kl_coef:       what the KL term counts for (0: it is measured, and has no part in the loss or the gradient).
         dual_clip:     bound of the ratio for negative advantages, above 1, or None.
         mask:          nonzero for the steps that take part, or None for all.
         reduction:     "steps" or "rows".
