@@ -59,19 +59,26 @@ at::Tensor policy_output(at::IntArrayRef sizes, at::ScalarType st, const at::Ten
 const void* data_or_null(const at::Tensor* t) { return t ? t->data_ptr() : nullptr; }
 
 // Scratch memory, one of each kind per (device, stream), as rl_triton.policy._native keeps it; none (declined) while
-// the stream is capturing a graph.
+// the stream is capturing a graph.  A backward pass asks for its own on torch's thread and without the interpreter lock, so the
+// map has a lock of its own.  What it holds is guarded by kind: `sums` and `rows`, which calls from Python alone use, by the
+// interpreter lock, `states` by StatesScratch's.  (An element stays where it is when others are added.)
 struct PolicyScratch {
   at::Tensor sums, rows, states;
 };
+PolicyScratch& scratch_of(int dev, uintptr_t stream) {
+  static auto* lock = new std::mutex;
+  static auto* all = new std::map<std::pair<int, uintptr_t>, PolicyScratch>();
+  const std::lock_guard<std::mutex> held(*lock);
+  return (*all)[{dev, stream}];
+}
 bool policy_scratch(const PolicyCall& c, at::Tensor PolicyScratch::* kind, size_t need, const at::Tensor& like, void** ptr,
                     size_t* bytes) {
   *ptr = nullptr, *bytes = 0;
   if (need == 0) return true;
-  static auto* all = new std::map<std::pair<int, uintptr_t>, PolicyScratch>();
   hipStream_t s = static_cast<hipStream_t>(c.stream());
   hipStreamCaptureStatus cs = hipStreamCaptureStatusNone;
   if (hipStreamIsCapturing(s, &cs) != hipSuccess || cs != hipStreamCaptureStatusNone) return false;
-  at::Tensor& buf = (*all)[{(int)c.dev, reinterpret_cast<uintptr_t>(s)}].*kind;
+  at::Tensor& buf = scratch_of((int)c.dev, reinterpret_cast<uintptr_t>(s)).*kind;
   if (!buf.defined() || (size_t)buf.numel() < need)
     buf = zeroed((int64_t)(buf.defined() ? std::max(need, 2 * (size_t)buf.numel()) : need), like);
   *ptr = buf.data_ptr(), *bytes = (size_t)buf.numel();
