@@ -171,7 +171,9 @@ def compute_linear_attention_step(
         state:     [num_envs, heads, dim_k, dim_v], float32, contiguous.
         dones:     nonzero where the step before ended its episode, [num_envs], float32, bfloat16 or bool, or None.
         scale:     default dim_k ** -0.5.
-        out_state: where to write the new state (`state` itself: in place), float32, contiguous; default a new tensor.
+        out_state: where to write the new state (`state` itself: in place), float32, contiguous; default a new tensor.  As for
+                   torch's in-place operations, a backward pass that needs what it held raises, and where gradients are
+                   enabled it must not require one.
 
     Returns:
         out:   [num_envs, heads, dim_v], the dtype of q.
@@ -187,6 +189,9 @@ def compute_linear_attention_step(
             out_state.shape == state.shape and out_state.is_contiguous(), "out_state must be a contiguous float32 tensor like state"
         apart = abs(out_state.data_ptr() - state.data_ptr())
         assert apart == 0 or apart >= 4 * state.numel(), "out_state overlaps state without being it"
+        if torch.is_grad_enabled() and out_state.requires_grad:
+            raise RuntimeError("out_state requires a gradient and cannot be written over")
+        torch.autograd.graph.increment_version(out_state)  # (a graph that saved what it held has to know)
     out = torch.empty(v.shape, dtype=v.dtype, device=v.device)
     if q.shape[0] and q.shape[1]:
         _native.linear_attention_step(decay.contiguous(), _dones(dones),
