@@ -10,20 +10,20 @@
 struct PolicyCall {
   c10::DeviceIndex dev = -1;
   bool ok = true;
-  bool wants_grad = false;  // by a tensor that the function is differentiable in
+  bool wants_grad = false;  // a gradient by one of the tensors looked at with `graph`
 
   const at::Tensor* fail() {
     ok = false;
     return nullptr;
   }
-  // A tensor on the current GPU that is an ordinary one; `graph`: the function is differentiable in it.
+  // A tensor on the current GPU that is an ordinary one; `graph`: one whose derivatives are given, or refused where they are asked for.
   const at::Tensor* tensor(PyObject* o, bool graph) {
     if (!ok || !THPVariable_Check(o)) return fail();
     const at::Tensor& t = THPVariable_Unpack(o);
     if (!t.is_cuda() || t.is_neg()) return fail();
-    if (graph && t.requires_grad() && at::GradMode::is_enabled()) {
-      if (t._fw_grad(0).defined()) return fail();  // (forward derivatives are refused by the Python path)
-      wants_grad = true;
+    if (graph) {
+      if (t._fw_grad(0).defined()) return fail();  // (a dual tensor, which need not require a gradient: refused by the Python path)
+      if (t.requires_grad() && at::GradMode::is_enabled()) wants_grad = true;
     }
     if (dev < 0) {
       dev = t.get_device();
@@ -285,8 +285,8 @@ PyObject* op_policy_loss_from_logits(PyObject* const* a, Py_ssize_t n) {
 // q, k, v of a sequence ([envs, steps, heads, dim]) or of a step ([envs, heads, dim]) and what goes with them.
 bool attention_args(PolicyCall& c, PyObject* q_, PyObject* k_, PyObject* v_, PyObject* decay_, PyObject* dones_, PyObject* state_,
                     PyObject* scale_, bool steps, rlk_attention* t, const at::Tensor** v, at::Tensor* flags) {
-  const at::Tensor *q = c.tensor(q_, steps), *k = c.tensor(k_, steps);
-  *v = c.tensor(v_, steps);
+  const at::Tensor *q = c.tensor(q_, true), *k = c.tensor(k_, true);
+  *v = c.tensor(v_, true);
   if (!c.ok || !float_type(q->scalar_type()) || k->scalar_type() != q->scalar_type() || (*v)->scalar_type() != q->scalar_type()) return false;
   const int64_t rank = steps ? 4 : 3;
   if (q->dim() != rank || (*v)->dim() != rank || k->sizes() != q->sizes() ||
@@ -301,14 +301,14 @@ bool attention_args(PolicyCall& c, PyObject* q_, PyObject* k_, PyObject* v_, PyO
   for (const at::Tensor* x : {q, k, *v})
     if (x->size(rank - 1) > 1 && x->stride(rank - 1) != 1) return false;
   t->q = seq(*q), t->k = seq(*k), t->v = seq(**v);
-  const at::Tensor* decay = c.array(decay_, at::kFloat, {t->heads});
+  const at::Tensor* decay = c.array(decay_, at::kFloat, {t->heads}, true);
   const at::Tensor* dones = dones_ == Py_None ? nullptr : c.tensor(dones_, false);
   if (!c.ok || (dones && (dones->scalar_type() != at::kFloat || dones->sizes() != q->sizes().slice(0, steps ? 2 : 1)))) return false;
   if (dones && !dones->is_contiguous()) {  // (a step's column of a rollout buffer)
     *flags = dones->contiguous();
     dones = flags;
   }
-  const at::Tensor* state = c.opt(state_, at::kFloat, {t->num_envs, t->heads, t->dim_k, t->dim_v}, steps);
+  const at::Tensor* state = c.opt(state_, at::kFloat, {t->num_envs, t->heads, t->dim_k, t->dim_v}, true);
   if (!c.ok || decay->requires_grad()) return false;  // (refused by the Python path)
   const double scale = scale_ == Py_None ? 1.0 / std::sqrt((double)t->dim_k) : c.number(scale_, -HUGE_VAL);
   if (!c.ok || (float)scale == 0.f || !std::isfinite((float)scale)) return false;

@@ -10,6 +10,7 @@ import ctypes
 import threading
 
 import torch
+from torch.autograd import forward_ad
 
 from rl_triton import _native
 
@@ -107,6 +108,12 @@ def _on_device(fn):
                     return fn(dev, _native._raw_stream(dev), lead, *args)
             return fn(dev, _native._raw_stream(dev), lead, *args)
     return call
+
+
+def refuse_forward_derivatives(*tensors):
+    """Raises for dual tensors, whose tangents the kernels would drop (they need not require a gradient)."""
+    if any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError("forward-mode derivatives of rl_triton.policy's functions are not implemented")
 
 
 def _ptr(t):

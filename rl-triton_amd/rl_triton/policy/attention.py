@@ -38,6 +38,7 @@ def _check_attention(q, k, v, decay, dones, state, scale, steps):
     if scale is None:
         scale = q.shape[-1] ** -0.5
     assert isinstance(scale, (int, float)) and math.isfinite(scale) and scale != 0, f"scale must be a number other than 0, got {scale!r}"
+    _native.refuse_forward_derivatives(q, k, v, decay, state)
     if _CORRECTNESS_WARNINGS():
         assert bool(((decay >= 0) & (decay <= 1)).all()), "decay must lie in [0, 1]"
     return float(scale)

@@ -92,6 +92,7 @@ def compute_action_log_probs(
         log_probs, entropies: [...], float32 whatever the logits' type (ratios of probabilities are taken of them).
     """
     _check_rows(logits, actions, temperature)
+    _native.refuse_forward_derivatives(logits)
     if torch.is_grad_enabled() and logits.requires_grad:
         return _ActionLogProbs.apply(logits, actions, float(temperature))
     return _forward(logits, actions, float(temperature), None)

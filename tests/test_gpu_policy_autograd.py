@@ -58,3 +58,27 @@ def test_a_tensor_with_a_gradient_is_not_written_over():
         frozen = state.clone()
         policy.compute_linear_attention_step(q, k, v, decay, frozen, out_state=frozen)
     assert torch.equal(frozen, want)
+
+
+def test_forward_derivatives_are_refused():
+    """A dual tensor need not require a gradient: its tangent must not be dropped in silence."""
+    q, k, v, decay, state = _step_args()
+    x, a = torch.randn(4, 7, device="cuda"), torch.zeros(4, dtype=torch.int64, device="cuda")
+    seq = torch.randn(3, 5, 2, 16, device="cuda")
+    for mode in (torch.enable_grad, torch.no_grad):
+        for wants in (False, True):
+            with mode(), fwAD.dual_level():
+                dual = lambda t: fwAD.make_dual(t.detach().clone().requires_grad_(wants), torch.ones_like(t))  # noqa: E731
+                calls = [lambda: policy.compute_action_log_probs(dual(x), a),
+                         lambda: policy.compute_linear_attention(dual(seq), seq, seq, decay),
+                         lambda: policy.compute_linear_attention(seq, dual(seq), seq, decay),
+                         lambda: policy.compute_linear_attention(seq, seq, dual(seq), decay),
+                         lambda: policy.compute_linear_attention(seq, seq, seq, decay, None, dual(state)),
+                         lambda: policy.compute_linear_attention(seq, seq, seq, fwAD.make_dual(decay, torch.ones_like(decay))),
+                         lambda: policy.compute_linear_attention_step(dual(q), k, v, decay, state),
+                         lambda: policy.compute_linear_attention_step(q, k, v, decay, dual(state))]
+                for call in calls:
+                    with pytest.raises((NotImplementedError, RuntimeError), match="[Ff]orward"):
+                        call()
+                policy.compute_linear_attention(seq, seq, seq, decay)  # (no dual among them: as ever)
+                policy.compute_action_log_probs(x, a)
