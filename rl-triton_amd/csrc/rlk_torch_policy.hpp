@@ -429,6 +429,17 @@ PyObject* op_linear_attention(PyObject* const* a, Py_ssize_t n) {
   return finish(rlk_linear_attention(&t, 1, c.stream()), "rlk_linear_attention", pair(out, last));
 }
 
+// A step's output where a gradient is wanted of it: it has none, and says so when it is asked for, not before.  The node's one input
+// is a tensor of its own, so nothing of the steps before is held; the state goes on without a graph.
+struct StepOutput : torch::autograd::Function<StepOutput> {
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext*, const at::Tensor&, const at::Tensor& v, rlk_attention* t) {
+    return {attention_out(v, t)};
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext*, torch::autograd::variable_list) {
+    TORCH_CHECK(false, "compute_linear_attention_step computes no gradient: a learner runs compute_linear_attention over the steps");
+  }
+};
+
 // linear_attention_step(q, k, v, decay, state, dones, scale, out_state)
 PyObject* op_linear_attention_step(PyObject* const* a, Py_ssize_t n) {
   if (n != 8 || a[7] != Py_None || correctness_warnings()) return decline();
@@ -437,7 +448,8 @@ PyObject* op_linear_attention_step(PyObject* const* a, Py_ssize_t n) {
   const at::Tensor* v;
   at::Tensor flags;
   if (!attention_args(c, a[0], a[1], a[2], a[3], a[5], a[4], a[6], false, &t, &v, &flags) || !t.state) return decline();
-  at::Tensor out = attention_out(*v, &t), next = policy_output({t.num_envs, t.heads, t.dim_k, t.dim_v}, at::kFloat, *v);
+  at::Tensor out = c.wants_grad ? StepOutput::apply(at::empty({0}, v->options()).requires_grad_(true), v->detach(), &t)[0] : attention_out(*v, &t);
+  at::Tensor next = policy_output({t.num_envs, t.heads, t.dim_k, t.dim_v}, at::kFloat, *v);
   t.state_out = static_cast<float*>(next.data_ptr());
   return finish(rlk_linear_attention_step(&t, c.stream()), "rlk_linear_attention_step", pair(out, next));
 }

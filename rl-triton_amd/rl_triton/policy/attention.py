@@ -100,6 +100,19 @@ class _LinearAttention(torch.autograd.Function):
         return (*grads, None, None, grad_state, None)
 
 
+class _StepOutput(torch.autograd.Function):
+    """A step's output where a gradient is wanted of it: it has none, and says so when it is asked for.  `asked` is a tensor of its
+    own, so that nothing of the steps before is held."""
+
+    @staticmethod
+    def forward(ctx, asked, out):
+        return out.view_as(out)
+
+    @staticmethod
+    def backward(ctx, grad_out):
+        raise RuntimeError("compute_linear_attention_step computes no gradient: a learner runs compute_linear_attention over the steps")
+
+
 def compute_linear_attention(
     q: torch.Tensor,
     k: torch.Tensor,
@@ -163,7 +176,8 @@ def compute_linear_attention_step(
 
     - S' = decay[h] * (1 - done) * state + k v^T,  out = scale * S'^T q
 
-    No gradient is computed (a learner runs whole sequences).
+    No gradient is computed (a learner runs whole sequences): where one of the inputs requires one, a backward pass through
+    the output raises.  The state comes without a graph.
 
     Args:
         q, k:      [num_envs, heads, dim_k], float32 or bfloat16, GPU.
@@ -198,4 +212,6 @@ def compute_linear_attention_step(
         _native.linear_attention_step(decay.contiguous(), _dones(dones),
                                       _native.Pass(_inner(q.detach()), _inner(k.detach()), _inner(v.detach()), out, state.detach(),
                                                    out_state, scale))
+    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, state)):
+        out = _StepOutput.apply(torch.empty(0, dtype=out.dtype, device=out.device, requires_grad=True), out)
     return out, out_state

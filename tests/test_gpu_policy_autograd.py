@@ -82,3 +82,38 @@ def test_forward_derivatives_are_refused():
                         call()
                 policy.compute_linear_attention(seq, seq, seq, decay)  # (no dual among them: as ever)
                 policy.compute_action_log_probs(x, a)
+
+
+def test_a_step_says_that_it_has_no_gradient():
+    """Steps that are unrolled into a loss: the error comes when the gradient is asked for, not a gradient without a part of it."""
+    q, k, v, decay, state = _step_args(True)
+    plain = policy.compute_linear_attention_step(q.detach(), k.detach(), v.detach(), decay, state)
+    for wrt in (q, k, v, state.clone().requires_grad_()):
+        args = [q.detach(), k.detach(), v.detach(), decay, state]
+        if wrt is q or wrt is k or wrt is v:
+            args[0 if wrt is q else 1 if wrt is k else 2] = wrt
+        else:
+            args[4] = wrt
+        out, new = policy.compute_linear_attention_step(*args)
+        assert torch.equal(out, plain[0]) and torch.equal(new, plain[1])
+        assert not new.requires_grad
+        weight = torch.ones((), device="cuda", requires_grad=True)
+        with pytest.raises(RuntimeError, match="compute_linear_attention_step"):
+            (weight * out).sum().backward()
+        out, new = policy.compute_linear_attention_step(*args, out_state=torch.empty_like(state))
+        assert torch.equal(out, plain[0]) and not new.requires_grad
+        with pytest.raises(RuntimeError, match="compute_linear_attention_step"):
+            out.sum().backward()
+        with torch.no_grad():
+            assert not any(t.requires_grad for t in policy.compute_linear_attention_step(*args))
+    assert not any(t.requires_grad for t in plain)
+
+
+def test_unrolled_steps_hold_nothing_back():
+    """What a step's results hold on to does not grow with the steps before them."""
+    q, k, v, decay, state = _step_args(True)
+    sizes = []
+    for _ in range(6):
+        out, state = policy.compute_linear_attention_step(q * 1, k * 1, v * 1, decay, state)
+        sizes.append(torch.cuda.memory_allocated())
+    assert sizes[-1] == sizes[1] and out.requires_grad
