@@ -628,7 +628,8 @@ __global__ __launch_bounds__(4 * D, 2) void walk_kernel(const Walks<E> walks) {
         for (int r = 0; r < 4; ++r) {
           const int d = 16 * m + 4 * v4 + r;
           const float b = load_one(reinterpret_cast<const E*>(tile + M::BT + M::transposed(d, i)));
-          U[m][r] = fmaf(b, c, cut || keep == 0.f ? 0.f : U[m][r] * keep);
+          // (a padded row stays 0: times an inf its zeros would be NaN, and in the sum over all rows)
+          U[m][r] = FULL || d < da ? fmaf(b, c, cut || keep == 0.f ? 0.f : U[m][r] * keep) : 0.f;
           if constexpr (!STATE) sum = fmaf(load_one(reinterpret_cast<const E*>(tile + M::A + i * M::ROW + d * M::S)), U[m][r], sum);
         }
         __builtin_amdgcn_sched_barrier(0);
