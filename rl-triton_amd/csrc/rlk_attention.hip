@@ -381,7 +381,7 @@ __global__ __launch_bounds__(4 * D, 2) void walk_kernel(const Walks<E> walks) {
 #pragma unroll
       for (int m = 0; m < MT; ++m)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) U[m][r] = 16 * m + 4 * l4 + r < da && j < dc ? U[m][r] * f : 0.f;
+        for (int r = 0; r < 4; ++r) U[m][r] = 16 * m + 4 * l4 + r < da && j < dc && f != 0.f ? U[m][r] * f : 0.f;
   }
 
   // This wavefront's part of p: rows i = 16 ti + l16, tiles of columns jt = wave % SHARE + SHARE u.  Computed
@@ -696,7 +696,8 @@ __global__ __launch_bounds__(256) void join_kernel(const Walks<E> walks) {
   float u = 0.f;
   if (w.state != nullptr) {
     const int64_t at = w.transposed ? (int64_t)(i % w.dc) * w.da + i / w.dc : i;
-    u = w.state[eh * n + at] * (w.reverse ? w.state_scale : w.state_scale * walks.decay[eh % walks.heads]);
+    const float f = w.reverse ? w.state_scale : w.state_scale * walks.decay[eh % walks.heads];
+    u = f == 0.f ? 0.f : w.state[eh * n + at] * f;  // (a decay of 0 leaves nothing of it, NaN included)
   }
   constexpr int AHEAD = 16;
   float* p = w.seg_states + eh * walks.segs * (int64_t)n + i;

@@ -24,8 +24,8 @@ __global__ __launch_bounds__(kNT) void step_kernel(const Walk<E> w, int heads, i
     qs[tid] = load_one(w.a.data + env * w.a.env_stride + head * w.a.head_stride + tid);
     ks[tid] = load_one(w.b.data + env * w.b.env_stride + head * w.b.head_stride + tid);
   }
-  const bool cut = dones != nullptr && dones[env] != 0.f;
   const float lambda = decay[head];
+  const bool cut = lambda == 0.f || (dones != nullptr && dones[env] != 0.f);
   const E* gv = w.c.data + env * w.c.env_stride + head * w.c.head_stride;
   float v[4];
 #pragma unroll
@@ -39,7 +39,7 @@ __global__ __launch_bounds__(kNT) void step_kernel(const Walk<E> w, int heads, i
     float4 x{0.f, 0.f, 0.f, 0.f};
     if (j < w.dc) {
       const int at = i * w.dc + j;
-      if (!cut) {  // (what a cut state held has no part, NaN included)
+      if (!cut) {  // (what a cut state held has no part, NaN included, nor what a decay of 0 leaves)
         if constexpr (VEC) {
           x = load_quad<NT>(src + at);
         } else {

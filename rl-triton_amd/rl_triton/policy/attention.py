@@ -141,7 +141,7 @@ def compute_linear_attention(
                (time-major views and slices of a joint projection are read in place, and heads that share keys or
                values may be expanded ones).  Dimensions of 1 to 128.
         v:     [num_envs, seq_len, heads, dim_v], the dtype of q.
-        decay: [heads], float32, in [0, 1].
+        decay: [heads], float32, in [0, 1].  (0 leaves nothing of a state, NaN included.)
         dones: nonzero where the episode ended with that step, [num_envs, seq_len], float32, bfloat16 or bool, or None.
         state: what the sequences go on from, [num_envs, heads, dim_k, dim_v], float32, or None (zeros).
         scale: default dim_k ** -0.5.

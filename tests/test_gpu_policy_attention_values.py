@@ -1,5 +1,5 @@
 """Linear attention at values and sizes where one path of it could answer otherwise than another: infinities at head dims that fill
-no whole tile."""
+no whole tile, decays of 0."""
 import math
 
 import pytest
@@ -35,3 +35,23 @@ def test_infinities_stay_infinities(dk, dv, dtype):
         x = x.detach().cpu().double()
         assert torch.equal(x.isnan(), w.isnan()), i
         assert torch.equal(x == math.inf, w == math.inf) and torch.equal(x == -math.inf, w == -math.inf), i
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+def test_a_decay_of_zero_forgets_what_is_not_finite(bad, dtype):
+    """A head that forgets everything forgets a state that is not finite too, in whole sequences (one segment and several) and in
+    single steps alike."""
+    for T in (3, 700):
+        g = torch.Generator().manual_seed(T)
+        q, k, v = (torch.randn(1, T, 2, 24, generator=g).to(dtype) for _ in range(3))
+        s = torch.randn(1, 2, 24, 24, generator=g)
+        s[0, 0, 3] = bad
+        decay = torch.tensor([0.0, 0.5])
+        out, last = policy.compute_linear_attention(*(t.cuda() for t in (q, k, v, decay)), None, s.cuda())
+        zero = torch.where(decay[None, :, None, None] == 0, 0.0, s)
+        want, wlast = policy.compute_linear_attention(*(t.cuda() for t in (q, k, v, decay)), None, zero.cuda())
+        assert bool(out.isfinite().all()) and torch.equal(out, want) and torch.equal(last, wlast)
+        o, new = policy.compute_linear_attention_step(*(t[:, 0].cuda() for t in (q, k, v)), decay.cuda(), s.cuda())
+        wo, wnew = policy.compute_linear_attention_step(*(t[:, 0].cuda() for t in (q, k, v)), decay.cuda(), zero.cuda())
+        assert bool(o.isfinite().all()) and torch.equal(o, wo) and torch.equal(new, wnew)
