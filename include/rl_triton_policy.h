@@ -92,7 +92,7 @@ typedef struct rlk_attention {
    * gradient of the state after the last one. */
   const float *state;
   int state_transposed; /* `state` is [num_envs, heads, dim_v, dim_k] */
-  /* NULL, or the state after the last step, zero if that step is done; reverse: the gradient of the state before
+  /* NULL, or the state after the last step, zero if that step is done (of no steps: `state`); reverse: the gradient of the state before
    * the first step. */
   float *state_out;
   float scale;                        /* of out */

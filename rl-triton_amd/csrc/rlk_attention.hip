@@ -718,6 +718,25 @@ __global__ __launch_bounds__(256) void join_kernel(const Walks<E> walks) {
   }
 }
 
+// The state that leaves a sequence of no steps: the one that enters it.
+__global__ __launch_bounds__(256) void no_steps_state_kernel(const float* state, float* state_out, int64_t pairs, int da, int dc, bool transposed,
+                                                             float scale) {
+  const int64_t n = (int64_t)da * dc, step = (int64_t)gridDim.x * 256;
+  for (int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x; at < pairs * n; at += step) {
+    const int64_t eh = at / n;
+    const int i = (int)(at - eh * n);
+    state_out[at] = state == nullptr ? 0.f : state[transposed ? eh * n + (int64_t)(i % dc) * da + i / dc : at] * scale;
+  }
+}
+
+int no_steps(const rlk_attention& c, hipStream_t s) {
+  if (!c.state_out) return RLK_OK;
+  const int64_t pairs = c.num_envs * c.heads, units = (pairs * c.dim_k * c.dim_v + 255) / 256;
+  no_steps_state_kernel<<<dim3((unsigned)(units < 4096 ? units : 4096)), dim3(256), 0, s>>>(
+      c.state, c.state_out, pairs, (int)c.dim_k, (int)c.dim_v, c.state_transposed != 0, c.state_scale * c.state_out_scale);
+  return hipGetLastError() == hipSuccess ? RLK_OK : RLK_ERR_LAUNCH;
+}
+
 template <class E, int D, int FORM>
 int launch_walks(Walks<E> k, int count, hipStream_t s) {
   const int64_t envs = k.num_envs, most = kMaxPairs / k.heads;
@@ -796,13 +815,18 @@ int rlk_linear_attention(const rlk_attention* calls, int count, void* stream) {
   if (!calls || count < 1 || count > 3) return RLK_ERR_INVALID_ARGUMENT;
   for (int i = 0; i < count; ++i) {
     const rlk_attention& c = calls[i];
-    if (!valid_attention(c) || c.seq_len < 0 || c.num_envs != calls->num_envs || c.seq_len != calls->seq_len ||
+    if (!valid_attention(c, c.seq_len != 0) || c.seq_len < 0 || c.num_envs != calls->num_envs || c.seq_len != calls->seq_len ||
         c.heads != calls->heads || c.decay != calls->decay || c.dones != calls->dones || c.bf16 != calls->bf16)
       return RLK_ERR_INVALID_ARGUMENT;
   }
-  if (calls->num_envs == 0 || calls->heads == 0 || calls->seq_len == 0) return RLK_OK;
+  if (calls->num_envs == 0 || calls->heads == 0) return RLK_OK;
   if (calls->heads > kMaxPairs || calls->seq_len > (int64_t{1} << 30)) return RLK_ERR_INVALID_ARGUMENT;
   const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  if (calls->seq_len == 0) {
+    int st = RLK_OK;
+    for (int i = 0; i < count && st == RLK_OK; ++i) st = no_steps(calls[i], s);
+    return st;
+  }
   return calls->bf16 ? walk_impl<bf16>(calls, count, s) : walk_impl<float>(calls, count, s);
 }
 

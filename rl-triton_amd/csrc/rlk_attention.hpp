@@ -43,13 +43,13 @@ Sequence<E> sequence(const rlk_sequence& x) {
   return {static_cast<E*>(const_cast<void*>(x.data)), x.env_stride, x.step_stride, x.head_stride};
 }
 
-inline bool valid_attention(const rlk_attention& c) {
+inline bool valid_attention(const rlk_attention& c, bool steps = true) {  // steps: there are any, so their arrays are
   if (c.num_envs < 0 || c.heads < 0 || c.dim_k < 1 || c.dim_k > 128 || c.dim_v < 1 || c.dim_v > 128) return false;
   if (!std::isfinite(c.scale) || !std::isfinite(c.state_scale) || !std::isfinite(c.state_out_scale)) return false;
   if (c.num_envs == 0 || c.heads == 0) return true;
   const uintptr_t low = c.bf16 ? 1u : 3u;
   for (const rlk_sequence* x : {&c.q, &c.k, &c.v, &c.out})
-    if (!x->data || (reinterpret_cast<uintptr_t>(x->data) & low) != 0) return false;
+    if (steps && (!x->data || (reinterpret_cast<uintptr_t>(x->data) & low) != 0)) return false;
   return c.decay != nullptr;
 }
 

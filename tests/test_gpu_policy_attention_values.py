@@ -1,5 +1,6 @@
 """Linear attention at values and sizes where one path of it could answer otherwise than another: infinities at head dims that fill
-no whole tile, decays of 0."""
+no whole tile, decays of 0, sequences of no steps."""
+import ctypes
 import math
 
 import pytest
@@ -7,6 +8,7 @@ import torch
 
 import rl_triton.policy as policy
 from _policy_reference import attention, attention_grads
+from rl_triton.policy import _native
 
 pytestmark = pytest.mark.gpu
 
@@ -55,3 +57,20 @@ def test_a_decay_of_zero_forgets_what_is_not_finite(bad, dtype):
         o, new = policy.compute_linear_attention_step(*(t[:, 0].cuda() for t in (q, k, v)), decay.cuda(), s.cuda())
         wo, wnew = policy.compute_linear_attention_step(*(t[:, 0].cuda() for t in (q, k, v)), decay.cuda(), zero.cuda())
         assert bool(o.isfinite().all()) and torch.equal(o, wo) and torch.equal(new, wnew)
+
+
+@pytest.mark.parametrize("reverse", [0, 1])
+@pytest.mark.parametrize("transposed", [0, 1])
+def test_the_c_entry_writes_the_states_of_no_steps(reverse, transposed):
+    """The header: empty inputs launch nothing, but for states, which are written."""
+    E, H, dk, dv = 3, 2, 5, 7
+    state = torch.randn(E, H, dk, dv, device="cuda")
+    given = state.transpose(-1, -2).contiguous() if transposed else state
+    decay = torch.tensor([0.5, 0.25], device="cuda")
+    none = _native.Sequence(None, 0, 0, 0)
+    for enters, want in ((given, state * 3), (None, torch.zeros_like(state))):
+        out = torch.full_like(state, 7.0)
+        call = _native.Attention(none, none, none, none, E, 0, H, dk, dv, decay.data_ptr(), None, None if enters is None else enters.data_ptr(),
+                                 transposed, out.data_ptr(), 1.0, 2.0, 1.5, reverse, 0, None, 0)
+        assert _native.load().rlk_linear_attention(ctypes.byref(call), 1, torch.cuda.current_stream().cuda_stream) == 0
+        assert torch.equal(out, want)
