@@ -86,13 +86,14 @@ bool policy_scratch(const PolicyCall& c, at::Tensor PolicyScratch::* kind, size_
 }
 
 // Scratch memory of sequences cut into segments, held from its choice to the launch: a backward pass runs on torch's own
-// thread.  `keep`: a call that is being captured has memory of its own, for the graph's replays; else there is none.
+// thread.  `own`: a call that is being captured has memory of its own, from the graph's pool, which keeps its place for the replays
+// (others of the graph's may have it after the launch, in the stream's order) and goes with the graph; else there is none.
 class StatesScratch {
  public:
   void* ptr = nullptr;
   size_t bytes = 0;
   bool ok = true;
-  StatesScratch(const PolicyCall& c, size_t need, const at::Tensor& like, bool keep) {
+  StatesScratch(const PolicyCall& c, size_t need, const at::Tensor& like, bool own) {
     if (!lock().try_lock()) {  // (whoever holds it may need the interpreter before they let go)
       PyThreadState* state = PyGILState_Check() ? PyEval_SaveThread() : nullptr;
       lock().lock();
@@ -100,10 +101,9 @@ class StatesScratch {
     }
     try {
       ok = policy_scratch(c, &PolicyScratch::states, need, like, &ptr, &bytes);
-      if (!ok && keep) {
-        static auto* kept = new std::vector<at::Tensor>();
-        kept->push_back(zeroed((int64_t)need, like));
-        ptr = kept->back().data_ptr(), bytes = need, ok = true;
+      if (!ok && own) {
+        captured = at::empty({(int64_t)need}, like.options().dtype(at::kByte));
+        ptr = captured.data_ptr(), bytes = need, ok = true;
       }
     } catch (...) {
       lock().unlock();
@@ -114,6 +114,7 @@ class StatesScratch {
   StatesScratch(const StatesScratch&) = delete;
 
  private:
+  at::Tensor captured;
   static std::mutex& lock() {
     static auto* m = new std::mutex;
     return *m;

@@ -81,21 +81,20 @@ _launching = threading.Lock()  # from a workspace's choice to the launch: a back
 
 
 def _workspace(kind: str, dev: int, stream: int, need: int):
-    """Scratch memory of the current call: kept per (device, stream), grown by doubling, zero-filled when made; a
-    call being captured into a graph gets memory of its own (zero-filled by a kernel the graph records), kept for
-    the life of the process."""
+    """Scratch memory of the current call, to be held until its launch: kept per (device, stream), grown by doubling, zero-filled
+    when made.  A call being captured into a graph has memory of its own from the graph's pool, which keeps its place for the replays
+    (other work of the same graph may have it in turn, in the stream's order) and goes with the graph; "sums" are zero-filled there by
+    a kernel that the graph records, the others need no initial contents."""
     if need == 0:
-        return None, 0
+        return None
     device = torch.device("cuda", dev)
     if _native._capturing():
-        ws = torch.zeros(need, dtype=torch.uint8, device=device)
-        _native._captured.append(ws)
-        return ws.data_ptr(), need
+        return (torch.zeros if kind == "sums" else torch.empty)(need, dtype=torch.uint8, device=device)
     ws = _workspaces.get((kind, dev, stream))
     if ws is None or ws.numel() < need:
         ws = torch.zeros(max(need, 2 * ws.numel() if ws is not None else 0), dtype=torch.uint8, device=device)
         _workspaces[(kind, dev, stream)] = ws
-    return ws.data_ptr(), ws.numel()
+    return ws
 
 
 def _on_device(fn):
@@ -120,6 +119,10 @@ def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
+def _bytes(ws):
+    return 0 if ws is None else ws.numel()
+
+
 def _rows(logits, actions, temperature):
     e, t, a = logits.shape
     se, st, _ = logits.stride()
@@ -130,7 +133,8 @@ def _rows(logits, actions, temperature):
 def action_log_probs(dev, stream, logits, actions, temperature, log_probs, entropies, norms):
     rows = _rows(logits, actions, temperature)
     if actions.numel() <= 256:
-        rows.workspace, rows.workspace_bytes = _workspace("rows", dev, stream, ROWS_WORKSPACE_BYTES)
+        ws = _workspace("rows", dev, stream, ROWS_WORKSPACE_BYTES)
+        rows.workspace, rows.workspace_bytes = ws.data_ptr(), ws.numel()
     _native._check((_lib or load()).rlk_action_log_probs(ctypes.byref(rows),
                                                         log_probs.data_ptr(), entropies.data_ptr(), _ptr(norms), stream),
                    "rlk_action_log_probs")
@@ -145,16 +149,16 @@ def action_log_probs_backward(dev, stream, logits, actions, temperature, entropi
 
 
 def _terms(dev, stream, num_envs, old, advantages, ref, mask, clip, kl_coef, entropy_coef, per_row, loss, means):
-    ws, wsb = _workspace("sums", dev, stream, (_lib or load()).rlk_policy_workspace_bytes(num_envs))
+    ws = _workspace("sums", dev, stream, (_lib or load()).rlk_policy_workspace_bytes(num_envs))
     low, high, dual = clip
-    return PolicyTerms(old.data_ptr(), advantages.data_ptr(), _ptr(ref), _ptr(mask), low, high, dual, kl_coef,
-                       entropy_coef, per_row, old.dtype is _BF16, loss.data_ptr(), means.data_ptr(), ws, wsb)
+    return ws, PolicyTerms(old.data_ptr(), advantages.data_ptr(), _ptr(ref), _ptr(mask), low, high, dual, kl_coef,
+                       entropy_coef, per_row, old.dtype is _BF16, loss.data_ptr(), means.data_ptr(), ws.data_ptr(), ws.numel())
 
 
 @_on_device
 def policy_loss(dev, stream, log_probs, old, advantages, ref, mask, clip, kl_coef, per_row, loss, means, grad):
     e, t = log_probs.shape
-    terms = _terms(dev, stream, e, old, advantages, ref, mask, clip, kl_coef, 0.0, per_row, loss, means)
+    ws, terms = _terms(dev, stream, e, old, advantages, ref, mask, clip, kl_coef, 0.0, per_row, loss, means)
     _native._check(_lib.rlk_policy_loss(log_probs.data_ptr(), e, t, ctypes.byref(terms), grad.data_ptr(), stream),
                    "rlk_policy_loss")
 
@@ -162,8 +166,8 @@ def policy_loss(dev, stream, log_probs, old, advantages, ref, mask, clip, kl_coe
 @_on_device
 def policy_loss_from_logits(dev, stream, logits, actions, temperature, old, advantages, ref, mask, clip, kl_coef,
                             entropy_coef, per_row, loss, means, grad):
-    terms = _terms(dev, stream, logits.shape[0], old, advantages, ref, mask, clip, kl_coef, entropy_coef, per_row, loss,
-                   means)
+    ws, terms = _terms(dev, stream, logits.shape[0], old, advantages, ref, mask, clip, kl_coef, entropy_coef, per_row, loss,
+                       means)
     _native._check(_lib.rlk_policy_loss_from_logits(ctypes.byref(_rows(logits, actions, temperature)),
                                                    ctypes.byref(terms), grad.data_ptr(), stream),
                    "rlk_policy_loss_from_logits")
@@ -198,8 +202,8 @@ def linear_attention(dev, stream, decay, dones, passes):
     lib = _lib or load()
     e, t, h = passes[0].a.shape[:3]
     need = sum(lib.rlk_attention_workspace_bytes(e, t, h, p.a.shape[-1], p.y.shape[-1]) for p in passes)
-    ws, wsb = _workspace("states", dev, stream, need)
-    calls = (Attention * len(passes))(*(p.struct(decay, dones, ws, wsb) for p in passes))
+    ws = _workspace("states", dev, stream, need)
+    calls = (Attention * len(passes))(*(p.struct(decay, dones, _ptr(ws), _bytes(ws)) for p in passes))
     _native._check(lib.rlk_linear_attention(calls, len(passes), stream), "rlk_linear_attention")
 
 
