@@ -355,7 +355,6 @@ struct LinearAttention : torch::autograd::Function<LinearAttention> {
     TORCH_CHECK(st == RLK_OK, "rlk_linear_attention failed: ", rlk_status_string(st));
     ctx->save_for_backward({q, k, v, call->state ? state : at::Tensor(), decay, call->dones});
     ctx->saved_data["scale"] = call->scale;
-    ctx->saved_data["state"] = call->state && state.requires_grad();
     ctx->set_materialize_grads(false);
     return {out, last};
   }
@@ -365,7 +364,9 @@ struct LinearAttention : torch::autograd::Function<LinearAttention> {
     const auto saved = ctx->get_saved_variables();
     const at::Tensor &q = saved[0], &k = saved[1], &v = saved[2], &state = saved[3], &decay = saved[4], &dones = saved[5];
     torch::autograd::variable_list out(6);
-    if (!grads[0].defined() && !grads[1].defined()) return out;
+    // the walks whose gradients are asked for (the state's comes with v's)
+    const bool asked[3] = {ctx->needs_input_grad(0), ctx->needs_input_grad(1), ctx->needs_input_grad(2) || ctx->needs_input_grad(3)};
+    if ((!grads[0].defined() && !grads[1].defined()) || !(asked[0] || asked[1] || asked[2])) return out;
     const at::Tensor g = !grads[0].defined() ? at::zeros(v.sizes(), v.options())
                          : grads[0].stride(3) == 1 || v.size(3) == 1 ? grads[0] : grads[0].contiguous();
     const at::Tensor last = grads[1].defined() ? grads[1].contiguous() : grads[1];
@@ -373,8 +374,10 @@ struct LinearAttention : torch::autograd::Function<LinearAttention> {
     rlk_attention t[3] = {};
     const at::Tensor* roles[3][3] = {{&g, &v, &k}, {&v, &g, &q}, {&k, &q, &g}};
     const at::Tensor* like[3] = {&q, &k, &v};
+    int count = 0;
     for (int i = 0; i < 3; ++i) {
-      rlk_attention& w = t[i];
+      if (!asked[i]) continue;
+      rlk_attention& w = t[count++];
       out[i] = policy_output(like[i]->sizes(), like[i]->scalar_type(), *like[i]);
       w.q = steps_of(*roles[i][0]), w.k = steps_of(*roles[i][1]), w.v = steps_of(*roles[i][2]), w.out = steps_of(out[i]);
       w.num_envs = q.size(0), w.seq_len = q.size(1), w.heads = q.size(2);
@@ -385,18 +388,21 @@ struct LinearAttention : torch::autograd::Function<LinearAttention> {
       w.state_transposed = i < 2, w.reverse = i > 0, w.bf16 = q.scalar_type() == at::kBFloat16;
       w.scale = (float)scale, w.state_scale = i > 0 ? (float)(1.0 / scale) : 1.f, w.state_out_scale = i > 0 ? (float)scale : 1.f;
     }
-    if (ctx->saved_data["state"].toBool()) {
+    if (ctx->needs_input_grad(3)) {
       out[3] = policy_output({q.size(0), q.size(2), q.size(3), v.size(3)}, at::kFloat, q);
-      t[2].state_out = static_cast<float*>(out[3].data_ptr());
+      t[count - 1].state_out = static_cast<float*>(out[3].data_ptr());
     }
     PolicyCall c;
     c.dev = q.get_device();
     size_t need = 0;
-    for (const rlk_attention& w : t) need += rlk_attention_workspace_bytes(w.num_envs, w.seq_len, w.heads, w.dim_k, w.dim_v);
+    for (int i = 0; i < count; ++i) {
+      const rlk_attention& w = t[i];
+      need += rlk_attention_workspace_bytes(w.num_envs, w.seq_len, w.heads, w.dim_k, w.dim_v);
+    }
     const int st = [&] {
       const StatesScratch scratch(c, need, q, true);
       for (rlk_attention& w : t) w.workspace = scratch.ptr, w.workspace_bytes = scratch.bytes;
-      return rlk_linear_attention(t, 3, c.stream());
+      return rlk_linear_attention(t, count, c.stream());
     }();
     TORCH_CHECK(st == RLK_OK, "rlk_linear_attention failed: ", rlk_status_string(st));
     once(out, {q, k, v, state, grads[0], grads[1]});

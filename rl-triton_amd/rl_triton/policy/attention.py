@@ -80,12 +80,14 @@ class _LinearAttention(torch.autograd.Function):
     def backward(ctx, grad_out, grad_last):
         q, k, v, decay, dones, state = ctx.saved_tensors
         scale = ctx.scale
-        if grad_out is None and grad_last is None:
+        wants_q, wants_k, wants_v, _, _, wants_state, _ = ctx.needs_input_grad
+        if (grad_out is None and grad_last is None) or not (wants_q or wants_k or wants_v or wants_state):
             return (None,) * 7
         e, t, h, _ = q.shape
-        grads = [torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in (q, k, v)]
-        grad_state = torch.empty(q.shape[0], h, q.shape[-1], v.shape[-1], dtype=torch.float32, device=q.device) \
-            if ctx.needs_input_grad[5] else None
+        # (the state's gradient comes with that of v)
+        grads = [torch.empty(x.shape, dtype=x.dtype, device=x.device) if wanted else None
+                 for x, wanted in ((q, wants_q), (k, wants_k), (v, wants_v or wants_state))]
+        grad_state = torch.empty(q.shape[0], h, q.shape[-1], v.shape[-1], dtype=torch.float32, device=q.device) if wants_state else None
         if t == 0:
             if grad_state is not None:
                 grad_state.zero_() if grad_last is None else grad_state.copy_(grad_last)
@@ -93,10 +95,14 @@ class _LinearAttention(torch.autograd.Function):
             g = torch.zeros(v.shape, dtype=v.dtype, device=v.device) if grad_out is None else _inner(grad_out)
             last = None if grad_last is None else grad_last.contiguous()
             back = dict(reverse=True, state_scale=1.0 / scale, out_scale=scale)
-            _native.linear_attention(decay, dones, [
-                _native.Pass(g, v, k, grads[0], state, None, scale, transposed=True),
-                _native.Pass(v, g, q, grads[1], last, None, scale, transposed=True, **back),
-                _native.Pass(k, q, g, grads[2], last, grad_state, scale, **back)])
+            passes = []
+            if grads[0] is not None:
+                passes.append(_native.Pass(g, v, k, grads[0], state, None, scale, transposed=True))
+            if grads[1] is not None:
+                passes.append(_native.Pass(v, g, q, grads[1], last, None, scale, transposed=True, **back))
+            if grads[2] is not None:
+                passes.append(_native.Pass(k, q, g, grads[2], last, grad_state, scale, **back))
+            _native.linear_attention(decay, dones, passes)
         return (*grads, None, None, grad_state, None)
 
 

@@ -117,3 +117,32 @@ def test_unrolled_steps_hold_nothing_back():
         out, state = policy.compute_linear_attention_step(q * 1, k * 1, v * 1, decay, state)
         sizes.append(torch.cuda.memory_allocated())
     assert sizes[-1] == sizes[1] and out.requires_grad
+
+
+@pytest.mark.parametrize("seq_len", [40, 700])  # (one segment and several)
+def test_only_the_gradients_that_are_asked_for_are_computed(seq_len):
+    """With some of the inputs frozen: the same gradients of the others, and no memory taken for those of the frozen ones."""
+    g = torch.Generator(device="cuda").manual_seed(1)
+    n = lambda *s: torch.randn(s, generator=g, device="cuda")  # noqa: E731
+    E = 64 if seq_len == 40 else 1
+    inputs = n(E, seq_len, 2, 64), n(E, seq_len, 2, 64), n(E, seq_len, 2, 64), n(E, 2, 64, 64)
+    decay, up, us = torch.tensor([0.99, 0.9], device="cuda"), n(E, seq_len, 2, 64), n(E, 2, 64, 64)
+
+    def run(wanted):
+        leaves = [t.clone().requires_grad_(w) for t, w in zip(inputs, wanted)]
+        outs = policy.compute_linear_attention(*leaves[:3], decay, None, leaves[3])
+        torch.cuda.synchronize()
+        torch.cuda.reset_peak_memory_stats()
+        before = torch.cuda.memory_allocated()
+        grads = torch.autograd.grad(outs, [t for t in leaves if t.requires_grad], (up, us))
+        return grads, torch.cuda.max_memory_allocated() - before
+
+    run((True,) * 4)  # (the scratch memory is there)
+    full, _ = run((True,) * 4)
+    for wanted in ((True, False, False, False), (False, True, False, False), (False, False, True, False), (False, False, False, True),
+                   (True, False, True, False), (False, True, False, True), (False, True, True, True)):
+        grads, peak = run(wanted)
+        assert all(torch.equal(a, b) for a, b in zip(grads, [x for x, w in zip(full, wanted) if w]))
+        # the state's gradient comes with v's: room for both, and 512 bytes a tensor for the allocator's rounding
+        room = sum(x.numel() * 4 + 512 for x, w in zip(inputs, (*wanted[:2], wanted[2] or wanted[3], wanted[3])) if w)
+        assert peak <= room, (wanted, peak, room)
