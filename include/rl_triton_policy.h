@@ -17,6 +17,10 @@
 extern "C" {
 #endif
 
+/* What logits are divided by is held as a reciprocal in float: outside this range that would be infinite or lose its digits. */
+#define RLK_LEAST_TEMPERATURE 1e-38
+#define RLK_LARGEST_TEMPERATURE 1e38
+
 /* Rows of logits: [num_envs, seq_len, num_actions], the actions of a row contiguous, and the action taken
  * at each step.  An action outside [0, num_actions) has a log-probability of NaN; nothing is read for it. */
 typedef struct rlk_action_rows {
@@ -24,7 +28,7 @@ typedef struct rlk_action_rows {
   const int64_t *actions; /* [num_envs, seq_len], contiguous */
   int64_t num_envs, seq_len, num_actions;
   int64_t env_stride, step_stride;
-  double temperature; /* logits are divided by it: > 0 */
+  double temperature; /* logits are divided by it */
   int bf16;          /* logits (and their gradient) */
   /* NULL, or RLK_ROWS_WORKSPACE_BYTES (no initial contents needed) with which log-probabilities of few long rows are
    * shared by several workgroups a row.  The losses use their own. */
@@ -92,8 +96,8 @@ typedef struct rlk_attention {
    * gradient of the state after the last one. */
   const float *state;
   int state_transposed; /* `state` is [num_envs, heads, dim_v, dim_k] */
-  /* NULL, or the state after the last step, zero if that step is done (of no steps: `state`); reverse: the gradient of the state before
-   * the first step. */
+  /* NULL, or the state after the last step, zero if that step is done (of no steps: `state`); reverse: the gradient of the
+   * state before the first step. */
   float *state_out;
   float scale;                        /* of out */
   float state_scale, state_out_scale; /* what `state` is multiplied with when read, `state_out` when written (the

@@ -527,7 +527,7 @@ int dispatch_update(int64_t vecs, F f) {
 
 inline bool valid_rows(const rlk_action_rows* r) {
   if (!r || r->num_envs < 0 || r->seq_len < 0 || r->num_actions < 1 || r->num_actions > (int64_t{1} << 30)) return false;
-  if (!(r->temperature > 0.0) || !std::isfinite(r->temperature)) return false;
+  if (!(r->temperature >= RLK_LEAST_TEMPERATURE && r->temperature <= RLK_LARGEST_TEMPERATURE)) return false;
   return r->num_envs * r->seq_len == 0 || (r->logits && r->actions && (reinterpret_cast<uintptr_t>(r->logits) & (r->bf16 ? 1u : 3u)) == 0);
 }
 

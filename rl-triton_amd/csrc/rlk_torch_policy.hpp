@@ -160,7 +160,7 @@ bool logit_rows(PolicyCall& c, PyObject* logits, PyObject* actions, PyObject* te
   if (!t || !float_type(t->scalar_type()) || t->dim() < 1 || t->numel() == 0 || !logit_layout(*t, r)) return false;
   *a = c.array(actions, at::kLong, t->sizes().slice(0, t->dim() - 1));
   const double tau = c.number(temperature, 0.0);
-  if (!c.ok || !(tau > 0.0)) return false;
+  if (!c.ok || !(tau >= RLK_LEAST_TEMPERATURE && tau <= RLK_LARGEST_TEMPERATURE)) return false;
   r->actions = static_cast<const int64_t*>((*a)->data_ptr());
   r->temperature = tau;
   return true;

@@ -15,8 +15,8 @@ def _check_rows(logits, actions, temperature):
     assert actions.get_device() == logits.get_device(), "actions must be on the device of logits"
     assert actions.dtype == torch.int64, f"actions: expected int64, got {actions.dtype}"
     assert actions.shape == logits.shape[:-1], f"actions shape {actions.shape} != logits shape {logits.shape} without its last axis"
-    assert isinstance(temperature, (int, float)) and math.isfinite(temperature) and temperature > 0, \
-        f"temperature must be a positive number, got {temperature!r}"
+    assert isinstance(temperature, (int, float)) and 1e-38 <= temperature <= 1e38, \
+        f"temperature must be a number from 1e-38 to 1e38 (float32 holds its reciprocal), got {temperature!r}"
     if _CORRECTNESS_WARNINGS():
         assert actions.numel() == 0 or bool(((actions >= 0) & (actions < logits.shape[-1])).all()), \
             "actions must lie in [0, num_actions)"
@@ -86,7 +86,7 @@ def compute_action_log_probs(
         logits:      [..., num_actions], float32 or bfloat16, GPU; usually [num_envs, seq_len, num_actions], of any
                      strides as long as the actions of a row are contiguous (others are copied).
         actions:     the taken actions, [...], int64.
-        temperature: what the logits are divided by (default 1).
+        temperature: what the logits are divided by (default 1), from 1e-38 to 1e38.
 
     Returns:
         log_probs, entropies: [...], float32 whatever the logits' type (ratios of probabilities are taken of them).

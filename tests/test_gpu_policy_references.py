@@ -99,3 +99,20 @@ def test_a_policy_that_forbids_the_action():
     assert float(means[1]) == math.inf and float(means[3]) == math.inf and bool(grad.isfinite().all()) and math.isfinite(float(loss))
     loss, grad, means = policy.compute_policy_loss(*(t.cuda() for t in (lp, old, adv, ref)), kl_coef=0.5)
     assert float(loss) == math.inf and float(grad[0, 1]) == -math.inf and bool(grad[0, ::2].isfinite().all())
+
+
+@pytest.mark.parametrize("tau", [1e-38, 1e-9, 1e9, 1e38])
+@pytest.mark.parametrize("A", [7, 300, 70001])
+def test_extreme_temperatures(A, tau):
+    """At the ends of what is allowed: all on the largest logit, or even over those that are allowed.  (x / tau in float64 loses no
+    digit; entropies and log-probabilities are off by a few u of log A.)"""
+    g = torch.Generator().manual_seed(A)
+    x = torch.randn(3, 2, A, generator=g)
+    x[..., 1::3] = -math.inf
+    x[..., 0] = 6.0  # (the largest, by far more than tau where tau is small)
+    for act in (0, 1, 2):
+        a = torch.full((3, 2), act)
+        lp, ent = policy.compute_action_log_probs(x.cuda(), a.cuda(), tau)
+        want, went, _, _ = softmax_rows(x, a, tau)
+        _close(lp, want.float(), 1e-6 * (1 + want.abs().nan_to_num(posinf=0)))
+        _close(ent, went, 1e-5 * (1 + math.log(A)))
