@@ -158,12 +158,24 @@ struct Lds {
   // Two chunks where they fit (160 KB a CU; two workgroups of it for bfloat16 dims of up to 64): the next one is put down
   // while this one is worked on.  float32 dims of up to 64 have one, and two workgroups a CU (training [64,1024,8,64] 645 us;
   // two chunks and one workgroup 818).
-  static constexpr int P_BYTES = C * PROW;                   // (a_i . b_j) lambda^{i-j} same(j, i)
+  // p, (a_i . b_j) lambda^{i-j} same(j, i).  bfloat16: as two numbers, the upper ones first, without the columns past the diagonal's
+  // tiles (rows 0 .. 31 have 32 columns, the others 64) and without padding: the 16-byte units of a row are exchanged with
+  // its number, so that a column of 16 rows' units lies in all banks.
+  static constexpr bool PARTS = S == 2;
+  static constexpr int P_PART = 32 * 32 * S + 32 * C * S;
+  static constexpr int P_BYTES = PARTS ? 2 * P_PART : C * PROW;
   static constexpr bool OVER = S == 4 && D == 64;            // p in the place of b's rows, which are read for nothing else
-  static constexpr int CHUNKS = !OVER && 2 * (CHUNK + 32) + P_BYTES <= 160 * 1024 ? 2 : 1;
+  static constexpr int CHUNKS = !OVER && 2 * CHUNK + P_BYTES <= 160 * 1024 ? 2 : 1;
   static constexpr int P = OVER ? B : CHUNKS * CHUNK;
-  static constexpr int TAINT = CHUNKS * CHUNK + (OVER ? 0 : P_BYTES);  // [CHUNKS][8]: whether a wavefront has put down an inf, a NaN or a value near the type's largest
-  static constexpr int BYTES = TAINT + CHUNKS * 32;
+  static constexpr int BYTES = CHUNKS * CHUNK + (OVER ? 0 : P_BYTES);
+  static_assert(D == 128 || 2 * BYTES <= 160 * 1024, "two workgroups a CU");
+  // whether wavefront w has put down an inf, a NaN or a value near the type's largest: in the padding of a's first rows
+  __device__ static constexpr int taint(int w) { return A + (w >> 2) * ROW + D * S + (w & 3) * 4; }
+  // where the upper numbers of p's row i, columns j .. j + 3 lie (bfloat16)
+  __device__ static int part(int i, int j) {
+    const int unit = j * S / 16;
+    return P + (i < 32 ? i * 64 + (unit ^ ((i >> 2) & 3)) * 16 : 2048 + (i - 32) * 128 + (unit ^ ((i >> 1) & 7)) * 16) + j * S % 16;
+  }
   // Where a transposed tile holds row d, column j.  The 16-byte units of a row are exchanged with d's low bits: a write has
   // lanes at every fourth row, a read at consecutive ones, and f takes all 8 values over either set, so both spread over
   // all banks (with padded rows the writes met in an eighth of them: 20 of 75 us of a [64,1024,8,64] call).
@@ -246,6 +258,10 @@ struct Part {
   }
 };
 
+// A number's upper 16 bits, as a float and for two as bfloat16.
+__device__ __forceinline__ float upper(float x) { return __uint_as_float(__float_as_uint(x) & 0xffff0000u); }
+__device__ __forceinline__ uint32_t uppers(float x, float y) { return __builtin_amdgcn_perm(__float_as_uint(y), __float_as_uint(x), 0x07060302u); }
+
 // acc += a (w * c) for an operand row c and weights w of its inner indices.  The weighted bfloat16 operand is taken as the sum
 // of three bfloat16 numbers, the product's upper, middle and lower 8 bits: the state is a float32 result and sums over
 // all steps (with one rounding of a term to 8 bits it would be off by 2^-9 of itself, with two numbers by 2.5e-6; three are
@@ -266,8 +282,6 @@ struct Weighted<bf16> {
   Frag<bf16> hi, mid, lo;
   __device__ Weighted(const Frag<bf16>& c, const float (&w)[8]) {
     union { bf16x8 v; uint32_t u[4]; } in{c.x}, h, m, l;
-    auto upper = [](float x) { return __uint_as_float(__float_as_uint(x) & 0xffff0000u); };
-    auto uppers = [](float x, float y) { return __builtin_amdgcn_perm(__float_as_uint(y), __float_as_uint(x), 0x07060302u); };
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       float a = Words<bf16>::get(in.u[i], 0) * w[2 * i], b = Words<bf16>::get(in.u[i], 1) * w[2 * i + 1];
@@ -280,6 +294,44 @@ struct Weighted<bf16> {
     hi.x = h.v, mid.x = m.v, lo.x = l.v;
   }
   __device__ f32x4 mma_with(const Frag<bf16>& a, f32x4 acc) const { return mma(a, hi, mma(a, mid, mma(a, lo, acc))); }
+};
+
+// A factor that is not one of the call's arrays, for products with one that is: the state where outputs are read from it, and p.
+// float32: itself.  bfloat16: the sum of two bfloat16 numbers, the upper 8 bits and the next 8 rounded, 2^-15 off at the most.
+// (As one number, 2^-8 off, outputs had half as much error again as their own rounding gives them.)  x is finite.
+template <class E>
+struct Factor;
+template <>
+struct Factor<float> {
+  Frag<float> x;
+  __device__ static Factor from(f32x4 a, f32x4 b) { return {Frag<float>::from(a, b)}; }
+  // acc[t] += this * rows[t]
+  template <int N>
+  __device__ void times(const Frag<float> (&rows)[N], f32x4* acc, bool half) const {
+#pragma unroll
+    for (int t = 0; t < N; ++t) acc[t] = half ? mma_half(x, rows[t], acc[t]) : mma(x, rows[t], acc[t]);
+  }
+};
+__device__ __forceinline__ u32x2 upper_quad(f32x4 x) { return {uppers(x[0], x[1]), uppers(x[2], x[3])}; }
+__device__ __forceinline__ u32x2 rest_quad(f32x4 x) {
+  return {bf16_pair(x[0] - upper(x[0]), x[1] - upper(x[1])), bf16_pair(x[2] - upper(x[2]), x[3] - upper(x[3]))};
+}
+template <>
+struct Factor<bf16> {
+  Frag<bf16> hi, lo;
+  __device__ static Factor from(f32x4 a, f32x4 b) {
+    union { u32x2 h[2]; bf16x8 v; } h, l;
+    h.h[0] = upper_quad(a), h.h[1] = upper_quad(b);
+    l.h[0] = rest_quad(a), l.h[1] = rest_quad(b);
+    return {{h.v}, {l.v}};
+  }
+  template <int N>
+  __device__ void times(const Frag<bf16> (&rows)[N], f32x4* acc, bool) const {
+#pragma unroll
+    for (int t = 0; t < N; ++t) acc[t] = mma(lo, rows[t], acc[t]);
+#pragma unroll
+    for (int t = 0; t < N; ++t) acc[t] = mma(hi, rows[t], acc[t]);
+  }
 };
 
 // Which walk of which environment and head a workgroup takes.  Workgroups go round the 8 XCDs, so the walks over the same
@@ -423,8 +475,10 @@ __global__ __launch_bounds__(4 * D, 2) void walk_kernel(const Walks<E> walks) {
   const int at_a = opaque(M::A + (16 * ti + l16) * M::ROW + PER * l4 * M::S);
   const int at_b = opaque(M::B + (16 * (wave % SHARE) + l16) * M::ROW + PER * l4 * M::S);
   const int at_a2 = opaque(M::A + l16 * M::ROW + 4 * l4 * M::S);
-  const int at_p_put = opaque(M::P + (16 * ti + l16) * M::PROW + (16 * (wave % SHARE) + 4 * l4) * M::S);
-  const int at_p = opaque(M::P + l16 * M::PROW + 8 * l4 * M::S);
+  const int at_p_put = opaque(M::PARTS ? M::part(16 * ti + l16, 16 * (wave % SHARE) + 4 * l4)
+                                       : M::P + (16 * ti + l16) * M::PROW + (16 * (wave % SHARE) + 4 * l4) * M::S);
+  const int at_p = opaque(M::PARTS ? M::part(l16, 8 * l4) : M::P + l16 * M::PROW + 8 * l4 * M::S);
+  const int at_p2[2] = {M::PARTS ? opaque(M::part(32 + l16, 8 * l4)) : 0, M::PARTS ? opaque(M::part(32 + l16, 32 + 8 * l4)) : 0};
   const int step2 = HALVES ? 4 : 32;
   const int at_bt[2][2] = {{opaque(M::transposed(l16, 8 * l4)), opaque(M::transposed(l16, 8 * l4 + step2))},
                            {opaque(M::transposed(16 + l16, 8 * l4)), opaque(M::transposed(16 + l16, 8 * l4 + step2))}};
@@ -441,6 +495,19 @@ __global__ __launch_bounds__(4 * D, 2) void walk_kernel(const Walks<E> walks) {
   };
 
   bool crossed = false;  // a cut anywhere in the segment
+  // a state that is not finite, in bfloat16: it has no two parts (inf - inf), so its chunks go step by step
+  bool wild = false;
+  auto look = [&] {
+    if constexpr (!STATE && M::PARTS) {
+      float sum = 0.f;
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) sum = fmaf(0.f, U[m][r], sum);
+      wild = __any(sum != 0.f);
+    }
+  };
+  look();
   // Puts the fetched chunk of the steps from s0 on down and has the one after it fetched; its cuts come back.
   auto put_down = [&](int64_t s0, int buffer) {
     const int L = (int)(last - s0 < C ? last - s0 : C);
@@ -454,7 +521,7 @@ __global__ __launch_bounds__(4 * D, 2) void walk_kernel(const Walks<E> walks) {
     float sum = pc.squares(pb.squares(0.f));
     if constexpr (!STATE) sum = pa.squares(sum);
     const bool tainted = __any(!(sum < 0x1p120f));  // (else each is below 2^60, and no product of two rows overflows)
-    if (lane == 0) *reinterpret_cast<int*>(lds + M::TAINT + (buffer != 0 ? 32 : 0) + 4 * wave) = tainted;
+    if (lane == 0) *reinterpret_cast<int*>(to + M::taint(wave)) = tainted;
     if constexpr (!STATE) {
       pa.put(to + at_row);
       pb.put(to + at_row + (M::B - M::A));
@@ -468,9 +535,11 @@ __global__ __launch_bounds__(4 * D, 2) void walk_kernel(const Walks<E> walks) {
   // One chunk, unless it is tainted.  PLAIN: whole, without a cut, and not the one that a state leaves the sequence with.
   auto chunk = [&](auto plain, int64_t s0, int L, uint64_t cuts, bool end, const char* tile) {
     constexpr bool PLAIN = decltype(plain)::value;
-    const int4* marks = reinterpret_cast<const int4*>(lds + M::TAINT + (tile != lds ? 32 : 0));
-    int4 mark = marks[0];
-    if constexpr (D == 128) mark.x |= marks[1].x | marks[1].y | marks[1].z | marks[1].w;
+    int4 mark = *reinterpret_cast<const int4*>(tile + M::taint(0));
+    if constexpr (D == 128) {
+      const int4 more = *reinterpret_cast<const int4*>(tile + M::taint(4));
+      mark.x |= more.x | more.y | more.z | more.w;
+    }
     // operands that take more registers: loads of more than the next two are kept from moving up
     auto apart = [] {
       if constexpr (sizeof(E) == 4 || D == 128) __builtin_amdgcn_sched_barrier(0);
@@ -512,11 +581,19 @@ __global__ __launch_bounds__(4 * D, 2) void walk_kernel(const Walks<E> walks) {
           for (int r = 0; r < 4; ++r)
             if (16 * jt + 4 * v4 + r < begin) pt[r] = 0.f;
         }
-        Quad<E>::of(pt).store(reinterpret_cast<E*>(lds + at_p_put + 16 * SHARE * u * M::S));
+        if constexpr (M::PARTS) {
+          // (the units' exchange is of the address's bits 4 to 6)
+          if (ti < 2 && SHARE * u >= 2) continue;  // past the diagonal's tiles
+          char* p = lds + (at_p_put ^ (16 * SHARE * u * M::S));
+          *reinterpret_cast<u32x2*>(p) = upper_quad(pt);
+          *reinterpret_cast<u32x2*>(p + M::P_PART) = rest_quad(pt);
+        } else {
+          Quad<E>::of(pt).store(reinterpret_cast<E*>(lds + at_p_put + 16 * SHARE * u * M::S));
+        }
       }
       __syncthreads();
     }
-    if (__builtin_amdgcn_readfirstlane(mark.x | mark.y | mark.z | mark.w) != 0) return false;
+    if (__builtin_amdgcn_readfirstlane(mark.x | mark.y | mark.z | mark.w) != 0 || wild) return false;
 
     Frag<E> fc[2];
 #pragma unroll
@@ -532,13 +609,13 @@ __global__ __launch_bounds__(4 * D, 2) void walk_kernel(const Walks<E> walks) {
       for (int kk = 0; kk < KK; ++kk) {
         if (!FULL && 32 * kk >= da) continue;
         const bool half = !FULL && da - 32 * kk <= 16;
-        const Frag<E> fu = Frag<E>::from(U[2 * kk], U[2 * kk + 1]);
+        const Factor<E> fu = Factor<E>::from(U[2 * kk], U[2 * kk + 1]);
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {
-          const char* row = tile + at_a2 + 16 * t * M::ROW + 32 * kk * M::S;
-          const Frag<E> fr = Frag<E>::load2(row, row + 16 * M::S);
-          y[t] = half ? mma_half(fu, fr, y[t]) : mma(fu, fr, y[t]);
-          if (t & 1) apart();
+        for (int t = 0; t < 4; t += 2) {
+          const char *row = tile + at_a2 + 16 * t * M::ROW + 32 * kk * M::S, *next = row + 16 * M::ROW;
+          const Frag<E> fr[2] = {Frag<E>::load2(row, row + 16 * M::S), Frag<E>::load2(next, next + 16 * M::S)};
+          fu.times(fr, y + t, half);
+          apart();
         }
       }
       if constexpr (!FULL) settle();
@@ -553,7 +630,12 @@ __global__ __launch_bounds__(4 * D, 2) void walk_kernel(const Walks<E> walks) {
       for (int kk = 0; kk < 2; ++kk)
 #pragma unroll
         for (int t = 2 * kk; t < 4; ++t) {  // (rows before the steps 32 kk + 0..31 have none of them)
-          y[t] = mma(fc[kk], Frag<E>::load(lds + at_p + 16 * t * M::PROW + 32 * kk * M::S), y[t]);
+          if constexpr (M::PARTS) {
+            const char* p = lds + (t < 2 ? at_p + 1024 * t : at_p2[kk] + 2048 * (t - 2));
+            y[t] = mma(fc[kk], Frag<E>::load(p), mma(fc[kk], Frag<E>::load(p + M::P_PART), y[t]));
+          } else {
+            y[t] = mma(fc[kk], Frag<E>::load(lds + at_p + 16 * t * M::PROW + 32 * kk * M::S), y[t]);
+          }
           if (t & 1) apart();
         }
       const int j = 16 * wave + 4 * l4;
@@ -646,6 +728,7 @@ __global__ __launch_bounds__(4 * D, 2) void walk_kernel(const Walks<E> walks) {
       for (int m = 0; m < MT; ++m)
 #pragma unroll
         for (int r = 0; r < 4; ++r) U[m][r] = lambda == 0.f ? 0.f : U[m][r] * lambda;
+    look();
   };
 
   int buffer = 0;

@@ -135,12 +135,13 @@ def compute_linear_attention(
     - out[t] = scale * S[t]^T q[t]
 
     the recurrence of compute_eligibility_traces with a matrix in place of the trace: no step reads from an episode
-    that ended before it.  Computed in chunks of steps with matrix instructions, float32 sums throughout; bfloat16
-    calls round the products of queries and keys, and the state where outputs are read from it, to bfloat16.
+    that ended before it.  Computed in chunks of steps with matrix instructions, float32 sums throughout; in
+    bfloat16 calls the products of queries and keys, and the state where outputs are read from it, are factors of two bfloat16
+    numbers each (2^-15 off), and an output is rounded once.
     Differentiable in q, k, v and state.
 
     What is not finite, in padded steps for one, reaches no step before it and none past its episode's end; a chunk that
-    holds such values is computed step by step, in some twenty times the time.
+    holds such values (or, in bfloat16, begins with a state that does) is computed step by step, in some twenty times the time.
 
     Args:
         q, k:  [num_envs, seq_len, heads, dim_k], float32 or bfloat16, GPU; any strides with a contiguous last axis

@@ -1,5 +1,5 @@
 """Linear attention at values and sizes where one path of it could answer otherwise than another: infinities at head dims that fill
-no whole tile, decays of 0, sequences of no steps, and how exact the float32 states of bfloat16 calls are."""
+no whole tile, decays of 0, sequences of no steps, and how exact bfloat16 calls are."""
 import ctypes
 import math
 
@@ -7,7 +7,7 @@ import pytest
 import torch
 
 import rl_triton.policy as policy
-from _policy_reference import U32, attention, attention_grads
+from _policy_reference import U16, U32, attention, attention_grads
 from rl_triton.policy import _native
 
 pytestmark = pytest.mark.gpu
@@ -96,3 +96,42 @@ def test_states_of_bfloat16_calls_are_float32(dims):
         for h in range(H):
             err = (x.detach().cpu().double() - w)[:, h].square().mean().sqrt() / w[:, h].abs().max()
             assert float(err) < 16 * U32, float(err)
+
+
+@pytest.mark.parametrize("E,T,H,dk,dv", [(2, 3, 2, 8, 8), (2, 65, 6, 64, 64), (3, 127, 2, 72, 24), (1, 130, 2, 128, 128), (2, 333, 4, 40, 72),
+                                         (1, 1000, 2, 64, 64), (1, 1025, 1, 128, 128), (2, 700, 2, 33, 16)])
+def test_outputs_of_bfloat16_calls_are_rounded_once(E, T, H, dk, dv):
+    """Outputs and gradients of bfloat16 calls: sums as exact as float32's, of which two factors in each term (the state, the weighted
+    product of query and key) are held in two bfloat16 numbers (the upper 8 bits leave less than 2^-7 of a number, 8 bits of that leave
+    2^-8 of it: 2^-15), and one rounding to bfloat16 at the end."""
+    g = torch.Generator().manual_seed(T)
+    q, k, v, go = (torch.randn(E, T, H, d, generator=g).bfloat16() for d in (dk, dk, dv, dv))
+    s, gs = torch.randn(E, H, dk, dv, generator=g), torch.randn(E, H, dk, dv, generator=g)
+    decay = torch.tensor([0.999, 0.5, 1.0, 0.05, 0.9, 0.0])[:H]
+    dones = (torch.rand(E, T, generator=g) < 0.01).float()
+    leaves = [t.cuda().requires_grad_() for t in (q, k, v)]
+    out, last = policy.compute_linear_attention(*leaves, decay.cuda(), dones.cuda(), s.cuda(), 0.3)
+    got = out, *torch.autograd.grad((out, last), leaves, (go.cuda(), gs.cuda()))
+    args, sizes = (q, k, v, decay, dones, s, 0.3), (q.abs(), k.abs(), v.abs(), decay, dones, s.abs(), 0.3)
+    want = attention(*args)[0], *attention_grads(*args, go, gs)[:3]
+    size = attention(*sizes)[0], *attention_grads(*sizes, go.abs(), gs.abs())[:3]
+    for i, (x, w, y) in enumerate(zip(got, want, size)):
+        err = (x.detach().cpu().double() - w).abs()
+        bound = y * ((T + 128) * U32 + 2.0 ** -15) + U16 * w.abs() + 1e-30
+        assert bool((err <= bound).all()), (i, float((err / bound).max()))
+
+
+def test_a_state_that_is_not_finite_in_bfloat16():
+    """An inf that a sequence goes on from is in every output that reads it, until its episode's end, as it is in float32."""
+    g = torch.Generator().manual_seed(1)
+    for d in (64, 128):
+        q, k, v = ((torch.rand(2, 300, 2, d, generator=g) + 0.5).bfloat16() for _ in range(3))
+        s = torch.randn(2, 2, d, d, generator=g)
+        s[0, 1, 3, 5], s[1, 0, 2, 40], s[1, 0, 7, 41] = math.inf, -math.inf, math.nan
+        decay, dones = torch.tensor([0.99, 0.95]), torch.zeros(2, 300)
+        dones[:, 200] = 1
+        out, last = policy.compute_linear_attention(*(t.cuda() for t in (q, k, v, decay, dones, s)))
+        want, wlast = attention(q, k, v, decay, dones, s, d ** -0.5)
+        x = out.cpu().double()
+        assert torch.equal(x.isnan(), want.isnan()) and torch.equal(x == math.inf, want == math.inf) and torch.equal(x == -math.inf, want == -math.inf)
+        assert bool(x[:, 201:].isfinite().all()) and bool(last.isfinite().all())
