@@ -377,6 +377,8 @@ __global__ __launch_bounds__(4 * D, 2) void walk_kernel(const Walks<E> walks) {
   const float lambda = walks.decay[head], lg = __log2f(lambda);
   const float* dones = walks.dones ? walks.dones + env * T : nullptr;
   const bool reverse = w.reverse;
+  // of the squares of a thread's values: below it each is below 2^60, 2^60 / scale, and no product of two rows overflows, scaled or not
+  const float limit = fabsf(w.scale) > 1.f ? 0x1p120f / w.scale / w.scale : 0x1p120f;
 
   Part<E, D> pa, pb, pc;
   if constexpr (!STATE) pa.start(w.a.data + env * w.a.env_stride + head * w.a.head_stride, w.a.step_stride, da, first, T, reverse);
@@ -520,7 +522,7 @@ __global__ __launch_bounds__(4 * D, 2) void walk_kernel(const Walks<E> walks) {
     char* to = lds + buffer;
     float sum = pc.squares(pb.squares(0.f));
     if constexpr (!STATE) sum = pa.squares(sum);
-    const bool tainted = __any(!(sum < 0x1p120f));  // (else each is below 2^60, and no product of two rows overflows)
+    const bool tainted = __any(!(sum < limit));
     if (lane == 0) *reinterpret_cast<int*>(to + M::taint(wave)) = tainted;
     if constexpr (!STATE) {
       pa.put(to + at_row);

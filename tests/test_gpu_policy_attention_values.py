@@ -135,3 +135,22 @@ def test_a_state_that_is_not_finite_in_bfloat16():
         x = out.cpu().double()
         assert torch.equal(x.isnan(), want.isnan()) and torch.equal(x == math.inf, want == math.inf) and torch.equal(x == -math.inf, want == -math.inf)
         assert bool(x[:, 201:].isfinite().all()) and bool(last.isfinite().all())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("d", [24, 64, 128])
+def test_products_that_a_scale_takes_out_of_range(d, dtype):
+    """Queries and keys whose products float32 holds, but not `scale` times them, with values that bring the output back into range: the
+    recurrence forms k v first.  (T + 128) u of the sizes, the output's rounding, and in bfloat16 2^-15 of the sizes."""
+    g = torch.Generator().manual_seed(d)
+    E, T, H = 1, 100, 2
+    q, k, v = ((torch.rand(E, T, H, d, generator=g) * 0.5 + 0.5).to(dtype) for _ in range(3))
+    q, k, v, scale = q * 2.0 ** 57, k * 2.0 ** 57, v * 2.0 ** -100, 2.0 ** 9 * 128 / d
+    decay = torch.tensor([0.9, 1.0])
+    out, last = policy.compute_linear_attention(*(t.cuda() for t in (q, k, v, decay)), scale=scale)
+    want, wlast = attention(q, k, v, decay, None, None, scale)
+    low = dtype == torch.bfloat16
+    assert bool(out.isfinite().all())
+    err = (out.cpu().double() - want).abs()
+    assert bool((err <= want * ((T + 128) * U32 + (2.0 ** -15 + U16 if low else 0))).all()), float((err / want).max())
+    assert bool(((last.cpu().double() - wlast).abs() <= (T + 128) * U32 * wlast).all())
