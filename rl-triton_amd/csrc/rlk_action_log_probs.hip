@@ -7,17 +7,17 @@
 namespace rlk {
 namespace {
 
-// What a row's statistics come to.
+// What a row's statistics come to, and the logit of its action (NaN: there is no such action).
+__device__ __forceinline__ void write_row(const RowStats& r, float x, float c, int64_t row, float* log_probs, float* entropies, float* norms) {
+  log_probs[row] = r.log_prob(x, c);
+  entropies[row] = r.entropy();
+  if (norms) norms[2 * row] = r.m, norms[2 * row + 1] = r.empty() ? INFINITY : r.log2s();  // (inf: p = 0)
+}
 template <class E>
 __device__ __forceinline__ void write_row(const ActionRows<E>& a, const E* base, int64_t row, const RowStats& r, float* log_probs,
                                           float* entropies, float* norms) {
   const int64_t act = a.actions[row];
-  const float x = act >= 0 && act < a.A ? load_one(base + act) : NAN;
-  const float log2s = r.log2s();
-  const bool empty = r.s == 0.f;
-  log_probs[row] = empty && x == x ? -INFINITY : ((x - r.m) * a.c - log2s) * kLn2;
-  entropies[row] = empty ? 0.f : (log2s - r.u / r.s) * kLn2;
-  if (norms) norms[2 * row] = r.m, norms[2 * row + 1] = empty ? INFINITY : log2s;  // (inf: p = 0)
+  write_row(r, act >= 0 && act < a.A ? load_one(base + act) : NAN, a.c, row, log_probs, entropies, norms);
 }
 
 template <class E, int LANES, int NV>
@@ -66,12 +66,7 @@ __global__ __launch_bounds__(kFewRows) void few_log_probs_kernel(const ActionRow
       FewLogits<K> h;
       h.load(mine, a.A);
       const RowStats r = h.stats(a.c);
-      const float x = act >= 0 && act < a.A ? mine[act] : NAN;
-      const float log2s = r.log2s();
-      const bool empty = r.s == 0.f;
-      log_probs[row] = empty && x == x ? -INFINITY : ((x - r.m) * a.c - log2s) * kLn2;
-      entropies[row] = empty ? 0.f : (log2s - r.u / r.s) * kLn2;
-      if (norms) norms[2 * row] = r.m, norms[2 * row + 1] = empty ? INFINITY : log2s;
+      write_row(r, act >= 0 && act < a.A ? mine[act] : NAN, a.c, row, log_probs, entropies, norms);
     }
     __syncthreads();
   }

@@ -129,12 +129,16 @@ __device__ __forceinline__ void softmax_add(float y, float& s, float& u) {
   u = fmaf(e, fmaxf(y, kDeep), u);  // (y = -inf: e = 0 counts as 0)
 }
 
+constexpr float kLn2 = 0.69314718055994531f;
+
 struct RowStats {
   float m, s, u;  // of a row without any finite logit: m = 0, s = u = 0
-  __device__ float log2s() const { return s == 0.f ? 0.f : __log2f(s); }
+  __device__ bool empty() const { return s == 0.f; }
+  __device__ float log2s() const { return empty() ? 0.f : __log2f(s); }
+  // of an action whose logit is x
+  __device__ float log_prob(float x, float c) const { return empty() && x == x ? -INFINITY : ((x - m) * c - log2s()) * kLn2; }
+  __device__ float entropy() const { return empty() ? 0.f : (log2s() - u / s) * kLn2; }
 };
-
-constexpr float kLn2 = 0.69314718055994531f;
 
 // What the writer of a gradient needs: p = 2^(y - log2 s), dx = p (a1 + b1 (y - log2 s)), plus g at the action.
 struct RowGrad {

@@ -44,12 +44,9 @@ __global__ __launch_bounds__(rows_threads<LANES>()) void logits_loss_kernel(cons
     } else {
       r = streamed_stats<E, LANES>(f, lane, a.c, lds, Part{0, f.nfull, true});
     }
-    const bool empty = r.s == 0.f;
-    const float log2s = r.log2s();
-    const float lp = empty && x == x ? -INFINITY : ((x - r.m) * a.c - log2s) * kLn2;
-    const float entropy = empty ? 0.f : (log2s - r.u / r.s) * kLn2;
-    const StepTerms st = step_terms(lp, t.old[row], t.adv[row], t.ref ? t.ref[row] : 0.f, t.ref != nullptr, c);
-    const RowGrad g(wt * st.slope, -(float)c.entropy_coef * wt, entropy, r.m, a.c, log2s, a.inv_tau, act, empty);
+    const float entropy = r.entropy();
+    const StepTerms st = step_terms(r.log_prob(x, a.c), t.old[row], t.adv[row], t.ref ? t.ref[row] : 0.f, t.ref != nullptr, c);
+    const RowGrad g(wt * st.slope, -(float)c.entropy_coef * wt, entropy, r.m, a.c, r.log2s(), a.inv_tau, act, r.empty());
     if constexpr (NV > 0)
       write_grad<E, LANES, NV>(f, &h, out, g, lane, Part{0, f.nfull, true});
     else
@@ -91,12 +88,9 @@ __global__ __launch_bounds__(256) void join_loss_kernel(const ActionRows<E> a, c
     const int64_t act = a.actions[row];
     const float x = act >= 0 && act < a.A ? load_one(f.base + act) : NAN;
     const RowStats r = join_parts(p, row, a.c);
-    const bool empty = r.s == 0.f;
-    const float log2s = r.log2s();
-    const float lp = empty && x == x ? -INFINITY : ((x - r.m) * a.c - log2s) * kLn2;
-    const float entropy = empty ? 0.f : (log2s - r.u / r.s) * kLn2;
-    const StepTerms st = step_terms(lp, t.old[row], t.adv[row], t.ref ? t.ref[row] : 0.f, t.ref != nullptr, c);
-    const RowGrad g(wt * st.slope, -(float)c.entropy_coef * wt, entropy, r.m, a.c, log2s, a.inv_tau, act, empty);
+    const float entropy = r.entropy();
+    const StepTerms st = step_terms(r.log_prob(x, a.c), t.old[row], t.adv[row], t.ref ? t.ref[row] : 0.f, t.ref != nullptr, c);
+    const RowGrad g(wt * st.slope, -(float)c.entropy_coef * wt, entropy, r.m, a.c, r.log2s(), a.inv_tau, act, r.empty());
     write_grad<E, 256, 0>(f, nullptr, out, g, threadIdx.x, p.part(part, f.nfull));
     if (threadIdx.x == 0 && part == 0) {
       add_terms(acc, st, wt);
@@ -133,15 +127,12 @@ __global__ __launch_bounds__(kFewRows) void few_loss_kernel(const ActionRows<E> 
       h.load(x, a.A);
       const RowStats r = h.stats(a.c);
       const float xa = act >= 0 && act < a.A ? x[act] : NAN;
-      const bool empty = r.s == 0.f;
-      const float log2s = r.log2s();
-        const float lp = empty && xa == xa ? -INFINITY : ((xa - r.m) * a.c - log2s) * kLn2;
-      const float entropy = empty ? 0.f : (log2s - r.u / r.s) * kLn2;
-      const StepTerms st = step_terms(lp, old, adv, ref, t.ref != nullptr, c);
-      const RowGrad g(wt * st.slope, -(float)c.entropy_coef * wt, entropy, r.m, a.c, log2s, a.inv_tau, act, empty);
-      if (__any(empty)) {
+      const float entropy = r.entropy();
+      const StepTerms st = step_terms(r.log_prob(xa, a.c), old, adv, ref, t.ref != nullptr, c);
+      const RowGrad g(wt * st.slope, -(float)c.entropy_coef * wt, entropy, r.m, a.c, r.log2s(), a.inv_tau, act, r.empty());
+      if (__any(r.empty())) {
 #pragma unroll
-        for (int j = 0; j < K; ++j) h.x[j] = empty ? 0.f : g(h.x[j], j);
+        for (int j = 0; j < K; ++j) h.x[j] = r.empty() ? 0.f : g(h.x[j], j);
         h.store(x, a.A);
       } else {
 #pragma unroll

@@ -57,9 +57,13 @@ __device__ __forceinline__ T block_sum(T x, T* s) {
 // clipped side, and where the dual clip caps it, the gradient is zero, elsewhere d/d(log pi) = -A r.  The KL
 // term is e^d - 1 - d with d = log pi_ref - log pi, derivative 1 - e^d.
 // ---------------------------------------------------------------------------------------
+
+// The bounds come as two floats each: terms of both signs leave a loss that is far smaller than they are, and a bound rounded
+// to one float is off alike in every step that it holds.  Their logarithms are one float each: a D that differs from one by
+// less than its rounding differs in the term by no more.
 struct LossConsts {
   float log_low, log_high, log_dual;  // thresholds of D; log_dual = inf: no cap
-  float low, high, dual;              // the values themselves, and what float32 leaves out of them
+  float low, high, dual;              // the bounds, and what float32 leaves out of them
   float low_rest, high_rest, dual_rest;
   float kl;  // kl_coef
   double kl_coef, entropy_coef;
@@ -67,8 +71,6 @@ struct LossConsts {
 
 constexpr int kTerms = 5;  // policy, KL, clipped share, KL to the old policy, entropy
 
-// The bounds come as two floats each: terms of both signs leave a loss that is far smaller than they are, and a bound rounded
-// to one float is off alike in every step that it holds.
 struct StepTerms {
   float policy, kl, clipped, old_kl;
   float slope;
