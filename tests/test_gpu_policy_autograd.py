@@ -14,6 +14,11 @@ def _path(request, monkeypatch):
     monkeypatch.setenv("RL_TRITON_CORRECTNESS_WARNINGS", request.param)
 
 
+def _requested(which):
+    """Bytes asked of the allocator (what it hands out depends on the blocks that it has from before)."""
+    return torch.cuda.memory_stats()[f"requested_bytes.all.{which}"]
+
+
 def _step_args(grad=False):
     g = torch.Generator(device="cuda").manual_seed(1)
     n = lambda *s: torch.randn(s, generator=g, device="cuda")  # noqa: E731
@@ -115,7 +120,7 @@ def test_unrolled_steps_hold_nothing_back():
     sizes = []
     for _ in range(6):
         out, state = policy.compute_linear_attention_step(q * 1, k * 1, v * 1, decay, state)
-        sizes.append(torch.cuda.memory_allocated())
+        sizes.append(_requested("current"))
     assert sizes[-1] == sizes[1] and out.requires_grad
 
 
@@ -133,9 +138,9 @@ def test_only_the_gradients_that_are_asked_for_are_computed(seq_len):
         outs = policy.compute_linear_attention(*leaves[:3], decay, None, leaves[3])
         torch.cuda.synchronize()
         torch.cuda.reset_peak_memory_stats()
-        before = torch.cuda.memory_allocated()
+        before = _requested("current")
         grads = torch.autograd.grad(outs, [t for t in leaves if t.requires_grad], (up, us))
-        return grads, torch.cuda.max_memory_allocated() - before
+        return grads, _requested("peak") - before
 
     run((True,) * 4)  # (the scratch memory is there)
     full, _ = run((True,) * 4)
@@ -143,6 +148,6 @@ def test_only_the_gradients_that_are_asked_for_are_computed(seq_len):
                    (True, False, True, False), (False, True, False, True), (False, True, True, True)):
         grads, peak = run(wanted)
         assert all(torch.equal(a, b) for a, b in zip(grads, [x for x, w in zip(full, wanted) if w]))
-        # the state's gradient comes with v's: room for both, and 512 bytes a tensor for the allocator's rounding
-        room = sum(x.numel() * 4 + 512 for x, w in zip(inputs, (*wanted[:2], wanted[2] or wanted[3], wanted[3])) if w)
+        # the state's gradient comes with v's: room for both
+        room = sum(x.numel() * 4 for x, w in zip(inputs, (*wanted[:2], wanted[2] or wanted[3], wanted[3])) if w)
         assert peak <= room, (wanted, peak, room)

@@ -56,7 +56,7 @@ def test_it_goes_with_the_graph():
         torch.cuda.synchronize()
         del graph, got
         gc.collect()
-        levels.append(torch.cuda.memory_allocated())
+        levels.append(torch.cuda.memory_stats()["requested_bytes.all.current"])
     assert levels == [levels[0]] * 4, levels
 
 
