@@ -18,12 +18,13 @@
 // accumulator layout (4 consecutive rows of a column per lane) is also an operand layout once the inner index is
 // taken in that order, so U feeds U^T a without a trip through LDS.
 //
-// Measured (us; floors are bytes at the 5.2 TB/s of a large copy): bfloat16 [64,1024,8,64] 75 forward (floor 52) and 185 for
-// the three walks back (90 with each array read once); float32 185 and 460 (103, 181).  [1,16384,16,128], a row of
-// segments: states 43, join 7.8, walks 83 (52 for all).  [37,333,4,40 and 72] float32: 60 and 113 (18 for both; the
+// Measured (us; floors are bytes at the 5.2 TB/s of a large copy): bfloat16 [64,1024,8,64] 79 forward (floor 52) and 196 for
+// the three walks back (90 with each array read once); float32 172 and 468 (103, 181).  [1,16384,16,128], a row of
+// segments: states 43, join 8.1, walks 88 (52 for all).  [37,333,4,40 and 72] float32: 59 and 111 (23 for both; the
 // useful products alone 13), on 148 of 256 CUs forward, each with the wavefronts' fifth tile of columns on one SIMD.
-// Neither HBM nor the matrix units are the bound in bfloat16: the vector units are busy for 43% of the time (a chunk costs a
-// wavefront some 450 instructions, a quarter of them the weights' split into three), matrix products for 15%, and
+// Neither HBM nor the matrix units are the bound in bfloat16: the vector units are busy for 46% of the time (a chunk costs a
+// wavefront some 490 instructions, two fifths of them splits: the weights' into three numbers, the state's and p's into two; without
+// the latter two it took 75 and 185), matrix products for 20%, and
 // the rest is waits for LDS and the two barriers of a chunk, with two wavefronts a SIMD to cover them.  In
 // float32 matrix products (16x16x4, a sixteenth of bfloat16's rate) take 34% of [37,333,4,40 and 72], over the SIMDs.
 #include "rlk_attention.hpp"
@@ -695,8 +696,8 @@ __global__ __launch_bounds__(4 * D, 2) void walk_kernel(const Walks<E> walks) {
   };
 
   // A chunk that holds an inf, a NaN or values whose products overflow, step by step: as products of matrices it would put
-  // them (0 inf = NaN) where the recurrence does not, in steps before them and past an episode's end.  bfloat16 [1,16384,16,128]: 122 us
-  // without such a chunk, 2539 with one in every chunk; looking for them costs 3% ([64,1024,8,64] training 264 -> 269).
+  // them (0 inf = NaN) where the recurrence does not, in steps before them and past an episode's end.  bfloat16 [1,16384,16,128]: 129 us
+  // without such a chunk, 2526 with one in every chunk; looking for them costs 3% ([64,1024,8,64] training 264 -> 269).
   auto careful = [&](int64_t s0, int L, uint64_t cuts, bool end, const char* tile) {
     int v16 = l16, v4 = l4;
     for (int i = 0; i < L; ++i) {

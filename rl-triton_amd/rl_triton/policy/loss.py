@@ -110,8 +110,9 @@ def compute_policy_loss_from_logits(
     of the logits.
 
     The log-probabilities are those of compute_action_log_probs.  A row of logits is read once, held while its
-    loss is found, and its gradient written from there (rows of up to 256 KB; longer ones are read twice).
-    Masked steps are not read and have zero gradients.  `logits.backward(grad)` goes on into the policy.
+    loss is found, and its gradient written from there (rows of up to 256 KB; longer ones are read twice, and so are up to 64 rows
+    of 64 KB and more, which several workgroups share).  Masked steps have zero gradients whatever their logits hold.
+    `logits.backward(grad)` goes on into the policy.
 
     Args:
         logits:       [num_envs, seq_len, num_actions], float32 or bfloat16, GPU.
