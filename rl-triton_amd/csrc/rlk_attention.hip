@@ -299,12 +299,14 @@ struct Weighted<bf16> {
 
 // A factor that is not one of the call's arrays, for products with one that is: the state where outputs are read from it, and p.
 // float32: itself.  bfloat16: the sum of two bfloat16 numbers, the upper 8 bits and the next 8 rounded, 2^-15 off at the most.
-// (As one number, 2^-8 off, outputs had half as much error again as their own rounding gives them.)  x is finite.
+// (As one number, 2^-8 off, outputs had half as much error again as their own rounding gives them.)  ANY: not only finite
+// numbers; an infinity's rest, inf - inf, is then a number that makes no difference to it.
 template <class E>
 struct Factor;
 template <>
 struct Factor<float> {
   Frag<float> x;
+  template <bool ANY>
   __device__ static Factor from(f32x4 a, f32x4 b) { return {Frag<float>::from(a, b)}; }
   // acc[t] += this * rows[t]
   template <int N>
@@ -314,16 +316,24 @@ struct Factor<float> {
   }
 };
 __device__ __forceinline__ u32x2 upper_quad(f32x4 x) { return {uppers(x[0], x[1]), uppers(x[2], x[3])}; }
+template <bool ANY>
 __device__ __forceinline__ u32x2 rest_quad(f32x4 x) {
-  return {bf16_pair(x[0] - upper(x[0]), x[1] - upper(x[1])), bf16_pair(x[2] - upper(x[2]), x[3] - upper(x[3]))};
+  float r[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    r[i] = x[i] - upper(x[i]);
+    if constexpr (ANY) r[i] = fminf(r[i], 0x1p126f);  // (of a NaN and a number the number)
+  }
+  return {bf16_pair(r[0], r[1]), bf16_pair(r[2], r[3])};
 }
 template <>
 struct Factor<bf16> {
   Frag<bf16> hi, lo;
+  template <bool ANY>
   __device__ static Factor from(f32x4 a, f32x4 b) {
     union { u32x2 h[2]; bf16x8 v; } h, l;
     h.h[0] = upper_quad(a), h.h[1] = upper_quad(b);
-    l.h[0] = rest_quad(a), l.h[1] = rest_quad(b);
+    l.h[0] = rest_quad<ANY>(a), l.h[1] = rest_quad<ANY>(b);
     return {{h.v}, {l.v}};
   }
   template <int N>
@@ -498,7 +508,7 @@ __global__ __launch_bounds__(4 * D, 2) void walk_kernel(const Walks<E> walks) {
   };
 
   bool crossed = false;  // a cut anywhere in the segment
-  // a state that is not finite, in bfloat16: it has no two parts (inf - inf), so its chunks go step by step
+  // a state of this wavefront's that is not finite, in bfloat16: its chunks are none of the plain ones
   bool wild = false;
   auto look = [&] {
     if constexpr (!STATE && M::PARTS) {
@@ -535,7 +545,8 @@ __global__ __launch_bounds__(4 * D, 2) void walk_kernel(const Walks<E> walks) {
     return found;
   };
 
-  // One chunk, unless it is tainted.  PLAIN: whole, without a cut, and not the one that a state leaves the sequence with.
+  // One chunk, unless it is tainted.  PLAIN: whole, without a cut, from a finite state, and not the one that a state leaves the
+  // sequence with.  (Wavefronts may go through different forms of a chunk: both have the same barriers.)
   auto chunk = [&](auto plain, int64_t s0, int L, uint64_t cuts, bool end, const char* tile) {
     constexpr bool PLAIN = decltype(plain)::value;
     int4 mark = *reinterpret_cast<const int4*>(tile + M::taint(0));
@@ -589,14 +600,14 @@ __global__ __launch_bounds__(4 * D, 2) void walk_kernel(const Walks<E> walks) {
           if (ti < 2 && SHARE * u >= 2) continue;  // past the diagonal's tiles
           char* p = lds + (at_p_put ^ (16 * SHARE * u * M::S));
           *reinterpret_cast<u32x2*>(p) = upper_quad(pt);
-          *reinterpret_cast<u32x2*>(p + M::P_PART) = rest_quad(pt);
+          *reinterpret_cast<u32x2*>(p + M::P_PART) = rest_quad<false>(pt);
         } else {
           Quad<E>::of(pt).store(reinterpret_cast<E*>(lds + at_p_put + 16 * SHARE * u * M::S));
         }
       }
       __syncthreads();
     }
-    if (__builtin_amdgcn_readfirstlane(mark.x | mark.y | mark.z | mark.w) != 0 || wild) return false;
+    if (__builtin_amdgcn_readfirstlane(mark.x | mark.y | mark.z | mark.w) != 0) return false;
 
     Frag<E> fc[2];
 #pragma unroll
@@ -612,7 +623,7 @@ __global__ __launch_bounds__(4 * D, 2) void walk_kernel(const Walks<E> walks) {
       for (int kk = 0; kk < KK; ++kk) {
         if (!FULL && 32 * kk >= da) continue;
         const bool half = !FULL && da - 32 * kk <= 16;
-        const Factor<E> fu = Factor<E>::from(U[2 * kk], U[2 * kk + 1]);
+        const Factor<E> fu = Factor<E>::template from<!PLAIN>(U[2 * kk], U[2 * kk + 1]);
 #pragma unroll
         for (int t = 0; t < 4; t += 2) {
           const char *row = tile + at_a2 + 16 * t * M::ROW + 32 * kk * M::S, *next = row + 16 * M::ROW;
@@ -741,7 +752,8 @@ __global__ __launch_bounds__(4 * D, 2) void walk_kernel(const Walks<E> walks) {
     const int L = (int)(last - s0 < C ? last - s0 : C);
     const bool end = !reverse && s0 + C >= T;
     crossed |= cuts != 0;
-    const bool whole_chunk = L == C && cuts == 0 && !end;
+    if (wild) look();  // (an episode's end may have come)
+    const bool whole_chunk = L == C && cuts == 0 && !end && !wild;
     if (!(whole_chunk ? chunk(std::true_type{}, s0, L, cuts, end, lds + buffer) : chunk(std::false_type{}, s0, L, cuts, end, lds + buffer)))
       careful(s0, L, cuts, end, lds + buffer);
     if (s0 + C >= last) break;

@@ -141,7 +141,7 @@ def compute_linear_attention(
     Differentiable in q, k, v and state.
 
     What is not finite, in padded steps for one, reaches no step before it and none past its episode's end; a chunk that
-    holds such values (or, in bfloat16, begins with a state that does) is computed step by step, in some twenty times the time.
+    holds such values is computed step by step, in some twenty times the time.
 
     Args:
         q, k:  [num_envs, seq_len, heads, dim_k], float32 or bfloat16, GPU; any strides with a contiguous last axis
