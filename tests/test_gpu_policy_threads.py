@@ -47,7 +47,7 @@ def test_losses_beside_backward_passes_over_segments(checked, monkeypatch):
         except Exception as e:  # (an exception of a thread would pass unseen)
             errors.append(repr(e))
 
-    threads = [threading.Thread(target=work, args=(fn, mine)) for fn, mine in zip((backward, losses, backward, losses), streams)]
+    threads = [threading.Thread(target=work, args=(fn, mine), daemon=True) for fn, mine in zip((backward, losses, backward, losses), streams)]
     for t in threads:
         t.start()
     for t in threads:
