@@ -116,6 +116,84 @@ int rlk_linear_attention(const rlk_attention *calls, int count, void *stream);
  * is read, `state_out` written; they may be the same. */
 int rlk_linear_attention_step(const rlk_attention *call, void *stream);
 
+/* The gated delta rule: S_t = a_t S_{t-1} + k_t u_t^T with u_t = beta_t (v_t - a_t S_{t-1}^T k_t), a_t = exp(log_decay_t), 0 where
+ * done_{t-1}; out_t = scale * S_t^T q_t.  A log-decay below -104 leaves nothing of the state, as -inf does. */
+typedef struct rlk_delta_rule {
+  rlk_sequence q, k, v, out; /* out.data is written */
+  int64_t num_envs, seq_len, heads, dim_k, dim_v; /* dims 1..128 */
+  const float *log_decays; /* NULL (zeros) or [num_envs, seq_len, heads], contiguous */
+  const float *betas;      /* [num_envs, seq_len, heads], contiguous */
+  const float *dones;      /* NULL or [num_envs, seq_len], contiguous */
+  const float *state;      /* before the first step, [num_envs, heads, dim_k, dim_v], contiguous; NULL: zeros */
+  float *state_out;        /* NULL, or the state after the last step, zero if that step is done (of no steps: `state`) */
+  float scale;
+  int bf16;                /* q, k, v, out */
+  void *workspace;         /* rlk_delta_rule_workspace_bytes(), 16-byte aligned, no initial contents needed */
+  size_t workspace_bytes;
+} rlk_delta_rule;
+
+/* Upstream gradients in `out` and `state_out` (NULL: none), the others are written; NULL data or pointers: not wanted.  Arrays of the gates
+ * are contiguous, those of states too. */
+typedef struct rlk_delta_rule_gradients {
+  rlk_sequence out, q, k, v;
+  const float *state_out;
+  float *state, *log_decays, *betas;
+} rlk_delta_rule_gradients;
+
+size_t rlk_delta_rule_workspace_bytes(int64_t num_envs, int64_t seq_len, int64_t heads, int64_t dim_k, int64_t dim_v, int backward);
+/* Of what a forward call leaves for the backward one (16-byte aligned). */
+size_t rlk_delta_rule_saved_bytes(int64_t num_envs, int64_t seq_len, int64_t heads, int64_t dim_k, int64_t dim_v);
+/* With `saved` (else NULL) the call needs no workspace.  heads * ceil(seq_len / 64) is at most 2^22. */
+int rlk_gated_delta_rule(const rlk_delta_rule *call, void *saved, size_t saved_bytes, void *stream);
+/* `call` as the forward one was, with a workspace for backward = 1; its out and state_out are not looked at, and of its
+ * state only whether there is one. */
+int rlk_gated_delta_rule_backward(const rlk_delta_rule *call, const rlk_delta_rule_gradients *grads, const void *saved, size_t saved_bytes,
+                                  void *stream);
+/* One step for every environment: step strides and seq_len unused, log_decays and betas [num_envs, heads], dones [num_envs].  `state` is
+ * read, `state_out` written; they may be the same. */
+int rlk_gated_delta_rule_step(const rlk_delta_rule *call, void *stream);
+
+/* Actions drawn from softmax(logits / temperature), truncated: of the actions ordered by their logits, the largest first and of equal ones the
+ * first, those are kept that top_k says, of these the shortest beginning that holds top_p of their probability, of these the ones at
+ * least min_p times as likely as the first.  The action is the first, in the order of their numbers, up to which the kept ones hold more
+ * than the uniform number's share.  Rows without an allowed action (all logits -inf) and rows with a NaN: -1. */
+typedef struct rlk_sampling {
+  const void *logits; /* [num_envs, seq_len, num_actions], the actions of a row contiguous */
+  int64_t num_envs, seq_len, num_actions; /* num_actions: 1 .. 2^20 */
+  int64_t env_stride, step_stride;
+  int bf16;
+  const float *uniforms; /* [num_envs, seq_len], contiguous, in [0, 1) */
+  double temperature;
+  int64_t top_k; /* 0: all */
+  double top_p;  /* above 0, up to 1: all */
+  double min_p;  /* 0 .. 1, 0: all */
+  int64_t *actions; /* [num_envs, seq_len] */
+  float *log_probs; /* of the actions among those kept: [num_envs, seq_len]; -inf without one, NaN in rows with a NaN */
+} rlk_sampling;
+
+#define RLK_MOST_SAMPLED_ACTIONS (1 << 20)
+
+int rlk_sample_actions(const rlk_sampling *call, void *stream);
+
+/* Queries and keys, head by head: x / sqrt(mean(x^2) + eps) * weight, then the pairs of the first rotary_dim elements turned by
+ * position * base^(-2 i / rotary_dim): elements i and i + rotary_dim / 2, or 2 i and 2 i + 1 (`interleaved`). */
+typedef struct rlk_head_norms {
+  rlk_sequence q, k;         /* heads of q_heads and k_heads; either number may be 0 */
+  rlk_sequence q_out, k_out; /* backward: gradients of q and k */
+  int64_t num_envs, seq_len, q_heads, k_heads, dim, rotary_dim; /* dim: 1 .. 256; rotary_dim: even, 0 .. dim */
+  int interleaved, bf16;
+  const float *q_weight, *k_weight; /* [dim] or NULL (ones) */
+  const int64_t *positions;         /* [num_envs, seq_len], contiguous; NULL: nothing is turned */
+  double base, eps;
+} rlk_head_norms;
+
+int rlk_query_key_norms(const rlk_head_norms *call, void *stream);
+/* Gradients: of q and k into q_out and k_out (NULL data: not wanted), of the weights into q_weight_grad and k_weight_grad (NULL: not
+ * wanted).  A workspace of rlk_head_norms_workspace_bytes() (no initial contents needed) where weights' gradients are. */
+size_t rlk_head_norms_workspace_bytes(const rlk_head_norms *call);
+int rlk_query_key_norms_backward(const rlk_head_norms *call, rlk_sequence grad_q, rlk_sequence grad_k, float *q_weight_grad,
+                                 float *k_weight_grad, void *workspace, size_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

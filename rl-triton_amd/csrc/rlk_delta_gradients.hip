@@ -1,0 +1,336 @@
+// rlk_delta_gradients.hip -- the gated delta rule: gradients of queries, keys, gates and betas, all chunks at once, from what the two walks
+// have left (rlk_delta.hpp): states S before the chunk, gradients R of the states after it, the corrections w and z.
+//
+// With u = b w, dv = b z, Y1_ij = scale D_ij G_i . u_j (i >= j) and Y2_ij = -D_ij dv_i . u_j (i > j):
+//   dq_i = scale back_i S G_i + sum_j Y1_ij k_j
+//   dk_i = dk+ + dk-,   dk+_i = -back_i S dv_i + sum_j Y2_ij k_j,   dk-_j = into_j R u_j + sum_i (Y1_ij q_i + Y2_ij k_i)
+//   db_i = z_i . w_i
+// A gate's gradient is the sum of every term that its factor is in.  Terms with D_ij have the gates from j + 1 to i; added at i and taken
+// away at j they sum up from the end: x_i = q_i . dq_i + k_i . (dk+_i - dk-_i), and at the chunk's last step also the terms of
+// S' (keep R . S + sum_j into_j k_j . R u_j); dg_t = sum of x_i from t to its episode's end, in float64.
+//
+// A workgroup per chunk, a wavefront per 16 rows of the state.  The sums over the state's columns go 64 columns at a time, G, u and dv in LDS;
+// then keys, queries and both Y take their place.
+#include "rlk_delta.hpp"
+
+namespace rlk {
+namespace delta {
+namespace {
+
+template <class E, int D>
+struct Lds {
+  typedef Tile<E, 64> G;
+  typedef Tile<float, 64> U;
+  typedef Tile<E, D> K;
+  typedef Tri<3> Y;
+  static constexpr int UT = G::BYTES, DT = UT + U::BYTES, FIRST = DT + U::BYTES;
+  static constexpr int QT = K::BYTES, Y1 = 2 * K::BYTES, Y2 = Y1 + Y::BYTES, SECOND = Y2 + Y::BYTES;
+  static constexpr int BYTES = FIRST > SECOND ? FIRST : SECOND;
+};
+
+// 64 columns from c0 on of a chunk's rows of w or z, each row times its beta, as parts in a tile.
+template <int NT>
+struct Corrections {
+  static constexpr int PER = C * 16 / NT;
+  f32x4 x[PER];
+  __device__ void fetch(const float* p, int c0, int dvp) {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int u = threadIdx.x + NT * i, c = c0 + u % 16 * 4;
+      x[i] = c < dvp ? *reinterpret_cast<const f32x4*>(p + u / 16 * dvp + c) : zero4();
+    }
+  }
+  __device__ void put(char* tile, const float* beta) const {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int u = threadIdx.x + NT * i;
+      Four<float>{x[i] * beta[u / 16]}.put(tile + Tile<float, 64>::row(u / 16) + u % 16 * 8, Tile<float, 64>::PART);
+    }
+  }
+};
+
+template <class E, int D, bool VEC>
+__global__ __launch_bounds__(4 * D, D == 128 || kParts<E> == 1 ? 2 : 1) void gradients_kernel(const Rule<E> r) {
+  constexpr int NT = 4 * D, WAVES = D / 16, N = kParts<E>;
+  typedef Lds<E, D> M;
+  typedef typename M::K T;
+  __shared__ __align__(16) char lds[M::BYTES];
+  __shared__ float sums[WAVES][C + 2];
+  __shared__ float beta[C];
+  __shared__ int found[WAVES];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l16 = lane & 15, l4 = lane >> 4;
+  const int64_t at = blockIdx.x, pair = at / r.chunks, chunk = at - pair * r.chunks, s0 = chunk * C;
+  const int64_t env = r.first_env + pair / r.heads;
+  const int head = (int)(pair % r.heads), dk = r.dk, dv = r.dv, dvp = pad16(dv);
+  const int n = (int)(r.seq_len - s0 < C ? r.seq_len - s0 : C);
+  const Record& rec = r.records[at];
+  const uint64_t cuts = rec.cuts[0] | (uint64_t)rec.cuts[1] << 32;
+
+  Rows<E, D, NT, VEC> k, q;
+  k.fetch(r.k.data + env * r.k.env + head * r.k.head + s0 * r.k.step, r.k.step, dk, n);
+  q.fetch(r.q.data + env * r.q.env + head * r.q.head + s0 * r.q.step, r.q.step, dk, n);
+  {
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < Rows<E, D, NT, VEC>::PER; ++i) {
+      const f32x4 a = k.x[i].floats(), b = q.x[i].floats();
+#pragma unroll
+      for (int x = 0; x < 4; ++x) sum = fmaf(0.f, a[x], fmaf(0.f, b[x], sum));
+    }
+    const bool any = __any(sum != 0.f);
+    if (lane == 0) found[wave] = any;
+  }
+  if (threadIdx.x < C) beta[threadIdx.x] = rec.beta[threadIdx.x];
+  const E* gg = r.gy.data + env * r.gy.env + head * r.gy.head + s0 * r.gy.step;
+  const float *w = r.w + at * C * dvp, *z = r.z + at * C * dvp;
+  const int64_t state = at * pad16(dk) * dvp;
+  const bool mine = 16 * wave < dk;
+
+  // transposed results: step 16 t + l16, dims 16 wave + 4 l4 + 0..3
+  f32x4 dq[4], up[4], down[4];  // (up, down: dk+ and dk-)
+#pragma unroll
+  for (int t = 0; t < 4; ++t) dq[t] = up[t] = down[t] = zero4();
+  // Y1 and Y2, rows ti: transposed too, steps i = 16 ti + l16, j = 16 tj + 4 l4 + 0..3.  8 wavefronts share: the first 4 have Y1, the others Y2
+  constexpr bool BOTH = WAVES == 4;
+  const int ti = wave & 3;
+  f32x4 ya[4], yb[4];
+#pragma unroll
+  for (int t = 0; t < 4; ++t) ya[t] = yb[t] = zero4();
+  const bool first = BOTH || wave < 4;
+  float kept = 0.f;
+  f32x4 db = zero4();  // (of the steps of this thread's parts of w and z)
+  constexpr int PER = Corrections<NT>::PER;
+  static_assert(PER <= 4);
+
+  for (int c0 = 0; c0 < dv; c0 += 64) {
+    Rows<E, 64, NT, VEC> gs;
+    Corrections<NT> ws, zs;
+    gs.fetch(gg + c0, r.gy.step, dv - c0, n);
+    ws.fetch(w, c0, dvp);
+    zs.fetch(z, c0, dvp);
+    if (c0 > 0) __syncthreads();
+    gs.put(lds, 0, n);
+    if (c0 == 0) __syncthreads();  // (beta is there)
+    ws.put(lds + M::UT, beta);
+    zs.put(lds + M::DT, beta);
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+#pragma unroll
+      for (int x = 0; x < 4; ++x) db[i] = fmaf(ws.x[i][x], zs.x[i][x], db[i]);
+    __syncthreads();
+    const int kks = dv - c0 > 32 ? 2 : 1;
+    for (int kk = 0; kk < kks; ++kk) {
+      {
+        const Op<N> g = rows_of<typename M::G>(lds, ti, kk);
+        const Op<3> d = rows_of<typename M::U>(lds + M::DT, ti, kk);
+#pragma unroll
+        for (int tj = 0; tj < 4; ++tj) {
+          if (tj > ti) continue;
+          const Op<3> u = rows_of<typename M::U>(lds + M::UT, tj, kk);
+          if constexpr (BOTH) {
+            ya[tj] = mul<2>(u, g, ya[tj]);
+            yb[tj] = mul<2>(u, d, yb[tj]);
+          } else if (first) {
+            ya[tj] = mul<2>(u, g, ya[tj]);
+          } else {
+            ya[tj] = mul<2>(u, d, ya[tj]);
+          }
+        }
+      }
+      settle();
+      if (mine) {
+        const int c = c0 + 32 * kk + 4 * l4;
+        const float *S = r.states + state + (16 * wave + l16) * dvp, *R = r.dstates + state + (16 * wave + l16) * dvp;
+        const f32x4 s_lo = *reinterpret_cast<const f32x4*>(S + (c < dvp ? c : 0)), s_hi = *reinterpret_cast<const f32x4*>(S + (c + 16 < dvp ? c + 16 : 0));
+        const f32x4 r_lo = *reinterpret_cast<const f32x4*>(R + (c < dvp ? c : 0)), r_hi = *reinterpret_cast<const f32x4*>(R + (c + 16 < dvp ? c + 16 : 0));
+        const f32x4 o = zero4();
+        const f32x4 a = c < dvp ? s_lo : o, b = c + 16 < dvp ? s_hi : o, e = c < dvp ? r_lo : o, f = c + 16 < dvp ? r_hi : o;
+#pragma unroll
+        for (int x = 0; x < 4; ++x) kept = fmaf(a[x], e[x], fmaf(b[x], f[x], kept));
+        const Op<3> s = split<3>(a, b), rr = split<3>(e, f);
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          dq[t] = mul<2>(s, rows_of<typename M::G>(lds, t, kk), dq[t]);
+          up[t] = mul<2>(s, rows_of<typename M::U>(lds + M::DT, t, kk), up[t]);
+          down[t] = mul<2>(rr, rows_of<typename M::U>(lds + M::UT, t, kk), down[t]);
+        }
+      }
+      settle();
+    }
+  }
+  // db: a row's 16 parts
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    float x = db[i];
+#pragma unroll
+    for (int d = 1; d < 16; d <<= 1) x += __shfl_xor(x, d);
+    const int row = (threadIdx.x + NT * i) / 16;
+    if (l16 == 0 && row < n && r.gb != nullptr) r.gb[(env * r.seq_len + s0 + row) * r.heads + head] = x;
+  }
+  const float keep = rec.keep;
+  kept = keep != 0.f ? kept * keep : 0.f;
+  float back[4], into[4];
+#pragma unroll
+  for (int t = 0; t < 4; ++t) {
+    back[t] = rec.back[16 * t + l16], into[t] = rec.into[16 * t + l16];
+    // (what does not reach a step has no part, NaN included)
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      dq[t][x] = back[t] != 0.f ? dq[t][x] * (back[t] * r.scale) : 0.f;
+      up[t][x] = back[t] != 0.f ? -up[t][x] * back[t] : 0.f;
+      down[t][x] = into[t] != 0.f ? down[t][x] * into[t] : 0.f;
+    }
+  }
+  __syncthreads();  // all have read the first arrays
+  {
+    const int i = 16 * ti + l16;
+    const uint64_t before = cuts & (((uint64_t)2 << i) - 1);
+    const int begin = before != 0 ? 63 - __clzll((long long)before) : 0;
+    const float hi = rec.ghi[i], lo = rec.glo[i];
+#pragma unroll
+    for (int tj = 0; tj < 4; ++tj) {
+      if (tj > (ti | 1)) continue;
+      f32x4 a = ya[tj], b = yb[tj];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int j = 16 * tj + 4 * l4 + e;
+        const bool same = tj <= ti && j >= begin;
+        const float d = same && j <= i ? expf((hi - rec.ghi[j]) + (lo - rec.glo[j])) : 0.f;
+        if constexpr (BOTH) {
+          a[e] = same && j <= i ? a[e] * (d * r.scale) : 0.f;
+          b[e] = same && j < i ? -b[e] * d : 0.f;
+        } else {
+          a[e] = first ? (same && j <= i ? a[e] * (d * r.scale) : 0.f) : (same && j < i ? -a[e] * d : 0.f);
+        }
+      }
+      const int place = M::Y::row(16 * ti) + l16 * (M::Y::row(16 * ti + 1) - M::Y::row(16 * ti)) + 2 * (16 * tj + 4 * l4);
+      Four<float>{a}.put(lds + (first ? M::Y1 : M::Y2) + place, M::Y::PART);
+      if constexpr (BOTH) Four<float>{b}.put(lds + M::Y2 + place, M::Y::PART);
+    }
+  }
+  // Keys and queries that are not finite would reach other episodes as 0 inf: then an episode at a time.
+  bool wild = false;
+#pragma unroll
+  for (int i = 0; i < WAVES; ++i) wild |= found[i] != 0;
+  for (int from = 0, to; from < n; from = to) {
+    to = n;
+    if (wild) {
+      const uint64_t later = cuts & ~(((uint64_t)2 << from) - 1);
+      to = later != 0 ? __ffsll((long long)later) - 1 : n;
+    }
+    if (from > 0) __syncthreads();
+    k.put(lds, from, to);
+    q.put(lds + M::QT, from, to);
+    __syncthreads();
+    float total = 0.f;
+    if (mine) {
+      // what the steps wrote into S'
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        const int i = 16 * t + l16;
+        if (i >= from && i < to && into[t] != 0.f)
+#pragma unroll
+          for (int x = 0; x < 4; ++x) total = fmaf(number_at<T>(lds, i, 16 * wave + 4 * l4 + x), down[t][x], total);
+      }
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        f32x4 a = dq[t], b = up[t], c = down[t];
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk) {
+          const Op<N> kc = columns_of<T>(lds, wave, kk), qc = columns_of<T>(lds + M::QT, wave, kk);
+          if (kk <= t / 2) {
+            a = mul<2>(kc, rows_of<typename M::Y>(lds + M::Y1, t, kk), a);
+            b = mul<2>(kc, rows_of<typename M::Y>(lds + M::Y2, t, kk), b);
+          }
+          if (kk >= t / 2) {
+            c = mul<2>(qc, columns_of<typename M::Y>(lds + M::Y1, t, kk), c);
+            c = mul<2>(kc, columns_of<typename M::Y>(lds + M::Y2, t, kk), c);
+          }
+        }
+        settle();
+        const int i = 16 * t + l16;
+        const bool inside = i >= from && i < to;
+        if (inside) dq[t] = a, up[t] = b, down[t] = c;
+        float x = 0.f;
+        if (inside)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int d = 16 * wave + 4 * l4 + e;
+            x = fmaf(number_at<T>(lds + M::QT, i, d), dq[t][e], fmaf(number_at<T>(lds, i, d), up[t][e] - down[t][e], x));
+          }
+        x += __shfl_xor(x, 16);
+        x += __shfl_xor(x, 32);
+        if (l4 == 0 && inside) sums[wave][i] = x;
+      }
+    }
+    if (to == n) {
+      total += kept;
+#pragma unroll
+      for (int d = 1; d < 64; d <<= 1) total += __shfl_xor(total, d);
+      if (lane == 0) sums[wave][C] = mine ? total : 0.f;
+    }
+  }
+  __syncthreads();
+  if (mine) {
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      const int i = 16 * t + l16, d = 16 * wave + 4 * l4;
+      if (i >= n) continue;
+      const f32x4 x = up[t] + down[t];
+      const int64_t s = s0 + i;
+      E* pq = r.gq.data != nullptr ? r.gq.data + env * r.gq.env + s * r.gq.step + head * r.gq.head + d : nullptr;
+      E* pk = r.gk.data != nullptr ? r.gk.data + env * r.gk.env + s * r.gk.step + head * r.gk.head + d : nullptr;
+      if constexpr (VEC) {
+        if (d < dk) {
+          if (pq != nullptr) store_quad<false>(pq, float4{dq[t][0], dq[t][1], dq[t][2], dq[t][3]});
+          if (pk != nullptr) store_quad<false>(pk, float4{x[0], x[1], x[2], x[3]});
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (d + e < dk) {
+            if (pq != nullptr) pq[e] = from_f32<E>(dq[t][e]);
+            if (pk != nullptr) pk[e] = from_f32<E>(x[e]);
+          }
+      }
+    }
+  }
+  if (wave == 0 && r.gg != nullptr) {
+    const int used = (dk + 15) / 16;
+    double x = 0.0;
+    if (lane < n)
+      for (int i = 0; i < used; ++i) x += (double)sums[i][lane];
+    if (lane == n - 1)
+      for (int i = 0; i < used; ++i) x += (double)sums[i][C];
+    const uint64_t later = lane < 63 ? cuts & ~(((uint64_t)2 << lane) - 1) : 0;
+    const int end = later != 0 ? __ffsll((long long)later) - 1 : n;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const double next = __shfl_down(x, d);
+      if (lane + d < end) x += next;
+    }
+    const float g = (cuts >> lane) & 1 || (r.from_zero && s0 + lane == 0) ? 0.f : (float)x;
+    if (lane < n) r.gg[(env * r.seq_len + s0 + lane) * r.heads + head] = g;
+  }
+}
+
+}  // namespace
+
+template <class E>
+int launch_gradients(const Rule<E>& r, int64_t envs, hipStream_t s) {
+  const dim3 grid((unsigned)(envs * r.heads * r.chunks));
+  const bool vec = fours(r.k, r.dk) && fours(r.q, r.dk) && fours(r.gy, r.dv) && fours(r.gq, r.dk) && fours(r.gk, r.dk);
+  if (r.dk <= 64 && r.dv <= 64) {
+    if (vec) gradients_kernel<E, 64, true><<<grid, dim3(256), 0, s>>>(r);
+    else gradients_kernel<E, 64, false><<<grid, dim3(256), 0, s>>>(r);
+  } else {
+    if (vec) gradients_kernel<E, 128, true><<<grid, dim3(512), 0, s>>>(r);
+    else gradients_kernel<E, 128, false><<<grid, dim3(512), 0, s>>>(r);
+  }
+  return hipGetLastError() == hipSuccess ? RLK_OK : RLK_ERR_LAUNCH;
+}
+template int launch_gradients<bf16>(const Rule<bf16>&, int64_t, hipStream_t);
+template int launch_gradients<float>(const Rule<float>&, int64_t, hipStream_t);
+
+}  // namespace delta
+}  // namespace rlk

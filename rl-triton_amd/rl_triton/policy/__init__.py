@@ -10,20 +10,31 @@ Not in the reference's API, whose surface rl_triton itself keeps:
 """
 from rl_triton._native import public_entry as _public_entry
 from rl_triton.policy import attention as _attention
+from rl_triton.policy import delta_rule as _delta_rule
+from rl_triton.policy import head_norms as _head_norms
 from rl_triton.policy import log_probs as _log_probs
 from rl_triton.policy import loss as _loss
+from rl_triton.policy import sampling as _sampling
 
 # The Python implementations, each behind the C++ fast path (rl_triton._native.public_entry).
 compute_action_log_probs = _public_entry(_log_probs.compute_action_log_probs, "action_log_probs")
+compute_gated_delta_rule = _delta_rule.compute_gated_delta_rule
+compute_gated_delta_rule_step = _delta_rule.compute_gated_delta_rule_step
 compute_linear_attention = _public_entry(_attention.compute_linear_attention, "linear_attention")
 compute_linear_attention_step = _public_entry(_attention.compute_linear_attention_step, "linear_attention_step")
 compute_policy_loss = _public_entry(_loss.compute_policy_loss, "policy_loss")
 compute_policy_loss_from_logits = _public_entry(_loss.compute_policy_loss_from_logits, "policy_loss_from_logits")
+compute_query_key_norms = _head_norms.compute_query_key_norms
+compute_sampled_actions = _sampling.compute_sampled_actions
 
 __all__ = [
     "compute_action_log_probs",
+    "compute_gated_delta_rule",
+    "compute_gated_delta_rule_step",
     "compute_linear_attention",
     "compute_linear_attention_step",
     "compute_policy_loss",
     "compute_policy_loss_from_logits",
+    "compute_query_key_norms",
+    "compute_sampled_actions",
 ]

@@ -45,6 +45,31 @@ class Attention(ctypes.Structure):
                 ("workspace_bytes", _SZ)]
 
 
+class DeltaRule(ctypes.Structure):
+    _fields_ = [("q", Sequence), ("k", Sequence), ("v", Sequence), ("out", Sequence), ("num_envs", _I64),
+                ("seq_len", _I64), ("heads", _I64), ("dim_k", _I64), ("dim_v", _I64), ("log_decays", _P), ("betas", _P),
+                ("dones", _P), ("state", _P), ("state_out", _P), ("scale", _F), ("bf16", _INT), ("workspace", _P),
+                ("workspace_bytes", _SZ)]
+
+
+class DeltaRuleGradients(ctypes.Structure):
+    _fields_ = [("out", Sequence), ("q", Sequence), ("k", Sequence), ("v", Sequence), ("state_out", _P), ("state", _P),
+                ("log_decays", _P), ("betas", _P)]
+
+
+class Sampling(ctypes.Structure):
+    _fields_ = [("logits", _P), ("num_envs", _I64), ("seq_len", _I64), ("num_actions", _I64), ("env_stride", _I64),
+                ("step_stride", _I64), ("bf16", _INT), ("uniforms", _P), ("temperature", _D), ("top_k", _I64), ("top_p", _D),
+                ("min_p", _D), ("actions", _P), ("log_probs", _P)]
+
+
+class HeadNorms(ctypes.Structure):
+    _fields_ = [("q", Sequence), ("k", Sequence), ("q_out", Sequence), ("k_out", Sequence), ("num_envs", _I64),
+                ("seq_len", _I64), ("q_heads", _I64), ("k_heads", _I64), ("dim", _I64), ("rotary_dim", _I64),
+                ("interleaved", _INT), ("bf16", _INT), ("q_weight", _P), ("k_weight", _P), ("positions", _P), ("base", _D),
+                ("eps", _D)]
+
+
 # name -> argtypes (must match include/rl_triton_policy.h)
 SIGNATURES = {
     "rlk_action_log_probs": [ctypes.POINTER(ActionRows), _P, _P, _P, _P],
@@ -55,8 +80,18 @@ SIGNATURES = {
     "rlk_attention_workspace_bytes": [_I64, _I64, _I64, _I64, _I64],
     "rlk_linear_attention": [ctypes.POINTER(Attention), _INT, _P],
     "rlk_linear_attention_step": [ctypes.POINTER(Attention), _P],
+    "rlk_delta_rule_workspace_bytes": [_I64, _I64, _I64, _I64, _I64, _INT],
+    "rlk_delta_rule_saved_bytes": [_I64, _I64, _I64, _I64, _I64],
+    "rlk_gated_delta_rule": [ctypes.POINTER(DeltaRule), _P, _SZ, _P],
+    "rlk_gated_delta_rule_backward": [ctypes.POINTER(DeltaRule), ctypes.POINTER(DeltaRuleGradients), _P, _SZ, _P],
+    "rlk_gated_delta_rule_step": [ctypes.POINTER(DeltaRule), _P],
+    "rlk_sample_actions": [ctypes.POINTER(Sampling), _P],
+    "rlk_query_key_norms": [ctypes.POINTER(HeadNorms), _P],
+    "rlk_head_norms_workspace_bytes": [ctypes.POINTER(HeadNorms)],
+    "rlk_query_key_norms_backward": [ctypes.POINTER(HeadNorms), Sequence, Sequence, _P, _P, _P, _SZ, _P],
 }
-_RESTYPES = {"rlk_policy_workspace_bytes": _SZ, "rlk_attention_workspace_bytes": _SZ}
+_RESTYPES = {"rlk_policy_workspace_bytes": _SZ, "rlk_attention_workspace_bytes": _SZ, "rlk_delta_rule_workspace_bytes": _SZ,
+             "rlk_delta_rule_saved_bytes": _SZ, "rlk_head_norms_workspace_bytes": _SZ}
 
 _lib = None
 
@@ -211,3 +246,83 @@ def linear_attention(dev, stream, decay, dones, passes):
 def linear_attention_step(dev, stream, decay, dones, step):
     _native._check((_lib or load()).rlk_linear_attention_step(ctypes.byref(step.struct(decay, dones, None, 0)), stream),
                    "rlk_linear_attention_step")
+
+
+def _delta_rule(q, k, v, out, log_decays, betas, dones, state, state_out, scale, ws):
+    seq = q.shape[1] if q.dim() == 4 else 1
+    return DeltaRule(_sequence(q), _sequence(k), _sequence(v), _sequence(out), q.shape[0], seq, q.shape[-2], q.shape[-1], v.shape[-1],
+                     _ptr(log_decays), betas.data_ptr(), _ptr(dones), _ptr(state), _ptr(state_out), scale, q.dtype is _BF16, _ptr(ws),
+                     _bytes(ws))
+
+
+def _scratch(need, like):
+    """Memory of one call, from torch's allocator: it may be some GB, so none is kept.  (Its later users follow on the stream.)"""
+    return torch.empty(need, dtype=torch.uint8, device=like.device)
+
+
+@_on_device
+def gated_delta_rule(dev, stream, q, k, v, out, log_decays, betas, dones, state, state_out, scale, keep):
+    """Returns what the backward pass reads (`keep`), else None."""
+    lib = _lib or load()
+    e, t, h, dk = q.shape
+    saved = _scratch(lib.rlk_delta_rule_saved_bytes(e, t, h, dk, v.shape[-1]), q) if keep else None
+    ws = None if keep else _scratch(lib.rlk_delta_rule_workspace_bytes(e, t, h, dk, v.shape[-1], 0), q)
+    call = _delta_rule(q, k, v, out, log_decays, betas, dones, state, state_out, scale, ws)
+    _native._check(lib.rlk_gated_delta_rule(ctypes.byref(call), _ptr(saved), _bytes(saved), stream), "rlk_gated_delta_rule")
+    return saved
+
+
+@_on_device
+def gated_delta_rule_backward(dev, stream, q, k, v, log_decays, betas, dones, state, scale, saved, grad_out, grad_last, grads, grad_state):
+    lib = _lib or load()
+    e, t, h, dk = q.shape
+    ws = _scratch(lib.rlk_delta_rule_workspace_bytes(e, t, h, dk, v.shape[-1], 1), q)
+    call = _delta_rule(q, k, v, grad_out, log_decays, betas, dones, state, None, scale, ws)
+    none = Sequence(None, 0, 0, 0)
+    gq, gk, gv, gg, gb = grads
+    to = DeltaRuleGradients(_sequence(grad_out), *(none if g is None else _sequence(g) for g in (gq, gk, gv)), _ptr(grad_last),
+                            _ptr(grad_state), _ptr(gg), _ptr(gb))
+    _native._check(lib.rlk_gated_delta_rule_backward(ctypes.byref(call), ctypes.byref(to), _ptr(saved), _bytes(saved), stream),
+                   "rlk_gated_delta_rule_backward")
+
+
+@_on_device
+def gated_delta_rule_step(dev, stream, q, k, v, out, log_decays, betas, dones, state, state_out, scale):
+    call = _delta_rule(q, k, v, out, log_decays, betas, dones, state, state_out, scale, None)
+    _native._check((_lib or load()).rlk_gated_delta_rule_step(ctypes.byref(call), stream), "rlk_gated_delta_rule_step")
+
+
+@_on_device
+def sample_actions(dev, stream, logits, uniforms, temperature, top_k, top_p, min_p, actions, log_probs):
+    e, t, a = logits.shape
+    se, st, _ = logits.stride()
+    call = Sampling(logits.data_ptr(), e, t, a, se, st, logits.dtype is _BF16, uniforms.data_ptr(), temperature, top_k, top_p, min_p,
+                    actions.data_ptr(), log_probs.data_ptr())
+    _native._check((_lib or load()).rlk_sample_actions(ctypes.byref(call), stream), "rlk_sample_actions")
+
+
+_NONE = Sequence(None, 0, 0, 0)
+
+
+def _head_norms(q, k, q_out, k_out, q_weight, k_weight, positions, base, rotary_dim, eps, interleaved):
+    steps = q.shape[1] if q.dim() == 4 else 1
+    out = [_NONE if t is None else _sequence(t) for t in (q_out, k_out)]
+    return HeadNorms(_sequence(q), _sequence(k), *out, q.shape[0], steps, q.shape[-2], k.shape[-2], q.shape[-1], rotary_dim, interleaved,
+                     q.dtype is _BF16, _ptr(q_weight), _ptr(k_weight), _ptr(positions), base, eps)
+
+
+@_on_device
+def query_key_norms(dev, stream, q, k, q_out, k_out, *settings):
+    call = _head_norms(q, k, q_out, k_out, *settings)
+    _native._check((_lib or load()).rlk_query_key_norms(ctypes.byref(call), stream), "rlk_query_key_norms")
+
+
+@_on_device
+def query_key_norms_backward(dev, stream, q, k, grad_q, grad_k, to_q, to_k, to_q_weight, to_k_weight, *settings):
+    lib = _lib or load()
+    call = _head_norms(q, k, to_q, to_k, *settings)
+    weights = to_q_weight is not None or to_k_weight is not None
+    ws = _scratch(lib.rlk_head_norms_workspace_bytes(ctypes.byref(call)), q) if weights else None
+    up = [_NONE if t is None else _sequence(t) for t in (grad_q, grad_k)]
+    _native._check(lib.rlk_query_key_norms_backward(ctypes.byref(call), *up, _ptr(to_q_weight), _ptr(to_k_weight), _ptr(ws), _bytes(ws),
+                                                    stream), "rlk_query_key_norms_backward")

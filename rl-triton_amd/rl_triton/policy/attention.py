@@ -9,8 +9,8 @@ from rl_triton.policy import _native
 MAX_HEAD_DIM = 128
 
 
-def _check_attention(q, k, v, decay, dones, state, scale, steps):
-    """Checks of both forms; `steps`: the tensors have a seq_len axis.  Returns the scale."""
+def check_heads(q, k, v, dones, state, steps):
+    """Checks of queries, keys, values, episode ends and states; `steps`: the tensors have a seq_len axis."""
     names = "[num_envs, seq_len, heads, dim]" if steps else "[num_envs, heads, dim]"
     assert q.is_cuda, "q must be on CUDA"
     assert q.dtype in (torch.float32, torch.bfloat16), f"q: expected float32 or bfloat16, got {q.dtype}"
@@ -22,10 +22,6 @@ def _check_attention(q, k, v, decay, dones, state, scale, steps):
     assert v.dim() == q.dim() and v.shape[:-1] == q.shape[:-1], f"v shape {v.shape} != q shape {q.shape} but for the last axis"
     for name, t in (("q", q), ("v", v)):
         assert 1 <= t.shape[-1] <= MAX_HEAD_DIM, f"{name}: head dimensions of 1 to {MAX_HEAD_DIM}, got {t.shape[-1]}"
-    envs, heads = q.shape[0], q.shape[-2]
-    assert decay.get_device() == q.get_device() and decay.dtype == torch.float32, "decay must be float32 on the device of q"
-    assert decay.shape == (heads,), f"decay must have shape [{heads}], got {tuple(decay.shape)}"
-    assert not decay.requires_grad, "decay is a constant of the layer: no gradient is computed for it"
     if dones is not None:
         assert dones.get_device() == q.get_device(), "dones must be on the device of q"
         assert dones.dtype in (torch.float32, torch.bfloat16, torch.bool), f"dones: expected float32, bfloat16 or bool, got {dones.dtype}"
@@ -33,8 +29,17 @@ def _check_attention(q, k, v, decay, dones, state, scale, steps):
         assert dones.shape == want, f"dones shape {dones.shape} != {want}"
     if state is not None:
         assert state.get_device() == q.get_device() and state.dtype == torch.float32, "state must be float32 on the device of q"
-        want = (envs, heads, q.shape[-1], v.shape[-1])
+        want = (q.shape[0], q.shape[-2], q.shape[-1], v.shape[-1])
         assert state.shape == want, f"state must have shape {list(want)}, got {list(state.shape)}"
+
+
+def _check_attention(q, k, v, decay, dones, state, scale, steps):
+    """Checks of both forms.  Returns the scale."""
+    check_heads(q, k, v, dones, state, steps)
+    heads = q.shape[-2]
+    assert decay.get_device() == q.get_device() and decay.dtype == torch.float32, "decay must be float32 on the device of q"
+    assert decay.shape == (heads,), f"decay must have shape [{heads}], got {tuple(decay.shape)}"
+    assert not decay.requires_grad, "decay is a constant of the layer: no gradient is computed for it"
     if scale is None:
         scale = q.shape[-1] ** -0.5
     assert isinstance(scale, (int, float)) and math.isfinite(scale) and scale != 0, f"scale must be a number other than 0, got {scale!r}"
@@ -42,6 +47,21 @@ def _check_attention(q, k, v, decay, dones, state, scale, steps):
     if _CORRECTNESS_WARNINGS():
         assert bool(((decay >= 0) & (decay <= 1)).all()), "decay must lie in [0, 1]"
     return float(scale)
+
+
+def check_out_state(state, out_state):
+    """Where a step writes its state: a new tensor, or `out_state` once it is known to be fit for it."""
+    assert state.is_contiguous(), "state must be contiguous"
+    if out_state is None:
+        return torch.empty(state.shape, dtype=state.dtype, device=state.device)
+    assert out_state.get_device() == state.get_device() and out_state.dtype == torch.float32 and \
+        out_state.shape == state.shape and out_state.is_contiguous(), "out_state must be a contiguous float32 tensor like state"
+    apart = abs(out_state.data_ptr() - state.data_ptr())
+    assert apart == 0 or apart >= 4 * state.numel(), "out_state overlaps state without being it"
+    if torch.is_grad_enabled() and out_state.requires_grad:
+        raise RuntimeError("out_state requires a gradient and cannot be written over")
+    torch.autograd.graph.increment_version(out_state)  # (a graph that saved what it held has to know)
+    return out_state
 
 
 def _dones(dones):
@@ -203,17 +223,7 @@ def compute_linear_attention_step(
     """
     assert state is not None, "state is required"
     scale = _check_attention(q, k, v, decay, dones, state, scale, False)
-    assert state.is_contiguous(), "state must be contiguous"
-    if out_state is None:
-        out_state = torch.empty(state.shape, dtype=state.dtype, device=state.device)
-    else:
-        assert out_state.get_device() == state.get_device() and out_state.dtype == torch.float32 and \
-            out_state.shape == state.shape and out_state.is_contiguous(), "out_state must be a contiguous float32 tensor like state"
-        apart = abs(out_state.data_ptr() - state.data_ptr())
-        assert apart == 0 or apart >= 4 * state.numel(), "out_state overlaps state without being it"
-        if torch.is_grad_enabled() and out_state.requires_grad:
-            raise RuntimeError("out_state requires a gradient and cannot be written over")
-        torch.autograd.graph.increment_version(out_state)  # (a graph that saved what it held has to know)
+    out_state = check_out_state(state, out_state)
     out = torch.empty(v.shape, dtype=v.dtype, device=v.device)
     if q.shape[0] and q.shape[1]:
         _native.linear_attention_step(decay.contiguous(), _dones(dones),
