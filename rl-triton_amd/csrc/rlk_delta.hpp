@@ -120,51 +120,76 @@ __device__ __forceinline__ Op<N> split(f32x4 a, f32x4 b) {
   return o;
 }
 
+// A number that the compiler takes for a new one: places that are formed from it are formed where they are used, not once before a loop and
+// held in registers for all of it.
+__device__ __forceinline__ int opaque(int x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
+
 // ---- tiles in LDS: parts of bfloat16, row by row.
 template <class E, int D>
 struct Tile {
   static constexpr int N = kParts<E>, ROW = 2 * D + 16, PART = C * ROW, BYTES = N * PART;
-  static __device__ int row(int i) { return i * ROW; }
+  static constexpr __host__ __device__ int row(int i) { return i * ROW; }
 };
 // A lower triangular matrix of a chunk's steps, of N parts: rows 0 .. 31 have 32 columns, the others 64.
 template <int N_>
 struct Tri {
   static constexpr int N = N_, PART = 32 * 80 + 32 * 144, BYTES = N * PART;
-  static __device__ int row(int i) { return i < 32 ? i * 80 : 32 * 80 + (i - 32) * 144; }
+  static constexpr __host__ __device__ int row(int i) { return i < 32 ? i * 80 : 32 * 80 + (i - 32) * 144; }
 };
 
-// Lane's part of the operand whose rows are the tile's rows 16 t .., inner indices its columns 32 kk ...
-template <class T>
-__device__ __forceinline__ Op<T::N> rows_of(const char* tile, int t, int kk) {
-  const int lane = threadIdx.x & 63, l16 = lane & 15, l4 = lane >> 4;
-  Op<T::N> o;
-#pragma unroll
-  for (int i = 0; i < T::N; ++i) {
-    const char* p = tile + i * T::PART + T::row(16 * t) + l16 * (T::row(16 * t + 1) - T::row(16 * t)) + 64 * kk + 8 * l4;
-    union { u32x2 h[2]; bf16x8 v; } u;
-    u.h[0] = *reinterpret_cast<const u32x2*>(p), u.h[1] = *reinterpret_cast<const u32x2*>(p + 32);
-    o.p[i] = u.v;
-  }
-  return o;
-}
-// ... whose rows are the tile's columns 16 t .., inner indices its rows 32 kk ..: read across by the LDS itself.
 __device__ __forceinline__ u32x2 read_across(const char* p) {
   return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p));
 }
-template <class T>
-__device__ __forceinline__ Op<T::N> columns_of(const char* tile, int t, int kk) {
-  const int lane = threadIdx.x & 63, l16 = lane & 15, l4 = lane >> 4;
-  const int stride = T::row(32 * kk + 1) - T::row(32 * kk);
-  Op<T::N> o;
-#pragma unroll
-  for (int i = 0; i < T::N; ++i) {
-    const char* p = tile + i * T::PART + T::row(32 * kk) + (4 * l4 + (l16 >> 2)) * stride + 32 * t + 8 * (l16 & 3);
-    union { u32x2 h[2]; bf16x8 v; } u;
-    u.h[0] = read_across(p), u.h[1] = read_across(p + 16 * stride);
-    o.p[i] = u.v;
+// A lane's places in tiles, formed once.  Opaque, or the compiler would fold tiles' places into an address of its own for every access
+// and hold them all.
+struct Places {
+  int l16, l4;     // (of the operand: row l16, quarter l4)
+  int quarter;     // in a row: 8 bytes of it
+  int across_row, across_col;  // read across: 4 rows of 16 columns, a lane 4 of them
+  __device__ Places() {
+    const int lane = threadIdx.x & 63;
+    l16 = lane & 15, l4 = lane >> 4;
+    quarter = 8 * l4, across_row = 4 * l4 + (l16 >> 2), across_col = 8 * (l16 & 3);
   }
-  return o;
-}
+};
+template <class T>
+struct At {
+  static constexpr int FIRST = T::row(1), SECOND = T::row(33) - T::row(32);  // bytes from row to row of the first 32 and of the others
+  static constexpr bool ONE = FIRST == SECOND;
+  int row[2], col[2];
+  __device__ At() {
+    const Places p;
+    row[0] = opaque(p.l16 * FIRST + p.quarter), col[0] = opaque(p.across_row * FIRST + p.across_col);
+    row[1] = ONE ? row[0] : opaque(p.l16 * SECOND + p.quarter), col[1] = ONE ? col[0] : opaque(p.across_row * SECOND + p.across_col);
+  }
+  // The operand whose rows are the tile's rows 16 t .., inner indices its columns 32 kk ..
+  __device__ __forceinline__ Op<T::N> rows(const char* tile, int t, int kk) const {
+    Op<T::N> o;
+#pragma unroll
+    for (int i = 0; i < T::N; ++i) {
+      const char* p = tile + (ONE || t < 2 ? row[0] : row[1]) + (i * T::PART + T::row(16 * t) + 64 * kk);
+      union { u32x2 h[2]; bf16x8 v; } u;
+      u.h[0] = *reinterpret_cast<const u32x2*>(p), u.h[1] = *reinterpret_cast<const u32x2*>(p + 32);
+      o.p[i] = u.v;
+    }
+    return o;
+  }
+  // ... whose rows are the tile's columns 16 t .., inner indices its rows 32 kk ..: read across by the LDS itself.
+  __device__ __forceinline__ Op<T::N> columns(const char* tile, int t, int kk) const {
+    Op<T::N> o;
+#pragma unroll
+    for (int i = 0; i < T::N; ++i) {
+      const char* p = tile + (ONE || kk == 0 ? col[0] : col[1]) + (i * T::PART + T::row(32 * kk) + 32 * t);
+      union { u32x2 h[2]; bf16x8 v; } u;
+      u.h[0] = read_across(p), u.h[1] = read_across(p + 16 * (kk ? SECOND : FIRST));
+      o.p[i] = u.v;
+    }
+    return o;
+  }
+};
 // The number at a tile's row and column.
 template <class T>
 __device__ __forceinline__ float number_at(const char* tile, int i, int d) {
@@ -200,42 +225,60 @@ struct Four<float> {
   __device__ void set(int i, float x) { w[i] = x; }
   __device__ f32x4 floats() const { return w; }
 };
-// The 4 elements from column `col` of a row on, of `dim`; those beyond are 0.
+// The 4 elements from column `col` of a row on, of `dim`.  What lies beyond is read from a place that exists and cleared when it is used: a
+// choice made here would wait for the load.
 template <class E, bool VEC>
 __device__ __forceinline__ Four<E> four(const E* row, int col, int dim) {
   Four<E> x;
   if constexpr (VEC) {
     x = *reinterpret_cast<const Four<E>*>(row + (col < dim ? col : 0));
-    if (col >= dim) x.clear();
   } else {
     x.clear();
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (col + i < dim) x.set(i, row[col + i]);
+    for (int i = 0; i < 4; ++i) x.set(i, row[col + i < dim ? col + i : 0]);
   }
   return x;
+}
+template <class E, bool VEC>
+__device__ __forceinline__ void clip(Four<E>& x, int col, int dim, bool row) {
+  if (!row || col >= dim) x.clear();
+  if constexpr (!VEC) {
+    const E zero = from_f32<E>(0.f);
+#pragma unroll
+    for (int i = 1; i < 4; ++i)
+      if (col + i >= dim) x.set(i, zero);
+  }
 }
 
 // A chunk's rows of an array on their way to a tile: NT threads, each 4 elements of 64 * D / 4 / NT rows.
 template <class E, int D, int NT, bool VEC>
 struct Rows {
   static constexpr int PER = C * D / 4 / NT, GROUPS = D / 4;
+  static constexpr int APART = NT / GROUPS;  // rows from one of a thread's to the next
   Four<E> x[PER];
-  __device__ void fetch(const E* first, int64_t step, int dim, int count) {
+  __device__ __forceinline__ void fetch(const E* first, int64_t step, int dim, int count) {
+    const int tid = opaque(threadIdx.x), r0 = tid / GROUPS, col = tid % GROUPS * 4;
+    if (count == C) {
+      const E* p = first + r0 * step;
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const int u = threadIdx.x + NT * i, r = u / GROUPS;
-      x[i] = four<E, VEC>(first + (r < count ? r : count - 1) * step, u % GROUPS * 4, dim);
+      for (int i = 0; i < PER; ++i) x[i] = four<E, VEC>(p + i * APART * step, col, dim);
+    } else {
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        const int r = r0 + APART * i;
+        x[i] = four<E, VEC>(first + (r < count ? r : count - 1) * step, col, dim);
+      }
     }
   }
   // rows [from, to) as they are, the others 0
-  __device__ void put(char* tile, int from, int to) {
+  __device__ __forceinline__ void put(char* tile, int dim, int from, int to) const {
+    const int tid = opaque(threadIdx.x), r0 = tid / GROUPS, col = tid % GROUPS * 4;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      const int u = threadIdx.x + NT * i, r = u / GROUPS;
+      const int r = r0 + APART * i;
       Four<E> y = x[i];
-      if (r < from || r >= to) y.clear();
-      y.put(tile + Tile<E, D>::row(r) + u % GROUPS * 8, Tile<E, D>::PART);
+      clip<E, VEC>(y, col, dim, r >= from && r < to);
+      y.put(tile + Tile<E, D>::row(r) + col * 2, Tile<E, D>::PART);
     }
   }
 };
@@ -255,6 +298,9 @@ __device__ __forceinline__ void wave_sync() {
   __builtin_amdgcn_wave_barrier();
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
+
+// Loads of operands are kept from moving up over this: held too early they fill the registers.
+__device__ __forceinline__ void apart() { __builtin_amdgcn_sched_barrier(0); }
 
 __device__ __forceinline__ bool finite(float x) { return fabsf(x) <= 3.402823466e38f; }
 

@@ -85,6 +85,10 @@ __global__ __launch_bounds__(4 * D, D == 128 || kParts<E> == 1 ? 2 : 1) void gra
   const float *w = r.w + at * C * dvp, *z = r.z + at * C * dvp;
   const int64_t state = at * pad16(dk) * dvp;
   const bool mine = 16 * wave < dk;
+  const At<typename M::G> at_g;
+  const At<typename M::U> at_u;
+  const At<T> at_k;
+  const At<typename M::Y> at_y;
 
   // transposed results: step 16 t + l16, dims 16 wave + 4 l4 + 0..3
   f32x4 dq[4], up[4], down[4];  // (up, down: dk+ and dk-)
@@ -109,7 +113,7 @@ __global__ __launch_bounds__(4 * D, D == 128 || kParts<E> == 1 ? 2 : 1) void gra
     ws.fetch(w, c0, dvp);
     zs.fetch(z, c0, dvp);
     if (c0 > 0) __syncthreads();
-    gs.put(lds, 0, n);
+    gs.put(lds, dv - c0, 0, n);
     if (c0 == 0) __syncthreads();  // (beta is there)
     ws.put(lds + M::UT, beta);
     zs.put(lds + M::DT, beta);
@@ -121,12 +125,12 @@ __global__ __launch_bounds__(4 * D, D == 128 || kParts<E> == 1 ? 2 : 1) void gra
     const int kks = dv - c0 > 32 ? 2 : 1;
     for (int kk = 0; kk < kks; ++kk) {
       {
-        const Op<N> g = rows_of<typename M::G>(lds, ti, kk);
-        const Op<3> d = rows_of<typename M::U>(lds + M::DT, ti, kk);
+        const Op<N> g = at_g.rows(lds, ti, kk);
+        const Op<3> d = at_u.rows(lds + M::DT, ti, kk);
 #pragma unroll
         for (int tj = 0; tj < 4; ++tj) {
           if (tj > ti) continue;
-          const Op<3> u = rows_of<typename M::U>(lds + M::UT, tj, kk);
+          const Op<3> u = at_u.rows(lds + M::UT, tj, kk);
           if constexpr (BOTH) {
             ya[tj] = mul<2>(u, g, ya[tj]);
             yb[tj] = mul<2>(u, d, yb[tj]);
@@ -150,9 +154,9 @@ __global__ __launch_bounds__(4 * D, D == 128 || kParts<E> == 1 ? 2 : 1) void gra
         const Op<3> s = split<3>(a, b), rr = split<3>(e, f);
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
-          dq[t] = mul<2>(s, rows_of<typename M::G>(lds, t, kk), dq[t]);
-          up[t] = mul<2>(s, rows_of<typename M::U>(lds + M::DT, t, kk), up[t]);
-          down[t] = mul<2>(rr, rows_of<typename M::U>(lds + M::UT, t, kk), down[t]);
+          dq[t] = mul<2>(s, at_g.rows(lds, t, kk), dq[t]);
+          up[t] = mul<2>(s, at_u.rows(lds + M::DT, t, kk), up[t]);
+          down[t] = mul<2>(rr, at_u.rows(lds + M::UT, t, kk), down[t]);
         }
       }
       settle();
@@ -219,8 +223,8 @@ __global__ __launch_bounds__(4 * D, D == 128 || kParts<E> == 1 ? 2 : 1) void gra
       to = later != 0 ? __ffsll((long long)later) - 1 : n;
     }
     if (from > 0) __syncthreads();
-    k.put(lds, from, to);
-    q.put(lds + M::QT, from, to);
+    k.put(lds, dk, from, to);
+    q.put(lds + M::QT, dk, from, to);
     __syncthreads();
     float total = 0.f;
     if (mine) {
@@ -237,14 +241,14 @@ __global__ __launch_bounds__(4 * D, D == 128 || kParts<E> == 1 ? 2 : 1) void gra
         f32x4 a = dq[t], b = up[t], c = down[t];
 #pragma unroll
         for (int kk = 0; kk < 2; ++kk) {
-          const Op<N> kc = columns_of<T>(lds, wave, kk), qc = columns_of<T>(lds + M::QT, wave, kk);
+          const Op<N> kc = at_k.columns(lds, wave, kk), qc = at_k.columns(lds + M::QT, wave, kk);
           if (kk <= t / 2) {
-            a = mul<2>(kc, rows_of<typename M::Y>(lds + M::Y1, t, kk), a);
-            b = mul<2>(kc, rows_of<typename M::Y>(lds + M::Y2, t, kk), b);
+            a = mul<2>(kc, at_y.rows(lds + M::Y1, t, kk), a);
+            b = mul<2>(kc, at_y.rows(lds + M::Y2, t, kk), b);
           }
           if (kk >= t / 2) {
-            c = mul<2>(qc, columns_of<typename M::Y>(lds + M::Y1, t, kk), c);
-            c = mul<2>(kc, columns_of<typename M::Y>(lds + M::Y2, t, kk), c);
+            c = mul<2>(qc, at_y.columns(lds + M::Y1, t, kk), c);
+            c = mul<2>(kc, at_y.columns(lds + M::Y2, t, kk), c);
           }
         }
         settle();

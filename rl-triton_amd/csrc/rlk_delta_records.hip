@@ -77,7 +77,8 @@ __global__ __launch_bounds__(64 * kWaves) void records_kernel(const Rule<E> r, i
       const int row = 16 * t + l16;
       const E* p = keys + (row < n ? row : n - 1) * r.k.step;
       Four<E> a = four<E, VEC>(p, d0 + 8 * l4, r.dk), b = four<E, VEC>(p, d0 + 8 * l4 + 4, r.dk);
-      if (row >= n) a.clear(), b.clear();
+      clip<E, VEC>(a, d0 + 8 * l4, r.dk, row < n);
+      clip<E, VEC>(b, d0 + 8 * l4 + 4, r.dk, row < n);
       if constexpr (kParts<E> == 1) {
         union { u32x2 h[2]; bf16x8 v; } u;
         u.h[0] = a.w, u.h[1] = b.w;

@@ -29,7 +29,7 @@ struct Shared {
   Rows<E, D, NT, VEC> k, q;
   f32x4 m[TILES_PER], rest_quad;
 
-  __device__ void fetch(const Rule<E>& r, int64_t env, int head, int64_t pair, int64_t chunk) {
+  __device__ __forceinline__ void fetch(const Rule<E>& r, int64_t env, int head, int64_t pair, int64_t chunk) {
     const int64_t s0 = chunk * C;
     const int n = (int)(r.seq_len - s0 < C ? r.seq_len - s0 : C);
     k.fetch(r.k.data + env * r.k.env + head * r.k.head + s0 * r.k.step, r.k.step, r.dk, n);
@@ -42,9 +42,9 @@ struct Shared {
     }
     rest_quad = rec[TILE_QUADS + (threadIdx.x < REST_QUADS ? threadIdx.x : 0)];
   }
-  __device__ void put(char* lds, int n) {
-    k.put(lds + M::K, 0, n);
-    q.put(lds + M::Q, 0, n);
+  __device__ __forceinline__ void put(char* lds, int dk, int n) const {
+    k.put(lds + M::K, dk, 0, n);
+    q.put(lds + M::Q, dk, 0, n);
 #pragma unroll
     for (int i = 0; i < TILES_PER; ++i) {
       const int u = threadIdx.x + NT * i;
@@ -60,7 +60,7 @@ struct Shared {
   __device__ static const Record& record(const char* lds) { return *reinterpret_cast<const Record*>(lds + M::REST - offsetof(Record, ghi)); }
 
   // P_ij = scale D_ij q_i . k_j.  Wavefronts share the 16 rows ti; computed transposed, so that a lane holds 4 consecutive j.
-  __device__ static void form_p(char* lds, float scale) {
+  __device__ static void form_p(char* lds, float scale, const At<typename M::Rows_>& at) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l16 = lane & 15, l4 = lane >> 4;
     constexpr int SHARE = D / 64;
     const Record& rec = record(lds);
@@ -73,7 +73,7 @@ struct Shared {
     for (int tj = wave % SHARE; tj <= upto; tj += SHARE) {
       f32x4 x = zero4();
 #pragma unroll
-      for (int kk = 0; kk < D / 32; ++kk) x = mul<2>(rows_of<typename M::Rows_>(lds + M::K, tj, kk), rows_of<typename M::Rows_>(lds + M::Q, ti, kk), x);
+      for (int kk = 0; kk < D / 32; ++kk) x = mul<2>(at.rows(lds + M::K, tj, kk), at.rows(lds + M::Q, ti, kk), x);
       settle();
       const f32x4 hj = *reinterpret_cast<const f32x4*>(rec.ghi + 16 * tj + 4 * l4), lj = *reinterpret_cast<const f32x4*>(rec.glo + 16 * tj + 4 * l4);
 #pragma unroll
@@ -120,30 +120,58 @@ __device__ __forceinline__ void load_state(const float* p, int dk, int dv, bool 
   }
 }
 template <int MT>
-__device__ __forceinline__ void store_state(float* p, int columns, int rows, bool none, const f32x4 (&S)[MT]) {
+__device__ __forceinline__ void store_state(float* p, int dk, int dv, bool none, const f32x4 (&S)[MT]) {
   const int lane = threadIdx.x & 63, l4 = lane >> 4, j = 16 * (threadIdx.x >> 6) + (lane & 15);
-  if (j >= columns) return;
+  if (j >= dv) return;
 #pragma unroll
   for (int m = 0; m < MT; ++m)
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const int d = 16 * m + 4 * l4 + e;
-      if (d < rows) p[d * columns + j] = none ? 0.f : S[m][e];
+      if (d < dk) p[d * dv + j] = none ? 0.f : S[m][e];
     }
+}
+// ... into the workspace, [rows, columns] of whole tiles.
+template <int MT>
+__device__ __forceinline__ void keep_state(float* p, int columns, int rows, const f32x4 (&S)[MT]) {
+  const int tid = opaque(threadIdx.x), lane = tid & 63;
+  p += 4 * (lane >> 4) * columns + 16 * (tid >> 6) + (lane & 15);
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+    if (16 * m < rows)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) p[(16 * m + e) * columns] = S[m][e];
+}
+// ... a chunk's rows of a wavefront's columns.
+__device__ __forceinline__ void keep_columns(float* p, int columns, const f32x4 (&x)[4]) {
+  const int tid = opaque(threadIdx.x), lane = tid & 63;
+  p += 4 * (lane >> 4) * columns + 16 * (tid >> 6) + (lane & 15);
+#pragma unroll
+  for (int t = 0; t < 4; ++t)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) p[(16 * t + e) * columns] = x[t][e];
 }
 
 // A wavefront's 16 columns of an array's chunk: column 16 wave + l16, rows 16 t + 4 l4 + 0..3.
 template <class E>
 __device__ __forceinline__ void load_columns(const E* first, int64_t step, int dim, int n, E (&x)[16]) {
-  const int lane = threadIdx.x & 63, l4 = lane >> 4, j = 16 * (threadIdx.x >> 6) + (lane & 15);
+  const int tid = opaque(threadIdx.x), lane = tid & 63, l4 = lane >> 4, j = 16 * (tid >> 6) + (lane & 15);
   const E* p = first + (j < dim ? j : dim - 1);
+  if (n == C) {
+    p += 4 * l4 * step;
 #pragma unroll
-  for (int t = 0; t < 4; ++t)
+    for (int t = 0; t < 4; ++t)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int i = 16 * t + 4 * l4 + e;
-      x[4 * t + e] = p[(i < n ? i : n - 1) * step];
-    }
+      for (int e = 0; e < 4; ++e) x[4 * t + e] = p[(16 * t + e) * step];
+  } else {
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int i = 16 * t + 4 * l4 + e;
+        x[4 * t + e] = p[(i < n ? i : n - 1) * step];
+      }
+  }
 }
 // ... as numbers, 0 where there is nothing.
 template <class E>
@@ -170,6 +198,9 @@ __global__ __launch_bounds__(4 * D, D == 128 || kParts<E> == 1 ? 2 : 1) void for
   const E* gv = r.v.data + env * r.v.env + head * r.v.head;
   E* gy = r.y.data + env * r.y.env + head * r.y.head;
 
+  const At<T> at;
+  const At<typename M::M> at_m;
+  const At<typename M::P> at_p;
   Sh sh;
   E v[16];
   sh.fetch(r, env, head, pair, 0);
@@ -180,10 +211,10 @@ __global__ __launch_bounds__(4 * D, D == 128 || kParts<E> == 1 ? 2 : 1) void for
   for (int64_t chunk = 0; chunk < r.chunks; ++chunk) {
     const int64_t s0 = chunk * C;
     const int n = (int)(r.seq_len - s0 < C ? r.seq_len - s0 : C);
-    sh.put(lds, n);
+    sh.put(lds, dk, n);
     __syncthreads();
     if (chunk + 1 < r.chunks) sh.fetch(r, env, head, pair, chunk + 1);
-    Sh::form_p(lds, r.scale);
+    Sh::form_p(lds, r.scale, at);
     const Record& rec = Sh::record(lds);
 
     f32x4 e[4], y[4];  // corrections (column j, steps 16 t + 4 l4 + ..); outputs, transposed (step 16 t + l16, columns 16 wave + 4 l4 + ..)
@@ -197,8 +228,9 @@ __global__ __launch_bounds__(4 * D, D == 128 || kParts<E> == 1 ? 2 : 1) void for
         const Op<3> s = split<3>(S[2 * kk], S[2 * kk + 1]);
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
-          ks[t] = mul<2>(rows_of<T>(lds + M::K, t, kk), s, ks[t]);
-          y[t] = mul<UPTO>(s, rows_of<T>(lds + M::Q, t, kk), y[t]);
+          ks[t] = mul<2>(at.rows(lds + M::K, t, kk), s, ks[t]);
+          y[t] = mul<UPTO>(s, at.rows(lds + M::Q, t, kk), y[t]);
+          if (t & 1) apart();
         }
       }
       f32x4 be[4];
@@ -221,8 +253,9 @@ __global__ __launch_bounds__(4 * D, D == 128 || kParts<E> == 1 ? 2 : 1) void for
       for (int t = 0; t < 4; ++t) {
         f32x4 mb = zero4();
 #pragma unroll
-        for (int kk = 0; kk <= t / 2; ++kk) mb = mul<2>(rows_of<typename M::M>(lds + M::MT, t, kk), b[kk], mb);
+        for (int kk = 0; kk <= t / 2; ++kk) mb = mul<2>(at_m.rows(lds + M::MT, t, kk), b[kk], mb);
         e[t] -= mb;
+        apart();
       }
 #pragma unroll
       for (int t = 0; t < 4; ++t) be[t] = e[t] * *reinterpret_cast<const f32x4*>(rec.beta + 16 * t + 4 * l4);
@@ -238,12 +271,12 @@ __global__ __launch_bounds__(4 * D, D == 128 || kParts<E> == 1 ? 2 : 1) void for
 #pragma unroll
       for (int t = 0; t < 4; ++t)
 #pragma unroll
-        for (int kk = 0; kk <= t / 2; ++kk) y[t] = mul<UPTO>(uo[kk], rows_of<typename M::P>(lds + M::PT, t, kk), y[t]);
+        for (int kk = 0; kk <= t / 2; ++kk) y[t] = mul<UPTO>(uo[kk], at_p.rows(lds + M::PT, t, kk), y[t]);
       float check = 0.f;
 #pragma unroll
       for (int t = 0; t < 4; ++t) check = odd(e[t], odd(y[t], check));
-      if (r.states != nullptr) store_state(r.states + (pair * r.chunks + chunk) * (int64_t)pad16(dk) * dvp, dvp, pad16(dk), false, S);
-      float* w = r.w != nullptr ? r.w + (pair * r.chunks + chunk) * (int64_t)C * dvp + j : nullptr;
+      if (r.states != nullptr) keep_state(r.states + (pair * r.chunks + chunk) * (int64_t)pad16(dk) * dvp, dvp, pad16(dk), S);
+      float* w = r.w != nullptr ? r.w + (pair * r.chunks + chunk) * (int64_t)C * dvp : nullptr;
       settle();
       if (rec.wild == 0 && __all(check == 0.f)) {
 #pragma unroll
@@ -259,10 +292,8 @@ __global__ __launch_bounds__(4 * D, D == 128 || kParts<E> == 1 ? 2 : 1) void for
                 if (c + x < dv) p[x] = from_f32<E>(y[t][x]);
             }
           }
-          if (w != nullptr)
-#pragma unroll
-            for (int x = 0; x < 4; ++x) w[(16 * t + 4 * l4 + x) * dvp] = e[t][x];
         }
+        if (w != nullptr) keep_columns(w, dvp, e);
         // S' = keep S + sum_j into_j k_j u_j^T
         f32x4 x[4];
 #pragma unroll
@@ -274,12 +305,14 @@ __global__ __launch_bounds__(4 * D, D == 128 || kParts<E> == 1 ? 2 : 1) void for
 #pragma unroll
           for (int z = 0; z < 4; ++z) S[m][z] = keep != 0.f ? S[m][z] * keep : 0.f;
 #pragma unroll
-          for (int kk = 0; kk < 2; ++kk) S[m] = mul<2>(columns_of<T>(lds + M::K, m, kk), a[kk], S[m]);
+          for (int kk = 0; kk < 2; ++kk) S[m] = mul<2>(at.columns(lds + M::K, m, kk), a[kk], S[m]);
+          if (m & 1) apart();
         }
         settle();
       } else {
         // step by step: what is not finite reaches no step before it, and none past its episode's end
         for (int i = 0; i < n; ++i) {
+          const int l16 = opaque(lane & 15), l4 = opaque(lane >> 4), j = 16 * wave + l16;
           const int64_t s = s0 + i;
           const float a = gate(r, env, head, s), b = r.betas[(env * r.seq_len + s) * r.heads + head];
           float sum = 0.f;
@@ -309,17 +342,17 @@ __global__ __launch_bounds__(4 * D, D == 128 || kParts<E> == 1 ? 2 : 1) void for
           out += __shfl_xor(out, 32);
           if (l4 == 0) {
             if (j < dv) gy[s * r.y.step + j] = from_f32<E>(out * r.scale);
-            if (w != nullptr) w[i * dvp] = c;
+            if (w != nullptr) w[i * dvp + j] = c;
           }
         }
         if (w != nullptr && l4 == 0)
-          for (int i = n; i < C; ++i) w[i * dvp] = 0.f;
+          for (int i = n; i < C; ++i) w[i * dvp + j] = 0.f;
       }
     }
     __syncthreads();
   }
   if (mine && r.state_out != nullptr)
-    store_state(r.state_out + eh * dk * dv, dv, dk, r.dones != nullptr && r.dones[env * r.seq_len + r.seq_len - 1] != 0.f, S);
+    store_state(r.state_out + eh * dk * dv, dk, dv, r.dones != nullptr && r.dones[env * r.seq_len + r.seq_len - 1] != 0.f, S);
 }
 
 // The way back: R, the gradient of the state, from the last chunk to the first.
@@ -338,6 +371,9 @@ __global__ __launch_bounds__(4 * D, D == 128 || kParts<E> == 1 ? 2 : 1) void bac
   const E* gg = r.gy.data + env * r.gy.env + head * r.gy.head;
   E* gv = r.gv.data + env * r.gv.env + head * r.gv.head;
 
+  const At<T> at;
+  const At<typename M::M> at_m;
+  const At<typename M::P> at_p;
   Sh sh;
   E g[16];
   const int64_t last = r.chunks - 1;
@@ -349,10 +385,10 @@ __global__ __launch_bounds__(4 * D, D == 128 || kParts<E> == 1 ? 2 : 1) void bac
   for (int64_t chunk = last; chunk >= 0; --chunk) {
     const int64_t s0 = chunk * C;
     const int n = (int)(r.seq_len - s0 < C ? r.seq_len - s0 : C);
-    sh.put(lds, n);
+    sh.put(lds, dk, n);
     __syncthreads();
     if (chunk > 0) sh.fetch(r, env, head, pair, chunk - 1);
-    Sh::form_p(lds, r.scale);
+    Sh::form_p(lds, r.scale, at);
     const Record& rec = Sh::record(lds);
 
     f32x4 z[4];
@@ -363,7 +399,10 @@ __global__ __launch_bounds__(4 * D, D == 128 || kParts<E> == 1 ? 2 : 1) void bac
       for (int kk = 0; kk < KK; ++kk) {
         const Op<3> s = split<3>(R[2 * kk], R[2 * kk + 1]);
 #pragma unroll
-        for (int t = 0; t < 4; ++t) z[t] = mul<2>(rows_of<T>(lds + M::K, t, kk), s, z[t]);
+        for (int t = 0; t < 4; ++t) {
+          z[t] = mul<2>(at.rows(lds + M::K, t, kk), s, z[t]);
+          if (t & 1) apart();
+        }
       }
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
@@ -382,7 +421,7 @@ __global__ __launch_bounds__(4 * D, D == 128 || kParts<E> == 1 ? 2 : 1) void bac
 #pragma unroll
         for (int t = 0; t < 4; ++t)
 #pragma unroll
-          for (int kk = t / 2; kk < 2; ++kk) z[t] = mul<2>(columns_of<typename M::P>(lds + M::PT, t, kk), a[kk], z[t]);
+          for (int kk = t / 2; kk < 2; ++kk) z[t] = mul<2>(at_p.columns(lds + M::PT, t, kk), a[kk], z[t]);
       }
       f32x4 x[4];
       {
@@ -393,8 +432,9 @@ __global__ __launch_bounds__(4 * D, D == 128 || kParts<E> == 1 ? 2 : 1) void bac
         for (int t = 0; t < 4; ++t) {
           f32x4 mb = zero4();
 #pragma unroll
-          for (int kk = t / 2; kk < 2; ++kk) mb = mul<2>(columns_of<typename M::M>(lds + M::MT, t, kk), a[kk], mb);
+          for (int kk = t / 2; kk < 2; ++kk) mb = mul<2>(at_m.columns(lds + M::MT, t, kk), a[kk], mb);
           z[t] -= mb;
+          apart();
         }
       }
       // the state's gradient before the chunk
@@ -420,13 +460,14 @@ __global__ __launch_bounds__(4 * D, D == 128 || kParts<E> == 1 ? 2 : 1) void bac
           for (int i = 0; i < 4; ++i) next[m][i] = keep != 0.f ? R[m][i] * keep : 0.f;
 #pragma unroll
           for (int kk = 0; kk < 2; ++kk) {
-            next[m] = mul<2>(columns_of<T>(lds + M::K, m, kk), a[kk], next[m]);
-            next[m] = mul<2>(columns_of<T>(lds + M::Q, m, kk), b[kk], next[m]);
+            next[m] = mul<2>(at.columns(lds + M::K, m, kk), a[kk], next[m]);
+            next[m] = mul<2>(at.columns(lds + M::Q, m, kk), b[kk], next[m]);
           }
+          apart();
         }
       }
-      if (r.dstates != nullptr) store_state(r.dstates + (pair * r.chunks + chunk) * (int64_t)pad16(dk) * dvp, dvp, pad16(dk), false, R);
-      float* gz = r.z + (pair * r.chunks + chunk) * (int64_t)C * dvp + j;
+      if (r.dstates != nullptr) keep_state(r.dstates + (pair * r.chunks + chunk) * (int64_t)pad16(dk) * dvp, dvp, pad16(dk), R);
+      float* gz = r.z + (pair * r.chunks + chunk) * (int64_t)C * dvp;
       float check = 0.f;
 #pragma unroll
       for (int t = 0; t < 4; ++t) check = odd(z[t], check);
@@ -439,13 +480,14 @@ __global__ __launch_bounds__(4 * D, D == 128 || kParts<E> == 1 ? 2 : 1) void bac
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int s = 16 * t + 4 * l4 + i;
-            gz[s * dvp] = z[t][i];
             if (r.gv.data != nullptr && s < n && j < dv) gv[(s0 + s) * r.gv.step + j] = from_f32<E>(dvs[t][i]);
           }
+        keep_columns(gz, dvp, z);
 #pragma unroll
         for (int m = 0; m < MT; ++m) R[m] = next[m];
       } else {
         for (int i = n - 1; i >= 0; --i) {
+          const int l16 = opaque(lane & 15), l4 = opaque(lane >> 4), j = 16 * wave + l16;
           const int64_t s = s0 + i;
           const float a = gate(r, env, head, s), b = r.betas[(env * r.seq_len + s) * r.heads + head];
           const float up = j < dv ? r.scale * to_f32(gg[s * r.gy.step + j]) : 0.f;
@@ -471,18 +513,18 @@ __global__ __launch_bounds__(4 * D, D == 128 || kParts<E> == 1 ? 2 : 1) void bac
               R[m][x] = a == 0.f ? 0.f : R[m][x] * a;
             }
           if (l4 == 0) {
-            gz[i * dvp] = sum;
+            gz[i * dvp + j] = sum;
             if (r.gv.data != nullptr && j < dv) gv[s * r.gv.step + j] = from_f32<E>(b * sum);
           }
         }
         if (l4 == 0)
-          for (int i = n; i < C; ++i) gz[i * dvp] = 0.f;
+          for (int i = n; i < C; ++i) gz[i * dvp + j] = 0.f;
       }
     }
     __syncthreads();
     if (mine && chunk > 0) load_columns(gg + (s0 - C) * r.gy.step, r.gy.step, dv, C, g);
   }
-  if (mine && r.state_out != nullptr) store_state(r.state_out + eh * dk * dv, dv, dk, false, R);
+  if (mine && r.state_out != nullptr) store_state(r.state_out + eh * dk * dv, dk, dv, false, R);
 }
 
 }  // namespace
