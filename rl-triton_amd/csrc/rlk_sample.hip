@@ -6,8 +6,9 @@
 // 2^20 actions is below 2^-24, a float32 uniform number's last bit.
 //
 // Truncations keep a beginning of the actions in the order (logit falling, number rising): what is kept is told by comparing with its last
-// member.  Rows of up to 64 actions: a lane per action compares itself with all others.  Longer rows: a workgroup finds the last member's
-// place from a histogram of the distances to the maximum, counts and weights added up in LDS, and in its bucket by bisection.
+// member.  Rows of up to 64 actions: a lane per action compares itself with all others.  Longer rows, a workgroup each: of a small top_k
+// it lists the candidates and compares them as above; else it finds the last member's place from a histogram of the distances
+// to the maximum, counts and weights added up in LDS, and in its bucket by comparison or bisection.
 #include "rlk_launch.hpp"
 #include "rlk_policy.hpp"
 
@@ -33,6 +34,7 @@ struct Sampling {
 typedef unsigned long long u64;
 
 // exp(z) for z <= 0 as a multiple of 2^-43, rounded to nearest.
+// (rows of few actions; fast_weight() is for longer ones)
 __device__ __forceinline__ u64 weight(double z) {
   if (!(z > -40.0)) return 0;  // (below half a unit)
   return (u64)__double2ll_rn(exp(z) * 0x1p43);
@@ -114,16 +116,22 @@ __global__ __launch_bounds__(256) void few_kernel(const Sampling s) {
   if (lane == __ffsll((long long)beyond) - 1) s.out[row] = lane, s.log_probs[row] = log_prob(z, total);
 }
 
-// ---- longer rows: a workgroup of NT threads a row.
+// ---- longer rows: a workgroup of NT threads a row.  Thread t has the vectors of 16 bytes t, t + NT, ..., which are read again for every pass: a
+// row held in registers is code for each of its elements in each pass, ten times what the instruction cache holds.
+constexpr int kTable = 64;
+constexpr int kShort = 512;  // lists that are ranked by comparing all with all
 template <int NT>
 struct Shared {
+  static constexpr int WAVES = NT / 64;
   u64 mass[kBuckets];
   uint32_t count[kBuckets];
   u64 list[kList];
-  u64 sums[NT / 64], sums2[NT / 64];
-  u64 scan[NT / 64 + 1];
+  u64 weights[kShort];
+  double table[kTable];
+  u64 sums[WAVES], sums2[WAVES];
+  u64 before, border;
   uint32_t listed;
-  int found;
+  int bucket, chunk;
 };
 
 template <int NT>
@@ -143,67 +151,142 @@ __device__ __forceinline__ int bucket(float x, float top, float scale) {
   const float d = (top - x) * scale;
   return x == top ? 0 : d < (float)(kBuckets - 1) ? (int)d : kBuckets - 1;  // (monotone in x; -inf and what lies far below are in the last)
 }
+__device__ __forceinline__ float value_of(u64 order) {
+  const uint32_t k = (uint32_t)(order >> 32);
+  return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
+}
+
+// exp(z), z <= 0, as weight() gives it: 2^(k / 64) from a table, what is left by its series (the first term left out is below 2^-44).
+__device__ __forceinline__ u64 fast_weight(double z, const double* table) {
+  const double t = z * (64.0 * 1.4426950408889634074);
+  const double n = rint(t);
+  const double y = (t - n) * (0.69314718055994530942 / 64.0);
+  const int k = (int)n;
+  double e = fma(y, 1.0 / 24.0, 1.0 / 6.0);
+  e = fma(e, y, 0.5);
+  e = fma(e, y, 1.0);
+  e = fma(e, y, 1.0);
+  e *= table[k & (kTable - 1)];
+  const double r = ldexp(e, (k >> 6) + 43);
+  // (rounded to a whole number by what float64 holds beside 2^52)
+  return z > -40.0 ? (u64)(__double_as_longlong(r + 0x1p52) & 0xfffffffffffffll) : 0;
+}
+
+template <class E>
+struct Vec {
+  static constexpr int N = 16 / (int)sizeof(E);
+  typedef uint32_t By2 __attribute__((ext_vector_type(4), aligned(2)));  // (an access need not be aligned to its size)
+  typedef uint32_t By4 __attribute__((ext_vector_type(4), aligned(4)));
+  typedef typename std::conditional<sizeof(E) == 2, By2, By4>::type Words_;
+  u32x4 w;
+  __device__ __forceinline__ void load(const E* row, int first, int count) {  // -inf behind the row's end
+    if (first + N <= count) {
+      w = *reinterpret_cast<const Words_*>(row + first);
+    } else {
+      const uint32_t none = sizeof(E) == 4 ? 0xff800000u : 0xff80ff80u;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] = none;
+      for (int i = 0; first + i < count; ++i) {
+        if constexpr (sizeof(E) == 4) {
+          const uint32_t b = __float_as_uint(load_one(row + first + i));
+#pragma unroll
+          for (int j = 0; j < 4; ++j) w[j] = i == j ? b : w[j];
+        } else {
+          const uint32_t b = (row + first + i)->bits;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) w[j] = i >> 1 != j ? w[j] : i & 1 ? (w[j] & 0xffffu) | b << 16 : (w[j] & 0xffff0000u) | b;
+        }
+      }
+    }
+  }
+  __device__ __forceinline__ float get(int i) const { return Words<E>::get(w[i / Words<E>::kPerWord], i % Words<E>::kPerWord); }
+};
+
+// Two elements at a time: the compiler would work on a whole vector's side by side, in twice the registers.
+__device__ __forceinline__ void apart(int e) {
+  if (e & 1) __builtin_amdgcn_sched_barrier(0);
+}
 
 template <class E, int NT>
-__global__ __launch_bounds__(NT) void row_kernel(const Sampling s) {
-  __shared__ Shared<NT> m;
+__global__ __launch_bounds__(NT, NT == 1024 ? 4 : 2) void row_kernel(const Sampling s) {
+  typedef Shared<NT> M;
+  constexpr int N = Vec<E>::N, WAVES = NT / 64;
+  __shared__ M m;
+  u64* const part = m.list;  // [trip][wavefront], once the list has had its use
+  static_assert(RLK_MOST_SAMPLED_ACTIONS / 4 / 64 <= kList && NT >= 256);
   const int64_t row = s.first + blockIdx.x;
   const E* p = row_of<E>(s, row);
-  const int A = s.actions, tid = threadIdx.x;
+  const int A = s.actions, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int trips = (A + NT * N - 1) / (NT * N);
 
-  float top = -INFINITY;
-  bool bad = false;
-  for (int i = tid; i < A; i += NT) {
-    const float x = load_one(p + i);
-    bad |= x != x;
-    top = fmaxf(top, x);
-  }
-  {
-    u64 b = order(top, 0);
-#pragma unroll
-    for (int d = 32; d > 0; d >>= 1) {
-      const u64 o = (u64)__shfl_xor((long long)b, d);
-      b = o > b ? o : b;
+  // Goes over the row, the next two vectors on their way: f(vector, its first action, trip).
+  auto each = [&](auto f) {
+    Vec<E> next[2];
+    next[0].load(p, tid * N, A), next[1].load(p, (NT + tid) * N, A);
+#pragma unroll 1
+    for (int c = 0; c < trips; c += 2) {
+      const Vec<E> x = next[0], y = next[1];
+      next[0].load(p, ((c + 2) * NT + tid) * N, A), next[1].load(p, ((c + 3) * NT + tid) * N, A);
+      f(x, (c * NT + tid) * N, c);
+      if (c + 1 < trips) f(y, ((c + 1) * NT + tid) * N, c + 1);
     }
+  };
+  // The same, one element after the other: for passes that are made seldom.
+  auto each_again = [&](auto f) {
+    for (int c = 0; c < trips; ++c) {
+#pragma unroll 1
+      for (int e = 0; e < N; ++e) {
+        const int i = (c * NT + tid) * N + e;
+        if (i < A) f(load_one(p + i), i);
+      }
+    }
+  };
+
+  for (int i = tid; i < kBuckets; i += NT) m.mass[i] = 0, m.count[i] = 0;
+  if (tid < kTable) m.table[tid] = exp2((double)tid / kTable);
+  if (tid == 0) m.listed = 0;
+  float top = -INFINITY, first_of = -INFINITY;
+  bool bad = false;
+  each([&](const Vec<E>& x, int, int) {
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      const float y = x.get(e);
+      bad |= y != y;
+      top = fmaxf(top, y);
+    }
+  });
+  first_of = top;  // of this thread's
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
+  {
     const bool any = __any(bad);
-    if ((tid & 63) == 0) m.sums[tid >> 6] = b, m.sums2[tid >> 6] = any;
+    if (lane == 0) m.sums[wave] = __float_as_uint(top), m.sums2[wave] = any;
     __syncthreads();
-    for (int i = 0; i < NT / 64; ++i) b = m.sums[i] > b ? m.sums[i] : b, bad |= m.sums2[i] != 0;
-    const uint32_t k = (uint32_t)(b >> 32);
-    top = __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
+#pragma unroll
+    for (int i = 0; i < WAVES; ++i) top = fmaxf(top, __uint_as_float((uint32_t)m.sums[i])), bad |= m.sums2[i] != 0;
   }
   if (bad || top == -INFINITY) {
     if (tid == 0) s.out[row] = -1, s.log_probs[row] = bad ? NAN : -INFINITY;
     return;
   }
+  const float scale = (float)s.inv_temperature * kPerNat;
+  auto take = [&](int action, float x, u64 total) { s.out[row] = action, s.log_probs[row] = log_prob(distance(x, top, s), total); };
 
-  u64 border = 0;  // the last that is kept, in order()
-  if (s.by_k || s.by_p) {
-    const float scale = (float)s.inv_temperature * kPerNat;
-    for (int i = tid; i < kBuckets; i += NT) m.mass[i] = 0, m.count[i] = 0;
+  // The bucket in which the counts or weights, added up from the first bucket on, reach `want`, and what lies before it.  `all`: their sum.
+  auto find_bucket = [&](bool counts, double want, u64* all) {
     __syncthreads();
-    for (int i = tid; i < A; i += NT) {
-      const float x = load_one(p + i);
-      const int b = bucket(x, top, scale);
-      if (s.by_k) atomicAdd(&m.count[b], 1u);
-      if (s.by_p) atomicAdd(&m.mass[b], weight(distance(x, top, s)));
-    }
-    __syncthreads();
-
-    // The last member of the shortest beginning that reaches `want`, of counts or weights; `held` becomes its weight.
-    auto last_of = [&](bool counts, double want, u64* held) {
-      // its bucket, and what lies before it: a wavefront's lanes take 32 buckets each
-      __syncthreads();
-      if (tid < 64) {
-        constexpr int PER = kBuckets / 64;
-        u64 x = 0;
-        for (int i = 0; i < PER; ++i) x += counts ? (u64)m.count[PER * tid + i] : m.mass[PER * tid + i];
-        u64 upto = x;
+    if (tid < 64) {
+      constexpr int PER = kBuckets / 64;
+      u64 x = 0;
+      for (int i = 0; i < PER; ++i) x += counts ? (u64)m.count[PER * tid + i] : m.mass[PER * tid + i];
+      u64 upto = x;
 #pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-          const u64 b = (u64)__shfl_up((long long)upto, d);
-          if (tid >= d) upto += b;
-        }
+      for (int d = 1; d < 64; d <<= 1) {
+        const u64 b = (u64)__shfl_up((long long)upto, d);
+        if (tid >= d) upto += b;
+      }
+      if (all != nullptr && tid == 63) m.border = upto;
+      if (all == nullptr) {
         const u64 reached = __ballot((double)upto >= want);
         const int first = reached != 0 ? __ffsll((long long)reached) - 1 : 63;
         if (tid == first) {
@@ -214,106 +297,246 @@ __global__ __launch_bounds__(NT) void row_kernel(const Sampling s) {
             if ((double)(c + n) >= want) break;
             c += n;
           }
-          m.found = b, m.scan[0] = c, m.listed = 0;
+          m.bucket = b, m.before = c, m.listed = 0;
         }
       }
-      __syncthreads();
-      const int b = m.found;
-      const u64 before = m.scan[0];
-      u64 lo = ~0ull, hi = 0;
-      for (int i = tid; i < A; i += NT) {
-        const float x = load_one(p + i);
-        if (bucket(x, top, scale) != b) continue;
-        const u64 o = order(x, i);
-        lo = o < lo ? o : lo, hi = o > hi ? o : hi;
-        const uint32_t at = atomicAdd(&m.listed, 1u);
-        if (at < kList) m.list[at] = o;
+    }
+    __syncthreads();
+    if (all != nullptr) *all = m.border;
+  };
+
+  u64 border = 0;  // the last that is kept, in order()
+  if (s.by_k && s.top_k <= 256) {
+    // As many of the threads' largest as top_k asks for are at least the border: what is before or in their last one's bucket are candidates.
+    if (first_of > -INFINITY) atomicAdd(&m.count[bucket(first_of, top, scale)], 1u);
+    find_bucket(true, (double)s.top_k, nullptr);
+    const int last = m.bucket;
+    const float reach = (float)(last + 1);
+    each([&](const Vec<E>& x, int first, int) {
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        const float y = x.get(e);
+        if (y == top || (y > -INFINITY && (last == kBuckets - 1 || (top - y) * scale < reach))) {
+          const uint32_t at = atomicAdd(&m.listed, 1u);
+          if (at < kShort) m.list[at] = order(y, first + e);
+        }
+        apart(e);
       }
+    });
+    __syncthreads();
+    const int n = (int)m.listed;
+    if (n <= kShort) {
+      constexpr int PER = (kShort + NT - 1) / NT;
+      u64 mine[PER], w[PER], before[PER];
+      int rank[PER];
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        const int at = tid + NT * i;
+        mine[i] = at < n ? m.list[at] : 0;
+        w[i] = at < n ? fast_weight(distance(value_of(mine[i]), top, s), m.table) : 0;
+        if (at < n) m.weights[at] = w[i];
+        before[i] = 0, rank[i] = 0;
+      }
+      __syncthreads();
+      if (wave * 64 < n)
+        for (int j = 0; j < n; ++j) {
+          const u64 other = m.list[j], wj = m.weights[j];
+#pragma unroll
+          for (int i = 0; i < PER; ++i) {
+            const bool first = other > mine[i];
+            rank[i] += first;
+            before[i] += first ? wj : 0;
+          }
+        }
+      u64 left = 0;  // what top_k leaves
+#pragma unroll
+      for (int i = 0; i < PER; ++i) left += tid + NT * i < n && rank[i] < s.top_k ? w[i] : 0;
+      left = all_sum<NT>(left, m.sums);
+      u64 total = 0;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        const int at = tid + NT * i;
+        const bool kept = at < n && rank[i] < s.top_k && (!s.by_p || (double)before[i] < s.top_p * (double)left) &&
+                          (!s.by_min || distance(value_of(mine[i]), top, s) >= s.least);
+        w[i] = kept ? w[i] : 0;
+        if (at < n) m.weights[at] = w[i];
+        total += w[i];
+      }
+      total = all_sum<NT>(total, m.sums);
+      const u64 want = share(s.uniforms[row], total);
+      __syncthreads();
+      u64 upto[PER];
+#pragma unroll
+      for (int i = 0; i < PER; ++i) upto[i] = 0;
+      if (wave * 64 < n)
+        for (int j = 0; j < n; ++j) {
+          const uint32_t other = (uint32_t)m.list[j];  // (~action: an earlier one has a larger number)
+          const u64 wj = m.weights[j];
+#pragma unroll
+          for (int i = 0; i < PER; ++i) upto[i] += other >= (uint32_t)mine[i] ? wj : 0;
+        }
+#pragma unroll
+      for (int i = 0; i < PER; ++i)
+        if (w[i] != 0 && upto[i] > want && upto[i] - w[i] <= want) take((int)~(uint32_t)mine[i], value_of(mine[i]), total);
+      return;
+    }
+    for (int i = tid; i < kBuckets; i += NT) m.count[i] = 0;
+    __syncthreads();
+  }
+
+  if (s.by_k || s.by_p) {
+    each([&](const Vec<E>& x, int, int) {
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        const float y = x.get(e);
+        if (y == -INFINITY) continue;
+        const int b = bucket(y, top, scale);
+        if (s.by_k) atomicAdd(&m.count[b], 1u);
+        if (s.by_p) atomicAdd(&m.mass[b], fast_weight(distance(y, top, s), m.table));
+        apart(e);
+      }
+    });
+
+    // The last member of the shortest beginning that reaches `want`: of counts, then of weights.
+    for (int round = s.by_k ? 0 : 1; round < (s.by_p ? 2 : 1); ++round) {
+      const bool counts = round == 0;
+      double want = (double)s.top_k;
+      if (!counts) {
+        u64 left = 0;  // what top_k leaves
+        if (s.by_k) {
+          each_again([&](float y, int i) { left += order(y, i) >= border ? fast_weight(distance(y, top, s), m.table) : 0; });
+          left = all_sum<NT>(left, m.sums);
+        } else {
+          find_bucket(false, 0.0, &left);
+        }
+        want = s.top_p * (double)left;
+      }
+      find_bucket(counts, want, nullptr);
+      const int b = m.bucket;
+      const u64 before = m.before;
+      u64 lo = ~0ull, hi = 0;
+      each([&](const Vec<E>& x, int first, int) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+          const float y = x.get(e);
+          if (y == -INFINITY || bucket(y, top, scale) != b) continue;
+          const u64 o = order(y, first + e);
+          lo = o < lo ? o : lo, hi = o > hi ? o : hi;
+          const uint32_t at = atomicAdd(&m.listed, 1u);
+          if (at < kList) m.list[at] = o;
+          apart(e);
+        }
+      });
 #pragma unroll
       for (int d = 32; d > 0; d >>= 1) {
         const u64 a = (u64)__shfl_xor((long long)lo, d), c = (u64)__shfl_xor((long long)hi, d);
         lo = a < lo ? a : lo, hi = c > hi ? c : hi;
       }
+      if (lane == 0) m.sums[wave] = lo, m.sums2[wave] = hi;
       __syncthreads();
-      if ((tid & 63) == 0) m.sums[tid >> 6] = lo, m.sums2[tid >> 6] = hi;
-      __syncthreads();
-      for (int i = 0; i < NT / 64; ++i) lo = m.sums[i] < lo ? m.sums[i] : lo, hi = m.sums2[i] > hi ? m.sums2[i] : hi;
+#pragma unroll
+      for (int i = 0; i < WAVES; ++i) lo = m.sums[i] < lo ? m.sums[i] : lo, hi = m.sums2[i] > hi ? m.sums2[i] : hi;
       const uint32_t n = m.listed;
-      auto value = [&](u64 o) {
-        const uint32_t k = (uint32_t)(o >> 32);
-        return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
-      };
-      auto from = [&](u64 least, bool weights) {  // the count or weight of the bucket's members from `least` on
-        u64 x = 0;
-        if (n <= kList) {
-          for (uint32_t i = tid; i < n; i += NT)
-            if (m.list[i] >= least) x += weights ? weight(distance(value(m.list[i]), top, s)) : 1;
-        } else {
-          for (int i = tid; i < A; i += NT) {
-            const float y = load_one(p + i);
-            if (bucket(y, top, scale) == b && order(y, i) >= least) x += weights ? weight(distance(y, top, s)) : 1;
-          }
+      if (n <= kShort) {
+        // each compares itself with all
+        if (tid == 0) m.border = lo;  // (all of the bucket, if it never is enough)
+        for (uint32_t i = tid; i < n; i += NT) m.weights[i] = counts ? 1 : fast_weight(distance(value_of(m.list[i]), top, s), m.table);
+        __syncthreads();
+        for (uint32_t i = tid; i < n; i += NT) {
+          const u64 mine = m.list[i];
+          u64 sum = before;
+          for (uint32_t j = 0; j < n; ++j) sum += m.list[j] > mine ? m.weights[j] : 0;
+          if ((double)sum < want && (double)(sum + m.weights[i]) >= want) m.border = mine;
         }
-        return all_sum<NT>(x, m.sums);
-      };
-      // the largest o in [lo, hi] from which on there is enough (all of the bucket, if it never is)
-      while (lo < hi) {
-        const u64 mid = lo + (hi - lo) / 2 + ((hi - lo) & 1);
-        if ((double)(before + from(mid, !counts)) >= want) lo = mid;
-        else hi = mid - 1;
+        __syncthreads();
+        lo = m.border;
+      } else {
+        // the largest order in [lo, hi] from which on there is enough
+        while (lo < hi) {
+          const u64 mid = lo + (hi - lo) / 2 + ((hi - lo) & 1);
+          u64 x = 0;
+          if (n <= kList) {
+            for (uint32_t i = tid; i < n; i += NT)
+              if (m.list[i] >= mid) x += counts ? 1 : fast_weight(distance(value_of(m.list[i]), top, s), m.table);
+          } else {
+            each_again([&](float y, int i) {
+              if (y > -INFINITY && bucket(y, top, scale) == b && order(y, i) >= mid) x += counts ? 1 : fast_weight(distance(y, top, s), m.table);
+            });
+          }
+          if ((double)(before + all_sum<NT>(x, m.sums)) >= want) lo = mid;
+          else hi = mid - 1;
+        }
       }
-      if (held != nullptr) {
-        // what the buckets before hold
-        u64 x = 0;
-        for (int i = tid; i < b; i += NT) x += m.mass[i];
-        x = all_sum<NT>(x, m.sums);
-        *held = x + from(lo, true);
-      }
-      return lo;
-    };
-    u64 held = 0;
-    if (s.by_k && s.top_k < A) border = last_of(true, (double)s.top_k, s.by_p ? &held : nullptr);
-    else if (s.by_p) {
-      for (int i = tid; i < kBuckets; i += NT) held += m.mass[i];
-      held = all_sum<NT>(held, m.sums);
-    }
-    if (s.by_p) {
-      const u64 other = last_of(false, s.top_p * (double)held, nullptr);
-      border = other > border ? other : border;
+      border = lo > border ? lo : border;
     }
   }
 
-  // Of the kept ones in the order of their numbers: NT at a time, their weights added up.
-  auto kept_weight = [&](int i, double* z) -> u64 {
-    if (i >= A) return 0;
-    const float x = load_one(p + i);
-    *z = distance(x, top, s);
-    return order(x, i) >= border && (!s.by_min || *z >= s.least) ? weight(*z) : 0;
+  // Of the kept ones in the order of their numbers: the weights of a wavefront's vectors of a trip, of these the one up to which there is enough, and in
+  // it the action.
+  __syncthreads();
+  const float border_value = border != 0 ? value_of(border) : -INFINITY;
+  auto kept_weight = [&](float x, int i) -> u64 {
+    if (x < border_value || x == -INFINITY) return 0;
+    const double z = distance(x, top, s);
+    return order(x, i) >= border && (!s.by_min || z >= s.least) ? fast_weight(z, m.table) : 0;
   };
+  each([&](const Vec<E>& x, int first, int c) {
+    u64 sum = 0;
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      sum += kept_weight(x.get(e), first + e);
+      apart(e);
+    }
+    if (__any(sum != 0)) {
+#pragma unroll
+      for (int d = 32; d > 0; d >>= 1) sum += (u64)__shfl_xor((long long)sum, d);
+    }
+    if (lane == 0) part[c * WAVES + wave] = sum;
+  });
+  __syncthreads();
+  const int parts = trips * WAVES;
   u64 total = 0;
-  double z = 0.0;
-  for (int i = tid; i < A; i += NT) total += kept_weight(i, &z);
+  for (int i = tid; i < parts; i += NT) total += part[i];
   total = all_sum<NT>(total, m.sums);
   const u64 want = share(s.uniforms[row], total);
+  if (wave != 0) return;
   u64 before = 0;
-  for (int i0 = 0; i0 < A; i0 += NT) {
-    const u64 w = kept_weight(i0 + tid, &z);
-    u64 sum = w;
+  int at = 0;
+  for (int i0 = 0;; i0 += 64) {  // (ends: `want` is below the total)
+    const u64 x = i0 + lane < parts ? part[i0 + lane] : 0;
+    u64 upto = x;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
-      const u64 b = (u64)__shfl_up((long long)sum, d);
-      if ((tid & 63) >= d) sum += b;
+      const u64 b = (u64)__shfl_up((long long)upto, d);
+      if (lane >= d) upto += b;
     }
-    __syncthreads();
-    if ((tid & 63) == 63) m.sums[tid >> 6] = sum;
-    __syncthreads();
-    u64 base = before;
-    for (int i = 0; i < NT / 64; ++i) {
-      if (i < tid >> 6) base += m.sums[i];
-      before += m.sums[i];
+    const u64 beyond = __ballot(before + upto > want);
+    if (beyond != 0 || i0 + 64 >= parts) {
+      const int l = beyond != 0 ? __ffsll((long long)beyond) - 1 : 63;
+      before += shfl64(upto - x, l, 64);
+      at = i0 + l;
+      break;
     }
-    if (base + sum > want && base + sum - w <= want) s.out[row] = i0 + tid, s.log_probs[row] = log_prob(z, total);
-    if (before > want) break;
+    before += shfl64(upto, 63, 64);
+  }
+  const int first = (at / WAVES * NT + at % WAVES * 64 + lane) * N;
+  Vec<E> x;
+  x.load(p, first, A);
+  u64 sum = 0;
+#pragma unroll
+  for (int e = 0; e < N; ++e) sum += kept_weight(x.get(e), first + e);
+  u64 upto = sum;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const u64 b = (u64)__shfl_up((long long)upto, d);
+    if (lane >= d) upto += b;
+  }
+  before += upto - sum;
+#pragma unroll
+  for (int e = 0; e < N; ++e) {
+    const u64 w = kept_weight(x.get(e), first + e);
+    if (w != 0 && before <= want && before + w > want) take(first + e, x.get(e), total);
+    before += w;
   }
 }
 
