@@ -147,30 +147,38 @@ __device__ __forceinline__ u64 all_sum(u64 x, u64* s) {
   return x;
 }
 
-__device__ __forceinline__ int bucket(float x, float top, float scale) {
-  const float d = (top - x) * scale;
-  return x == top ? 0 : d < (float)(kBuckets - 1) ? (int)d : kBuckets - 1;  // (monotone in x; -inf and what lies far below are in the last)
+// How many 64ths of a nat x lies below the largest, held to the buckets there are: 0 for its equals (inf - inf and 0 inf too), the last for
+// -inf and what lies far below; monotone in x.
+__device__ __forceinline__ float depth(float x, float top, float scale) {
+  return fminf(fmaxf((top - x) * scale, 0.f), (float)(kBuckets - 1));
 }
+__device__ __forceinline__ int bucket(float x, float top, float scale) { return (int)depth(x, top, scale); }
 __device__ __forceinline__ float value_of(u64 order) {
   const uint32_t k = (uint32_t)(order >> 32);
   return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
 }
 
-// exp(z), z <= 0, as weight() gives it: 2^(k / 64) from a table, what is left by its series (the first term left out is below 2^-44).
-__device__ __forceinline__ u64 fast_weight(double z, const double* table) {
-  const double t = z * (64.0 * 1.4426950408889634074);
-  const double n = rint(t);
-  const double y = (t - n) * (0.69314718055994530942 / 64.0);
-  const int k = (int)n;
-  double e = fma(y, 1.0 / 24.0, 1.0 / 6.0);
-  e = fma(e, y, 0.5);
-  e = fma(e, y, 1.0);
-  e = fma(e, y, 1.0);
-  e *= table[k & (kTable - 1)];
-  const double r = ldexp(e, (k >> 6) + 43);
-  // (rounded to a whole number by what float64 holds beside 2^52)
-  return z > -40.0 ? (u64)(__double_as_longlong(r + 0x1p52) & 0xfffffffffffffll) : 0;
-}
+// What a row's weights are formed with: `unit` turns a difference of logits into 64ths of an octave.
+struct Weights {
+  const double* table;  // 2^(43 + i / 64)
+  double top, unit;
+  // The distance of x below the largest, in 64ths of an octave: 0 for its equals (inf - inf too), at least what still rounds to no weight.
+  __device__ __forceinline__ double steps(float x) const { return fmax(fmin(((double)x - top) * unit, 0.0), -3693.0); }
+  // exp as weight() gives it: 2^(n / 64) from the table, what is left by its series (the first term left out is below 2^-44), rounded to a whole
+  // number by what float64 holds beside 2^52.
+  __device__ __forceinline__ u64 of_steps(double t) const {
+    constexpr double U = 0.69314718055994530942 / 64.0;
+    const double n = rint(t), f = t - n;
+    const int k = (int)n;
+    double e = fma(f, U * U * U * U / 24.0, U * U * U / 6.0);
+    e = fma(e, f, U * U / 2.0);
+    e = fma(e, f, U);
+    e = fma(e, f, 1.0);
+    const double r = ldexp(e * table[k & (kTable - 1)], k >> 6);
+    return (u64)(__double_as_longlong(r + 0x1p52) & 0xfffffffffffffll);
+  }
+  __device__ __forceinline__ u64 operator()(float x) const { return of_steps(steps(x)); }
+};
 
 template <class E>
 struct Vec {
@@ -179,24 +187,17 @@ struct Vec {
   typedef uint32_t By4 __attribute__((ext_vector_type(4), aligned(4)));
   typedef typename std::conditional<sizeof(E) == 2, By2, By4>::type Words_;
   u32x4 w;
-  __device__ __forceinline__ void load(const E* row, int first, int count) {  // -inf behind the row's end
-    if (first + N <= count) {
-      w = *reinterpret_cast<const Words_*>(row + first);
-    } else {
-      const uint32_t none = sizeof(E) == 4 ? 0xff800000u : 0xff80ff80u;
+  __device__ __forceinline__ void load(const E* row, int first) { w = *reinterpret_cast<const Words_*>(row + first); }
+  __device__ __forceinline__ void load_some(const E* row, int first, int count) {  // -inf behind the row's end
+    if (first + N <= count) return load(row, first);
+    const uint32_t none = sizeof(E) == 4 ? 0xff800000u : 0xff80ff80u;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) w[i] = none;
-      for (int i = 0; first + i < count; ++i) {
-        if constexpr (sizeof(E) == 4) {
-          const uint32_t b = __float_as_uint(load_one(row + first + i));
+    for (int i = 0; i < 4; ++i) w[i] = none;
 #pragma unroll
-          for (int j = 0; j < 4; ++j) w[j] = i == j ? b : w[j];
-        } else {
-          const uint32_t b = (row + first + i)->bits;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) w[j] = i >> 1 != j ? w[j] : i & 1 ? (w[j] & 0xffffu) | b << 16 : (w[j] & 0xffff0000u) | b;
-        }
-      }
+    for (int i = 0; i < N; ++i) {
+      if (first + i >= count) continue;
+      if constexpr (sizeof(E) == 4) w[i] = __float_as_uint(load_one(row + first + i));
+      else w[i / 2] = i & 1 ? (w[i / 2] & 0xffffu) | (uint32_t)(row + first + i)->bits << 16 : (w[i / 2] & 0xffff0000u) | (row + first + i)->bits;
     }
   }
   __device__ __forceinline__ float get(int i) const { return Words<E>::get(w[i / Words<E>::kPerWord], i % Words<E>::kPerWord); }
@@ -208,29 +209,45 @@ __device__ __forceinline__ void apart(int e) {
 }
 
 template <class E, int NT>
-__global__ __launch_bounds__(NT, NT == 1024 ? 4 : 2) void row_kernel(const Sampling s) {
+__global__ __launch_bounds__(NT, NT >= 512 ? 4 : 2) void row_kernel(const Sampling s) {
   typedef Shared<NT> M;
   constexpr int N = Vec<E>::N, WAVES = NT / 64;
   __shared__ M m;
   u64* const part = m.list;  // [trip][wavefront], once the list has had its use
-  static_assert(RLK_MOST_SAMPLED_ACTIONS / 4 / 64 <= kList && NT >= 256);
+  static_assert(RLK_MOST_SAMPLED_ACTIONS / 4 / 64 <= kList);
   const int64_t row = s.first + blockIdx.x;
   const E* p = row_of<E>(s, row);
   const int A = s.actions, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int trips = (A + NT * N - 1) / (NT * N);
 
-  // Goes over the row, the next two vectors on their way: f(vector, its first action, trip).
-  auto each = [&](auto f) {
-    Vec<E> next[2];
-    next[0].load(p, tid * N, A), next[1].load(p, (NT + tid) * N, A);
+  // Goes over the row, the next U vectors on their way: f(vector, its first action, trip).
+  const int whole = A / (NT * N);  // trips in which all threads have whole vectors
+  auto each = [&](auto ahead, auto f) {
+    constexpr int U = decltype(ahead)::value;
+    Vec<E> next[U];
+#pragma unroll
+    for (int i = 0; i < U; ++i)
+      if (i < whole) next[i].load(p, (i * NT + tid) * N);
 #pragma unroll 1
-    for (int c = 0; c < trips; c += 2) {
-      const Vec<E> x = next[0], y = next[1];
-      next[0].load(p, ((c + 2) * NT + tid) * N, A), next[1].load(p, ((c + 3) * NT + tid) * N, A);
-      f(x, (c * NT + tid) * N, c);
-      if (c + 1 < trips) f(y, ((c + 1) * NT + tid) * N, c + 1);
+    for (int c = 0; c < whole; c += U) {
+      Vec<E> x[U];
+#pragma unroll
+      for (int i = 0; i < U; ++i) {
+        x[i] = next[i];
+        if (c + U + i < whole) next[i].load(p, ((c + U + i) * NT + tid) * N);
+      }
+#pragma unroll
+      for (int i = 0; i < U; ++i)
+        if (c + i < whole) f(x[i], ((c + i) * NT + tid) * N, c + i);
+    }
+    if (whole < trips) {
+      Vec<E> x;
+      x.load_some(p, (whole * NT + tid) * N, A);
+      f(x, (whole * NT + tid) * N, whole);
     }
   };
+  const std::integral_constant<int, 4> light{};  // (passes of a few instructions an element)
+  const std::integral_constant<int, 2> heavy{};
   // The same, one element after the other: for passes that are made seldom.
   auto each_again = [&](auto f) {
     for (int c = 0; c < trips; ++c) {
@@ -243,11 +260,11 @@ __global__ __launch_bounds__(NT, NT == 1024 ? 4 : 2) void row_kernel(const Sampl
   };
 
   for (int i = tid; i < kBuckets; i += NT) m.mass[i] = 0, m.count[i] = 0;
-  if (tid < kTable) m.table[tid] = exp2((double)tid / kTable);
+  if (tid < kTable) m.table[tid] = exp2((double)tid / kTable) * 0x1p43;
   if (tid == 0) m.listed = 0;
   float top = -INFINITY, first_of = -INFINITY;
   bool bad = false;
-  each([&](const Vec<E>& x, int, int) {
+  each(light, [&](const Vec<E>& x, int, int) {
 #pragma unroll
     for (int e = 0; e < N; ++e) {
       const float y = x.get(e);
@@ -270,6 +287,7 @@ __global__ __launch_bounds__(NT, NT == 1024 ? 4 : 2) void row_kernel(const Sampl
     return;
   }
   const float scale = (float)s.inv_temperature * kPerNat;
+  const Weights weights{m.table, (double)top, s.inv_temperature * (64.0 * 1.4426950408889634074)};
   auto take = [&](int action, float x, u64 total) { s.out[row] = action, s.log_probs[row] = log_prob(distance(x, top, s), total); };
 
   // The bucket in which the counts or weights, added up from the first bucket on, reach `want`, and what lies before it.  `all`: their sum.
@@ -311,16 +329,18 @@ __global__ __launch_bounds__(NT, NT == 1024 ? 4 : 2) void row_kernel(const Sampl
     if (first_of > -INFINITY) atomicAdd(&m.count[bucket(first_of, top, scale)], 1u);
     find_bucket(true, (double)s.top_k, nullptr);
     const int last = m.bucket;
-    const float reach = (float)(last + 1);
-    each([&](const Vec<E>& x, int first, int) {
+    const float reach = (float)(last + 1);  // (the last bucket's depths are its number)
+    each(light, [&](const Vec<E>& x, int first, int) {
+      bool any = false;
 #pragma unroll
-      for (int e = 0; e < N; ++e) {
-        const float y = x.get(e);
-        if (y == top || (y > -INFINITY && (last == kBuckets - 1 || (top - y) * scale < reach))) {
-          const uint32_t at = atomicAdd(&m.listed, 1u);
-          if (at < kShort) m.list[at] = order(y, first + e);
-        }
-        apart(e);
+      for (int e = 0; e < N; ++e) any |= depth(x.get(e), top, scale) < reach;
+      if (!any) return;
+#pragma unroll 1
+      for (int i = first; i < first + N && i < A; ++i) {
+        const float y = load_one(p + i);
+        if (!(depth(y, top, scale) < reach) || y == -INFINITY) continue;
+        const uint32_t at = atomicAdd(&m.listed, 1u);
+        if (at < kShort) m.list[at] = order(y, i);
       }
     });
     __syncthreads();
@@ -333,7 +353,7 @@ __global__ __launch_bounds__(NT, NT == 1024 ? 4 : 2) void row_kernel(const Sampl
       for (int i = 0; i < PER; ++i) {
         const int at = tid + NT * i;
         mine[i] = at < n ? m.list[at] : 0;
-        w[i] = at < n ? fast_weight(distance(value_of(mine[i]), top, s), m.table) : 0;
+        w[i] = at < n ? weights(value_of(mine[i])) : 0;
         if (at < n) m.weights[at] = w[i];
         before[i] = 0, rank[i] = 0;
       }
@@ -385,17 +405,20 @@ __global__ __launch_bounds__(NT, NT == 1024 ? 4 : 2) void row_kernel(const Sampl
   }
 
   if (s.by_k || s.by_p) {
-    each([&](const Vec<E>& x, int, int) {
+    if (s.by_k)
+      each(light, [&](const Vec<E>& x, int, int) {
 #pragma unroll
-      for (int e = 0; e < N; ++e) {
-        const float y = x.get(e);
-        if (y == -INFINITY) continue;
-        const int b = bucket(y, top, scale);
-        if (s.by_k) atomicAdd(&m.count[b], 1u);
-        if (s.by_p) atomicAdd(&m.mass[b], fast_weight(distance(y, top, s), m.table));
-        apart(e);
-      }
-    });
+        for (int e = 0; e < N; ++e)
+          if (x.get(e) > -INFINITY) atomicAdd(&m.count[bucket(x.get(e), top, scale)], 1u);
+      });
+    if (s.by_p)
+      each(heavy, [&](const Vec<E>& x, int, int) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+          atomicAdd(&m.mass[bucket(x.get(e), top, scale)], weights(x.get(e)));
+          apart(e);
+        }
+      });
 
     // The last member of the shortest beginning that reaches `want`: of counts, then of weights.
     for (int round = s.by_k ? 0 : 1; round < (s.by_p ? 2 : 1); ++round) {
@@ -404,7 +427,7 @@ __global__ __launch_bounds__(NT, NT == 1024 ? 4 : 2) void row_kernel(const Sampl
       if (!counts) {
         u64 left = 0;  // what top_k leaves
         if (s.by_k) {
-          each_again([&](float y, int i) { left += order(y, i) >= border ? fast_weight(distance(y, top, s), m.table) : 0; });
+          each_again([&](float y, int i) { left += order(y, i) >= border ? weights(y) : 0; });
           left = all_sum<NT>(left, m.sums);
         } else {
           find_bucket(false, 0.0, &left);
@@ -415,16 +438,22 @@ __global__ __launch_bounds__(NT, NT == 1024 ? 4 : 2) void row_kernel(const Sampl
       const int b = m.bucket;
       const u64 before = m.before;
       u64 lo = ~0ull, hi = 0;
-      each([&](const Vec<E>& x, int first, int) {
+      each(light, [&](const Vec<E>& x, int first, int) {
+        bool any = false;
 #pragma unroll
         for (int e = 0; e < N; ++e) {
-          const float y = x.get(e);
-          if (y == -INFINITY || bucket(y, top, scale) != b) continue;
-          const u64 o = order(y, first + e);
+          const float d = depth(x.get(e), top, scale);
+          any |= d >= (float)b && d < (float)(b + 1);
+        }
+        if (!any) return;
+#pragma unroll 1
+        for (int i = first; i < first + N && i < A; ++i) {
+          const float y = load_one(p + i);
+          if (bucket(y, top, scale) != b) continue;
+          const u64 o = order(y, i);
           lo = o < lo ? o : lo, hi = o > hi ? o : hi;
           const uint32_t at = atomicAdd(&m.listed, 1u);
           if (at < kList) m.list[at] = o;
-          apart(e);
         }
       });
 #pragma unroll
@@ -440,7 +469,7 @@ __global__ __launch_bounds__(NT, NT == 1024 ? 4 : 2) void row_kernel(const Sampl
       if (n <= kShort) {
         // each compares itself with all
         if (tid == 0) m.border = lo;  // (all of the bucket, if it never is enough)
-        for (uint32_t i = tid; i < n; i += NT) m.weights[i] = counts ? 1 : fast_weight(distance(value_of(m.list[i]), top, s), m.table);
+        for (uint32_t i = tid; i < n; i += NT) m.weights[i] = counts ? 1 : weights(value_of(m.list[i]));
         __syncthreads();
         for (uint32_t i = tid; i < n; i += NT) {
           const u64 mine = m.list[i];
@@ -457,10 +486,10 @@ __global__ __launch_bounds__(NT, NT == 1024 ? 4 : 2) void row_kernel(const Sampl
           u64 x = 0;
           if (n <= kList) {
             for (uint32_t i = tid; i < n; i += NT)
-              if (m.list[i] >= mid) x += counts ? 1 : fast_weight(distance(value_of(m.list[i]), top, s), m.table);
+              if (m.list[i] >= mid) x += counts ? 1 : weights(value_of(m.list[i]));
           } else {
             each_again([&](float y, int i) {
-              if (y > -INFINITY && bucket(y, top, scale) == b && order(y, i) >= mid) x += counts ? 1 : fast_weight(distance(y, top, s), m.table);
+              if (bucket(y, top, scale) == b && order(y, i) >= mid) x += counts ? 1 : weights(y);
             });
           }
           if ((double)(before + all_sum<NT>(x, m.sums)) >= want) lo = mid;
@@ -475,12 +504,14 @@ __global__ __launch_bounds__(NT, NT == 1024 ? 4 : 2) void row_kernel(const Sampl
   // it the action.
   __syncthreads();
   const float border_value = border != 0 ? value_of(border) : -INFINITY;
+  const int border_action = border != 0 ? (int)~(uint32_t)border : A;
+  const double least = s.least * (64.0 * 1.4426950408889634074);
   auto kept_weight = [&](float x, int i) -> u64 {
-    if (x < border_value || x == -INFINITY) return 0;
-    const double z = distance(x, top, s);
-    return order(x, i) >= border && (!s.by_min || z >= s.least) ? fast_weight(z, m.table) : 0;
+    if (!(x > border_value || (x == border_value && i <= border_action))) return 0;
+    const double t = weights.steps(x);
+    return !s.by_min || t >= least ? weights.of_steps(t) : 0;
   };
-  each([&](const Vec<E>& x, int first, int c) {
+  each(heavy, [&](const Vec<E>& x, int first, int c) {
     u64 sum = 0;
 #pragma unroll
     for (int e = 0; e < N; ++e) {
@@ -521,7 +552,7 @@ __global__ __launch_bounds__(NT, NT == 1024 ? 4 : 2) void row_kernel(const Sampl
   }
   const int first = (at / WAVES * NT + at % WAVES * 64 + lane) * N;
   Vec<E> x;
-  x.load(p, first, A);
+  x.load_some(p, first, A);
   u64 sum = 0;
 #pragma unroll
   for (int e = 0; e < N; ++e) sum += kept_weight(x.get(e), first + e);
@@ -557,8 +588,11 @@ int launch(Sampling s, hipStream_t stream) {
   } else {
     for (s.first = 0; s.first < rows; s.first += most) {
       const dim3 grid((unsigned)(rows - s.first < most ? rows - s.first : most));
+      // A row to a CU: by 1024 threads ([64] of 131072, top-k: 26 us, 33 by 512).  More: two workgroups of 512 a CU, one of which works while the
+      // other waits (top-p, [512] of 50001: 105 us, 127 by 1024).
       if (s.actions <= 4096) row_kernel<E, 256><<<grid, dim3(256), 0, stream>>>(s);
-      else row_kernel<E, 1024><<<grid, dim3(1024), 0, stream>>>(s);
+      else if (rows <= device_cus()) row_kernel<E, 1024><<<grid, dim3(1024), 0, stream>>>(s);
+      else row_kernel<E, 512><<<grid, dim3(512), 0, stream>>>(s);
     }
   }
   return hipGetLastError() == hipSuccess ? RLK_OK : RLK_ERR_LAUNCH;
