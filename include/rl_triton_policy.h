@@ -143,7 +143,7 @@ typedef struct rlk_delta_rule_gradients {
 size_t rlk_delta_rule_workspace_bytes(int64_t num_envs, int64_t seq_len, int64_t heads, int64_t dim_k, int64_t dim_v, int backward);
 /* Of what a forward call leaves for the backward one (16-byte aligned). */
 size_t rlk_delta_rule_saved_bytes(int64_t num_envs, int64_t seq_len, int64_t heads, int64_t dim_k, int64_t dim_v);
-/* With `saved` (else NULL) the call needs no workspace.  heads * ceil(seq_len / 64) is at most 2^22. */
+/* `saved`: NULL, or what the backward call is to read.  heads * ceil(seq_len / 64) is at most 2^22. */
 int rlk_gated_delta_rule(const rlk_delta_rule *call, void *saved, size_t saved_bytes, void *stream);
 /* `call` as the forward one was, with a workspace for backward = 1; its out and state_out are not looked at, and of its
  * state only whether there is one. */

@@ -77,8 +77,19 @@ int forward(const rlk_delta_rule& c, void* saved, hipStream_t s) {
   const int64_t most = envs_at_once(c.num_envs, c.heads, r.chunks, sizeof(Record));
   for (r.first_env = 0; r.first_env < c.num_envs; r.first_env += most) {
     const int64_t envs = c.num_envs - r.first_env < most ? c.num_envs - r.first_env : most;
+    r.records = static_cast<Record*>(c.workspace);
+    const int64_t pairs = envs * c.heads;
+    const Segments plan = plan_segments(pairs, r.chunks);
+    r.segs = plan.segs, r.seg_chunks = plan.chunks;
+    if (plan.segs > 1) {
+      float* p = reinterpret_cast<float*>(r.records + pairs * r.chunks);
+      r.wild = reinterpret_cast<int*>(p);
+      r.phi = p + (pairs + 3) / 4 * 4;
+      r.seg_states = r.phi + (size_t)(pairs * plan.segs) * pad16(r.dk) * pad16(r.dk);
+    } else {
+      r.wild = nullptr;
+    }
     if (saved != nullptr) Saved(saved, c).at(r);
-    else r.records = static_cast<Record*>(c.workspace);
     int st = launch_records(r, envs, s);
     if (st == RLK_OK) st = launch_forward(r, envs, s);
     if (st != RLK_OK) return st;
@@ -252,7 +263,17 @@ size_t rlk_delta_rule_workspace_bytes(int64_t num_envs, int64_t seq_len, int64_t
     return 0;
   const int64_t chunks = chunks_of(seq_len);
   const size_t each = backward ? backward_chunk_bytes(dim_k, dim_v) : sizeof(Record);
-  return (size_t)(envs_at_once(num_envs, heads, chunks, each) * heads * chunks) * each;
+  const int64_t envs = envs_at_once(num_envs, heads, chunks, each);
+  size_t bytes = (size_t)(envs * heads * chunks) * each;
+  if (!backward) {  // (the last set of environments, the smaller one, may be the one that is cut)
+    size_t floats = segment_floats(envs * heads, plan_segments(envs * heads, chunks), (int)dim_k, (int)dim_v);
+    if (const int64_t left = num_envs % envs) {
+      const size_t last = segment_floats(left * heads, plan_segments(left * heads, chunks), (int)dim_k, (int)dim_v);
+      if (last > floats) floats = last;
+    }
+    bytes += floats * sizeof(float);
+  }
+  return bytes;
 }
 
 size_t rlk_delta_rule_saved_bytes(int64_t num_envs, int64_t seq_len, int64_t heads, int64_t dim_k, int64_t dim_v) {
@@ -266,9 +287,9 @@ int rlk_gated_delta_rule(const rlk_delta_rule* call, void* saved, size_t saved_b
   const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   if (call->seq_len == 0) return same_state(*call, call->state, call->state_out, s);
   if (!fits(*call)) return RLK_ERR_INVALID_ARGUMENT;
-  if (saved != nullptr ? !scratch_fits(saved, saved_bytes, Saved(saved, *call).bytes())
-                       : !scratch_fits(call->workspace, call->workspace_bytes,
-                                       rlk_delta_rule_workspace_bytes(call->num_envs, call->seq_len, call->heads, call->dim_k, call->dim_v, 0)))
+  if ((saved != nullptr && !scratch_fits(saved, saved_bytes, Saved(saved, *call).bytes())) ||
+      !scratch_fits(call->workspace, call->workspace_bytes,
+                    rlk_delta_rule_workspace_bytes(call->num_envs, call->seq_len, call->heads, call->dim_k, call->dim_v, 0)))
     return RLK_ERR_WORKSPACE;
   return call->bf16 ? forward<bf16>(*call, saved, s) : forward<float>(*call, saved, s);
 }

@@ -76,6 +76,13 @@ struct Rule {
   // it, and z.  NULL: not kept.
   float *states, *w, *dstates, *z;
   float *gg, *gb;  // gradients of gates and betas
+  // Sequences cut into segments of seg_chunks chunks, where there are few pairs.  A segment turns the state S that enters it into phi S + n:
+  // [pair, segment] phi [pad16(dk), pad16(dk)], and in seg_states [pair, segment, pad16(dk), pad16(dv)] n of the segment before, then the state
+  // that enters.  wild: [pair], a segment that can only be walked from the state itself; such a pair is walked by one workgroup.
+  int segs;
+  int64_t seg_chunks;
+  float *phi, *seg_states;
+  int* wild;
   bool from_zero;  // the sequences begin without a state: the first gate has nothing to act on, and no gradient
 };
 
@@ -308,11 +315,30 @@ __device__ __forceinline__ bool finite(float x) { return fabsf(x) <= 3.402823466
 template <class E>
 int launch_records(const Rule<E>& r, int64_t envs, hipStream_t s);
 template <class E>
-int launch_forward(const Rule<E>& r, int64_t envs, hipStream_t s);
+int launch_forward(const Rule<E>& r, int64_t envs, hipStream_t s);  // (with its segments)
 template <class E>
 int launch_backward(const Rule<E>& r, int64_t envs, hipStream_t s);
 template <class E>
 int launch_gradients(const Rule<E>& r, int64_t envs, hipStream_t s);
+
+// Segments: none where the pairs fill the GPU by themselves; else for two workgroups a CU, of at least 8 chunks, and no fewer than 4 (cutting
+// costs two more walks without outputs, which that many segments make up for).
+struct Segments {
+  int segs;
+  int64_t chunks;
+};
+inline Segments plan_segments(int64_t pairs, int64_t chunks) {
+  int64_t segs = 2 * device_cus() / pairs;
+  if (segs > chunks / 8) segs = chunks / 8;
+  if (segs < 4) return {1, chunks};
+  const int64_t per = (chunks + segs - 1) / segs;
+  return {(int)((chunks + per - 1) / per), per};
+}
+// Scratch memory of the segments, in floats.
+inline size_t segment_floats(int64_t pairs, const Segments& s, int dk, int dv) {
+  if (s.segs <= 1) return 0;
+  return (size_t)((pairs + 3) / 4 * 4) + (size_t)(pairs * s.segs) * pad16(dk) * (pad16(dk) + pad16(dv));
+}
 
 // Whether an array's rows can be read 4 elements at a time.
 template <class E>

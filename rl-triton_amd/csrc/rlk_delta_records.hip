@@ -32,6 +32,7 @@ __global__ __launch_bounds__(64 * kWaves) void records_kernel(const Rule<E> r, i
   const int head = (int)(pair % r.heads), n = (int)(T - s0 < C ? T - s0 : C);
   Record& rec = r.records[at];
   bool wild = false;
+  if (r.wild != nullptr && chunk == 0 && lane == 0) r.wild[pair] = 0;
 
   // gates and betas, a step per lane
   uint64_t cuts;

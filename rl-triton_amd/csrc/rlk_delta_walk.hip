@@ -21,7 +21,8 @@ struct Lds {
 };
 
 // The shared part of a walk: a chunk's arrays on their way to LDS, and the weighted q . k.
-template <class E, int D, bool VEC, int PARTS_OF_P>
+// QUERIES: else only the keys and M are.
+template <class E, int D, bool VEC, int PARTS_OF_P, bool QUERIES = true>
 struct Shared {
   static constexpr int NT = 4 * D;
   typedef Lds<E, D, PARTS_OF_P> M;
@@ -33,7 +34,7 @@ struct Shared {
     const int64_t s0 = chunk * C;
     const int n = (int)(r.seq_len - s0 < C ? r.seq_len - s0 : C);
     k.fetch(r.k.data + env * r.k.env + head * r.k.head + s0 * r.k.step, r.k.step, r.dk, n);
-    q.fetch(r.q.data + env * r.q.env + head * r.q.head + s0 * r.q.step, r.q.step, r.dk, n);
+    if constexpr (QUERIES) q.fetch(r.q.data + env * r.q.env + head * r.q.head + s0 * r.q.step, r.q.step, r.dk, n);
     const f32x4* rec = reinterpret_cast<const f32x4*>(r.records + pair * r.chunks + chunk);
 #pragma unroll
     for (int i = 0; i < TILES_PER; ++i) {
@@ -44,7 +45,7 @@ struct Shared {
   }
   __device__ __forceinline__ void put(char* lds, int dk, int n) const {
     k.put(lds + M::K, dk, 0, n);
-    q.put(lds + M::Q, dk, 0, n);
+    if constexpr (QUERIES) q.put(lds + M::Q, dk, 0, n);
 #pragma unroll
     for (int i = 0; i < TILES_PER; ++i) {
       const int u = threadIdx.x + NT * i;
@@ -183,18 +184,27 @@ __device__ __forceinline__ f32x4 columns_quad(const E (&x)[16], int t, int dim, 
   return y;
 }
 
-template <class E, int D, bool VEC>
+// TRANSITION: no outputs, but what a segment does to the state that enters it: the state that it leaves from none (blockIdx.z 1), and from the
+// unit vectors with no values (0).
+template <class E, int D, bool VEC, bool TRANSITION>
 __global__ __launch_bounds__(4 * D, D == 128 || kParts<E> == 1 ? 2 : 1) void forward_kernel(const Rule<E> r) {
   constexpr int MT = D / 16, KK = D / 32, N = kParts<E>, NO = N == 1 ? 2 : 3, UPTO = NO - 1;  // (parts of a factor of the outputs)
-  typedef Shared<E, D, VEC, NO> Sh;
+  typedef Shared<E, D, VEC, NO, !TRANSITION> Sh;
   typedef typename Sh::M M;
   typedef typename M::Rows_ T;
   __shared__ __align__(16) char lds[M::BYTES];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l16 = lane & 15, l4 = lane >> 4;
   const int64_t pair = blockIdx.x, env = r.first_env + pair / r.heads, eh = r.first_env * r.heads + pair;
-  const int head = (int)(pair % r.heads), dk = r.dk, dv = r.dv, dvp = pad16(dv);
+  const int head = (int)(pair % r.heads), dk = r.dk, seg = blockIdx.y;
+  const bool units = TRANSITION && blockIdx.z == 0;
+  const int dv = units ? dk : r.dv, dvp = pad16(dv);
   const bool mine = 16 * wave < dv;
   const int j = 16 * wave + l16;
+  int64_t first = seg * r.seg_chunks, last = first + r.seg_chunks < r.chunks ? first + r.seg_chunks : r.chunks;
+  if (!TRANSITION && r.segs > 1 && r.wild[pair] != 0) {
+    if (seg > 0) return;
+    last = r.chunks;
+  }
   const E* gv = r.v.data + env * r.v.env + head * r.v.head;
   E* gy = r.y.data + env * r.y.env + head * r.y.head;
 
@@ -203,18 +213,31 @@ __global__ __launch_bounds__(4 * D, D == 128 || kParts<E> == 1 ? 2 : 1) void for
   const At<typename M::P> at_p;
   Sh sh;
   E v[16];
-  sh.fetch(r, env, head, pair, 0);
-  if (mine) load_columns(gv, r.v.step, dv, (int)(r.seq_len < C ? r.seq_len : C), v);
+  sh.fetch(r, env, head, pair, first);
+  if (mine && !units) load_columns(gv + first * C * r.v.step, r.v.step, dv, (int)(r.seq_len - first * C < C ? r.seq_len - first * C : C), v);
   f32x4 S[MT];
-  load_state(r.state ? r.state + eh * dk * dv : nullptr, dk, dv, false, S);
+  if constexpr (TRANSITION) {
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int x = 0; x < 4; ++x) S[m][x] = units && 16 * m + 4 * l4 + x == j && j < dk ? 1.f : 0.f;
+  } else if (seg == 0) {
+    load_state(r.state ? r.state + eh * dk * dv : nullptr, dk, dv, false, S);
+  } else {
+    const float* p = r.seg_states + (pair * r.segs + seg) * (int64_t)pad16(dk) * dvp + j;
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int x = 0; x < 4; ++x) S[m][x] = mine && 16 * m < dk ? p[(16 * m + 4 * l4 + x) * dvp] : 0.f;
+  }
 
-  for (int64_t chunk = 0; chunk < r.chunks; ++chunk) {
+  for (int64_t chunk = first; chunk < last; ++chunk) {
     const int64_t s0 = chunk * C;
     const int n = (int)(r.seq_len - s0 < C ? r.seq_len - s0 : C);
     sh.put(lds, dk, n);
     __syncthreads();
-    if (chunk + 1 < r.chunks) sh.fetch(r, env, head, pair, chunk + 1);
-    Sh::form_p(lds, r.scale, at);
+    if (chunk + 1 < last) sh.fetch(r, env, head, pair, chunk + 1);
+    if constexpr (!TRANSITION) Sh::form_p(lds, r.scale, at);
     const Record& rec = Sh::record(lds);
 
     f32x4 e[4], y[4];  // corrections (column j, steps 16 t + 4 l4 + ..); outputs, transposed (step 16 t + l16, columns 16 wave + 4 l4 + ..)
@@ -229,7 +252,7 @@ __global__ __launch_bounds__(4 * D, D == 128 || kParts<E> == 1 ? 2 : 1) void for
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
           ks[t] = mul<2>(at.rows(lds + M::K, t, kk), s, ks[t]);
-          y[t] = mul<UPTO>(s, at.rows(lds + M::Q, t, kk), y[t]);
+          if constexpr (!TRANSITION) y[t] = mul<UPTO>(s, at.rows(lds + M::Q, t, kk), y[t]);
           if (t & 1) apart();
         }
       }
@@ -237,7 +260,7 @@ __global__ __launch_bounds__(4 * D, D == 128 || kParts<E> == 1 ? 2 : 1) void for
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
         const f32x4 back = *reinterpret_cast<const f32x4*>(rec.back + 16 * t + 4 * l4);
-        e[t] = columns_quad(v, t, dv, n);
+        e[t] = units ? zero4() : columns_quad(v, t, dv, n);
 #pragma unroll
         for (int x = 0; x < 4; ++x)
           if (back[x] != 0.f) e[t][x] = fmaf(-back[x], ks[t][x], e[t][x]);  // (a state that does not reach a step has no part, NaN included)
@@ -246,7 +269,7 @@ __global__ __launch_bounds__(4 * D, D == 128 || kParts<E> == 1 ? 2 : 1) void for
 #pragma unroll
         for (int x = 0; x < 4; ++x) y[t][x] = into_step != 0.f ? y[t][x] * (into_step * r.scale) : 0.f;
       }
-      if (chunk + 1 < r.chunks)
+      if (chunk + 1 < last && !units)
         load_columns(gv + (s0 + C) * r.v.step, r.v.step, dv, (int)(r.seq_len - s0 - C < C ? r.seq_len - s0 - C : C), v);
       const Op<3> b[2] = {split<3>(be[0], be[1]), split<3>(be[2], be[3])};
 #pragma unroll
@@ -261,7 +284,7 @@ __global__ __launch_bounds__(4 * D, D == 128 || kParts<E> == 1 ? 2 : 1) void for
       for (int t = 0; t < 4; ++t) be[t] = e[t] * *reinterpret_cast<const f32x4*>(rec.beta + 16 * t + 4 * l4);
       u[0] = split<3>(be[0], be[1]), u[1] = split<3>(be[2], be[3]);
     }
-    __syncthreads();
+    if constexpr (!TRANSITION) __syncthreads();
     if (mine) {
       Op<NO> uo[2];
 #pragma unroll
@@ -271,18 +294,18 @@ __global__ __launch_bounds__(4 * D, D == 128 || kParts<E> == 1 ? 2 : 1) void for
 #pragma unroll
       for (int t = 0; t < 4; ++t)
 #pragma unroll
-        for (int kk = 0; kk <= t / 2; ++kk) y[t] = mul<UPTO>(uo[kk], at_p.rows(lds + M::PT, t, kk), y[t]);
+        for (int kk = 0; kk <= t / 2; ++kk) if constexpr (!TRANSITION) y[t] = mul<UPTO>(uo[kk], at_p.rows(lds + M::PT, t, kk), y[t]);
       float check = 0.f;
 #pragma unroll
       for (int t = 0; t < 4; ++t) check = odd(e[t], odd(y[t], check));
-      if (r.states != nullptr) keep_state(r.states + (pair * r.chunks + chunk) * (int64_t)pad16(dk) * dvp, dvp, pad16(dk), S);
-      float* w = r.w != nullptr ? r.w + (pair * r.chunks + chunk) * (int64_t)C * dvp : nullptr;
+      if (!TRANSITION && r.states != nullptr) keep_state(r.states + (pair * r.chunks + chunk) * (int64_t)pad16(dk) * dvp, dvp, pad16(dk), S);
+      float* w = !TRANSITION && r.w != nullptr ? r.w + (pair * r.chunks + chunk) * (int64_t)C * dvp : nullptr;
       settle();
       if (rec.wild == 0 && __all(check == 0.f)) {
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
           const int i = 16 * t + l16, c = 16 * wave + 4 * l4;
-          if (i < n) {
+          if (!TRANSITION && i < n) {
             E* p = gy + (s0 + i) * r.y.step + c;
             if constexpr (VEC) {
               if (c < dv) store_quad<false>(p, float4{y[t][0], y[t][1], y[t][2], y[t][3]});
@@ -309,6 +332,8 @@ __global__ __launch_bounds__(4 * D, D == 128 || kParts<E> == 1 ? 2 : 1) void for
           if (m & 1) apart();
         }
         settle();
+      } else if (TRANSITION) {
+        if (lane == 0) r.wild[pair] = 1;
       } else {
         // step by step: what is not finite reaches no step before it, and none past its episode's end
         for (int i = 0; i < n; ++i) {
@@ -351,8 +376,77 @@ __global__ __launch_bounds__(4 * D, D == 128 || kParts<E> == 1 ? 2 : 1) void for
     }
     __syncthreads();
   }
-  if (mine && r.state_out != nullptr)
+  if constexpr (TRANSITION) {
+    if (!mine) return;
+    float check = 0.f;
+#pragma unroll
+    for (int m = 0; m < MT; ++m) check = odd(S[m], check);
+    if (__any(check != 0.f) && lane == 0) r.wild[pair] = 1;
+    const int64_t rows = pad16(dk);
+    keep_state(units ? r.phi + (pair * r.segs + seg) * rows * rows : r.seg_states + (pair * r.segs + seg + 1) * rows * dvp, dvp, (int)rows, S);
+    return;
+  }
+  if (mine && r.state_out != nullptr && last == r.chunks)
     store_state(r.state_out + eh * dk * dv, dk, dv, r.dones != nullptr && r.dones[env * r.seq_len + r.seq_len - 1] != 0.f, S);
+}
+
+// The states that enter the segments, one after the other: S' = phi S + n.  A workgroup per pair and 16 columns, a wavefront per 16 rows; the
+// columns are exchanged through LDS, and the next segment's rows of phi are on their way.
+template <int D>
+__global__ __launch_bounds__(4 * D) void join_kernel(const Rule<float> r, const float* state) {
+  constexpr int KK = D / 32, ROW = D + 4;
+  __shared__ __align__(16) float S[2][16 * ROW];  // [column, row]
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l16 = lane & 15, l4 = lane >> 4;
+  const int64_t pair = blockIdx.x, eh = r.first_env * r.heads + pair;
+  const int dk = r.dk, dv = r.dv, rows = pad16(dk), dvp = pad16(dv), j = 16 * blockIdx.y + l16, d0 = 16 * wave + 4 * l4;
+  const bool mine = 16 * wave < rows;
+  if (r.wild[pair] != 0) return;
+#pragma unroll
+  for (int x = 0; x < 4; ++x)
+    S[0][l16 * ROW + d0 + x] = state != nullptr && d0 + x < dk && j < dv ? state[eh * dk * dv + (int64_t)(d0 + x) * dv + j] : 0.f;
+  const float* phi = r.phi + pair * r.segs * (int64_t)rows * rows + (16 * wave + l16) * rows;
+  float* n = r.seg_states + (pair * r.segs + 1) * (int64_t)rows * dvp + d0 * dvp + j;
+  f32x4 next[KK][2], add;
+  auto fetch = [&] {
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int d = 32 * kk + 16 * h + 4 * l4;
+        next[kk][h] = *reinterpret_cast<const f32x4*>(phi + (d < rows ? d : 0));
+      }
+#pragma unroll
+    for (int x = 0; x < 4; ++x) add[x] = n[x * dvp];
+  };
+  if (mine) fetch();
+  for (int s = 1; s < r.segs; ++s) {
+    __syncthreads();
+    const float* from = S[(s - 1) & 1];
+    if (mine) {
+      f32x4 acc = add;
+      Op<3> a[KK];
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk) a[kk] = split<3>(next[kk][0], next[kk][1]);
+      float* out = n;
+      phi += (int64_t)rows * rows, n += (int64_t)rows * dvp;
+      if (s + 1 < r.segs) fetch();
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk) {
+        // (rows past the last are 0 in S, and what phi has in their place is finite)
+        const f32x4 lo = *reinterpret_cast<const f32x4*>(from + l16 * ROW + 32 * kk + 4 * l4), hi = *reinterpret_cast<const f32x4*>(from + l16 * ROW + 32 * kk + 16 + 4 * l4);
+        acc = mul<2>(a[kk], split<3>(lo, hi), acc);
+      }
+      settle();
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        out[x * dvp] = acc[x];
+        S[s & 1][l16 * ROW + d0 + x] = acc[x];
+      }
+    } else {
+#pragma unroll
+      for (int x = 0; x < 4; ++x) S[s & 1][l16 * ROW + d0 + x] = 0.f;
+    }
+  }
 }
 
 // The way back: R, the gradient of the state, from the last chunk to the first.
@@ -529,17 +623,22 @@ __global__ __launch_bounds__(4 * D, D == 128 || kParts<E> == 1 ? 2 : 1) void bac
 
 }  // namespace
 
+template <class E, int D, bool VEC>
+void forward_launches(const Rule<E>& r, int64_t pairs, hipStream_t s) {
+  if (r.segs > 1) {
+    forward_kernel<E, D, VEC, true><<<dim3((unsigned)pairs, (unsigned)r.segs - 1, 2), dim3(4 * D), 0, s>>>(r);
+    Rule<float> j = {};
+    j.first_env = r.first_env, j.heads = r.heads, j.dk = r.dk, j.dv = r.dv, j.segs = r.segs, j.phi = r.phi, j.seg_states = r.seg_states, j.wild = r.wild;
+    join_kernel<D><<<dim3((unsigned)pairs, (unsigned)pad16(r.dv) / 16), dim3(4 * D), 0, s>>>(j, r.state);
+  }
+  forward_kernel<E, D, VEC, false><<<dim3((unsigned)pairs, (unsigned)r.segs), dim3(4 * D), 0, s>>>(r);
+}
 template <class E>
 int launch_forward(const Rule<E>& r, int64_t envs, hipStream_t s) {
-  const dim3 grid((unsigned)(envs * r.heads));
+  const int64_t pairs = envs * r.heads;
   const bool vec = fours(r.k, r.dk) && fours(r.q, r.dk) && fours(r.y, r.dv);
-  if (r.dk <= 64 && r.dv <= 64) {
-    if (vec) forward_kernel<E, 64, true><<<grid, dim3(256), 0, s>>>(r);
-    else forward_kernel<E, 64, false><<<grid, dim3(256), 0, s>>>(r);
-  } else {
-    if (vec) forward_kernel<E, 128, true><<<grid, dim3(512), 0, s>>>(r);
-    else forward_kernel<E, 128, false><<<grid, dim3(512), 0, s>>>(r);
-  }
+  if (r.dk <= 64 && r.dv <= 64) vec ? forward_launches<E, 64, true>(r, pairs, s) : forward_launches<E, 64, false>(r, pairs, s);
+  else vec ? forward_launches<E, 128, true>(r, pairs, s) : forward_launches<E, 128, false>(r, pairs, s);
   return hipGetLastError() == hipSuccess ? RLK_OK : RLK_ERR_LAUNCH;
 }
 template <class E>

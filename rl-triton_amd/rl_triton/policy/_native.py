@@ -266,7 +266,7 @@ def gated_delta_rule(dev, stream, q, k, v, out, log_decays, betas, dones, state,
     lib = _lib or load()
     e, t, h, dk = q.shape
     saved = _scratch(lib.rlk_delta_rule_saved_bytes(e, t, h, dk, v.shape[-1]), q) if keep else None
-    ws = None if keep else _scratch(lib.rlk_delta_rule_workspace_bytes(e, t, h, dk, v.shape[-1], 0), q)
+    ws = _scratch(lib.rlk_delta_rule_workspace_bytes(e, t, h, dk, v.shape[-1], 0), q)
     call = _delta_rule(q, k, v, out, log_decays, betas, dones, state, state_out, scale, ws)
     _native._check(lib.rlk_gated_delta_rule(ctypes.byref(call), _ptr(saved), _bytes(saved), stream), "rlk_gated_delta_rule")
     return saved

@@ -95,6 +95,53 @@ def test_gradients_against_differences():
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", [(1, 2500, 2, 40, 64), (2, 2049, 1, 128, 100), (1, 4100, 3, 16, 24)])
+def test_long_sequences_of_few_heads(shape, dtype):
+    """Sequences that are cut into segments, with and without episode ends in them, and the same with gradients."""
+    E, T, H, dk, dv = shape
+    for ends, state in ((None, True), (0.002, True), (0.02, False)):
+        x = inputs(*shape, dtype, T + dv, ends, state)
+        d = _cuda(*x)
+        out, last = policy.compute_gated_delta_rule(*d, 0.7)
+        g = torch.Generator().manual_seed(T)
+        go, gs = torch.randn(E, T, H, dv, generator=g).to(dtype), torch.randn(E, H, dk, dv, generator=g)
+        want, wlast, grads = rule(*x, 0.7, go, gs)
+        _hold(out, want, dtype, T, dk, "out")
+        held(last, wlast, relative(T, dk), "state")
+        leaves = [d[i].requires_grad_() for i in (0, 1, 2, 3, 4, 6) if d[i] is not None]
+        again, again_last = policy.compute_gated_delta_rule(*d, 0.7)
+        assert torch.equal(again, out) and torch.equal(again_last, last)
+        got = torch.autograd.grad((again, again_last), leaves, _cuda(go, gs))
+        size = float((x[0].double() * grads[0]).norm() + (x[1].double() * grads[1]).norm())
+        for i, (a, b) in enumerate(zip(got, grads)):
+            if i < 3:
+                _hold(a, b, dtype, T, dk, i)
+            else:
+                held(a, b, relative(T, dk), i, size if i == 3 else 0.0)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_bad_numbers_in_long_sequences(dtype):
+    """A head with a NaN, and one whose state grows out of float32 though none is there at first, are walked without segments; the others as before."""
+    shape = (1, 2600, 4, 24, 32)
+    x = list(inputs(*shape, dtype, 21, None, False, gates=False))
+    x[5] = torch.zeros(1, 2600)
+    x[5][:, 1400] = x[5][:, 2000] = 1.0
+    clean = policy.compute_gated_delta_rule(*_cuda(*x), 1.0)
+    x[2][0, 1700, 1, 3] = math.nan
+    x[1][0, 1401:2001, 2] *= 20.0
+    x[2][0, :2001, 2] = 0.0  # (nothing is written before)
+    out, last = policy.compute_gated_delta_rule(*_cuda(*x), 1.0)
+    want, wlast = rule(*x, 1.0)
+    for h in (0, 3):
+        assert torch.equal(out[:, :, h], clean[0][:, :, h]) and torch.equal(last[:, h], clean[1][:, h])
+    _hold(out[:, :1700, 1], want[:, :1700, 1], dtype, 2600, 24, "before")
+    _hold(out[:, 2001:, 1], want[:, 2001:, 1], dtype, 2600, 24, "after")
+    _hold(out[:, :, 2], want[:, :, 2], dtype, 2600, 24, "a state of zeros stays one")
+    held(last, wlast, relative(2600, 24))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_layouts(dtype):
     """Time-major views, slices of a joint projection, misaligned and element-strided tensors, shared heads: the same bits."""
     x = inputs(3, 90, 4, 32, 32, dtype, 3)
