@@ -134,6 +134,12 @@ __device__ __forceinline__ int opaque(int x) {
   return x;
 }
 
+// The same for a stride, which all lanes have: multiples of it are formed again by the scalar unit, and not held in more scalar registers than there are.
+__device__ __forceinline__ int64_t opaque_stride(int64_t x) {
+  asm volatile("" : "+s"(x));
+  return x;
+}
+
 // ---- tiles in LDS: parts of bfloat16, row by row.
 template <class E, int D>
 struct Tile {
@@ -263,7 +269,8 @@ struct Rows {
   static constexpr int PER = C * D / 4 / NT, GROUPS = D / 4;
   static constexpr int APART = NT / GROUPS;  // rows from one of a thread's to the next
   Four<E> x[PER];
-  __device__ __forceinline__ void fetch(const E* first, int64_t step, int dim, int count) {
+  __device__ __forceinline__ void fetch(const E* first, int64_t stride, int dim, int count) {
+    const int64_t step = opaque_stride(stride);
     const int tid = opaque(threadIdx.x), r0 = tid / GROUPS, col = tid % GROUPS * 4;
     if (count == C) {
       const E* p = first + r0 * step;
@@ -328,7 +335,7 @@ struct Segments {
   int64_t chunks;
 };
 inline Segments plan_segments(int64_t pairs, int64_t chunks) {
-  int64_t segs = 2 * device_cus() / pairs;
+  int64_t segs = device_cus() / pairs;
   if (segs > chunks / 8) segs = chunks / 8;
   if (segs < 4) return {1, chunks};
   const int64_t per = (chunks + segs - 1) / segs;

@@ -134,7 +134,8 @@ __device__ __forceinline__ void store_state(float* p, int dk, int dv, bool none,
 }
 // ... into the workspace, [rows, columns] of whole tiles.
 template <int MT>
-__device__ __forceinline__ void keep_state(float* p, int columns, int rows, const f32x4 (&S)[MT]) {
+__device__ __forceinline__ void keep_state(float* p, int stride, int rows, const f32x4 (&S)[MT]) {
+  const int64_t columns = opaque_stride(stride);
   const int tid = opaque(threadIdx.x), lane = tid & 63;
   p += 4 * (lane >> 4) * columns + 16 * (tid >> 6) + (lane & 15);
 #pragma unroll
@@ -144,7 +145,8 @@ __device__ __forceinline__ void keep_state(float* p, int columns, int rows, cons
       for (int e = 0; e < 4; ++e) p[(16 * m + e) * columns] = S[m][e];
 }
 // ... a chunk's rows of a wavefront's columns.
-__device__ __forceinline__ void keep_columns(float* p, int columns, const f32x4 (&x)[4]) {
+__device__ __forceinline__ void keep_columns(float* p, int stride, const f32x4 (&x)[4]) {
+  const int64_t columns = opaque_stride(stride);
   const int tid = opaque(threadIdx.x), lane = tid & 63;
   p += 4 * (lane >> 4) * columns + 16 * (tid >> 6) + (lane & 15);
 #pragma unroll
@@ -155,7 +157,8 @@ __device__ __forceinline__ void keep_columns(float* p, int columns, const f32x4 
 
 // A wavefront's 16 columns of an array's chunk: column 16 wave + l16, rows 16 t + 4 l4 + 0..3.
 template <class E>
-__device__ __forceinline__ void load_columns(const E* first, int64_t step, int dim, int n, E (&x)[16]) {
+__device__ __forceinline__ void load_columns(const E* first, int64_t stride, int dim, int n, E (&x)[16]) {
+  const int64_t step = opaque_stride(stride);
   const int tid = opaque(threadIdx.x), lane = tid & 63, l4 = lane >> 4, j = 16 * (tid >> 6) + (lane & 15);
   const E* p = first + (j < dim ? j : dim - 1);
   if (n == C) {
@@ -177,6 +180,8 @@ __device__ __forceinline__ void load_columns(const E* first, int64_t step, int d
 // ... as numbers, 0 where there is nothing.
 template <class E>
 __device__ __forceinline__ f32x4 columns_quad(const E (&x)[16], int t, int dim, int n) {
+  if (n == C && 16 * __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) + 16 <= dim)
+    return f32x4{to_f32(x[4 * t]), to_f32(x[4 * t + 1]), to_f32(x[4 * t + 2]), to_f32(x[4 * t + 3])};
   const int lane = threadIdx.x & 63, l4 = lane >> 4, j = 16 * (threadIdx.x >> 6) + (lane & 15);
   f32x4 y;
 #pragma unroll
@@ -261,13 +266,11 @@ __global__ __launch_bounds__(4 * D, D == 128 || kParts<E> == 1 ? 2 : 1) void for
       for (int t = 0; t < 4; ++t) {
         const f32x4 back = *reinterpret_cast<const f32x4*>(rec.back + 16 * t + 4 * l4);
         e[t] = units ? zero4() : columns_quad(v, t, dv, n);
+        // (a state that is not finite makes these NaN, where it does not reach a step too: then the chunk goes step by step)
 #pragma unroll
-        for (int x = 0; x < 4; ++x)
-          if (back[x] != 0.f) e[t][x] = fmaf(-back[x], ks[t][x], e[t][x]);  // (a state that does not reach a step has no part, NaN included)
+        for (int x = 0; x < 4; ++x) e[t][x] = fmaf(-back[x], ks[t][x], e[t][x]);
         be[t] = e[t] * *reinterpret_cast<const f32x4*>(rec.beta + 16 * t + 4 * l4);
-        const float into_step = rec.back[16 * t + l16];
-#pragma unroll
-        for (int x = 0; x < 4; ++x) y[t][x] = into_step != 0.f ? y[t][x] * (into_step * r.scale) : 0.f;
+        if constexpr (!TRANSITION) y[t] *= rec.back[16 * t + l16] * r.scale;
       }
       if (chunk + 1 < last && !units)
         load_columns(gv + (s0 + C) * r.v.step, r.v.step, dv, (int)(r.seq_len - s0 - C < C ? r.seq_len - s0 - C : C), v);
@@ -326,7 +329,7 @@ __global__ __launch_bounds__(4 * D, D == 128 || kParts<E> == 1 ? 2 : 1) void for
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
 #pragma unroll
-          for (int z = 0; z < 4; ++z) S[m][z] = keep != 0.f ? S[m][z] * keep : 0.f;
+          for (int z = 0; z < 4; ++z) S[m][z] *= keep;
 #pragma unroll
           for (int kk = 0; kk < 2; ++kk) S[m] = mul<2>(at.columns(lds + M::K, m, kk), a[kk], S[m]);
           if (m & 1) apart();
@@ -500,9 +503,7 @@ __global__ __launch_bounds__(4 * D, D == 128 || kParts<E> == 1 ? 2 : 1) void bac
       }
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
-        const f32x4 into = *reinterpret_cast<const f32x4*>(rec.into + 16 * t + 4 * l4);
-#pragma unroll
-        for (int x = 0; x < 4; ++x) z[t][x] = into[x] != 0.f ? z[t][x] * into[x] : 0.f;
+        z[t] *= *reinterpret_cast<const f32x4*>(rec.into + 16 * t + 4 * l4);  // (NaN if R is not finite: then step by step)
       }
     }
     __syncthreads();
@@ -540,18 +541,14 @@ __global__ __launch_bounds__(4 * D, D == 128 || kParts<E> == 1 ? 2 : 1) void bac
         for (int t = 0; t < 4; ++t) {
           const f32x4 back = *reinterpret_cast<const f32x4*>(rec.back + 16 * t + 4 * l4);
           dvs[t] = z[t] * *reinterpret_cast<const f32x4*>(rec.beta + 16 * t + 4 * l4);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            x[t][i] = back[i] != 0.f ? -back[i] * dvs[t][i] : 0.f;
-            bg[t][i] = back[i] != 0.f ? r.scale * back[i] * go[t][i] : 0.f;
-          }
+          x[t] = -(back * dvs[t]), bg[t] = (back * r.scale) * go[t];
         }
         const Op<3> a[2] = {split<3>(x[0], x[1]), split<3>(x[2], x[3])}, b[2] = {split<3>(bg[0], bg[1]), split<3>(bg[2], bg[3])};
         const float keep = rec.keep;
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) next[m][i] = keep != 0.f ? R[m][i] * keep : 0.f;
+          for (int i = 0; i < 4; ++i) next[m][i] = R[m][i] * keep;
 #pragma unroll
           for (int kk = 0; kk < 2; ++kk) {
             next[m] = mul<2>(at.columns(lds + M::K, m, kk), a[kk], next[m]);
