@@ -212,6 +212,18 @@ __device__ __forceinline__ float number_at(const char* tile, int i, int d) {
   return x;
 }
 
+// ... and of 4 columns from d on.
+template <class T>
+__device__ __forceinline__ f32x4 numbers_at(const char* tile, int i, int d) {
+  f32x4 x = zero4();
+#pragma unroll
+  for (int n = T::N - 1; n >= 0; --n) {
+    const u32x2 w = *reinterpret_cast<const u32x2*>(tile + n * T::PART + T::row(i) + 2 * d);
+    x += f32x4{__uint_as_float(w[0] << 16), __uint_as_float(w[0] & 0xffff0000u), __uint_as_float(w[1] << 16), __uint_as_float(w[1] & 0xffff0000u)};
+  }
+  return x;
+}
+
 // 4 consecutive elements as they are stored.
 template <class E>
 struct Four;

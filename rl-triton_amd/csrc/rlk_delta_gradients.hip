@@ -56,35 +56,43 @@ __global__ __launch_bounds__(4 * D, D == 128 || kParts<E> == 1 ? 2 : 1) void gra
   typedef typename M::K T;
   __shared__ __align__(16) char lds[M::BYTES];
   __shared__ float sums[WAVES][C + 2];
-  __shared__ float beta[C];
   __shared__ int found[WAVES];
+  constexpr int REST_QUADS = (int)(sizeof(Record) - offsetof(Record, ghi)) / 16;
+  __shared__ f32x4 rest_of_record[REST_QUADS];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l16 = lane & 15, l4 = lane >> 4;
   const int64_t at = blockIdx.x, pair = at / r.chunks, chunk = at - pair * r.chunks, s0 = chunk * C;
   const int64_t env = r.first_env + pair / r.heads;
   const int head = (int)(pair % r.heads), dk = r.dk, dv = r.dv, dvp = pad16(dv);
   const int n = (int)(r.seq_len - s0 < C ? r.seq_len - s0 : C);
-  const Record& rec = r.records[at];
-  const uint64_t cuts = rec.cuts[0] | (uint64_t)rec.cuts[1] << 32;
+  const Record& rec = *reinterpret_cast<const Record*>(reinterpret_cast<const char*>(rest_of_record) - offsetof(Record, ghi));  // (in LDS, without M)
 
+  // all of the first loads together
+  const bool mine = 16 * wave < dk;
+  const float *w = r.w + at * C * dvp, *z = r.z + at * C * dvp;
+  const int64_t state = at * pad16(dk) * dvp + (int64_t)(16 * wave + l16) * dvp;
+  Corrections<NT> ws, zs;
+  Rows<E, 64, NT, VEC> gs;
+  const E* gg = r.gy.data + env * r.gy.env + head * r.gy.head + s0 * r.gy.step;
+  f32x4 sq[2][2], rq[2][2];  // 64 columns of the wavefront's rows of S and R
+  auto fetch = [&](int c0) {
+    gs.fetch(gg + c0, r.gy.step, dv - c0, n);
+    ws.fetch(w, c0, dvp);
+    zs.fetch(z, c0, dvp);
+    if (mine)
+#pragma unroll
+      for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int c = c0 + 32 * kk + 16 * h + 4 * l4, cc = c < dvp ? c : 0;
+          sq[kk][h] = *reinterpret_cast<const f32x4*>(r.states + state + cc);
+          rq[kk][h] = *reinterpret_cast<const f32x4*>(r.dstates + state + cc);
+        }
+  };
+  if (threadIdx.x < REST_QUADS) rest_of_record[threadIdx.x] = reinterpret_cast<const f32x4*>(r.records[at].ghi)[threadIdx.x];
+  fetch(0);
   Rows<E, D, NT, VEC> k, q;
   k.fetch(r.k.data + env * r.k.env + head * r.k.head + s0 * r.k.step, r.k.step, dk, n);
   q.fetch(r.q.data + env * r.q.env + head * r.q.head + s0 * r.q.step, r.q.step, dk, n);
-  {
-    float sum = 0.f;
-#pragma unroll
-    for (int i = 0; i < Rows<E, D, NT, VEC>::PER; ++i) {
-      const f32x4 a = k.x[i].floats(), b = q.x[i].floats();
-#pragma unroll
-      for (int x = 0; x < 4; ++x) sum = fmaf(0.f, a[x], fmaf(0.f, b[x], sum));
-    }
-    const bool any = __any(sum != 0.f);
-    if (lane == 0) found[wave] = any;
-  }
-  if (threadIdx.x < C) beta[threadIdx.x] = rec.beta[threadIdx.x];
-  const E* gg = r.gy.data + env * r.gy.env + head * r.gy.head + s0 * r.gy.step;
-  const float *w = r.w + at * C * dvp, *z = r.z + at * C * dvp;
-  const int64_t state = at * pad16(dk) * dvp;
-  const bool mine = 16 * wave < dk;
   const At<typename M::G> at_g;
   const At<typename M::U> at_u;
   const At<T> at_k;
@@ -94,74 +102,71 @@ __global__ __launch_bounds__(4 * D, D == 128 || kParts<E> == 1 ? 2 : 1) void gra
   f32x4 dq[4], up[4], down[4];  // (up, down: dk+ and dk-)
 #pragma unroll
   for (int t = 0; t < 4; ++t) dq[t] = up[t] = down[t] = zero4();
-  // Y1 and Y2, rows ti: transposed too, steps i = 16 ti + l16, j = 16 tj + 4 l4 + 0..3.  8 wavefronts share: the first 4 have Y1, the others Y2
-  constexpr bool BOTH = WAVES == 4;
-  const int ti = wave & 3;
-  f32x4 ya[4], yb[4];
+  // Y1 and Y2: transposed too, steps i = 16 ti + l16, j = 16 tj + 4 l4 + 0..3.  A wavefront has rows of one of them: of 4 wavefronts two have
+  // rows 3 and 0, two 2 and 1, 5 tiles each; of 8 each has one row.
+  constexpr int ROWS = WAVES == 4 ? 2 : 1, TILES = WAVES == 4 ? 5 : 4;
+  const bool second = wave & 1;
+  const int row_a = ROWS == 2 ? 3 - (wave >> 1) : wave >> 1, row_b = wave >> 1;
+  auto tile_of = [&](int slot, int& ti, int& tj) {  // whether there is one
+    ti = ROWS == 2 && slot > row_a ? row_b : row_a, tj = ROWS == 2 && slot > row_a ? slot - row_a - 1 : slot;
+    return tj <= ti;
+  };
+  f32x4 ya[TILES];
 #pragma unroll
-  for (int t = 0; t < 4; ++t) ya[t] = yb[t] = zero4();
-  const bool first = BOTH || wave < 4;
+  for (int t = 0; t < TILES; ++t) ya[t] = zero4();
   float kept = 0.f;
-  f32x4 db = zero4();  // (of the steps of this thread's parts of w and z)
   constexpr int PER = Corrections<NT>::PER;
   static_assert(PER <= 4);
+  float db[PER];  // (of the steps of this thread's parts of w and z)
+#pragma unroll
+  for (int i = 0; i < PER; ++i) db[i] = 0.f;
 
+  __syncthreads();  // the record is there
+  const uint64_t cuts = rec.cuts[0] | (uint64_t)rec.cuts[1] << 32;
   for (int c0 = 0; c0 < dv; c0 += 64) {
-    Rows<E, 64, NT, VEC> gs;
-    Corrections<NT> ws, zs;
-    gs.fetch(gg + c0, r.gy.step, dv - c0, n);
-    ws.fetch(w, c0, dvp);
-    zs.fetch(z, c0, dvp);
     if (c0 > 0) __syncthreads();
     gs.put(lds, dv - c0, 0, n);
-    if (c0 == 0) __syncthreads();  // (beta is there)
-    ws.put(lds + M::UT, beta);
-    zs.put(lds + M::DT, beta);
+    ws.put(lds + M::UT, rec.beta);
+    zs.put(lds + M::DT, rec.beta);
 #pragma unroll
     for (int i = 0; i < PER; ++i)
 #pragma unroll
       for (int x = 0; x < 4; ++x) db[i] = fmaf(ws.x[i][x], zs.x[i][x], db[i]);
     __syncthreads();
-    const int kks = dv - c0 > 32 ? 2 : 1;
-    for (int kk = 0; kk < kks; ++kk) {
-      {
-        const Op<N> g = at_g.rows(lds, ti, kk);
-        const Op<3> d = at_u.rows(lds + M::DT, ti, kk);
 #pragma unroll
-        for (int tj = 0; tj < 4; ++tj) {
-          if (tj > ti) continue;
-          const Op<3> u = at_u.rows(lds + M::UT, tj, kk);
-          if constexpr (BOTH) {
-            ya[tj] = mul<2>(u, g, ya[tj]);
-            yb[tj] = mul<2>(u, d, yb[tj]);
-          } else if (first) {
-            ya[tj] = mul<2>(u, g, ya[tj]);
-          } else {
-            ya[tj] = mul<2>(u, d, ya[tj]);
-          }
-        }
+    for (int kk = 0; kk < 2; ++kk) {
+      if (c0 + 32 * kk >= dv) continue;
+#pragma unroll
+      for (int slot = 0; slot < TILES; ++slot) {
+        int ti, tj;
+        if (!tile_of(slot, ti, tj)) continue;
+        const Op<3> u = at_u.rows(lds + M::UT, tj, kk);
+        if (second) ya[slot] = mul<2>(u, at_u.rows(lds + M::DT, ti, kk), ya[slot]);
+        else ya[slot] = mul<2>(u, at_g.rows(lds, ti, kk), ya[slot]);
       }
       settle();
       if (mine) {
-        const int c = c0 + 32 * kk + 4 * l4;
-        const float *S = r.states + state + (16 * wave + l16) * dvp, *R = r.dstates + state + (16 * wave + l16) * dvp;
-        const f32x4 s_lo = *reinterpret_cast<const f32x4*>(S + (c < dvp ? c : 0)), s_hi = *reinterpret_cast<const f32x4*>(S + (c + 16 < dvp ? c + 16 : 0));
-        const f32x4 r_lo = *reinterpret_cast<const f32x4*>(R + (c < dvp ? c : 0)), r_hi = *reinterpret_cast<const f32x4*>(R + (c + 16 < dvp ? c + 16 : 0));
-        const f32x4 o = zero4();
-        const f32x4 a = c < dvp ? s_lo : o, b = c + 16 < dvp ? s_hi : o, e = c < dvp ? r_lo : o, f = c + 16 < dvp ? r_hi : o;
 #pragma unroll
-        for (int x = 0; x < 4; ++x) kept = fmaf(a[x], e[x], fmaf(b[x], f[x], kept));
-        const Op<3> s = split<3>(a, b), rr = split<3>(e, f);
+        for (int h = 0; h < 2; ++h) {
+          if (c0 + 32 * kk + 16 * h + 4 * l4 >= dvp) sq[kk][h] = rq[kk][h] = zero4();
+#pragma unroll
+          for (int x = 0; x < 4; ++x) kept = fmaf(sq[kk][h][x], rq[kk][h][x], kept);
+        }
+        const Op<3> s = split<3>(sq[kk][0], sq[kk][1]), rr = split<3>(rq[kk][0], rq[kk][1]);
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
           dq[t] = mul<2>(s, at_g.rows(lds, t, kk), dq[t]);
           up[t] = mul<2>(s, at_u.rows(lds + M::DT, t, kk), up[t]);
           down[t] = mul<2>(rr, at_u.rows(lds + M::UT, t, kk), down[t]);
+          apart();
         }
       }
       settle();
     }
+    if (c0 + 64 < dv) fetch(c0 + 64);
   }
+  k.fetch(r.k.data + env * r.k.env + head * r.k.head + s0 * r.k.step, r.k.step, dk, n);
+  q.fetch(r.q.data + env * r.q.env + head * r.q.head + s0 * r.q.step, r.q.step, dk, n);
   // db: a row's 16 parts
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
@@ -185,32 +190,39 @@ __global__ __launch_bounds__(4 * D, D == 128 || kParts<E> == 1 ? 2 : 1) void gra
       down[t][x] = into[t] != 0.f ? down[t][x] * into[t] : 0.f;
     }
   }
-  __syncthreads();  // all have read the first arrays
   {
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < Rows<E, D, NT, VEC>::PER; ++i) {
+      const f32x4 a = k.x[i].floats(), b = q.x[i].floats();
+#pragma unroll
+      for (int x = 0; x < 4; ++x) sum = fmaf(0.f, a[x], fmaf(0.f, b[x], sum));
+    }
+    const bool any = __any(sum != 0.f);
+    if (lane == 0) found[wave] = any;
+  }
+  __syncthreads();  // all have read the first arrays
+#pragma unroll
+  for (int slot = 0; slot < TILES; ++slot) {
+    int ti, tj;
+    if (!tile_of(slot, ti, tj)) continue;
     const int i = 16 * ti + l16;
     const uint64_t before = cuts & (((uint64_t)2 << i) - 1);
     const int begin = before != 0 ? 63 - __clzll((long long)before) : 0;
     const float hi = rec.ghi[i], lo = rec.glo[i];
+    const f32x4 hj = *reinterpret_cast<const f32x4*>(rec.ghi + 16 * tj + 4 * l4), lj = *reinterpret_cast<const f32x4*>(rec.glo + 16 * tj + 4 * l4);
+    f32x4 a = ya[slot];
 #pragma unroll
-    for (int tj = 0; tj < 4; ++tj) {
-      if (tj > (ti | 1)) continue;
-      f32x4 a = ya[tj], b = yb[tj];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int j = 16 * tj + 4 * l4 + e;
-        const bool same = tj <= ti && j >= begin;
-        const float d = same && j <= i ? expf((hi - rec.ghi[j]) + (lo - rec.glo[j])) : 0.f;
-        if constexpr (BOTH) {
-          a[e] = same && j <= i ? a[e] * (d * r.scale) : 0.f;
-          b[e] = same && j < i ? -b[e] * d : 0.f;
-        } else {
-          a[e] = first ? (same && j <= i ? a[e] * (d * r.scale) : 0.f) : (same && j < i ? -a[e] * d : 0.f);
-        }
-      }
-      const int place = M::Y::row(16 * ti) + l16 * (M::Y::row(16 * ti + 1) - M::Y::row(16 * ti)) + 2 * (16 * tj + 4 * l4);
-      Four<float>{a}.put(lds + (first ? M::Y1 : M::Y2) + place, M::Y::PART);
-      if constexpr (BOTH) Four<float>{b}.put(lds + M::Y2 + place, M::Y::PART);
+    for (int e = 0; e < 4; ++e) {
+      const int j = 16 * tj + 4 * l4 + e;
+      const float d = __expf((hi - hj[e]) + (lo - lj[e]));
+      a[e] = j >= begin && (second ? j < i : j <= i) ? a[e] * (second ? -d : d * r.scale) : 0.f;
     }
+    char* y = lds + (second ? M::Y2 : M::Y1);
+    const int first = M::Y::row(16 * ti), stride = ti < 2 ? M::Y::row(1) : M::Y::row(33) - M::Y::row(32);
+    Four<float>{a}.put(y + first + l16 * stride + 2 * (16 * tj + 4 * l4), M::Y::PART);
+    if (tj == ti && (ti & 1) == 0)  // the tile above the diagonal that products go over
+      Four<float>{zero4()}.put(y + first + l16 * stride + 2 * (16 * tj + 16 + 4 * l4), M::Y::PART);
   }
   // Keys and queries that are not finite would reach other episodes as 0 inf: then an episode at a time.
   bool wild = false;
@@ -232,9 +244,10 @@ __global__ __launch_bounds__(4 * D, D == 128 || kParts<E> == 1 ? 2 : 1) void gra
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
         const int i = 16 * t + l16;
-        if (i >= from && i < to && into[t] != 0.f)
-#pragma unroll
-          for (int x = 0; x < 4; ++x) total = fmaf(number_at<T>(lds, i, 16 * wave + 4 * l4 + x), down[t][x], total);
+        if (i >= from && i < to && into[t] != 0.f) {
+          const f32x4 x = numbers_at<T>(lds, i, 16 * wave + 4 * l4) * down[t];
+          total += (x[0] + x[1]) + (x[2] + x[3]);
+        }
       }
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
@@ -256,12 +269,10 @@ __global__ __launch_bounds__(4 * D, D == 128 || kParts<E> == 1 ? 2 : 1) void gra
         const bool inside = i >= from && i < to;
         if (inside) dq[t] = a, up[t] = b, down[t] = c;
         float x = 0.f;
-        if (inside)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int d = 16 * wave + 4 * l4 + e;
-            x = fmaf(number_at<T>(lds + M::QT, i, d), dq[t][e], fmaf(number_at<T>(lds, i, d), up[t][e] - down[t][e], x));
-          }
+        if (inside) {
+          const f32x4 a = numbers_at<T>(lds + M::QT, i, 16 * wave + 4 * l4) * dq[t] + numbers_at<T>(lds, i, 16 * wave + 4 * l4) * (up[t] - down[t]);
+          x = (a[0] + a[1]) + (a[2] + a[3]);
+        }
         x += __shfl_xor(x, 16);
         x += __shfl_xor(x, 32);
         if (l4 == 0 && inside) sums[wave][i] = x;

@@ -11,7 +11,9 @@ namespace delta {
 namespace {
 
 constexpr int kWaves = 4;
-constexpr int LROW = 68;  // floats of a row of L in LDS: 16 rows of 4 columns reach all banks
+// Floats of a row of L in LDS: 16 rows of 4 columns reach all banks.  Rows 0 .. 31 have 32 columns, so that a CU holds three workgroups.
+constexpr int SHORT = 36, LONG = 68, LFLOATS = 32 * SHORT + 32 * LONG;
+__device__ __forceinline__ constexpr int row_at(int i) { return i < 32 ? i * SHORT : 32 * SHORT + (i - 32) * LONG; }
 
 // acc + a b for 16x16 blocks: a's rows from LDS, b as a result lies in a lane.
 __device__ __forceinline__ f32x4 block_mma(f32x4 a, f32x4 b, f32x4 acc) {
@@ -22,11 +24,11 @@ __device__ __forceinline__ f32x4 block_mma(f32x4 a, f32x4 b, f32x4 acc) {
 
 template <class E, bool VEC>
 __global__ __launch_bounds__(64 * kWaves) void records_kernel(const Rule<E> r, int64_t count) {
-  __shared__ __align__(16) float lds[kWaves][C * LROW + 3 * C];
+  __shared__ __align__(16) float lds[kWaves][LFLOATS + 3 * C];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l16 = lane & 15, l4 = lane >> 4;
   const int64_t at = (int64_t)blockIdx.x * kWaves + wave;
   if (at >= count) return;  // (no barrier below: a wavefront has its own part of LDS)
-  float *L = lds[wave], *ghi = L + C * LROW, *glo = ghi + C, *beta = glo + C;
+  float *L = lds[wave], *ghi = L + LFLOATS, *glo = ghi + C, *beta = glo + C;
   const int64_t pair = at / r.chunks, chunk = at - pair * r.chunks;
   const int64_t env = r.first_env + pair / r.heads, T = r.seq_len, s0 = chunk * C;
   const int head = (int)(pair % r.heads), n = (int)(T - s0 < C ? T - s0 : C);
@@ -110,7 +112,7 @@ __global__ __launch_bounds__(64 * kWaves) void records_kernel(const Rule<E> r, i
         wild |= !finite(x[e]);
         // no episode begins in (j, i]
         const uint64_t between = (cuts >> j >> 1) << 1 << j & (((uint64_t)2 << i) - 1);
-        L[i * LROW + j] = i > j && between == 0 ? x[e] * expf((ghi[i] - hj) + (glo[i] - lj)) : 0.f;
+        L[row_at(16 * ti) + (4 * l4 + e) * (ti < 2 ? SHORT : LONG) + j] = i > j && between == 0 ? x[e] * __expf((ghi[i] - hj) + (glo[i] - lj)) : 0.f;
       }
     }
   }
@@ -118,34 +120,35 @@ __global__ __launch_bounds__(64 * kWaves) void records_kernel(const Rule<E> r, i
 
   // diagonal blocks: lane (block l4, column l16)
   {
-    const float* block = L + 16 * l4 * LROW + 16 * l4;
+    float* block = L + row_at(16 * l4) + 16 * l4;
+    const int row = l4 < 2 ? SHORT : LONG;
     const float* b = beta + 16 * l4;
     float m[16], bm[16];
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-      m[i] = block[i * LROW + l16];
+      m[i] = block[i * row + l16];
 #pragma unroll
-      for (int j = 0; j < i; ++j) m[i] = fmaf(-block[i * LROW + j], bm[j], m[i]);
+      for (int j = 0; j < i; ++j) m[i] = fmaf(-block[i * row + j], bm[j], m[i]);
       bm[i] = b[i] * m[i];
     }
     wave_sync();
 #pragma unroll
-    for (int i = 0; i < 16; ++i) L[(16 * l4 + i) * LROW + 16 * l4 + l16] = m[i];
+    for (int i = 0; i < 16; ++i) block[i * row + l16] = m[i];
   }
   wave_sync();
 
   // a block's rows as the left factor, a block as a result lies in a lane (the right factor or a sum)
-  auto left = [&](int ti, int tj) { return *reinterpret_cast<const f32x4*>(L + (16 * ti + l16) * LROW + 16 * tj + 4 * l4); };
+  auto left = [&](int ti, int tj) { return *reinterpret_cast<const f32x4*>(L + row_at(16 * ti) + l16 * (ti < 2 ? SHORT : LONG) + 16 * tj + 4 * l4); };
   auto result = [&](int ti, int tj) {
     f32x4 x;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) x[e] = L[(16 * ti + 4 * l4 + e) * LROW + 16 * tj + l16];
+    for (int e = 0; e < 4; ++e) x[e] = L[row_at(16 * ti) + (4 * l4 + e) * (ti < 2 ? SHORT : LONG) + 16 * tj + l16];
     return x;
   };
   auto betas = [&](int t) { return *reinterpret_cast<const f32x4*>(beta + 16 * t + 4 * l4); };  // (of columns of a left factor, of rows of a right one)
   auto put = [&](int ti, int tj, f32x4 x) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) L[(16 * ti + 4 * l4 + e) * LROW + 16 * tj + l16] = x[e];
+    for (int e = 0; e < 4; ++e) L[row_at(16 * ti) + (4 * l4 + e) * (ti < 2 ? SHORT : LONG) + 16 * tj + l16] = x[e];
   };
 #pragma unroll
   for (int h = 0; h < 4; h += 2) {
@@ -186,7 +189,7 @@ __global__ __launch_bounds__(64 * kWaves) void records_kernel(const Rule<E> r, i
   for (int ti = 0; ti < 4; ++ti)
 #pragma unroll
     for (int tj = 0; tj <= ti; ++tj) {
-      const f32x4 x = *reinterpret_cast<const f32x4*>(L + (16 * ti + (lane >> 2)) * LROW + 16 * tj + 4 * (lane & 3));
+      const f32x4 x = *reinterpret_cast<const f32x4*>(L + row_at(16 * ti) + (lane >> 2) * (ti < 2 ? SHORT : LONG) + 16 * tj + 4 * (lane & 3));
       wild |= !finite(x[0]) || !finite(x[1]) || !finite(x[2]) || !finite(x[3]);
       *reinterpret_cast<f32x4*>(rec.tiles[ti * (ti + 1) / 2 + tj] + 4 * lane) = x;
     }
