@@ -11,9 +11,10 @@ namespace delta {
 namespace {
 
 constexpr int kWaves = 4;
-// Floats of a row of L in LDS: 16 rows of 4 columns reach all banks.  Rows 0 .. 31 have 32 columns, so that a CU holds three workgroups.
-constexpr int SHORT = 36, LONG = 68, LFLOATS = 32 * SHORT + 32 * LONG;
-__device__ __forceinline__ constexpr int row_at(int i) { return i < 32 ? i * SHORT : 32 * SHORT + (i - 32) * LONG; }
+// Floats of a row of L in LDS, for its 16, 32 or 64 columns: 16 rows of 4 columns reach all banks, and a CU holds three workgroups.
+__device__ __forceinline__ constexpr int row_floats(int tile) { return tile == 0 ? 20 : tile == 1 ? 36 : 68; }
+__device__ __forceinline__ constexpr int row_at(int tile) { return tile == 0 ? 0 : 16 * 20 + (tile == 1 ? 0 : 16 * 36 + (tile - 2) * 16 * 68); }
+constexpr int LFLOATS = 16 * (20 + 36 + 68 + 68);
 
 // acc + a b for 16x16 blocks: a's rows from LDS, b as a result lies in a lane.
 __device__ __forceinline__ f32x4 block_mma(f32x4 a, f32x4 b, f32x4 acc) {
@@ -112,7 +113,7 @@ __global__ __launch_bounds__(64 * kWaves) void records_kernel(const Rule<E> r, i
         wild |= !finite(x[e]);
         // no episode begins in (j, i]
         const uint64_t between = (cuts >> j >> 1) << 1 << j & (((uint64_t)2 << i) - 1);
-        L[row_at(16 * ti) + (4 * l4 + e) * (ti < 2 ? SHORT : LONG) + j] = i > j && between == 0 ? x[e] * __expf((ghi[i] - hj) + (glo[i] - lj)) : 0.f;
+        L[row_at(ti) + (4 * l4 + e) * row_floats(ti) + j] = i > j && between == 0 ? x[e] * __expf((ghi[i] - hj) + (glo[i] - lj)) : 0.f;
       }
     }
   }
@@ -120,8 +121,8 @@ __global__ __launch_bounds__(64 * kWaves) void records_kernel(const Rule<E> r, i
 
   // diagonal blocks: lane (block l4, column l16)
   {
-    float* block = L + row_at(16 * l4) + 16 * l4;
-    const int row = l4 < 2 ? SHORT : LONG;
+    float* block = L + row_at(l4) + 16 * l4;
+    const int row = row_floats(l4);
     const float* b = beta + 16 * l4;
     float m[16], bm[16];
 #pragma unroll
@@ -138,17 +139,17 @@ __global__ __launch_bounds__(64 * kWaves) void records_kernel(const Rule<E> r, i
   wave_sync();
 
   // a block's rows as the left factor, a block as a result lies in a lane (the right factor or a sum)
-  auto left = [&](int ti, int tj) { return *reinterpret_cast<const f32x4*>(L + row_at(16 * ti) + l16 * (ti < 2 ? SHORT : LONG) + 16 * tj + 4 * l4); };
+  auto left = [&](int ti, int tj) { return *reinterpret_cast<const f32x4*>(L + row_at(ti) + l16 * row_floats(ti) + 16 * tj + 4 * l4); };
   auto result = [&](int ti, int tj) {
     f32x4 x;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) x[e] = L[row_at(16 * ti) + (4 * l4 + e) * (ti < 2 ? SHORT : LONG) + 16 * tj + l16];
+    for (int e = 0; e < 4; ++e) x[e] = L[row_at(ti) + (4 * l4 + e) * row_floats(ti) + 16 * tj + l16];
     return x;
   };
   auto betas = [&](int t) { return *reinterpret_cast<const f32x4*>(beta + 16 * t + 4 * l4); };  // (of columns of a left factor, of rows of a right one)
   auto put = [&](int ti, int tj, f32x4 x) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) L[row_at(16 * ti) + (4 * l4 + e) * (ti < 2 ? SHORT : LONG) + 16 * tj + l16] = x[e];
+    for (int e = 0; e < 4; ++e) L[row_at(ti) + (4 * l4 + e) * row_floats(ti) + 16 * tj + l16] = x[e];
   };
 #pragma unroll
   for (int h = 0; h < 4; h += 2) {
@@ -189,7 +190,7 @@ __global__ __launch_bounds__(64 * kWaves) void records_kernel(const Rule<E> r, i
   for (int ti = 0; ti < 4; ++ti)
 #pragma unroll
     for (int tj = 0; tj <= ti; ++tj) {
-      const f32x4 x = *reinterpret_cast<const f32x4*>(L + row_at(16 * ti) + (lane >> 2) * (ti < 2 ? SHORT : LONG) + 16 * tj + 4 * (lane & 3));
+      const f32x4 x = *reinterpret_cast<const f32x4*>(L + row_at(ti) + (lane >> 2) * row_floats(ti) + 16 * tj + 4 * (lane & 3));
       wild |= !finite(x[0]) || !finite(x[1]) || !finite(x[2]) || !finite(x[3]);
       *reinterpret_cast<f32x4*>(rec.tiles[ti * (ti + 1) / 2 + tj] + 4 * lane) = x;
     }
