@@ -91,8 +91,6 @@ __global__ __launch_bounds__(4 * D, D == 128 || kParts<E> == 1 ? 2 : 1) void gra
   if (threadIdx.x < REST_QUADS) rest_of_record[threadIdx.x] = reinterpret_cast<const f32x4*>(r.records[at].ghi)[threadIdx.x];
   fetch(0);
   Rows<E, D, NT, VEC> k, q;
-  k.fetch(r.k.data + env * r.k.env + head * r.k.head + s0 * r.k.step, r.k.step, dk, n);
-  q.fetch(r.q.data + env * r.q.env + head * r.q.head + s0 * r.q.step, r.q.step, dk, n);
   const At<typename M::G> at_g;
   const At<typename M::U> at_u;
   const At<T> at_k;

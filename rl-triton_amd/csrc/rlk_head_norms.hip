@@ -36,6 +36,7 @@ template <class E>
 struct Norms {
   Side<E> side[2];  // queries, keys
   int64_t tokens, steps;
+  int64_t stride_envs, stride_steps;  // from a group's token to its next one
   int dim, rotary;
   const int64_t* positions;
   float eps, inv_dim;
@@ -86,19 +87,25 @@ struct Turn {
   bool on;
   __device__ void set(const Unit<N, HALVES>& u, const Frequencies& f, const int64_t* position) {
     on = position != nullptr && u.there && u.pair >= 0;
+    const double where = on ? (double)*position : 0.0;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       c[i] = 1.f, s[i] = 0.f;
       if (!on) continue;
-      double t = (double)*position * f.turns[u.pair + i];
-      t -= floor(t);
+      // in turns, less whole ones, and of these less quarters: what is left is within an eighth
+      const double t = __builtin_amdgcn_fract(where * f.turns[u.pair + i]);
       const double quarters = rint(4.0 * t);
-      const float rest = (float)(t - 0.25 * quarters);
-      float sn, cs;
-      sincospif(2.f * rest, &sn, &cs);
-      const int n = (int)quarters & 3;
-      c[i] = n == 0 ? cs : n == 1 ? -sn : n == 2 ? -cs : sn;
-      s[i] = n == 0 ? sn : n == 1 ? cs : n == 2 ? -sn : -cs;
+      const float x = (float)((t - 0.25 * quarters) * 6.283185307179586476925), y = x * x;
+      // (series up to pi / 4: the first terms left out are below 2^-28)
+      float sn = fmaf(y, 1.f / 362880.f, -1.f / 5040.f), cs = fmaf(y, -1.f / 3628800.f, 1.f / 40320.f);
+      sn = fmaf(sn, y, 1.f / 120.f), cs = fmaf(cs, y, -1.f / 720.f);
+      sn = fmaf(sn, y, -1.f / 6.f), cs = fmaf(cs, y, 1.f / 24.f);
+      sn = fmaf(sn * y, x, x), cs = fmaf(cs, y, -0.5f);
+      cs = fmaf(cs, y, 1.f);
+      const int n = (int)quarters;
+      const float a = n & 1 ? sn : cs, b = n & 1 ? cs : sn;
+      c[i] = (n + 1) & 2 ? -a : a;
+      s[i] = n & 2 ? -b : b;
     }
   }
   // pairs of a unit: element i of both runs, or neighbours across the two runs
@@ -144,8 +151,10 @@ __global__ __launch_bounds__(256) void norms_kernel(const Norms<E> n, const Freq
       ga[u].x[i] = gb[u].x[i] = 0.f;
     }
   }
-  for (int64_t token = (int64_t)blockIdx.x * GROUPS + group; token < n.tokens; token += (int64_t)gridDim.x * GROUPS) {
-    const int64_t env = token / n.steps, step = token - env * n.steps;
+  int64_t token = (int64_t)blockIdx.x * GROUPS + group;
+  // (a division in 64 bits is as much work as a row)
+  int64_t env = n.tokens >> 32 == 0 ? (int64_t)((uint32_t)token / (uint32_t)n.steps) : token / n.steps, step = token - env * n.steps;
+  for (; token < n.tokens; token += (int64_t)gridDim.x * GROUPS) {
     const E* px = d.x + env * d.env + step * d.step + head0 * d.head;
     Elements<E, N> xa[kHeads][UNITS], xb[kHeads][UNITS], ya[BACK ? kHeads : 1][UNITS], yb[BACK ? kHeads : 1][UNITS];
 #pragma unroll
@@ -180,7 +189,9 @@ __global__ __launch_bounds__(256) void norms_kernel(const Norms<E> n, const Freq
       for (int u = 0; u < UNITS; ++u)
 #pragma unroll
         for (int i = 0; i < N; ++i) sum = fmaf(xa[h][u].x[i], xa[h][u].x[i], fmaf(xb[h][u].x[i], xb[h][u].x[i], sum));
-      const float r = 1.f / sqrtf(fmaf(group_sum<G>(sum), n.inv_dim, n.eps));
+      const float square = fmaf(group_sum<G>(sum), n.inv_dim, n.eps);
+      float r = __builtin_amdgcn_rsqf(square);
+      r = square < 1e-30f || square > 1e30f ? 1.f / sqrtf(square) : fmaf(r * fmaf(-square * r, r, 1.f), 0.5f, r);  // (one step to the last bit)
       if constexpr (!BACK) {
 #pragma unroll
         for (int u = 0; u < UNITS; ++u) {
@@ -220,6 +231,8 @@ __global__ __launch_bounds__(256) void norms_kernel(const Norms<E> n, const Freq
           }
       }
     }
+    env += n.stride_envs, step += n.stride_steps;
+    if (step >= n.steps) step -= n.steps, ++env;
   }
   if constexpr (BACK) {
     if (n.partial == nullptr) return;
@@ -306,6 +319,7 @@ int run(const rlk_head_norms& c, const rlk_sequence* grads, float* const* weight
     along = (n.tokens + groups - 1) / groups;
     const int64_t most = BACK ? kBackBlocks : int64_t{1} << 20;
     if (along > most) along = most;
+    n.stride_envs = along * groups / n.steps, n.stride_steps = along * groups % n.steps;
     if (blocks > 0 && along > 0)
       norms_kernel<E, decltype(N)::value, decltype(G)::value, decltype(U)::value, decltype(halves)::value, BACK>
           <<<dim3((unsigned)along, (unsigned)blocks), dim3(256), 0, s>>>(n, f);
