@@ -15,8 +15,9 @@ namespace rlk {
 namespace {
 
 constexpr int kMostDim = 256;
-constexpr int kHeads = 4;  // heads of a step that a group takes
-constexpr int kBackBlocks = 512;  // workgroups along the steps whose sums of weights' gradients are added up afterwards
+template <bool BACK>
+constexpr int kHeads = BACK ? 2 : 4;  // heads of a step that a group takes
+constexpr int kBackBlocks = 256;  // workgroups along the steps whose sums of weights' gradients are added up afterwards
 
 struct Frequencies {
   double turns[kMostDim / 2];  // of a position, by pair
@@ -29,7 +30,7 @@ struct Side {
   const E* g;  // backward
   int64_t env, step, head, yenv, ystep, yhead, genv, gstep, ghead;
   const float* weight;
-  int heads, blocks;  // blocks of kHeads heads
+  int heads, blocks;  // blocks of heads that a group takes together
 };
 
 template <class E>
@@ -139,7 +140,7 @@ __global__ __launch_bounds__(256) void norms_kernel(const Norms<E> n, const Freq
   constexpr int GROUPS = 256 / G;
   const bool keys = (int)blockIdx.y >= n.side[0].blocks;
   const Side<E>& d = n.side[keys];
-  const int head0 = ((int)blockIdx.y - (keys ? n.side[0].blocks : 0)) * kHeads, heads = d.heads - head0 < kHeads ? d.heads - head0 : kHeads;
+  const int head0 = ((int)blockIdx.y - (keys ? n.side[0].blocks : 0)) * kHeads<BACK>, heads = d.heads - head0 < kHeads<BACK> ? d.heads - head0 : kHeads<BACK>;
   Elements<E, N> wa[UNITS], wb[UNITS], ga[UNITS], gb[UNITS];
 #pragma unroll
   for (int u = 0; u < UNITS; ++u) {
@@ -156,9 +157,9 @@ __global__ __launch_bounds__(256) void norms_kernel(const Norms<E> n, const Freq
   int64_t env = n.tokens >> 32 == 0 ? (int64_t)((uint32_t)token / (uint32_t)n.steps) : token / n.steps, step = token - env * n.steps;
   for (; token < n.tokens; token += (int64_t)gridDim.x * GROUPS) {
     const E* px = d.x + env * d.env + step * d.step + head0 * d.head;
-    Elements<E, N> xa[kHeads][UNITS], xb[kHeads][UNITS], ya[BACK ? kHeads : 1][UNITS], yb[BACK ? kHeads : 1][UNITS];
+    Elements<E, N> xa[kHeads<BACK>][UNITS], xb[kHeads<BACK>][UNITS], ya[BACK ? kHeads<BACK> : 1][UNITS], yb[BACK ? kHeads<BACK> : 1][UNITS];
 #pragma unroll
-    for (int h = 0; h < kHeads; ++h) {
+    for (int h = 0; h < kHeads<BACK>; ++h) {
       if (h >= heads) continue;
 #pragma unroll
       for (int u = 0; u < UNITS; ++u) {
@@ -182,7 +183,7 @@ __global__ __launch_bounds__(256) void norms_kernel(const Norms<E> n, const Freq
       turn[u].set(Unit<N, HALVES>(lane + G * u, n.dim, n.rotary), f, n.positions != nullptr ? n.positions + token : nullptr);
     E* py = d.y != nullptr ? d.y + env * d.yenv + step * d.ystep + head0 * d.yhead : nullptr;
 #pragma unroll
-    for (int h = 0; h < kHeads; ++h) {
+    for (int h = 0; h < kHeads<BACK>; ++h) {
       if (h >= heads) continue;
       float sum = 0.f;
 #pragma unroll
@@ -236,23 +237,24 @@ __global__ __launch_bounds__(256) void norms_kernel(const Norms<E> n, const Freq
   }
   if constexpr (BACK) {
     if (n.partial == nullptr) return;
-    // the workgroup's sums, group after group
-    __shared__ float sums[kMostDim];
-    for (int k = 0; k < GROUPS; ++k) {
-      __syncthreads();
-      if (group == k)
+    // the workgroup's sums: a wavefront's groups, then the wavefronts
+    __shared__ float sums[4][kMostDim];
 #pragma unroll
-        for (int u = 0; u < UNITS; ++u) {
-          const Unit<N, HALVES> at(lane + G * u, n.dim, n.rotary);
+    for (int u = 0; u < UNITS; ++u) {
+      const Unit<N, HALVES> at(lane + G * u, n.dim, n.rotary);
 #pragma unroll
-          for (int i = 0; i < N; ++i) {
-            if (at.there) sums[at.a + i] = (k ? sums[at.a + i] : 0.f) + ga[u].x[i];
-            if (at.second) sums[at.b + i] = (k ? sums[at.b + i] : 0.f) + gb[u].x[i];
-          }
-        }
+      for (int i = 0; i < N; ++i) {
+        float a = ga[u].x[i], b = gb[u].x[i];
+#pragma unroll
+        for (int d = G; d < 64; d <<= 1) a += __shfl_xor(a, d), b += __shfl_xor(b, d);
+        if ((threadIdx.x & 63) < G && at.there) sums[threadIdx.x >> 6][at.a + i] = a;
+        if ((threadIdx.x & 63) < G && at.second) sums[threadIdx.x >> 6][at.b + i] = b;
+      }
     }
     __syncthreads();
-    if ((int)threadIdx.x < n.dim) n.partial[((int64_t)blockIdx.x * gridDim.y + blockIdx.y) * n.dim + threadIdx.x] = sums[threadIdx.x];
+    if ((int)threadIdx.x < n.dim)
+      n.partial[((int64_t)blockIdx.x * gridDim.y + blockIdx.y) * n.dim + threadIdx.x] =
+          (sums[0][threadIdx.x] + sums[1][threadIdx.x]) + (sums[2][threadIdx.x] + sums[3][threadIdx.x]);
   }
 }
 
@@ -264,6 +266,7 @@ __global__ __launch_bounds__(256) void weights_kernel(const float* partial, int 
   __shared__ double s[256];
   double x = 0.0;
   if (e < dim)
+#pragma unroll 4
     for (int i = threadIdx.x / 4; i < blocks * count; i += 64) x += (double)partial[((int64_t)(i / count) * all + first + i % count) * dim + e];
   s[threadIdx.x] = x;
   __syncthreads();
@@ -307,7 +310,7 @@ int run(const rlk_head_norms& c, const rlk_sequence* grads, float* const* weight
     d.weight = i ? c.k_weight : c.q_weight, d.heads = (int)(i ? c.k_heads : c.q_heads);
     if (grads) d.g = static_cast<const E*>(grads[i].data), d.genv = grads[i].env_stride, d.gstep = grads[i].step_stride, d.ghead = grads[i].head_stride;
     if (BACK && d.g == nullptr) d.heads = 0;
-    d.blocks = (d.heads + kHeads - 1) / kHeads;
+    d.blocks = (d.heads + kHeads<BACK> - 1) / kHeads<BACK>;
     if (d.heads > 0) vec = vec && quads<E>(d.x, d.env, d.step, d.head) && quads<E>(d.y, d.yenv, d.ystep, d.yhead) && quads<E>(d.g, d.genv, d.gstep, d.ghead);
   }
   const Frequencies& f = frequencies(c.base, n.rotary);
@@ -379,7 +382,7 @@ int rlk_query_key_norms(const rlk_head_norms* c, void* stream) {
 
 size_t rlk_head_norms_workspace_bytes(const rlk_head_norms* c) {
   if (!valid_norms(c)) return 0;
-  const int64_t blocks = (c->q_heads + kHeads - 1) / kHeads + (c->k_heads + kHeads - 1) / kHeads;
+  const int64_t blocks = (c->q_heads + kHeads<true> - 1) / kHeads<true> + (c->k_heads + kHeads<true> - 1) / kHeads<true>;
   return sizeof(float) * (size_t)(kBackBlocks * blocks * c->dim);
 }
 

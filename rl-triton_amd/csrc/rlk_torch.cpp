@@ -708,6 +708,7 @@ PyObject* op_affine_scan(PyObject* const* a, Py_ssize_t n) {
 }
 
 #include "rlk_torch_policy.hpp"
+#include "rlk_torch_operators.hpp"
 
 // C++ exceptions (an allocation that fails, say) must not cross into the interpreter: such
 // a call is declined, and the Python path raises torch's own exception for it.  Python's own (a saved tensor's hook that
@@ -842,6 +843,10 @@ const OpName kOps[] = {
     {"policy_loss_from_logits", guarded<op_policy_loss_from_logits>},
     {"linear_attention", guarded<op_linear_attention>},
     {"linear_attention_step", guarded<op_linear_attention_step>},
+    {"gated_delta_rule", guarded<op_gated_delta_rule>},
+    {"gated_delta_rule_step", guarded<op_gated_delta_rule_step>},
+    {"query_key_norms", guarded<op_query_key_norms>},
+    {"sampled_actions", guarded<op_sampled_actions>},
 };
 
 // entry(op, names, npos, defaults, required, fallback): a public function over fast op `op`
