@@ -251,7 +251,8 @@ PyObject* op_gated_delta_rule(PyObject* const* a, Py_ssize_t n) {
     return pair(o[0], o[1]);
   }
   at::Tensor out = policy_output(x.v->sizes(), x.v->scalar_type(), *x.v), last = policy_output({t.num_envs, t.heads, t.dim_k, t.dim_v}, at::kFloat, *x.v);
-  return finish(delta_forward(&t, out, last, nullptr), "rlk_gated_delta_rule", pair(out, last));
+  const int st = delta_forward(&t, out, last, nullptr);  // (before pair() takes the tensors: arguments have no order)
+  return finish(st, "rlk_gated_delta_rule", pair(out, last));
 }
 
 // A step's output where a gradient is wanted of it (as StepOutput).

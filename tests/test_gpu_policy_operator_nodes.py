@@ -193,3 +193,33 @@ def test_two_threads_at_once():
     assert not errors, errors
     for a, b in zip(got, want):
         assert all(torch.equal(p, q) for p, q in zip(a, b))
+
+
+def test_calls_keep_nothing():
+    """What a call allocates and does not return is free when it is over, and so is what it returns when the caller lets go; calls without a
+    gradient are C++'s to the end."""
+    import gc
+    from rl_triton._native import fast
+    q, k, v, g, beta, dones, state = (t.cuda() for t in inputs(2, 300, 2, 24, 40, torch.float32, 1))
+    w = torch.ones(24, device="cuda")
+    leaf = q.clone().requires_grad_()
+    step = [t[:, 0].contiguous() for t in (q, k, v, g, beta)]
+    x, u = torch.randn(9, 700, device="cuda"), torch.rand(9, device="cuda")
+    calls = [(4, lambda: policy.compute_gated_delta_rule(q, k, v, g, beta, dones, state)),
+             (0, lambda: policy.compute_gated_delta_rule(leaf, k, v, g, beta)),
+             (0, lambda: torch.autograd.grad(policy.compute_gated_delta_rule(leaf, k, v, g, beta)[0].sum(), leaf)),
+             (4, lambda: policy.compute_gated_delta_rule_step(*step, state)), (4, lambda: policy.compute_query_key_norms(q, k, w, w)),
+             (0, lambda: torch.autograd.grad(policy.compute_query_key_norms(leaf, k, w, w)[0].sum(), leaf)),
+             (4, lambda: policy.compute_sampled_actions(x, u, top_k=5, top_p=0.9))]
+    for launches, call in calls:
+        call()
+        torch.cuda.synchronize()
+        gc.collect()
+        before, taken = torch.cuda.memory_allocated(), fast.launched()
+        gc.disable()
+        for _ in range(4):
+            call()
+        torch.cuda.synchronize()
+        gc.enable()
+        assert torch.cuda.memory_allocated() == before
+        assert fast.launched() - taken == launches
