@@ -3,13 +3,15 @@
 Every episode shows one of `cues` symbols at its first step and blanks after it; at its last step, which a flag announces, the
 action named by the symbol earns 1.  Episodes last from 2 to `longest` steps, so windows of a rollout begin and end inside them.
 
-    python examples/recall.py [--updates 150] [--dtype bfloat16] [--from-log-probs]
+    python examples/recall.py [--updates 150] [--dtype bfloat16] [--from-log-probs] [--memory gated]
 
 The operators as a learner uses them:
   acting    compute_linear_attention_step, with the state written in place; compute_action_log_probs
   targets   rl_triton.compute_gae
   learning  compute_linear_attention over the window, from the state that it began with; compute_policy_loss_from_logits
             and `logits.backward(grad)`, or, with --from-log-probs, compute_action_log_probs and compute_policy_loss
+With --memory gated the policy sets its memory's gates itself: compute_query_key_norms, rotated by the steps since the episode began,
+compute_gated_delta_rule and its step; it acts by compute_sampled_actions.
 """
 import argparse
 import os
@@ -89,36 +91,70 @@ class Policy(nn.Module):
         return self.heads_of(x, memory)
 
 
-def train(updates=150, envs=256, steps=64, cues=4, longest=12, epochs=4, dtype=torch.float32, from_log_probs=False, seed=0, say=print):
+class GatedPolicy(Policy):
+    """The same with a gated delta rule for its memory: keys of length 1, gates from the observation, positions counted from the episode's
+    beginning."""
+
+    def __init__(self, inputs, actions, heads=2, dim=32, width=64, dtype=torch.float32):
+        super().__init__(inputs, actions, heads, dim, width, dtype)
+        self.gates = nn.Linear(width, 2 * heads)
+        self.q_norm, self.k_norm = (nn.Parameter(torch.full((dim,), dim ** -0.5)) for _ in range(2))
+
+    def parts(self, obs, positions):
+        x, q, k, v = super().parts(obs)
+        q, k = policy.compute_query_key_norms(q, k, self.q_norm, self.k_norm, positions)
+        forget, write = self.gates(x).float().chunk(2, -1)
+        return x, q, k, v, -0.1 * nn.functional.softplus(forget), torch.sigmoid(write)
+
+    @torch.no_grad()
+    def act(self, obs, state, done, positions):
+        x, q, k, v, log_decays, betas = self.parts(obs, positions)
+        memory, _ = policy.compute_gated_delta_rule_step(q, k, v, log_decays, betas, state, done, 1.0, out_state=state)
+        return self.heads_of(x, memory)
+
+    def forward(self, obs, state, dones, positions):
+        x, q, k, v, log_decays, betas = self.parts(obs, positions)
+        memory, _ = policy.compute_gated_delta_rule(q, k, v, log_decays, betas, dones, state, 1.0)
+        return self.heads_of(x, memory)
+
+
+def train(updates=150, envs=256, steps=64, cues=4, longest=12, epochs=4, dtype=torch.float32, from_log_probs=False, seed=0, say=print, memory="linear"):
     """Trains a policy; returns the share of episodes that ended with the right action, one number an update."""
     device = torch.device("cuda")
     torch.manual_seed(seed)
     generator = torch.Generator(device=device).manual_seed(seed)
     task = Recall(envs, cues, longest, device, generator)
-    net = Policy(cues + 1, cues, dtype=dtype).to(device)
+    gated = memory == "gated"
+    net = (GatedPolicy if gated else Policy)(cues + 1, cues, dtype=dtype).to(device)
     adam = torch.optim.Adam(net.parameters(), lr=3e-3)
     state = torch.zeros(envs, net.heads, net.dim, net.dim, device=device)
     done = torch.zeros(envs, device=device)
+    position = torch.zeros(envs, dtype=torch.int64, device=device)  # steps since the episode began
     right = []
     for update in range(updates):
         begin = torch.where(done[:, None, None, None] != 0, 0.0, state)  # (the step takes the flag with it, a window the state alone)
         played = []
         for _ in range(steps):
             obs = task.observe()
-            logits, value = net.act(obs, state, done)
-            action = torch.multinomial(torch.softmax(logits, -1), 1, generator=generator).squeeze(-1)
-            log_prob, _ = policy.compute_action_log_probs(logits, action)
+            place = position
+            logits, value = net.act(obs, state, done, *(place,) * gated)
+            if gated:
+                action, log_prob = policy.compute_sampled_actions(logits, torch.rand(envs, generator=generator, device=device))
+            else:
+                action = torch.multinomial(torch.softmax(logits, -1), 1, generator=generator).squeeze(-1)
+                log_prob, _ = policy.compute_action_log_probs(logits, action)
             reward, done = task.step(action)
-            played.append((obs, action, log_prob, value, reward, done))
-        obs, actions, old, values, rewards, dones = (torch.stack(x, 1) for x in zip(*played))
+            position = torch.where(done != 0, 0, position + 1)
+            played.append((obs, action, log_prob, value, reward, done, place))
+        obs, actions, old, values, rewards, dones, places = (torch.stack(x, 1) for x in zip(*played))
         with torch.no_grad():
-            last_value = net.act(task.observe(), state.clone(), done)[1]
+            last_value = net.act(task.observe(), state.clone(), done, *(position,) * gated)[1]
         advantages = rl_triton.compute_gae(rewards, values, dones, gamma=0.95, lambda_=0.95, last_value=last_value)
         returns = advantages + values
         advantages = (advantages - advantages.mean()) / (advantages.std() + 1e-6)
 
         for _ in range(epochs):
-            logits, value = net(obs, begin, dones)
+            logits, value = net(obs, begin, dones, *(places,) * gated)
             if from_log_probs:
                 log_probs, entropies = policy.compute_action_log_probs(logits, actions)
                 loss, grad, means = policy.compute_policy_loss(log_probs, old, advantages)
@@ -141,5 +177,6 @@ if __name__ == "__main__":
     parser.add_argument("--updates", type=int, default=150)
     parser.add_argument("--dtype", choices=("float32", "bfloat16"), default="float32")
     parser.add_argument("--from-log-probs", action="store_true")
+    parser.add_argument("--memory", choices=("linear", "gated"), default="linear")
     args = parser.parse_args()
-    train(args.updates, dtype=getattr(torch, args.dtype), from_log_probs=args.from_log_probs)
+    train(args.updates, dtype=getattr(torch, args.dtype), from_log_probs=args.from_log_probs, memory=args.memory)
