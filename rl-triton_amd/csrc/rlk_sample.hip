@@ -335,18 +335,20 @@ __global__ __launch_bounds__(NT, NT >= 512 ? 4 : 2) void row_kernel(const Sampli
 #pragma unroll
       for (int e = 0; e < N; ++e) any |= depth(x.get(e), top, scale) < reach;
       if (!any) return;
-#pragma unroll 1
-      for (int i = first; i < first + N && i < A; ++i) {
-        const float y = load_one(p + i);
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        const float y = x.get(e);
         if (!(depth(y, top, scale) < reach) || y == -INFINITY) continue;
         const uint32_t at = atomicAdd(&m.listed, 1u);
-        if (at < kShort) m.list[at] = order(y, i);
+        if (at < kShort) m.list[at] = order(y, first + e);
       }
     });
     __syncthreads();
     const int n = (int)m.listed;
     if (n <= kShort) {
+      // (comparisons by eights: one after the other each would wait for the LDS)
       constexpr int PER = (kShort + NT - 1) / NT;
+      const int padded = (n + 7) & ~7;
       u64 mine[PER], w[PER], before[PER];
       int rank[PER];
 #pragma unroll
@@ -355,18 +357,23 @@ __global__ __launch_bounds__(NT, NT >= 512 ? 4 : 2) void row_kernel(const Sampli
         mine[i] = at < n ? m.list[at] : 0;
         w[i] = at < n ? weights(value_of(mine[i])) : 0;
         if (at < n) m.weights[at] = w[i];
+        else if (at < padded) m.list[at] = m.weights[at] = 0;
         before[i] = 0, rank[i] = 0;
       }
       __syncthreads();
       if (wave * 64 < n)
-        for (int j = 0; j < n; ++j) {
-          const u64 other = m.list[j], wj = m.weights[j];
+        for (int j0 = 0; j0 < padded; j0 += 8) {
+          u64 other[8], wj[8];
 #pragma unroll
-          for (int i = 0; i < PER; ++i) {
-            const bool first = other > mine[i];
-            rank[i] += first;
-            before[i] += first ? wj : 0;
-          }
+          for (int j = 0; j < 8; ++j) other[j] = m.list[j0 + j], wj[j] = m.weights[j0 + j];
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+#pragma unroll
+            for (int i = 0; i < PER; ++i) {
+              const bool first = other[j] > mine[i];
+              rank[i] += first;
+              before[i] += first ? wj[j] : 0;
+            }
         }
       u64 left = 0;  // what top_k leaves
 #pragma unroll
@@ -389,11 +396,15 @@ __global__ __launch_bounds__(NT, NT >= 512 ? 4 : 2) void row_kernel(const Sampli
 #pragma unroll
       for (int i = 0; i < PER; ++i) upto[i] = 0;
       if (wave * 64 < n)
-        for (int j = 0; j < n; ++j) {
-          const uint32_t other = (uint32_t)m.list[j];  // (~action: an earlier one has a larger number)
-          const u64 wj = m.weights[j];
+        for (int j0 = 0; j0 < padded; j0 += 8) {
+          uint32_t other[8];  // (~action: an earlier one has a larger number)
+          u64 wj[8];
 #pragma unroll
-          for (int i = 0; i < PER; ++i) upto[i] += other >= (uint32_t)mine[i] ? wj : 0;
+          for (int j = 0; j < 8; ++j) other[j] = (uint32_t)m.list[j0 + j], wj[j] = m.weights[j0 + j];
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+#pragma unroll
+            for (int i = 0; i < PER; ++i) upto[i] += other[j] >= (uint32_t)mine[i] ? wj[j] : 0;
         }
 #pragma unroll
       for (int i = 0; i < PER; ++i)
@@ -446,11 +457,11 @@ __global__ __launch_bounds__(NT, NT >= 512 ? 4 : 2) void row_kernel(const Sampli
           any |= d >= (float)b && d < (float)(b + 1);
         }
         if (!any) return;
-#pragma unroll 1
-        for (int i = first; i < first + N && i < A; ++i) {
-          const float y = load_one(p + i);
-          if (bucket(y, top, scale) != b) continue;
-          const u64 o = order(y, i);
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+          const float y = x.get(e);
+          if (bucket(y, top, scale) != b || first + e >= A) continue;
+          const u64 o = order(y, first + e);
           lo = o < lo ? o : lo, hi = o > hi ? o : hi;
           const uint32_t at = atomicAdd(&m.listed, 1u);
           if (at < kList) m.list[at] = o;
@@ -468,13 +479,23 @@ __global__ __launch_bounds__(NT, NT >= 512 ? 4 : 2) void row_kernel(const Sampli
       const uint32_t n = m.listed;
       if (n <= kShort) {
         // each compares itself with all
+        const uint32_t padded = (n + 7) & ~7u;
         if (tid == 0) m.border = lo;  // (all of the bucket, if it never is enough)
-        for (uint32_t i = tid; i < n; i += NT) m.weights[i] = counts ? 1 : weights(value_of(m.list[i]));
+        for (uint32_t i = tid; i < padded; i += NT) {
+          if (i >= n) m.list[i] = 0;
+          m.weights[i] = i >= n ? 0 : counts ? 1 : weights(value_of(m.list[i]));
+        }
         __syncthreads();
         for (uint32_t i = tid; i < n; i += NT) {
           const u64 mine = m.list[i];
           u64 sum = before;
-          for (uint32_t j = 0; j < n; ++j) sum += m.list[j] > mine ? m.weights[j] : 0;
+          for (uint32_t j0 = 0; j0 < padded; j0 += 8) {
+            u64 other[8], wj[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) other[j] = m.list[j0 + j], wj[j] = m.weights[j0 + j];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) sum += other[j] > mine ? wj[j] : 0;
+          }
           if ((double)sum < want && (double)(sum + m.weights[i]) >= want) m.border = mine;
         }
         __syncthreads();
@@ -588,7 +609,7 @@ int launch(Sampling s, hipStream_t stream) {
   } else {
     for (s.first = 0; s.first < rows; s.first += most) {
       const dim3 grid((unsigned)(rows - s.first < most ? rows - s.first : most));
-      // A row to a CU: by 1024 threads ([64] of 131072, top-k: 26 us, 33 by 512).  More: two workgroups of 512 a CU, one of which works while the
+      // A row to a CU: by 1024 threads ([64] of 131072, top-k: 26 us against 33 by 512; by now 20).  More: two workgroups of 512 a CU, one of which works while the
       // other waits (top-p, [512] of 50001: 105 us, 127 by 1024).
       if (s.actions <= 4096) row_kernel<E, 256><<<grid, dim3(256), 0, stream>>>(s);
       else if (rows <= device_cus()) row_kernel<E, 1024><<<grid, dim3(1024), 0, stream>>>(s);
