@@ -333,6 +333,8 @@ template <class E>
 int launch_gradients(const Rule<E>& r, int64_t envs, hipStream_t s) {
   const dim3 grid((unsigned)(envs * r.heads * r.chunks));
   const bool vec = fours(r.k, r.dk) && fours(r.q, r.dk) && fours(r.gy, r.dv) && fours(r.gq, r.dk) && fours(r.gk, r.dk);
+  // (longer values of short keys: the second 4 wavefronts have no rows of the state, but their part of Y and the loads; [37,333,4,40+72] float32
+  // 86 us, 98 by 4)
   if (r.dk <= 64 && r.dv <= 64) {
     if (vec) gradients_kernel<E, 64, true><<<grid, dim3(256), 0, s>>>(r);
     else gradients_kernel<E, 64, false><<<grid, dim3(256), 0, s>>>(r);

@@ -10,7 +10,7 @@ namespace rlk {
 namespace delta {
 namespace {
 
-// D: dims padded to 64 or 128; D / 16 wavefronts.
+// D: dims of the keys padded to 64 or 128.
 template <class E, int D, int PARTS_OF_P>
 struct Lds {
   typedef Tile<E, D> Rows_;
@@ -22,9 +22,9 @@ struct Lds {
 
 // The shared part of a walk: a chunk's arrays on their way to LDS, and the weighted q . k.
 // QUERIES: else only the keys and M are.
-template <class E, int D, bool VEC, int PARTS_OF_P, bool QUERIES = true>
+template <class E, int D, int WAVES, bool VEC, int PARTS_OF_P, bool QUERIES = true>
 struct Shared {
-  static constexpr int NT = 4 * D;
+  static constexpr int NT = 64 * WAVES;
   typedef Lds<E, D, PARTS_OF_P> M;
   static constexpr int TILE_QUADS = 640, REST_QUADS = (int)(sizeof(Record) - offsetof(Record, ghi)) / 16, TILES_PER = (TILE_QUADS + NT - 1) / NT;
   Rows<E, D, NT, VEC> k, q;
@@ -63,7 +63,7 @@ struct Shared {
   // P_ij = scale D_ij q_i . k_j.  Wavefronts share the 16 rows ti; computed transposed, so that a lane holds 4 consecutive j.
   __device__ static void form_p(char* lds, float scale, const At<typename M::Rows_>& at) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l16 = lane & 15, l4 = lane >> 4;
-    constexpr int SHARE = D / 64;
+    constexpr int SHARE = WAVES / 4;
     const Record& rec = record(lds);
     const uint64_t cuts = rec.cuts[0] | (uint64_t)rec.cuts[1] << 32;
     const int ti = wave / SHARE, i = 16 * ti + l16;
@@ -191,10 +191,10 @@ __device__ __forceinline__ f32x4 columns_quad(const E (&x)[16], int t, int dim, 
 
 // TRANSITION: no outputs, but what a segment does to the state that enters it: the state that it leaves from none (blockIdx.z 1), and from the
 // unit vectors with no values (0).
-template <class E, int D, bool VEC, bool TRANSITION>
-__global__ __launch_bounds__(4 * D, D == 128 || kParts<E> == 1 ? 2 : 1) void forward_kernel(const Rule<E> r) {
+template <class E, int D, int WAVES, bool VEC, bool TRANSITION>
+__global__ __launch_bounds__(64 * WAVES, WAVES == 8 || kParts<E> == 1 ? 2 : 1) void forward_kernel(const Rule<E> r) {
   constexpr int MT = D / 16, KK = D / 32, N = kParts<E>, NO = N == 1 ? 2 : 3, UPTO = NO - 1;  // (parts of a factor of the outputs)
-  typedef Shared<E, D, VEC, NO, !TRANSITION> Sh;
+  typedef Shared<E, D, WAVES, VEC, NO, !TRANSITION> Sh;
   typedef typename Sh::M M;
   typedef typename M::Rows_ T;
   __shared__ __align__(16) char lds[M::BYTES];
@@ -453,10 +453,10 @@ __global__ __launch_bounds__(4 * D) void join_kernel(const Rule<float> r, const 
 }
 
 // The way back: R, the gradient of the state, from the last chunk to the first.
-template <class E, int D, bool VEC>
-__global__ __launch_bounds__(4 * D, D == 128 || kParts<E> == 1 ? 2 : 1) void backward_kernel(const Rule<E> r) {
+template <class E, int D, int WAVES, bool VEC>
+__global__ __launch_bounds__(64 * WAVES, WAVES == 8 || kParts<E> == 1 ? 2 : 1) void backward_kernel(const Rule<E> r) {
   constexpr int MT = D / 16, KK = D / 32, N = kParts<E>;
-  typedef Shared<E, D, VEC, 3> Sh;
+  typedef Shared<E, D, WAVES, VEC, 3> Sh;
   typedef typename Sh::M M;
   typedef typename M::Rows_ T;
   __shared__ __align__(16) char lds[M::BYTES];
@@ -620,35 +620,47 @@ __global__ __launch_bounds__(4 * D, D == 128 || kParts<E> == 1 ? 2 : 1) void bac
 
 }  // namespace
 
-template <class E, int D, bool VEC>
-void forward_launches(const Rule<E>& r, int64_t pairs, hipStream_t s) {
-  if (r.segs > 1) {
-    forward_kernel<E, D, VEC, true><<<dim3((unsigned)pairs, (unsigned)r.segs - 1, 2), dim3(4 * D), 0, s>>>(r);
-    Rule<float> j = {};
-    j.first_env = r.first_env, j.heads = r.heads, j.dk = r.dk, j.dv = r.dv, j.segs = r.segs, j.phi = r.phi, j.seg_states = r.seg_states, j.wild = r.wild;
-    join_kernel<D><<<dim3((unsigned)pairs, (unsigned)pad16(r.dv) / 16), dim3(4 * D), 0, s>>>(j, r.state);
-  }
-  forward_kernel<E, D, VEC, false><<<dim3((unsigned)pairs, (unsigned)r.segs), dim3(4 * D), 0, s>>>(r);
+// f(dims of the keys in whole tiles, wavefronts): of the values' 64 or 128 columns, a wavefront for 16; keys of over 64 elements always have 8,
+// which share their loads and hold a segment's as many unit vectors.
+template <class F>
+void by_dims(int dk, int dv, F f) {
+  typedef std::integral_constant<int, 64> D64;
+  typedef std::integral_constant<int, 128> D128;
+  typedef std::integral_constant<int, 4> Four_;
+  typedef std::integral_constant<int, 8> Eight;
+  if (dk > 64) f(D128{}, Eight{});
+  else if (dv > 64) f(D64{}, Eight{});
+  else f(D64{}, Four_{});
 }
 template <class E>
 int launch_forward(const Rule<E>& r, int64_t envs, hipStream_t s) {
-  const int64_t pairs = envs * r.heads;
+  const unsigned pairs = (unsigned)(envs * r.heads);
   const bool vec = fours(r.k, r.dk) && fours(r.q, r.dk) && fours(r.y, r.dv);
-  if (r.dk <= 64 && r.dv <= 64) vec ? forward_launches<E, 64, true>(r, pairs, s) : forward_launches<E, 64, false>(r, pairs, s);
-  else vec ? forward_launches<E, 128, true>(r, pairs, s) : forward_launches<E, 128, false>(r, pairs, s);
+  by_dims(r.dk, r.dv, [&](auto d, auto waves) {
+    constexpr int D = decltype(d)::value, W = decltype(waves)::value;
+    if (r.segs > 1) {
+      const dim3 grid(pairs, (unsigned)r.segs - 1, 2);
+      if (vec) forward_kernel<E, D, W, true, true><<<grid, dim3(64 * W), 0, s>>>(r);
+      else forward_kernel<E, D, W, false, true><<<grid, dim3(64 * W), 0, s>>>(r);
+      Rule<float> j = {};
+      j.first_env = r.first_env, j.heads = r.heads, j.dk = r.dk, j.dv = r.dv, j.segs = r.segs, j.phi = r.phi, j.seg_states = r.seg_states, j.wild = r.wild;
+      join_kernel<D><<<dim3(pairs, (unsigned)pad16(r.dv) / 16), dim3(4 * D), 0, s>>>(j, r.state);
+    }
+    const dim3 grid(pairs, (unsigned)r.segs);
+    if (vec) forward_kernel<E, D, W, true, false><<<grid, dim3(64 * W), 0, s>>>(r);
+    else forward_kernel<E, D, W, false, false><<<grid, dim3(64 * W), 0, s>>>(r);
+  });
   return hipGetLastError() == hipSuccess ? RLK_OK : RLK_ERR_LAUNCH;
 }
 template <class E>
 int launch_backward(const Rule<E>& r, int64_t envs, hipStream_t s) {
   const dim3 grid((unsigned)(envs * r.heads));
   const bool vec = fours(r.k, r.dk) && fours(r.q, r.dk);
-  if (r.dk <= 64 && r.dv <= 64) {
-    if (vec) backward_kernel<E, 64, true><<<grid, dim3(256), 0, s>>>(r);
-    else backward_kernel<E, 64, false><<<grid, dim3(256), 0, s>>>(r);
-  } else {
-    if (vec) backward_kernel<E, 128, true><<<grid, dim3(512), 0, s>>>(r);
-    else backward_kernel<E, 128, false><<<grid, dim3(512), 0, s>>>(r);
-  }
+  by_dims(r.dk, r.dv, [&](auto d, auto waves) {
+    constexpr int D = decltype(d)::value, W = decltype(waves)::value;
+    if (vec) backward_kernel<E, D, W, true><<<grid, dim3(64 * W), 0, s>>>(r);
+    else backward_kernel<E, D, W, false><<<grid, dim3(64 * W), 0, s>>>(r);
+  });
   return hipGetLastError() == hipSuccess ? RLK_OK : RLK_ERR_LAUNCH;
 }
 template int launch_forward<bf16>(const Rule<bf16>&, int64_t, hipStream_t);
