@@ -15,9 +15,15 @@ namespace rlk {
 namespace {
 
 constexpr int kMostDim = 256;
+// Heads of a step that a group takes: 4, forward, share their angles; back, where a row is two arrays', 2 of them leave room for more wavefronts
+// ([64,1024,8+8,64] bf16: 144 us, 190 with 4).
 template <bool BACK>
-constexpr int kHeads = BACK ? 2 : 4;  // heads of a step that a group takes
-constexpr int kBackBlocks = 256;  // workgroups along the steps whose sums of weights' gradients are added up afterwards
+constexpr int kHeads = BACK ? 2 : 4;
+// Back: as many workgroups along the steps, for all blocks of heads together, as are resident at once, 5 a CU: each goes on over the steps until
+// all are done, and leaves its sums of the weights' gradients ([64,1024,8+8,64] bf16: 118 us; 130 with 4 a CU, 137 with 8, whose last ones
+// run by themselves).
+constexpr int kResident = 5;
+int64_t back_blocks(int64_t blocks) { return std::max<int64_t>(1, kResident * device_cus() / std::max<int64_t>(1, blocks)); }
 
 struct Frequencies {
   double turns[kMostDim / 2];  // of a position, by pair
@@ -41,7 +47,7 @@ struct Norms {
   int dim, rotary;
   const int64_t* positions;
   float eps, inv_dim;
-  float* partial;  // backward: [kBackBlocks at most][blocks of queries + keys][dim]
+  float* partial;  // backward: [back_blocks() at most][blocks of queries + keys][dim]
 };
 
 // N consecutive elements of E.
@@ -135,7 +141,7 @@ __device__ __forceinline__ float group_sum(float x) {
 
 // G lanes a row, UNITS units of N pairs a lane.
 template <class E, int N, int G, int UNITS, bool HALVES, bool BACK>
-__global__ __launch_bounds__(256) void norms_kernel(const Norms<E> n, const Frequencies f) {
+__global__ __launch_bounds__(256, BACK ? kResident : 4) void norms_kernel(const Norms<E> n, const Frequencies f) {
   const int lane = threadIdx.x & (G - 1), group = threadIdx.x / G;
   constexpr int GROUPS = 256 / G;
   const bool keys = (int)blockIdx.y >= n.side[0].blocks;
@@ -320,7 +326,7 @@ int run(const rlk_head_norms& c, const rlk_sequence* grads, float* const* weight
   auto launch = [&](auto N, auto G, auto U, auto halves) {
     constexpr int groups = 256 / decltype(G)::value;
     along = (n.tokens + groups - 1) / groups;
-    const int64_t most = BACK ? kBackBlocks : int64_t{1} << 20;
+    const int64_t most = BACK ? back_blocks(blocks) : int64_t{1} << 20;
     if (along > most) along = most;
     n.stride_envs = along * groups / n.steps, n.stride_steps = along * groups % n.steps;
     if (blocks > 0 && along > 0)
@@ -383,7 +389,7 @@ int rlk_query_key_norms(const rlk_head_norms* c, void* stream) {
 size_t rlk_head_norms_workspace_bytes(const rlk_head_norms* c) {
   if (!valid_norms(c)) return 0;
   const int64_t blocks = (c->q_heads + kHeads<true> - 1) / kHeads<true> + (c->k_heads + kHeads<true> - 1) / kHeads<true>;
-  return sizeof(float) * (size_t)(kBackBlocks * blocks * c->dim);
+  return sizeof(float) * (size_t)(std::max<int64_t>(kResident * device_cus(), blocks) * c->dim);  // (also of one side alone, whose blocks are fewer)
 }
 
 int rlk_query_key_norms_backward(const rlk_head_norms* c, rlk_sequence grad_q, rlk_sequence grad_k, float* q_weight_grad, float* k_weight_grad,

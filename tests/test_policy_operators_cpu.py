@@ -134,3 +134,13 @@ def test_head_norms_refusals():
                             ((x, x, None, None, p), dict(base=0), "base"), ((x, x, None, None, p), dict(eps=-1e-6), "eps"), ((x, x), dict(eps=float("nan")), "eps")):
         with pytest.raises(AssertionError, match=match):
             f(*args, **kw)
+
+
+def test_head_norms_workspace_serves_either_side_alone():
+    """A backward call with the gradient of one output has fewer blocks of heads, so more workgroups along the steps."""
+    lib = _native.load()
+    size = lambda q, k: lib.rlk_head_norms_workspace_bytes(ctypes.byref(_native.HeadNorms(  # noqa: E731
+        q=_native.Sequence(4096, 0, 0, 0), k=_native.Sequence(4096, 0, 0, 0), num_envs=8, seq_len=8192, q_heads=q, k_heads=k, dim=64, base=1e4, eps=1e-6)))
+    for q in (1, 2, 3, 5, 64, 4096):
+        for k in (0, 1, 2, 7, 4096):
+            assert size(q, k) >= max(size(q, 0), size(0, k) if k else 0) > 0
