@@ -1,7 +1,8 @@
 /*
  * rl_triton_policy.h -- C ABI of the operators around the return estimators: what a learner computes
- * before them (log-probabilities of the taken actions, a memory over the steps of an episode) and after
- * them (the clipped policy loss and its gradient).  The reference has no counterpart of these.
+ * before them (heads normed and rotated by their positions, a memory over the steps of an episode, the
+ * sampling of actions, log-probabilities of the taken ones) and after them (the clipped policy loss and its
+ * gradient).  The reference has no counterpart of these.
  *
  * As in rl_triton_amd.h: device pointers, work enqueued on `stream` (a hipStream_t), nothing allocates or
  * synchronises, inputs are never written, RLK_OK or a negative RLK_ERR_* code comes back.  Empty inputs

@@ -121,7 +121,7 @@ int backward(const rlk_delta_rule& c, const rlk_delta_rule_gradients& g, const v
 
 // One step: a workgroup per (environment, head) holds the state in registers, a thread a quad of columns of every ROWS-th row; what keys and
 // queries read from it is added up over the rows, then the state goes back with the correction.  The state is read and written once and
-// is nearly all there is to move.
+// is nearly all there is to move: [512] of 16 heads of 128 + 128 198 us, 5.4 TB/s; [8] of 4 heads of 64 + 64 5.5 us, a launch.
 template <class E, int LANES, int PER, bool VEC, bool NT>
 __global__ __launch_bounds__(256) void step_kernel(const Rule<E> r, int64_t first) {
   constexpr int ROWS = 256 / LANES;

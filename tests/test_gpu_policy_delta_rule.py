@@ -393,3 +393,31 @@ def test_values_are_checked_where_that_is_asked_for(monkeypatch):
         policy.compute_gated_delta_rule(x, x, x, g + 0.1, g)
     with pytest.raises(AssertionError, match="betas must lie"):
         policy.compute_gated_delta_rule(x, x, x, None, g - 0.1)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_padded_batches(dtype):
+    """Steps whose betas and log_decays are 0 write nothing: sequences of several lengths, padded, end with the states of the short ones, and
+    what is behind a sequence's end has no part in its gradients.  (The same sums, some of them with zeros: float32's rounding of the state, 64 steps of
+    2^-24 of its size at most, and of an output its own.)"""
+    q, k, v, g, beta, _, state = _cuda(*inputs(3, 150, 2, 24, 40, dtype, 23))
+    lengths = (150, 70, 1)
+    for e, n in enumerate(lengths):
+        g[e, n:] = 0.0
+        beta[e, n:] = 0.0
+    xs = [t.detach().clone().requires_grad_() for t in (q, k, v, g, beta, state)]
+    out, last = policy.compute_gated_delta_rule(*xs[:5], None, xs[5])
+    valid = torch.zeros(3, 150, 1, 1, device="cuda", dtype=dtype)
+    for e, n in enumerate(lengths):
+        valid[e, :n] = 1.0
+    grads = torch.autograd.grad((out, last), xs, (valid.expand_as(out).contiguous(), torch.ones_like(last)))
+    for e, n in enumerate(lengths):
+        ys = [t[e:e + 1, :n].detach().clone().requires_grad_() for t in (q, k, v, g, beta)] + [state[e:e + 1].detach().clone().requires_grad_()]
+        alone, end = policy.compute_gated_delta_rule(*ys[:5], None, ys[5])
+        step = torch.finfo(dtype).eps
+        assert torch.allclose(out[e:e + 1, :n].float(), alone.float(), rtol=step, atol=64 * 2.0 ** -24 * float(alone.detach().abs().max()))
+        assert torch.allclose(last[e:e + 1], end, rtol=0, atol=64 * 2.0 ** -24 * float(end.detach().abs().max()))
+        want = torch.autograd.grad((alone, end), ys, (torch.ones_like(alone), torch.ones_like(end)))
+        for a, b in zip((*(t[e:e + 1, :n] for t in grads[:5]), grads[5][e:e + 1]), want):
+            # (a gradient sums over up to 150 steps and 40 columns)
+            assert torch.allclose(a.float(), b.float(), rtol=torch.finfo(a.dtype).eps, atol=256 * 2.0 ** -24 * max(1.0, float(b.abs().max())))
