@@ -223,3 +223,35 @@ def test_calls_keep_nothing():
         gc.enable()
         assert torch.cuda.memory_allocated() == before
         assert fast.launched() - taken == launches
+
+
+def test_offsets_past_32_bits():
+    """Views whose environments or steps lie 2^31 elements and more apart: the bits of contiguous copies."""
+    big = torch.empty((1 << 33) + (1 << 16), dtype=torch.bfloat16, device="cuda")  # 17 GB, of which a few rows are written
+    q, k, v, g, beta, dones, state = (t.cuda() for t in inputs(3, 5, 2, 16, 16, torch.bfloat16, 5))
+
+    def spread(x, env, step):
+        y = big.as_strided(x.shape, (env, step, 16, 1))
+        return y.copy_(x)
+
+    for env, step in ((1 << 32, 64), (128, 1 << 31)):
+        for slot in range(3):  # (one array at a time lies in the buffer)
+            xs = [t.clone() for t in (q, k, v)]
+            near = [t.clone().requires_grad_() for t in (q, k, v)]
+            xs[slot] = spread(xs[slot], env, step)
+            far = [t.detach().requires_grad_() for t in xs]
+            outs = []
+            for x in (far, near):
+                y, last = policy.compute_gated_delta_rule(*x, g, beta, dones, state)
+                outs.append((y, last, *torch.autograd.grad(y, x, torch.ones_like(y))))
+            assert all(torch.equal(a, b) for a, b in zip(*outs))
+        up = spread(torch.randn(q.shape, device="cuda").bfloat16(), env, step)
+        y, _ = policy.compute_gated_delta_rule(*near, g, beta, dones, state)
+        y2, _ = policy.compute_gated_delta_rule(*near, g, beta, dones, state)
+        assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(y, near, up), torch.autograd.grad(y2, near, up.clone())))
+    for actions in (20, 5000):
+        x = big.as_strided((2, 2, actions), ((1 << 32) - 8, 1 << 31, 1))
+        x.copy_(torch.randn(x.shape, device="cuda"))
+        u = torch.rand(2, 2, device="cuda")
+        for kw in ({}, dict(top_k=9), dict(top_p=0.7)):
+            assert all(torch.equal(a, b) for a, b in zip(policy.compute_sampled_actions(x, u, **kw), policy.compute_sampled_actions(x.clone(), u, **kw)))
