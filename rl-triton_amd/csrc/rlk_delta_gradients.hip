@@ -12,8 +12,10 @@
 // A workgroup per chunk, a wavefront per 16 rows of the state.  The sums over the state's columns go 64 columns at a time, G, u and dv in LDS;
 // then keys, queries and both Y take their place.
 //
-// Bound by matrix products of three parts and by LDS: five operands of two or three parts each are read again for every 16 rows; two workgroups a CU.
-// [64,1024,8,64+64] bf16 361 us (1.9 TB/s); slices of 32 columns and three workgroups a CU 439, registers spilled.
+// [64,1024,8,64+64] bf16 361 us, 2.4 TB/s of 104 KB a chunk.  Bound by waits, half of a wavefront's time, with two workgroups a CU: vector units
+// issue for 37% of it, matrix units for 14, LDS conflicts take 21.  Slices of 32 columns and three workgroups a CU: 439, registers spilled;
+// keys and queries fetched with the first arrays: as before; workgroups that go from chunk to chunk with the next one's arrays on their way: 360 bytes a
+// lane spilled.
 #include "rlk_delta.hpp"
 
 namespace rlk {

@@ -5,7 +5,7 @@
 // below them from halves, M_21 = (1 - M_22 b) L_21 (1 - b M_11), for blocks of 16 and then of 32, by float32 matrix products.
 // Gates are added up in float64: D is a quotient of their sums' exponentials, and a head that forgets fast has large sums.
 //
-// Bound by the steps of a substitution after each other, 3 workgroups a CU: [64,1024,8,64] bf16 55 us (2.8 TB/s of keys in and records out; 66 with
+// Bound by the steps of a substitution after each other, 3 workgroups a CU: [64,1024,8,64] bf16 55 us (2.9 TB/s of keys in and records out; 66 with
 // two workgroups a CU), [1,16384,16,128] 40 us.
 #include "rlk_delta.hpp"
 
