@@ -444,7 +444,13 @@ __global__ __launch_bounds__(NT, NT >= 512 ? 4 : 2) void row_kernel(const Sampli
       if (!counts) {
         u64 left = 0;  // what top_k leaves
         if (s.by_k) {
-          each_again([&](float y, int i) { left += order(y, i) >= border ? weights(y) : 0; });
+          each(heavy, [&](const Vec<E>& x, int first, int) {
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+              left += order(x.get(e), first + e) >= border ? weights(x.get(e)) : 0;
+              apart(e);
+            }
+          });
           left = all_sum<NT>(left, m.sums);
         } else {
           find_bucket(false, 0.0, &left);
