@@ -9,7 +9,7 @@
 // loads first, with the angles formed once.  Angles: position times frequency in turns, in float64, and what is left of the nearest quarter
 // turn in float32, so that a position of a million is as exact as the first one.
 //
-// GPU time, bf16: [1,16384,16+4,128] 42 us (4.0 TB/s), [64,1024,8+8,64] forward 75 us (3.6 TB/s), back 118 us (3.4 TB/s) and 4 for the weights; what
+// GPU time, bf16: [1,16384,16+4,128] 42 us (4.0 TB/s; 52 where nothing is in the caches yet), [64,1024,8+8,64] forward 75 us (3.6 TB/s), back 118 us (3.4 TB/s) and 4 for the weights; what
 // keeps it from the copy's 4.8 are the angles, some third of the instructions.  One group for queries and keys alike, to share them: 42 -> 59
 // and 77 -> 92 us.
 #include "rlk_launch.hpp"
@@ -48,7 +48,7 @@ struct Norms {
   Side<E> side[2];  // queries, keys
   int64_t tokens, steps;
   int64_t stride_envs, stride_steps;  // from a group's token to its next one
-  int dim, rotary;
+  int dim, rotary, blocks;  // blocks: of heads, queries' and keys'
   const int64_t* positions;
   float eps, inv_dim;
   float* partial;  // backward: [back_blocks() at most][blocks of queries + keys][dim]
@@ -148,9 +148,12 @@ template <class E, int N, int G, int UNITS, bool HALVES, bool BACK>
 __global__ __launch_bounds__(256, BACK ? kResident : 4) void norms_kernel(const Norms<E> n, const Frequencies f) {
   const int lane = threadIdx.x & (G - 1), group = threadIdx.x / G;
   constexpr int GROUPS = 256 / G;
-  const bool keys = (int)blockIdx.y >= n.side[0].blocks;
+  // (the blocks of heads of the same steps run together, as a step's heads lie: [1,16384,16+4,128] 52 us, 55 with all steps of a block first)
+  const uint32_t slot = blockIdx.x / (uint32_t)n.blocks, slots = gridDim.x / (uint32_t)n.blocks;
+  const int block = (int)(blockIdx.x - slot * (uint32_t)n.blocks);
+  const bool keys = block >= n.side[0].blocks;
   const Side<E>& d = n.side[keys];
-  const int head0 = ((int)blockIdx.y - (keys ? n.side[0].blocks : 0)) * kHeads<BACK>, heads = d.heads - head0 < kHeads<BACK> ? d.heads - head0 : kHeads<BACK>;
+  const int head0 = (block - (keys ? n.side[0].blocks : 0)) * kHeads<BACK>, heads = d.heads - head0 < kHeads<BACK> ? d.heads - head0 : kHeads<BACK>;
   Elements<E, N> wa[UNITS], wb[UNITS], ga[UNITS], gb[UNITS];
 #pragma unroll
   for (int u = 0; u < UNITS; ++u) {
@@ -162,10 +165,10 @@ __global__ __launch_bounds__(256, BACK ? kResident : 4) void norms_kernel(const 
       ga[u].x[i] = gb[u].x[i] = 0.f;
     }
   }
-  int64_t token = (int64_t)blockIdx.x * GROUPS + group;
+  int64_t token = (int64_t)slot * GROUPS + group;
   // (a division in 64 bits is as much work as a row)
   int64_t env = n.tokens >> 32 == 0 ? (int64_t)((uint32_t)token / (uint32_t)n.steps) : token / n.steps, step = token - env * n.steps;
-  for (; token < n.tokens; token += (int64_t)gridDim.x * GROUPS) {
+  for (; token < n.tokens; token += (int64_t)slots * GROUPS) {
     const E* px = d.x + env * d.env + step * d.step + head0 * d.head;
     Elements<E, N> xa[kHeads<BACK>][UNITS], xb[kHeads<BACK>][UNITS], ya[BACK ? kHeads<BACK> : 1][UNITS], yb[BACK ? kHeads<BACK> : 1][UNITS];
 #pragma unroll
@@ -263,7 +266,7 @@ __global__ __launch_bounds__(256, BACK ? kResident : 4) void norms_kernel(const 
     }
     __syncthreads();
     if ((int)threadIdx.x < n.dim)
-      n.partial[((int64_t)blockIdx.x * gridDim.y + blockIdx.y) * n.dim + threadIdx.x] =
+      n.partial[(int64_t)blockIdx.x * n.dim + threadIdx.x] =
           (sums[0][threadIdx.x] + sums[1][threadIdx.x]) + (sums[2][threadIdx.x] + sums[3][threadIdx.x]);
   }
 }
@@ -325,17 +328,17 @@ int run(const rlk_head_norms& c, const rlk_sequence* grads, float* const* weight
   }
   const Frequencies& f = frequencies(c.base, n.rotary);
   const int blocks = n.side[0].blocks + n.side[1].blocks;
-  if (blocks > 65535) return RLK_ERR_INVALID_ARGUMENT;
+  n.blocks = blocks;
   int64_t along = 0;
   auto launch = [&](auto N, auto G, auto U, auto halves) {
     constexpr int groups = 256 / decltype(G)::value;
     along = (n.tokens + groups - 1) / groups;
-    const int64_t most = BACK ? back_blocks(blocks) : int64_t{1} << 20;
+    const int64_t most = BACK ? back_blocks(blocks) : std::max<int64_t>(1, (int64_t{1} << 23) / std::max(1, blocks));
     if (along > most) along = most;
     n.stride_envs = along * groups / n.steps, n.stride_steps = along * groups % n.steps;
     if (blocks > 0 && along > 0)
       norms_kernel<E, decltype(N)::value, decltype(G)::value, decltype(U)::value, decltype(halves)::value, BACK>
-          <<<dim3((unsigned)along, (unsigned)blocks), dim3(256), 0, s>>>(n, f);
+          <<<dim3((unsigned)(along * blocks)), dim3(256), 0, s>>>(n, f);
   };
   auto by_size = [&](auto halves) {
     const auto one = std::integral_constant<int, 1>{};

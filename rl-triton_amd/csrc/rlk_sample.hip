@@ -14,7 +14,7 @@
 // us of a CU's share, the rest waits for maxima, candidates and their sums.  [512] of 50001 float32, top-p, 92 us: 25.6 million exponentials
 // in float64 for the histogram and once more for the action's place, and three reads, of which the caches serve two.  Rows cut into slices
 // with lists of their own, a second launch to join them: 2 to 10 us more up to 131072 actions, half the time only from 2^20 on.  Sorting the
-// candidates in place of comparing all: 5 us more for 50, 3 to 12 less for 256.
+// candidates in place of comparing all: 5 us more for 50, from 4 more to 12 less for 256.
 #include "rlk_launch.hpp"
 #include "rlk_policy.hpp"
 
