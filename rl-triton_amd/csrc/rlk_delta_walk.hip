@@ -8,9 +8,8 @@
 // Bound by a chunk's chain: three products and the splits between them after each other (1200 vector instructions and 125 matrix products a wavefront and
 // chunk of 64 rows), two barriers, two wavefronts a SIMD to fill the waits (registers: a state of 128 rows, its split and the next chunk on its
 // way; LDS: 70 KB in bf16, 146 KB in float32).  GPU time, us: [64,1024,8,64+64] bf16 forward 183 (3.4 TB/s of what it reads and leaves for
-// the way back), back 174 (3.5 TB/s); [1,16384,16,128+128] bf16 177 in 16
-// segments, the segments' states 181 before them and 43 for joining; [37,333,4,40+72] float32 forward 75, back 67 (111 and 124 while keys were padded to
-// the dims of the values).  A third workgroup a CU, smaller tiles and states in LDS were slower or did not fit.
+// the way back), back 174 (3.5 TB/s); [1,16384,16,128+128] bf16 177 in 16 segments, the segments' states 181 before them and 43 for joining;
+// [37,333,4,40+72] float32 forward 75, back 67 (111 and 124 while keys were padded to the dims of the values).
 #include "rlk_delta.hpp"
 
 namespace rlk {

@@ -10,11 +10,11 @@
 // it lists the candidates and compares them as above; else it finds the last member's place from a histogram of the distances
 // to the maximum, counts and weights added up in LDS, and in its bucket by comparison or bisection.
 //
-// GPU time: [256] of 18 3.8 us, a launch.  [64] of 131072 bf16, top-k 50 with top-p and min-p, 21 us: a workgroup a row, whose two reads are 6 to 8
-// us of a CU's share, the rest waits for maxima, candidates and their sums.  [512] of 50001 float32, top-p, 92 us: 25.6 million exponentials
-// in float64 for the histogram and once more for the action's place, and three reads, of which the caches serve two.  Rows cut into slices
-// with lists of their own, a second launch to join them: 2 to 10 us more up to 131072 actions, half the time only from 2^20 on.  Sorting the
-// candidates in place of comparing all: 5 us more for 50, from 4 more to 12 less for 256.
+// GPU time: [256] of 18 3.8 us, a launch.  [64] of 131072 bf16, top-k 50 with top-p and min-p, 21 us: a workgroup a row, whose two reads are
+// some 9 of them (a row of 4096 takes 12), the rest waits for maxima, candidates and their sums.  [512] of 50001 float32, top-p, 92 us: 25.6
+// million exponentials in float64 for the histogram and once more for the action's place, and three reads, of which the caches serve two.
+// Rows cut into slices with lists of their own, a second launch to join them: 2 to 10 us more up to 131072 actions, half the time only from 2^20
+// on.  Sorting the candidates in place of comparing all: 5 us more for 50, from 4 more to 12 less for 256.
 #include "rlk_launch.hpp"
 #include "rlk_policy.hpp"
 
