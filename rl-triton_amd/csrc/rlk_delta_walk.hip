@@ -17,21 +17,20 @@ namespace delta {
 namespace {
 
 // D: dims of the keys padded to 64 or 128.
-template <class E, int D, int PARTS_OF_P>
+template <class E, int D>
 struct Lds {
   typedef Tile<E, D> Rows_;
-  typedef Tri<3> M;
-  typedef Tri<PARTS_OF_P> P;
-  static constexpr int K = 0, Q = Rows_::BYTES, MT = 2 * Rows_::BYTES, PT = MT + M::BYTES, REST = PT + P::BYTES;
+  typedef Tri<3> M;  // (the weighted q . k too)
+  static constexpr int K = 0, Q = Rows_::BYTES, MT = 2 * Rows_::BYTES, PT = MT + M::BYTES, REST = PT + M::BYTES;
   static constexpr int BYTES = REST + (int)(sizeof(Record) - offsetof(Record, ghi));
 };
 
 // The shared part of a walk: a chunk's arrays on their way to LDS, and the weighted q . k.
 // QUERIES: else only the keys and M are.
-template <class E, int D, int WAVES, bool VEC, int PARTS_OF_P, bool QUERIES = true>
+template <class E, int D, int WAVES, bool VEC, bool QUERIES = true>
 struct Shared {
   static constexpr int NT = 64 * WAVES;
-  typedef Lds<E, D, PARTS_OF_P> M;
+  typedef Lds<E, D> M;
   static constexpr int TILE_QUADS = 640, REST_QUADS = (int)(sizeof(Record) - offsetof(Record, ghi)) / 16, TILES_PER = (TILE_QUADS + NT - 1) / NT;
   Rows<E, D, NT, VEC> k, q;
   f32x4 m[TILES_PER], rest_quad;
@@ -88,12 +87,7 @@ struct Shared {
         const int j = 16 * tj + 4 * l4 + e;
         x[e] = j <= i && j >= begin ? x[e] * (scale * __expf((hi - hj[e]) + (lo - lj[e]))) : 0.f;
       }
-      char* p = lds + M::PT + M::P::row(16 * ti) + l16 * (M::P::row(16 * ti + 1) - M::P::row(16 * ti)) + 2 * (16 * tj + 4 * l4);
-#pragma unroll
-      for (int n = 0; n < PARTS_OF_P; ++n) {
-        *reinterpret_cast<u32x2*>(p + n * M::P::PART) = upper_quad(x);
-        x = rest(x);
-      }
+      Four<float>{x}.put(lds + M::PT + M::M::row(16 * ti) + l16 * (M::M::row(16 * ti + 1) - M::M::row(16 * ti)) + 2 * (16 * tj + 4 * l4), M::M::PART);
     }
   }
 };
@@ -199,8 +193,8 @@ __device__ __forceinline__ f32x4 columns_quad(const E (&x)[16], int t, int dim, 
 // unit vectors with no values (0).
 template <class E, int D, int WAVES, bool VEC, bool TRANSITION>
 __global__ __launch_bounds__(64 * WAVES, WAVES == 8 || kParts<E> == 1 ? 2 : 1) void forward_kernel(const Rule<E> r) {
-  constexpr int MT = D / 16, KK = D / 32, N = kParts<E>, NO = N == 1 ? 2 : 3, UPTO = NO - 1;  // (parts of a factor of the outputs)
-  typedef Shared<E, D, WAVES, VEC, NO, !TRANSITION> Sh;
+  constexpr int MT = D / 16, KK = D / 32;
+  typedef Shared<E, D, WAVES, VEC, !TRANSITION> Sh;
   typedef typename Sh::M M;
   typedef typename M::Rows_ T;
   __shared__ __align__(16) char lds[M::BYTES];
@@ -221,7 +215,6 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 || kParts<E> == 1 ? 2 : 1) v
 
   const At<T> at;
   const At<typename M::M> at_m;
-  const At<typename M::P> at_p;
   Sh sh;
   E v[16];
   sh.fetch(r, env, head, pair, first);
@@ -263,7 +256,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 || kParts<E> == 1 ? 2 : 1) v
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
           ks[t] = mul<2>(at.rows(lds + M::K, t, kk), s, ks[t]);
-          if constexpr (!TRANSITION) y[t] = mul<UPTO>(s, at.rows(lds + M::Q, t, kk), y[t]);
+          if constexpr (!TRANSITION) y[t] = mul<2>(s, at.rows(lds + M::Q, t, kk), y[t]);
           if (t & 1) apart();
         }
       }
@@ -295,15 +288,10 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 || kParts<E> == 1 ? 2 : 1) v
     }
     if constexpr (!TRANSITION) __syncthreads();
     if (mine) {
-      Op<NO> uo[2];
-#pragma unroll
-      for (int kk = 0; kk < 2; ++kk)
-#pragma unroll
-        for (int i = 0; i < NO; ++i) uo[kk].p[i] = u[kk].p[i];
 #pragma unroll
       for (int t = 0; t < 4; ++t)
 #pragma unroll
-        for (int kk = 0; kk <= t / 2; ++kk) if constexpr (!TRANSITION) y[t] = mul<UPTO>(uo[kk], at_p.rows(lds + M::PT, t, kk), y[t]);
+        for (int kk = 0; kk <= t / 2; ++kk) if constexpr (!TRANSITION) y[t] = mul<2>(u[kk], at_m.rows(lds + M::PT, t, kk), y[t]);
       float check = 0.f;
 #pragma unroll
       for (int t = 0; t < 4; ++t) check = odd(e[t], odd(y[t], check));
@@ -462,7 +450,7 @@ __global__ __launch_bounds__(4 * D) void join_kernel(const Rule<float> r, const 
 template <class E, int D, int WAVES, bool VEC>
 __global__ __launch_bounds__(64 * WAVES, WAVES == 8 || kParts<E> == 1 ? 2 : 1) void backward_kernel(const Rule<E> r) {
   constexpr int MT = D / 16, KK = D / 32, N = kParts<E>;
-  typedef Shared<E, D, WAVES, VEC, 3> Sh;
+  typedef Shared<E, D, WAVES, VEC> Sh;
   typedef typename Sh::M M;
   typedef typename M::Rows_ T;
   __shared__ __align__(16) char lds[M::BYTES];
@@ -476,7 +464,6 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 || kParts<E> == 1 ? 2 : 1) v
 
   const At<T> at;
   const At<typename M::M> at_m;
-  const At<typename M::P> at_p;
   Sh sh;
   E g[16];
   const int64_t last = r.chunks - 1;
@@ -522,7 +509,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 || kParts<E> == 1 ? 2 : 1) v
 #pragma unroll
         for (int t = 0; t < 4; ++t)
 #pragma unroll
-          for (int kk = t / 2; kk < 2; ++kk) z[t] = mul<2>(at_p.columns(lds + M::PT, t, kk), a[kk], z[t]);
+          for (int kk = t / 2; kk < 2; ++kk) z[t] = mul<2>(at_m.columns(lds + M::PT, t, kk), a[kk], z[t]);
       }
       f32x4 x[4];
       {
