@@ -78,7 +78,8 @@ struct Rule {
   float *gg, *gb;  // gradients of gates and betas
   // Sequences cut into segments of seg_chunks chunks, where there are few pairs.  A segment turns the state S that enters it into phi S + n:
   // [pair, segment] phi [pad16(dk), pad16(dk)], and in seg_states [pair, segment, pad16(dk), pad16(dv)] n of the segment before, then the state
-  // that enters.  wild: [pair], a segment that can only be walked from the state itself; such a pair is walked by one workgroup.
+  // that enters.  wild: [pair], a segment that can only be walked from the state itself, or one that a state enters that
+  // is not finite; such a pair is walked by one workgroup.
   int segs;
   int64_t seg_chunks;
   float *phi, *seg_states;

@@ -388,16 +388,20 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 || kParts<E> == 1 ? 2 : 1) v
 }
 
 // The states that enter the segments, one after the other: S' = phi S + n.  A workgroup per pair and 16 columns, a wavefront per 16 rows; the
-// columns are exchanged through LDS, and the next segment's rows of phi are on their way.
+// columns are exchanged through LDS, and the next segment's rows of phi are on their way.  A state that is not finite leaves a sum that is not
+// finite in every row, where phi is 0 behind an episode's end too: such a pair is walked from the state itself.
 template <int D>
 __global__ __launch_bounds__(4 * D) void join_kernel(const Rule<float> r, const float* state) {
   constexpr int KK = D / 32, ROW = D + 4;
   __shared__ __align__(16) float S[2][16 * ROW];  // [column, row]
+  __shared__ int wild;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l16 = lane & 15, l4 = lane >> 4;
   const int64_t pair = blockIdx.x, eh = r.first_env * r.heads + pair;
   const int dk = r.dk, dv = r.dv, rows = pad16(dk), dvp = pad16(dv), j = 16 * blockIdx.y + l16, d0 = 16 * wave + 4 * l4;
   const bool mine = 16 * wave < rows;
-  if (r.wild[pair] != 0) return;
+  if (threadIdx.x == 0) wild = r.wild[pair];  // (once for all: a workgroup of other columns may write it)
+  __syncthreads();
+  if (wild != 0) return;
 #pragma unroll
   for (int x = 0; x < 4; ++x)
     S[0][l16 * ROW + d0 + x] = state != nullptr && d0 + x < dk && j < dv ? state[eh * dk * dv + (int64_t)(d0 + x) * dv + j] : 0.f;
@@ -434,6 +438,7 @@ __global__ __launch_bounds__(4 * D) void join_kernel(const Rule<float> r, const 
         acc = mul<2>(a[kk], split<3>(lo, hi), acc);
       }
       settle();
+      if (__any(odd(acc, 0.f) != 0.f) && lane == 0) r.wild[pair] = 1;
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
         out[x * dvp] = acc[x];
