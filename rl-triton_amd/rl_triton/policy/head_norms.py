@@ -43,7 +43,7 @@ def _check(q, k, q_weight, k_weight, positions, base, rotary_dim, eps):
 
 def _forward(q, k, q_weight, k_weight, positions, settings):
     outs = [torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in (q, k)]
-    if q.shape[0] and q.shape[1] and (q.numel() or k.numel()):
+    if q.numel() or k.numel():
         _native.query_key_norms(q, k, *outs, q_weight, k_weight, positions, *settings)
     return tuple(outs)
 
@@ -65,7 +65,7 @@ class _QueryKeyNorms(torch.autograd.Function):
         to = [torch.empty(x.shape, dtype=x.dtype, device=x.device) if wanted and g is not None else None
               for x, wanted, g in ((q, wants[0], ups[0]), (k, wants[1], ups[1]), (q_weight, wants[2], ups[0]), (k_weight, wants[3], ups[1]))]
         if any(t is not None for t in to):
-            if q.shape[0] and q.shape[1] and (q.numel() or k.numel()):
+            if q.numel() or k.numel():
                 _native.query_key_norms_backward(q, k, *ups, *to, q_weight, k_weight, positions, *ctx.settings)
             else:
                 for t in to[2:]:
