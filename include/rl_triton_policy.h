@@ -6,7 +6,7 @@
  *
  * As in rl_triton_amd.h: device pointers, work enqueued on `stream` (a hipStream_t), nothing allocates or
  * synchronises, inputs are never written, RLK_OK or a negative RLK_ERR_* code comes back.  Empty inputs
- * return RLK_OK without a launch (losses and states excepted: those are written).  `bf16` non-zero: the arrays it names
+ * return RLK_OK without a launch (losses, states and the weights' gradients of the norms excepted: those are written).  `bf16` non-zero: the arrays it names
  * are rlk_bf16, otherwise float.  Sizes are counted and strides given in elements; every offset is formed in 64 bits.
  */
 #ifndef RL_TRITON_POLICY_H

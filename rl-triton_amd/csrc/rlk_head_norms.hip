@@ -271,7 +271,7 @@ __global__ __launch_bounds__(256, BACK ? kResident : 4) void norms_kernel(const 
   }
 }
 
-// The weights' gradients from the workgroups' sums: a workgroup per 4 elements and side, in float64 and a fixed order.
+// The weights' gradients from the workgroups' sums: a workgroup per 4 elements and side, in float64 and a fixed order.  0 where there are no rows.
 __global__ __launch_bounds__(256) void weights_kernel(const float* partial, int blocks, int q_blocks, int k_blocks, int dim, float* gq, float* gk) {
   float* out = blockIdx.y ? gk : gq;
   if (out == nullptr) return;
@@ -331,14 +331,14 @@ int run(const rlk_head_norms& c, const rlk_sequence* grads, float* const* weight
   n.blocks = blocks;
   int64_t along = 0;
   auto launch = [&](auto N, auto G, auto U, auto halves) {
+    if (n.tokens == 0 || blocks == 0) return;
     constexpr int groups = 256 / decltype(G)::value;
     along = (n.tokens + groups - 1) / groups;
     const int64_t most = BACK ? back_blocks(blocks) : std::max<int64_t>(1, (int64_t{1} << 23) / std::max(1, blocks));
     if (along > most) along = most;
     n.stride_envs = along * groups / n.steps, n.stride_steps = along * groups % n.steps;
-    if (blocks > 0 && along > 0)
-      norms_kernel<E, decltype(N)::value, decltype(G)::value, decltype(U)::value, decltype(halves)::value, BACK>
-          <<<dim3((unsigned)(along * blocks)), dim3(256), 0, s>>>(n, f);
+    norms_kernel<E, decltype(N)::value, decltype(G)::value, decltype(U)::value, decltype(halves)::value, BACK>
+        <<<dim3((unsigned)(along * blocks)), dim3(256), 0, s>>>(n, f);
   };
   auto by_size = [&](auto halves) {
     const auto one = std::integral_constant<int, 1>{};
@@ -407,6 +407,7 @@ int rlk_query_key_norms_backward(const rlk_head_norms* c, rlk_sequence grad_q, r
   const bool weights = q_weight_grad || k_weight_grad;
   if (weights && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 3u) != 0 || workspace_bytes < rlk_head_norms_workspace_bytes(c)))
     return RLK_ERR_WORKSPACE;
+  if (!weights && (c->num_envs == 0 || c->seq_len == 0 || c->q_heads + c->k_heads == 0)) return RLK_OK;
   const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   const rlk_sequence grads[2] = {grad_q, grad_k};
   float* const to[2] = {q_weight_grad, k_weight_grad};
