@@ -6,8 +6,10 @@ namespace rlk {
 namespace delta {
 namespace {
 
-// How many environments go into one set of launches: their records (and a backward pass's gradients of states) are scratch memory, of some GB at
-// most where that still leaves every CU pairs to walk, and a launch has at most 2^31 work-items.
+// How many environments go into one set of launches: their records (11.5 KB a chunk of a pair, environment and head) or a backward pass's gradients
+// of states and z (up to 96 KB) are scratch memory.  As many as 1 GB holds, but at least 512 pairs, so that every CU has some to walk, and at
+// least one environment: a backward pass of 512 pairs over 16384 steps asks for 12 GB at 128 + 128 dims, one environment of 16 heads and 2^20 steps for
+// 24.  A launch has at most 2^31 work-items.
 constexpr size_t kScratch = size_t{1} << 30;
 constexpr int64_t kMostChunks = int64_t{1} << 22;
 inline int64_t envs_at_once(int64_t envs, int64_t heads, int64_t chunks, size_t chunk_bytes) {

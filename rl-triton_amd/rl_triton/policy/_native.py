@@ -256,7 +256,8 @@ def _delta_rule(q, k, v, out, log_decays, betas, dones, state, state_out, scale,
 
 
 def _scratch(need, like):
-    """Memory of one call, from torch's allocator: it may be some GB, so none is kept.  (Its later users follow on the stream.)"""
+    """Memory of one call, from torch's allocator: it may be GBs (1, or what 512 pairs of environments and heads ask for, or one environment), so none is
+    kept.  (Its later users follow on the stream.)"""
     return torch.empty(need, dtype=torch.uint8, device=like.device)
 
 
