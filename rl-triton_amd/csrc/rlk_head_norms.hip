@@ -205,7 +205,20 @@ __global__ __launch_bounds__(256, BACK ? kResident : 4) void norms_kernel(const 
         for (int i = 0; i < N; ++i) sum = fmaf(xa[h][u].x[i], xa[h][u].x[i], fmaf(xb[h][u].x[i], xb[h][u].x[i], sum));
       const float square = fmaf(group_sum<G>(sum), n.inv_dim, n.eps);
       float r = __builtin_amdgcn_rsqf(square);
-      r = square < 1e-30f || square > 1e30f ? 1.f / sqrtf(square) : fmaf(r * fmaf(-square * r, r, 1.f), 0.5f, r);  // (one step to the last bit)
+      r = fmaf(r * fmaf(-square * r, r, 1.f), 0.5f, r);  // (one step to the last bit)
+      if (square < 1e-30f || square > 1e30f) {
+        // Squares near or past the ends of float32, in all lanes of the group alike: of elements and a root of eps taken times a power of two.
+        const float times = square < 1.f ? 0x1p80f : 0x1p-80f;
+        sum = 0.f;
+#pragma unroll
+        for (int u = 0; u < UNITS; ++u)
+#pragma unroll
+          for (int i = 0; i < N; ++i) {
+            const float a = xa[h][u].x[i] * times, b = xb[h][u].x[i] * times;
+            sum = fmaf(a, a, fmaf(b, b, sum));
+          }
+        r = times / sqrtf(fmaf(group_sum<G>(sum), n.inv_dim, n.eps * times * times));
+      }
       if constexpr (!BACK) {
 #pragma unroll
         for (int u = 0; u < UNITS; ++u) {
