@@ -213,17 +213,20 @@ __device__ __forceinline__ float number_at(const char* tile, int i, int d) {
   return x;
 }
 
-// ... and of 4 columns from d on.
+// ... and 4 of them from a place on.
 template <class T>
-__device__ __forceinline__ f32x4 numbers_at(const char* tile, int i, int d) {
-  f32x4 x = zero4();
+__device__ __forceinline__ f32x4 parts_at(const char* place) {
+  f32x4 x;
 #pragma unroll
   for (int n = T::N - 1; n >= 0; --n) {
-    const u32x2 w = *reinterpret_cast<const u32x2*>(tile + n * T::PART + T::row(i) + 2 * d);
-    x += f32x4{__uint_as_float(w[0] << 16), __uint_as_float(w[0] & 0xffff0000u), __uint_as_float(w[1] << 16), __uint_as_float(w[1] & 0xffff0000u)};
+    const u32x2 w = *reinterpret_cast<const u32x2*>(place + n * T::PART);
+    const f32x4 y{__uint_as_float(w[0] << 16), __uint_as_float(w[0] & 0xffff0000u), __uint_as_float(w[1] << 16), __uint_as_float(w[1] & 0xffff0000u)};
+    x = n == T::N - 1 ? y : x + y;
   }
   return x;
 }
+template <class T>
+__device__ __forceinline__ f32x4 numbers_at(const char* tile, int i, int d) { return parts_at<T>(tile + T::row(i) + 2 * d); }
 
 // 4 consecutive elements as they are stored.
 template <class E>

@@ -5,17 +5,19 @@
 //   dq_i = scale back_i S G_i + sum_j Y1_ij k_j
 //   dk_i = dk+ + dk-,   dk+_i = -back_i S dv_i + sum_j Y2_ij k_j,   dk-_j = into_j R u_j + sum_i (Y1_ij q_i + Y2_ij k_i)
 //   db_i = z_i . w_i
-// A gate's gradient is the sum of every term that its factor is in.  Terms with D_ij have the gates from j + 1 to i; added at i and taken
-// away at j they sum up from the end: x_i = q_i . dq_i + k_i . (dk+_i - dk-_i), and at the chunk's last step also the terms of
-// S' (keep R . S + sum_j into_j k_j . R u_j); dg_t = sum of x_i from t to its episode's end, in float64.
+// A gate's gradient is the sum of every term that its factor is in: with W_ij = Y1_ij q_i . k_j + Y2_ij k_i . k_j, which has the gates from j + 1 to i,
+//   dg_t = keep R . S + sum_{i >= t} back_i (scale q_i . S G_i - k_i . S dv_i) + sum_{j < t} into_j k_j . R u_j + sum_{i >= t > j} W_ij.
+// Nothing is taken off again, so the gradient of a gate that leaves little of the state is as exact as its terms, which are as small.  (As a sum from the
+// end, of each W_ij added at i and taken away at j, it was a difference of numbers up to exp(-g) times its size: nothing was left of it from
+// g = -16 on.)  The last sum by tiles of 16 steps: a tile's sums by rows (i) and by columns (j), and what one on the diagonal gives for each t.
 //
 // A workgroup per chunk, a wavefront per 16 rows of the state.  The sums over the state's columns go 64 columns at a time, G, u and dv in LDS;
 // then keys, queries and both Y take their place.
 //
-// [64,1024,8,64+64] bf16 361 us, 2.4 TB/s of 104 KB a chunk.  Bound by waits, half of a wavefront's time, with two workgroups a CU: vector units
-// issue for 37% of it, matrix units for 14, LDS conflicts take 21.  Slices of 32 columns and three workgroups a CU: 439, registers spilled;
-// keys and queries fetched with the first arrays: as before; workgroups that go from chunk to chunk with the next one's arrays on their way: 360 bytes a
-// lane spilled.
+// [64,1024,8,64+64] bf16 390 us, 2.2 TB/s of 104 KB a chunk.  Bound by waits, half of a wavefront's time, with two workgroups a CU: vector units
+// issue for 42% of it, matrix units for 16, LDS conflicts take 27.  The gates' sums are 27 more than one sum from the end was.  Slices of 32
+// columns and three workgroups a CU: 439 against 361 then, registers spilled; keys and queries fetched with the first arrays: as before;
+// workgroups that go from chunk to chunk with the next one's arrays on their way: 360 bytes a lane spilled.
 #include "rlk_delta.hpp"
 
 namespace rlk {
@@ -54,13 +56,39 @@ struct Corrections {
   }
 };
 
+// Of a quarter's 16 lanes: the value of the lane N further on (UP: or before), 0 past the quarter's end.  All lanes have to take part.
+template <int N, bool UP>
+__device__ __forceinline__ float beside(float x) {
+  return __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(x), (UP ? 0x110 : 0x100) + N, 0xf, 0xf, true));
+}
+// The sum over these lanes from the first (UP) or the last one to this one.
+template <bool UP>
+__device__ __forceinline__ float added_up(float x) {
+  x += beside<1, UP>(x);
+  x += beside<2, UP>(x);
+  x += beside<4, UP>(x);
+  x += beside<8, UP>(x);
+  return x;
+}
+// x of the two quarters 0 + 1 and 2 + 3, and y's between them: (x, y, x, y) by quarters.
+__device__ __forceinline__ float by_twos(float x, float y) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(y), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+// ... of the two halves: x in the lower one, y in the upper one.
+__device__ __forceinline__ float by_halves(float x, float y) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(y), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+__device__ __forceinline__ float of_lane(float x, int lane) { return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(x), lane)); }
+
 template <class E, int D, bool VEC>
 __global__ __launch_bounds__(4 * D, D == 128 || kParts<E> == 1 ? 2 : 1) void gradients_kernel(const Rule<E> r) {
   constexpr int NT = 4 * D, WAVES = D / 16, N = kParts<E>;
   typedef Lds<E, D> M;
   typedef typename M::K T;
   __shared__ __align__(16) char lds[M::BYTES];
-  __shared__ float sums[WAVES][C + 2];
+  __shared__ float kept_sums[WAVES];
   __shared__ int found[WAVES];
   constexpr int REST_QUADS = (int)(sizeof(Record) - offsetof(Record, ghi)) / 16;
   __shared__ f32x4 rest_of_record[REST_QUADS];
@@ -221,11 +249,83 @@ __global__ __launch_bounds__(4 * D, D == 128 || kParts<E> == 1 ? 2 : 1) void gra
       const float d = __expf((hi - hj[e]) + (lo - lj[e]));
       a[e] = j >= begin && (second ? j < i : j <= i) ? a[e] * (second ? -d : d * r.scale) : 0.f;
     }
+    ya[slot] = a;
     char* y = lds + (second ? M::Y2 : M::Y1);
     const int first = M::Y::row(16 * ti), stride = ti < 2 ? M::Y::row(1) : M::Y::row(33) - M::Y::row(32);
     Four<float>{a}.put(y + first + l16 * stride + 2 * (16 * tj + 4 * l4), M::Y::PART);
     if (tj == ti && (ti & 1) == 0)  // the tile above the diagonal that products go over
       Four<float>{zero4()}.put(y + first + l16 * stride + 2 * (16 * tj + 16 + 4 * l4), M::Y::PART);
+  }
+  // Where the gates' sums are kept: the record's gates have had their use, and there are 16 bytes behind each of Y's rows.  Of W's tiles, of Y1 and
+  // of Y2, the sums of their rows (on the diagonal: what a tile gives for each step) and of their columns; a wavefront's sums of a step.
+  float* by_row = reinterpret_cast<float*>(rest_of_record);
+  static_assert(320 * sizeof(float) <= offsetof(Record, keep) - offsetof(Record, ghi));
+  auto behind = [&](int y, int part, int i) { return lds + y + part * M::Y::PART + M::Y::row(i) + (i < 32 ? 64 : 128); };
+  auto by_column = [&](bool y2, int tile, int quarter) { return reinterpret_cast<f32x4*>(behind(y2 ? M::Y2 : M::Y1, 2, 4 * tile + quarter)); };
+  auto of_step = [&](int y, int w, int i) { return reinterpret_cast<float*>(behind(y, w >> 2, i)) + (w & 3); };
+  k.put(lds, dk, 0, n);
+  q.put(lds + M::QT, dk, 0, n);
+  __syncthreads();
+  if (r.gg != nullptr) {
+    const char* rows_i = lds + (second ? 0 : M::QT);
+    f32x4 qk[TILES];  // or k . k
+#pragma unroll
+    for (int slot = 0; slot < TILES; ++slot) qk[slot] = zero4();
+#pragma unroll
+    for (int kk = 0; kk < D / 32; ++kk) {
+      if (32 * kk >= dk) continue;
+#pragma unroll
+      for (int slot = 0; slot < TILES; ++slot) {
+        int ti, tj;
+        if (tile_of(slot, ti, tj)) qk[slot] = mul<2>(at_k.rows(lds, tj, kk), at_k.rows(rows_i, ti, kk), qk[slot]);
+      }
+    }
+    settle();
+#pragma unroll
+    for (int slot = 0; slot < TILES; ++slot) {
+      int ti, tj;
+      if (!tile_of(slot, ti, tj)) continue;
+      const int i = 16 * ti + l16;
+      f32x4 later;  // sums over the tile's rows from i on
+      float row = 0.f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int j = 16 * tj + 4 * l4 + e;
+        // (Y is 0 between episodes, where q . k may be anything)
+        const float y = ya[slot][e], w = y != 0.f && j < i ? y * qk[slot][e] : 0.f;
+        row += w;
+        later[e] = added_up<false>(w);
+      }
+      if (ti == tj) {
+        row = 0.f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) row += 4 * l4 + e < l16 ? later[e] : 0.f;
+      }
+      row = by_twos(row, row);
+      row = by_halves(row, row);
+      const int tile = ti * (ti + 1) / 2 + tj;
+      if (l4 == 0) by_row[160 * second + 16 * tile + l16] = row;
+      if (l16 == 0) *by_column(second, tile, l4) = later;
+    }
+    if (mine) {
+      // what the state before the chunk gives to a step, and what a step gives to the one after it
+      float given[4];
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        const int i = 16 * t + l16;
+        const f32x4 q4 = numbers_at<T>(lds + M::QT, i, 16 * wave + 4 * l4), k4 = numbers_at<T>(lds, i, 16 * wave + 4 * l4);
+        float x = 0.f, y = 0.f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x = fmaf(q4[e], dq[t][e], fmaf(k4[e], up[t][e], x)), y = fmaf(k4[e], down[t][e], y);
+        given[t] = by_twos(back[t] != 0.f ? x : 0.f, into[t] != 0.f ? y : 0.f);
+      }
+#pragma unroll
+      for (int t = 0; t < 4; t += 2) {
+        const int i = 16 * (t + (l4 >> 1)) + l16;
+        const float x = by_halves(given[t], given[t + 1]);  // (x, y of t, x, y of t + 1)
+        *of_step(l4 & 1 ? M::Y1 : M::Y2, wave, i) = x;
+      }
+    }
   }
   // Keys and queries that are not finite would reach other episodes as 0 inf: then an episode at a time.
   bool wild = false;
@@ -236,25 +336,17 @@ __global__ __launch_bounds__(4 * D, D == 128 || kParts<E> == 1 ? 2 : 1) void gra
     if (wild) {
       const uint64_t later = cuts & ~(((uint64_t)2 << from) - 1);
       to = later != 0 ? __ffsll((long long)later) - 1 : n;
+      __syncthreads();
+      k.put(lds, dk, from, to);
+      q.put(lds + M::QT, dk, from, to);
+      __syncthreads();
     }
-    if (from > 0) __syncthreads();
-    k.put(lds, dk, from, to);
-    q.put(lds + M::QT, dk, from, to);
-    __syncthreads();
-    float total = 0.f;
     if (mine) {
-      // what the steps wrote into S'
-#pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        const int i = 16 * t + l16;
-        if (i >= from && i < to && into[t] != 0.f) {
-          const f32x4 x = numbers_at<T>(lds, i, 16 * wave + 4 * l4) * down[t];
-          total += (x[0] + x[1]) + (x[2] + x[3]);
-        }
-      }
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
         f32x4 a = dq[t], b = up[t], c = down[t];
+        const int i = 16 * t + l16;
+        const bool inside = i >= from && i < to;
 #pragma unroll
         for (int kk = 0; kk < 2; ++kk) {
           const Op<N> kc = at_k.columns(lds, wave, kk), qc = at_k.columns(lds + M::QT, wave, kk);
@@ -268,26 +360,13 @@ __global__ __launch_bounds__(4 * D, D == 128 || kParts<E> == 1 ? 2 : 1) void gra
           }
         }
         settle();
-        const int i = 16 * t + l16;
-        const bool inside = i >= from && i < to;
         if (inside) dq[t] = a, up[t] = b, down[t] = c;
-        float x = 0.f;
-        if (inside) {
-          const f32x4 a = numbers_at<T>(lds + M::QT, i, 16 * wave + 4 * l4) * dq[t] + numbers_at<T>(lds, i, 16 * wave + 4 * l4) * (up[t] - down[t]);
-          x = (a[0] + a[1]) + (a[2] + a[3]);
-        }
-        x += __shfl_xor(x, 16);
-        x += __shfl_xor(x, 32);
-        if (l4 == 0 && inside) sums[wave][i] = x;
       }
     }
-    if (to == n) {
-      total += kept;
-#pragma unroll
-      for (int d = 1; d < 64; d <<= 1) total += __shfl_xor(total, d);
-      if (lane == 0) sums[wave][C] = mine ? total : 0.f;
-    }
   }
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) kept += __shfl_xor(kept, d);
+  if (lane == 0) kept_sums[wave] = kept;
   __syncthreads();
   if (mine) {
 #pragma unroll
@@ -314,20 +393,39 @@ __global__ __launch_bounds__(4 * D, D == 128 || kParts<E> == 1 ? 2 : 1) void gra
     }
   }
   if (wave == 0 && r.gg != nullptr) {
-    const int used = (dk + 15) / 16;
-    double x = 0.0;
-    if (lane < n)
-      for (int i = 0; i < used; ++i) x += (double)sums[i][lane];
-    if (lane == n - 1)
-      for (int i = 0; i < used; ++i) x += (double)sums[i][C];
-    const uint64_t later = lane < 63 ? cuts & ~(((uint64_t)2 << lane) - 1) : 0;
-    const int end = later != 0 ? __ffsll((long long)later) - 1 : n;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const double next = __shfl_down(x, d);
-      if (lane + d < end) x += next;
+    const int used = (dk + 15) / 16, T = lane >> 4;
+    float x = 0.f, before = 0.f, all = 0.f;  // of the steps from here on, of those before, of the whole chunk
+    for (int i = 0; i < used; ++i) {
+      if (lane < n) x += *of_step(M::Y2, i, lane), before += *of_step(M::Y1, i, lane);
+      all += kept_sums[i];
     }
-    const float g = (cuts >> lane) & 1 || (r.from_zero && s0 + lane == 0) ? 0.f : (float)x;
+    // W's tiles in this step's rows, in its columns, and those that lie beyond it both ways
+    float rows = 0.f, columns = 0.f, beyond = 0.f;
+#pragma unroll
+    for (int ti = 0; ti < 4; ++ti)
+#pragma unroll
+      for (int tj = 0; tj <= ti; ++tj) {
+        const int tile = ti * (ti + 1) / 2 + tj;
+        const float f = by_row[16 * tile + l16] + by_row[160 + 16 * tile + l16];
+        if (ti == tj) {
+          all += T == ti ? f : 0.f;
+        } else {
+          rows += T == ti ? f : 0.f;
+          beyond += tj < T && T < ti ? f : 0.f;
+          const int at = l16 & 3;
+          columns += T == tj ? reinterpret_cast<const float*>(by_column(false, tile, l16 >> 2))[at] + reinterpret_cast<const float*>(by_column(true, tile, l16 >> 2))[at] : 0.f;
+        }
+      }
+    // (each of these sums has terms of this gate alone, so nothing that is not finite comes in from another episode)
+    x = added_up<false>(x), rows = added_up<false>(rows), beyond = added_up<false>(beyond);
+    before = added_up<true>(before), columns = added_up<true>(columns);
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      const float later = of_lane(x, 16 * t), earlier = of_lane(before, 16 * t + 15), past = of_lane(beyond, 16 * t);
+      all += (t > T ? later : 0.f) + (t < T ? earlier : 0.f) + (t == T ? past : 0.f);
+    }
+    all += (x + rows) + beside<1, true>(before + columns);
+    const float g = (cuts >> lane) & 1 || (r.from_zero && s0 + lane == 0) ? 0.f : all;
     if (lane < n) r.gg[(env * r.seq_len + s0 + lane) * r.heads + head] = g;
   }
 }
