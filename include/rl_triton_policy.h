@@ -141,12 +141,16 @@ typedef struct rlk_delta_rule_gradients {
   float *state, *log_decays, *betas;
 } rlk_delta_rule_gradients;
 
-size_t rlk_delta_rule_workspace_bytes(int64_t num_envs, int64_t seq_len, int64_t heads, int64_t dim_k, int64_t dim_v, int backward);
+/* Of a forward call, of a backward one, of a forward call with `saved` (whose records lie there; NULL will do where 0 bytes are asked for). */
+#define RLK_DELTA_FORWARD 0
+#define RLK_DELTA_BACKWARD 1
+#define RLK_DELTA_FORWARD_SAVED 2
+size_t rlk_delta_rule_workspace_bytes(int64_t num_envs, int64_t seq_len, int64_t heads, int64_t dim_k, int64_t dim_v, int pass);
 /* Of what a forward call leaves for the backward one (16-byte aligned). */
 size_t rlk_delta_rule_saved_bytes(int64_t num_envs, int64_t seq_len, int64_t heads, int64_t dim_k, int64_t dim_v);
 /* `saved`: NULL, or what the backward call is to read.  heads * ceil(seq_len / 64) is at most 2^22. */
 int rlk_gated_delta_rule(const rlk_delta_rule *call, void *saved, size_t saved_bytes, void *stream);
-/* `call` as the forward one was, with a workspace for backward = 1; its out and state_out are not looked at, and of its
+/* `call` as the forward one was, with a workspace of its own; its out and state_out are not looked at, and of its
  * state only whether there is one. */
 int rlk_gated_delta_rule_backward(const rlk_delta_rule *call, const rlk_delta_rule_gradients *grads, const void *saved, size_t saved_bytes,
                                   void *stream);

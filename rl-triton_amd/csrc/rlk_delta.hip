@@ -34,7 +34,7 @@ bool valid(const rlk_delta_rule& c, bool steps) {
 }
 // Whether heads and chunks are few enough for the launches of one environment.
 bool fits(const rlk_delta_rule& c) { return c.seq_len <= (int64_t{1} << 30) && c.heads <= kMostChunks && c.heads * chunks_of(c.seq_len) <= kMostChunks; }
-bool scratch_fits(const void* p, size_t have, size_t need) { return have >= need && p != nullptr && (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+bool scratch_fits(const void* p, size_t have, size_t need) { return need == 0 || (have >= need && p != nullptr && (reinterpret_cast<uintptr_t>(p) & 15u) == 0); }
 
 template <class E>
 Rule<E> rule(const rlk_delta_rule& c) {
@@ -79,12 +79,12 @@ int forward(const rlk_delta_rule& c, void* saved, hipStream_t s) {
   const int64_t most = envs_at_once(c.num_envs, c.heads, r.chunks, sizeof(Record));
   for (r.first_env = 0; r.first_env < c.num_envs; r.first_env += most) {
     const int64_t envs = c.num_envs - r.first_env < most ? c.num_envs - r.first_env : most;
-    r.records = static_cast<Record*>(c.workspace);
     const int64_t pairs = envs * c.heads;
+    r.records = static_cast<Record*>(c.workspace);
+    float* p = reinterpret_cast<float*>(r.records + (saved != nullptr ? 0 : pairs * r.chunks));
     const Segments plan = plan_segments(pairs, r.chunks);
     r.segs = plan.segs, r.seg_chunks = plan.chunks;
     if (plan.segs > 1) {
-      float* p = reinterpret_cast<float*>(r.records + pairs * r.chunks);
       r.wild = reinterpret_cast<int*>(p);
       r.phi = p + (pairs + 3) / 4 * 4;
       r.seg_states = r.phi + (size_t)(pairs * plan.segs) * pad16(r.dk) * pad16(r.dk);
@@ -259,14 +259,15 @@ using namespace rlk::delta;
 
 extern "C" {
 
-size_t rlk_delta_rule_workspace_bytes(int64_t num_envs, int64_t seq_len, int64_t heads, int64_t dim_k, int64_t dim_v, int backward) {
+size_t rlk_delta_rule_workspace_bytes(int64_t num_envs, int64_t seq_len, int64_t heads, int64_t dim_k, int64_t dim_v, int pass) {
+  const bool backward = pass == RLK_DELTA_BACKWARD;
   if (num_envs <= 0 || seq_len <= 0 || heads <= 0 || dim_k <= 0 || dim_v <= 0 || dim_k > 128 || dim_v > 128 || heads > kMostChunks ||
       seq_len > (int64_t{1} << 30) || heads * chunks_of(seq_len) > kMostChunks)
     return 0;
   const int64_t chunks = chunks_of(seq_len);
   const size_t each = backward ? backward_chunk_bytes(dim_k, dim_v) : sizeof(Record);
   const int64_t envs = envs_at_once(num_envs, heads, chunks, each);
-  size_t bytes = (size_t)(envs * heads * chunks) * each;
+  size_t bytes = pass == RLK_DELTA_FORWARD_SAVED ? 0 : (size_t)(envs * heads * chunks) * each;
   if (!backward) {  // (the last set of environments, the smaller one, may be the one that is cut)
     size_t floats = segment_floats(envs * heads, plan_segments(envs * heads, chunks), (int)dim_k, (int)dim_v);
     if (const int64_t left = num_envs % envs) {
@@ -291,7 +292,8 @@ int rlk_gated_delta_rule(const rlk_delta_rule* call, void* saved, size_t saved_b
   if (!fits(*call)) return RLK_ERR_INVALID_ARGUMENT;
   if ((saved != nullptr && !scratch_fits(saved, saved_bytes, Saved(saved, *call).bytes())) ||
       !scratch_fits(call->workspace, call->workspace_bytes,
-                    rlk_delta_rule_workspace_bytes(call->num_envs, call->seq_len, call->heads, call->dim_k, call->dim_v, 0)))
+                    rlk_delta_rule_workspace_bytes(call->num_envs, call->seq_len, call->heads, call->dim_k, call->dim_v,
+                                                   saved != nullptr ? RLK_DELTA_FORWARD_SAVED : RLK_DELTA_FORWARD)))
     return RLK_ERR_WORKSPACE;
   return call->bf16 ? forward<bf16>(*call, saved, s) : forward<float>(*call, saved, s);
 }
@@ -310,7 +312,7 @@ int rlk_gated_delta_rule_backward(const rlk_delta_rule* call, const rlk_delta_ru
   if (c.seq_len == 0) return same_state(c, grads->state_out, grads->state, s);
   if (!fits(c)) return RLK_ERR_INVALID_ARGUMENT;
   if (!scratch_fits(saved, saved_bytes, Saved(nullptr, c).bytes()) ||
-      !scratch_fits(c.workspace, c.workspace_bytes, rlk_delta_rule_workspace_bytes(c.num_envs, c.seq_len, c.heads, c.dim_k, c.dim_v, 1)))
+      !scratch_fits(c.workspace, c.workspace_bytes, rlk_delta_rule_workspace_bytes(c.num_envs, c.seq_len, c.heads, c.dim_k, c.dim_v, RLK_DELTA_BACKWARD)))
     return RLK_ERR_WORKSPACE;
   return c.bf16 ? backward<bf16>(c, *grads, saved, s) : backward<float>(c, *grads, saved, s);
 }

@@ -179,7 +179,8 @@ bool delta_args(PolicyCall& c, PyObject* const* a, PyObject* dones_, PyObject* s
 // The launch of a sequence's forward pass; with `saved`, what the backward pass reads.
 int delta_forward(rlk_delta_rule* t, const at::Tensor& out, const at::Tensor& last, const at::Tensor* saved) {
   t->out = rows_of(out), t->state_out = static_cast<float*>(last.data_ptr());
-  const at::Tensor scratch = call_scratch(rlk_delta_rule_workspace_bytes(t->num_envs, t->seq_len, t->heads, t->dim_k, t->dim_v, 0), out);
+  const at::Tensor scratch = call_scratch(rlk_delta_rule_workspace_bytes(t->num_envs, t->seq_len, t->heads, t->dim_k, t->dim_v,
+                                                                         saved ? RLK_DELTA_FORWARD_SAVED : RLK_DELTA_FORWARD), out);
   t->workspace = scratch.data_ptr(), t->workspace_bytes = (size_t)scratch.numel();
   return rlk_gated_delta_rule(t, saved ? saved->data_ptr() : nullptr, saved ? (size_t)saved->numel() : 0,
                               c10::hip::getCurrentHIPStream(out.get_device()).stream());
@@ -229,7 +230,7 @@ struct GatedDeltaRule : torch::autograd::Function<GatedDeltaRule> {
     for (int i = 0; i < 3; ++i)
       if (out[i].defined()) *sequences[i] = rows_of(out[i]);
     to.log_decays = floats(out[3]), to.betas = floats(out[4]), to.state = floats(out[5]);
-    const at::Tensor scratch = call_scratch(rlk_delta_rule_workspace_bytes(t.num_envs, t.seq_len, t.heads, t.dim_k, t.dim_v, 1), q);
+    const at::Tensor scratch = call_scratch(rlk_delta_rule_workspace_bytes(t.num_envs, t.seq_len, t.heads, t.dim_k, t.dim_v, RLK_DELTA_BACKWARD), q);
     t.workspace = scratch.data_ptr(), t.workspace_bytes = (size_t)scratch.numel();
     const int st = rlk_gated_delta_rule_backward(&t, &to, saved.data_ptr(), (size_t)saved.numel(), c10::hip::getCurrentHIPStream(q.get_device()).stream());
     TORCH_CHECK(st == RLK_OK, "rlk_gated_delta_rule_backward failed: ", rlk_status_string(st));

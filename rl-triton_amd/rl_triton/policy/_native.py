@@ -255,6 +255,9 @@ def _delta_rule(q, k, v, out, log_decays, betas, dones, state, state_out, scale,
                      _bytes(ws))
 
 
+_FORWARD, _BACKWARD, _FORWARD_SAVED = 0, 1, 2  # RLK_DELTA_*
+
+
 def _scratch(need, like):
     """Memory of one call, from torch's allocator: it may be GBs (1, or what 512 pairs of environments and heads ask for, or one environment), so none is
     kept.  (Its later users follow on the stream.)"""
@@ -267,7 +270,7 @@ def gated_delta_rule(dev, stream, q, k, v, out, log_decays, betas, dones, state,
     lib = _lib or load()
     e, t, h, dk = q.shape
     saved = _scratch(lib.rlk_delta_rule_saved_bytes(e, t, h, dk, v.shape[-1]), q) if keep else None
-    ws = _scratch(lib.rlk_delta_rule_workspace_bytes(e, t, h, dk, v.shape[-1], 0), q)
+    ws = _scratch(lib.rlk_delta_rule_workspace_bytes(e, t, h, dk, v.shape[-1], _FORWARD_SAVED if keep else _FORWARD), q)
     call = _delta_rule(q, k, v, out, log_decays, betas, dones, state, state_out, scale, ws)
     _native._check(lib.rlk_gated_delta_rule(ctypes.byref(call), _ptr(saved), _bytes(saved), stream), "rlk_gated_delta_rule")
     return saved
@@ -277,7 +280,7 @@ def gated_delta_rule(dev, stream, q, k, v, out, log_decays, betas, dones, state,
 def gated_delta_rule_backward(dev, stream, q, k, v, log_decays, betas, dones, state, scale, saved, grad_out, grad_last, grads, grad_state):
     lib = _lib or load()
     e, t, h, dk = q.shape
-    ws = _scratch(lib.rlk_delta_rule_workspace_bytes(e, t, h, dk, v.shape[-1], 1), q)
+    ws = _scratch(lib.rlk_delta_rule_workspace_bytes(e, t, h, dk, v.shape[-1], _BACKWARD), q)
     call = _delta_rule(q, k, v, grad_out, log_decays, betas, dones, state, None, scale, ws)
     none = Sequence(None, 0, 0, 0)
     gq, gk, gv, gg, gb = grads
