@@ -345,7 +345,7 @@ template <class E>
 int launch_gradients(const Rule<E>& r, int64_t envs, hipStream_t s);
 
 // Segments: none where the pairs fill the GPU by themselves; else for one workgroup a CU ([1,16384,16,128+128] bf16: 465 us; 535 for two, more
-// to join and no faster walks; 3218 in one piece), of at least 8 chunks, and no fewer than 4 (cutting costs two more walks without outputs,
+// to join and no faster walks; 2490 in one piece), of at least 8 chunks, and no fewer than 4 (cutting costs two more walks without outputs,
 // which that many segments make up for).
 struct Segments {
   int segs;

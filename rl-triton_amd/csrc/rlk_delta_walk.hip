@@ -5,11 +5,12 @@
 // each other -- what the keys read, the corrections, the state's update -- pass results on as operands in registers: a result's lane holds a
 // column and 4 consecutive rows, which is the next product's inner index.  Columns do not meet, so neither do wavefronts.
 //
-// Bound by a chunk's chain: three products and the splits between them after each other (1200 vector instructions and 125 matrix products a wavefront and
+// Bound by a chunk's chain: three products and the splits between them after each other (1300 vector instructions and 150 matrix products a wavefront and
 // chunk of 64 rows), two barriers, two wavefronts a SIMD to fill the waits (registers: a state of 128 rows, its split and the next chunk on its
-// way; LDS: 70 KB in bf16, 146 KB in float32).  GPU time, us: [64,1024,8,64+64] bf16 forward 183 (3.4 TB/s of what it reads and leaves for
-// the way back), back 174 (3.5 TB/s); [1,16384,16,128+128] bf16 177 in 16 segments, the segments' states 181 before them and 43 for joining;
-// [37,333,4,40+72] float32 forward 75, back 67 (111 and 124 while keys were padded to the dims of the values).
+// way; LDS: 77 KB in bf16, 145 KB in float32).  GPU time, us: [64,1024,8,64+64] bf16 forward 194 (3.2 TB/s of what it reads and leaves for
+// the way back), back 176 (3.5 TB/s); [1,16384,16,128+128] bf16 194 in 16 segments, the segments' states 185 before them and 43 for joining;
+// [37,333,4,40+72] float32 forward 75, back 66 (111 and 124 while keys were padded to the dims of the values).  The walk back is one workgroup a pair
+// however few there are: training [1,16384,16,128+128] 3980.
 #include "rlk_delta.hpp"
 
 namespace rlk {

@@ -1,9 +1,9 @@
 // rlk_sample.hip -- actions sampled from logits with truncation (include/rl_triton_policy.h).
 //
 // A weight is exp((x - max) / temperature) as a whole number of 2^-43: computed in float64, and from then on every sum is exact and does not
-// depend on its order, so the action is the same however a row is split, and that of the definition in real numbers but for uniform numbers within
-// some 1e-13 of a border.  (Sums in float32 would be off by more than a probability of a large vocabulary.)  What the rounding leaves out of
-// 2^20 actions is below 2^-24, a float32 uniform number's last bit.
+// depend on its order, so the action is the same however a row is split, and that of the definition in real numbers but for uniform numbers as near
+// to a border as the weights' roundings add up to: 2^-44 each, some 1e-13 of a few actions, 1e-11 of a vocabulary's and at most 2^-24 of 2^20, a
+// float32 uniform number's last bit.  (Sums in float32 would be off by more than a probability of a large vocabulary.)
 //
 // Truncations keep a beginning of the actions in the order (logit falling, number rising): what is kept is told by comparing with its last
 // member.  Rows of up to 64 actions: a lane per action compares itself with all others.  Longer rows, a workgroup each: of a small top_k
@@ -40,7 +40,7 @@ struct Sampling {
 typedef unsigned long long u64;
 
 // exp(z) for z <= 0 as a multiple of 2^-43, rounded to nearest.
-// (rows of few actions; fast_weight() is for longer ones)
+// (rows of few actions; Weights is for longer ones)
 __device__ __forceinline__ u64 weight(double z) {
   if (!(z > -40.0)) return 0;  // (below half a unit)
   return (u64)__double2ll_rn(exp(z) * 0x1p43);
@@ -137,7 +137,7 @@ struct Shared {
   u64 sums[WAVES], sums2[WAVES];
   u64 before, border;
   uint32_t listed;
-  int bucket, chunk;
+  int bucket;
 };
 
 template <int NT>
@@ -621,7 +621,7 @@ int launch(Sampling s, hipStream_t stream) {
   } else {
     for (s.first = 0; s.first < rows; s.first += most) {
       const dim3 grid((unsigned)(rows - s.first < most ? rows - s.first : most));
-      // A row to a CU: by 1024 threads ([64] of 131072, top-k: 26 us against 33 by 512; by now 20).  More: two workgroups of 512 a CU, one of which works while the
+      // A row to a CU: by 1024 threads ([64] of 131072, top-k: 26 us against 33 by 512; by now 21).  More: two workgroups of 512 a CU, one of which works while the
       // other waits (top-p, [512] of 50001: 105 us, 127 by 1024).
       if (s.actions <= 4096) row_kernel<E, 256><<<grid, dim3(256), 0, stream>>>(s);
       else if (rows <= device_cus()) row_kernel<E, 1024><<<grid, dim3(1024), 0, stream>>>(s);

@@ -94,7 +94,8 @@ def compute_query_key_norms(
       (y[a] cos - y[b] sin, y[b] cos + y[a] sin), with (a, b) = (i, i + rotary_dim / 2), or (2 i, 2 i + 1) if `interleaved`
 
     Keys of length 1, as compute_gated_delta_rule expects them, have a weight of dim ** -0.5 in all places.  The angles are formed in
-    float64, so far positions are turned as exactly as near ones; the rest in float32, rounded once.
+    float64, so positions of a million are turned as exactly as near ones (from some 10^9 on 2^-53 of an angle's turns is more than float32's
+    rounding); the rest in float32, rounded once.
     Differentiable in q, k, q_weight and k_weight.
 
     Args:

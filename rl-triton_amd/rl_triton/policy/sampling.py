@@ -30,7 +30,8 @@ def compute_sampled_actions(
     p[0] + .. + p[action] > uniform.
 
     Probabilities are summed as whole numbers of 2^-43 of the largest, formed in float64, so an action depends neither on the order of
-    the sums nor on the storage of the rows, and is the definition's unless a uniform number lies within about 1e-13 of a border.  An action that is
+    the sums nor on the storage of the rows, and is the definition's unless a uniform number lies as near to a border as the roundings add up to:
+    some 1e-13 for a few actions, 1e-11 for a vocabulary, never above num_actions * 2^-44.  An action that is
     not allowed has a logit of -inf and is never taken; of a row of nothing else the action is -1 and the log-probability -inf, of a row with
     a NaN -1 and NaN.  A largest logit of +inf shares everything among its equals.  No gradient is computed.
 
