@@ -115,3 +115,24 @@ def test_a_state_that_leaves_float32_without_an_end(dtype):
     out, last, _ = _run(x, ups)
     assert not bool(torch.isfinite(last[:, 1]).any())
     assert torch.equal(out[:, :, 0], clean[0][:, :, 0]) and torch.equal(last[:, 0], clean[1][:, 0])
+
+
+def test_a_replay_does_not_remember_the_last_state():
+    """Captured once, replayed with a state that is not finite and with finite ones before and after: as the eager calls."""
+    x, *_ = _inputs(torch.bfloat16, 700, 34)
+    static = [t.cuda() for t in x]
+    fine = static[6].clone()
+    bad = fine.clone()
+    bad[0, 0, 3, 5], bad[0, 1, 0, 0] = math.nan, math.inf
+    policy.compute_gated_delta_rule(*static, 0.7)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out, last = policy.compute_gated_delta_rule(*static, 0.7)
+    for state in (fine, bad, fine, bad, bad, fine):
+        static[6].copy_(state)
+        graph.replay()
+        want = policy.compute_gated_delta_rule(*static, 0.7)
+        torch.cuda.synchronize()
+        for a, b in zip((out, last), want):
+            assert torch.equal(torch.isnan(a), torch.isnan(b)) and torch.equal(a.nan_to_num(), b.nan_to_num())
